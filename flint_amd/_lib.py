@@ -31,7 +31,9 @@ EXPORTS = [
     "fl_decode_step", "fl_decode_sample", "fl_decode_hidden", "fl_verify", "fl_kv_move", "fl_sample",
     "fl_sample_noalloc", "fl_probe_handoff", "fl_tile_int4", "fl_dequant_int4_tiled", "fl_gemv_int4_tiled",
     "fl_probe_dequant", "fl_gemm_rows_workspace", "fl_gemm_rows_int4",
-    "fl_prefill_workspace", "fl_prefill",
+    "fl_prefill_workspace", "fl_prefill", "fl_prefill_feat",
+    "fl_quantize_int8", "fl_gemm_int8_workspace", "fl_gemm_int8", "fl_linear_int8_workspace", "fl_linear_int8",
+    "fl_logprobs_workspace", "fl_logprobs", "fl_head_logprobs_workspace", "fl_head_logprobs",
 ]
 
 
@@ -76,6 +78,7 @@ def load(path=LIB_PATH):
         raise RuntimeError(f"{path} not found: run `python -m flint_amd.build` (HIP library required)")
     lib = ctypes.CDLL(path)
     vp, i32, f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_float
+    i64, pi64 = ctypes.c_int64, ctypes.POINTER(ctypes.c_int64)
     sig = {
         "fl_version": ([], i32),
         "fl_device_info": ([vp, vp], i32),
@@ -101,6 +104,16 @@ def load(path=LIB_PATH):
         "fl_verify": ([ctypes.POINTER(Weights), vp, vp, i32, vp, vp, i32, vp, vp, vp, vp], i32),
         "fl_prefill_workspace": ([vp, i32, ctypes.POINTER(ctypes.c_int64)], i32),
         "fl_prefill": ([ctypes.POINTER(Weights), vp, vp, i32, i32, vp, vp, vp], i32),
+        "fl_prefill_feat": ([ctypes.POINTER(Weights), vp, vp, i32, i32, vp, vp, vp, vp], i32),
+        "fl_quantize_int8": ([vp, vp, vp, i32, i32, vp], i32),
+        "fl_gemm_int8_workspace": ([i32, i32, i32, pi64], i32),
+        "fl_gemm_int8": ([vp, vp, vp, vp, vp, i32, vp, i32, i32, i32, vp], i32),
+        "fl_linear_int8_workspace": ([i32, i32, i32, pi64], i32),
+        "fl_linear_int8": ([vp, vp, vp, vp, i32, vp, i32, i32, i32, vp], i32),
+        "fl_logprobs_workspace": ([i32, i32, i32, pi64], i32),
+        "fl_logprobs": ([vp, i32, i64, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp], i32),
+        "fl_head_logprobs_workspace": ([i32, i32, i32, i32, pi64], i32),
+        "fl_head_logprobs": ([vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp], i32),
         "fl_kv_move": ([vp, vp, vp, i32, vp], i32),
         "fl_sample": ([vp, i32, i32, f32, i32, ctypes.c_uint64, ctypes.c_uint64, vp, vp, vp, vp], i32),
         "fl_sample_noalloc": ([vp, i32, i32, f32, i32, ctypes.c_uint64, ctypes.c_uint64, vp, vp, vp, vp], i32),

@@ -534,7 +534,9 @@ void pf_attention(const fl_state* st, const PfWs& w, int l, int T, int pos, hipS
     hipLaunchKernelGGL(k_pf_attn_merge, dim3((a.nkv * T * a.rep + 3) / 4), dim3(256), 0, s, a);
 }
 
-void pf_pass(const fl_weights* w, fl_state* st, const PfWs& ws, const int32_t* tokens, int T, int pos, hipStream_t s) {
+// last: where the final-normed rows go (ws.xn, or the caller's features)
+void pf_pass(const fl_weights* w, fl_state* st, const PfWs& ws, const int32_t* tokens, int T, int pos, uint16_t* last,
+             hipStream_t s) {
   const fl_model_desc& d = st->d;
   const int D = d.dim, F = d.inter, NQKV = (d.n_head + 2 * d.n_kv_head) * FL_HEAD_DIM, L = d.n_layer;
   auto mat = [&](const uint32_t* p, int l, int n, int k, int per) { return p + (size_t)l * n * (k / per); };
@@ -556,8 +558,33 @@ void pf_pass(const fl_weights* w, fl_state* st, const PfWs& ws, const int32_t* t
                           EpiSum{ws.part, T, D}, s);
     const uint16_t* next = l + 1 < L ? w->attn_norm + (size_t)(l + 1) * D : w->final_norm;
     hipLaunchKernelGGL(k_pf_norm, dim3(T), dim3(PF_NT), 0, s, ws.part, parts, T, D, tokens, w->embed, d.vocab,
-                       d.resid_mult, next, d.norm_eps, ws.h, ws.xn, st->err);
+                       d.resid_mult, next, d.norm_eps, ws.h, l + 1 < L ? ws.xn : last, st->err);
   }
+}
+
+// feat / token_out: null where not asked for
+int pf_run(const fl_weights* w, fl_state* st, const int32_t* tokens, int32_t n, int32_t pos, int32_t* token_out,
+           uint16_t* feat, void* workspace, void* stream) {
+  if (!st || !tokens || !workspace || n < 1 || !fl_weights_ok(w)) return FL_E_ARG;
+  // what fl_verify needs too: the tiled weight copies, a model that its kernels take
+  if (!w->wqkv_t || !w->wo_t || !w->wgu_t || !w->wd_t || !st->verify_ok) return FL_E_ARG;
+  if (pos < 0 || pos > st->max_seq - n || pos > w->rope_len - n) return FL_E_POS;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int most = std::min(n, PF_TOKENS);
+  const PfWs ws = pf_layout(st->d, most, static_cast<uint8_t*>(workspace));
+  int T = 0;
+  uint16_t* last = ws.xn;
+  for (int at = 0; at < n; at += T) {
+    T = std::min(most, n - at);
+    if (feat) last = feat + (size_t)at * st->d.dim;
+    pf_pass(w, st, ws, tokens + at, T, pos + at, last, s);
+  }
+  if (token_out) {
+    hipLaunchKernelGGL(k_pf_lmhead, dim3(PF_LM_GRID), dim3(PF_NT), 0, s, last + (size_t)(T - 1) * st->d.dim, w->embed,
+                       st->d.vocab, st->d.dim, st->d.logits_scaling, ws.best);
+    hipLaunchKernelGGL(k_pf_argmax, dim3(1), dim3(64), 0, s, ws.best, PF_LM_GRID, token_out);
+  }
+  return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
 }
 
 }  // namespace
@@ -572,22 +599,14 @@ int fl_prefill_workspace(fl_state* st, int32_t n, int64_t* bytes) {
 
 int fl_prefill(const fl_weights* w, fl_state* st, const int32_t* tokens, int32_t n, int32_t pos, int32_t* token_out,
                void* workspace, void* stream) {
-  if (!st || !tokens || !token_out || !workspace || n < 1 || !fl_weights_ok(w)) return FL_E_ARG;
-  // what fl_verify needs too: the tiled weight copies, a model that its kernels take
-  if (!w->wqkv_t || !w->wo_t || !w->wgu_t || !w->wd_t || !st->verify_ok) return FL_E_ARG;
-  if (pos < 0 || pos > st->max_seq - n || pos > w->rope_len - n) return FL_E_POS;
-  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int most = std::min(n, PF_TOKENS);
-  const PfWs ws = pf_layout(st->d, most, static_cast<uint8_t*>(workspace));
-  int T = 0;
-  for (int at = 0; at < n; at += T) {
-    T = std::min(most, n - at);
-    pf_pass(w, st, ws, tokens + at, T, pos + at, s);
-  }
-  hipLaunchKernelGGL(k_pf_lmhead, dim3(PF_LM_GRID), dim3(PF_NT), 0, s, ws.xn + (size_t)(T - 1) * st->d.dim, w->embed,
-                     st->d.vocab, st->d.dim, st->d.logits_scaling, ws.best);
-  hipLaunchKernelGGL(k_pf_argmax, dim3(1), dim3(64), 0, s, ws.best, PF_LM_GRID, token_out);
-  return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
+  if (!token_out) return FL_E_ARG;
+  return pf_run(w, st, tokens, n, pos, token_out, nullptr, workspace, stream);
+}
+
+int fl_prefill_feat(const fl_weights* w, fl_state* st, const int32_t* tokens, int32_t n, int32_t pos,
+                    int32_t* token_out, uint16_t* feat, void* workspace, void* stream) {
+  if (!feat || (reinterpret_cast<uintptr_t>(feat) & 15)) return FL_E_ARG;
+  return pf_run(w, st, tokens, n, pos, token_out, feat, workspace, stream);
 }
 
 }  // extern "C"

@@ -8,6 +8,9 @@
 // to every tensor it points into, so none can be freed under it.
 #include <torch/extension.h>
 
+#include <c10/core/impl/VirtualGuardImpl.h>
+
+#include <optional>
 #include <vector>
 
 #include "../../include/flint_amd.h"
@@ -224,6 +227,143 @@ pybind11::object linear_fast(const torch::Tensor& x, const torch::Tensor& q, con
   return pybind11::cast(y);
 }
 
+bool plain(const torch::Tensor& t, torch::ScalarType dt, int64_t dim) {
+  return t.defined() && t.is_cuda() && t.scalar_type() == dt && t.layout() == torch::kStrided && t.dim() == dim &&
+         t.is_contiguous();
+}
+bool on16(const torch::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+torch::Tensor bytes_of(int64_t n, const torch::Tensor& like) {
+  return n > 0 ? torch::empty({n}, like.options().dtype(torch::kUInt8).requires_grad(false)) : torch::Tensor();
+}
+void* data_of(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// every tensor on the device that is current and of the stream
+bool here(const torch::Tensor& a, std::initializer_list<const torch::Tensor*> rest) {
+  if (a.device().index() != c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getDevice().index()) return false;
+  for (const torch::Tensor* t : rest)
+    if (t->defined() && t->device() != a.device()) return false;
+  return true;
+}
+
+// quantize.gemm_int8 (xs given, x int8) and quantize.linear_int8 (no xs, x bf16) in one call, for the
+// arguments they take as they are; None for any other, which the caller's general path decides, as linear_fast.
+pybind11::object int8_fast(const torch::Tensor& x, const std::optional<torch::Tensor>& xs, const torch::Tensor& wq,
+                           const torch::Tensor& ws, bool f32, int64_t stream) {
+  if (!plain(wq, torch::kInt8, 2) || !plain(ws, torch::kFloat32, 1) || ws.size(0) != wq.size(0)) return pybind11::none();
+  const int64_t n = wq.size(0), k = wq.size(1);
+  if (x.dim() < 1 || !plain(x, xs ? torch::kInt8 : torch::kBFloat16, xs ? 2 : x.dim()) || k == 0 || n == 0 ||
+      x.size(-1) != k || x.numel() == 0)
+    return pybind11::none();
+  const int64_t m = x.numel() / k;
+  if (xs && (!plain(*xs, torch::kFloat32, 1) || xs->size(0) != m)) return pybind11::none();
+  if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX || !on16(x) || !on16(wq) ||
+      !here(x, {xs ? &*xs : &x, &wq, &ws}))
+    return pybind11::none();
+  int64_t need = 0;
+  const int32_t m_ = (int32_t)m, n_ = (int32_t)n, k_ = (int32_t)k;
+  if ((xs ? fl_gemm_int8_workspace(m_, n_, k_, &need) : fl_linear_int8_workspace(m_, n_, k_, &need)) != FL_OK)
+    return pybind11::none();
+  torch::Tensor y;
+  int rc = FL_E_HIP;
+  try {
+    pybind11::gil_scoped_release nogil;  // a launch may wait for room in the queue
+    auto sizes = x.sizes().vec();
+    sizes.back() = n;
+    y = torch::empty(sizes, x.options().dtype(f32 ? torch::kFloat32 : torch::kBFloat16).requires_grad(false));
+    const torch::Tensor work = bytes_of(need, x);
+    const auto* w = static_cast<const int8_t*>(wq.data_ptr());
+    const auto* s = static_cast<const float*>(ws.data_ptr());
+    rc = xs ? fl_gemm_int8(static_cast<const int8_t*>(x.data_ptr()), static_cast<const float*>(xs->data_ptr()), w, s,
+                           y.data_ptr(), f32, data_of(work), m_, n_, k_, stream_of(stream))
+            : fl_linear_int8(static_cast<const uint16_t*>(x.data_ptr()), w, s, y.data_ptr(), f32, data_of(work), m_, n_,
+                             k_, stream_of(stream));
+  } catch (const c10::OutOfMemoryError&) {
+  }
+  if (rc != FL_OK) return pybind11::none();  // the general path raises it
+  return pybind11::cast(y);
+}
+
+// Outputs of generate.logprobs and generate.head_logprobs, rows of them
+struct LogprobOut {
+  torch::Tensor logprob, entropy, rank, ids, top;
+  void make(int64_t rows, int64_t n, bool tokens, const torch::Tensor& like) {
+    const auto f = like.options().dtype(torch::kFloat32).requires_grad(false);
+    const auto i = f.dtype(torch::kInt32);
+    if (tokens) logprob = torch::empty({rows}, f), rank = torch::empty({rows}, i);
+    entropy = torch::empty({rows}, f);
+    if (n > 0) ids = torch::empty({rows, n}, i), top = torch::empty({rows, n}, f);
+  }
+  pybind11::object cast() const {
+    auto one = [](const torch::Tensor& t) -> pybind11::object {
+      return t.defined() ? pybind11::cast(t) : pybind11::object(pybind11::none());
+    };
+    return pybind11::make_tuple(one(logprob), one(entropy), one(rank), one(ids), one(top));
+  }
+};
+
+bool tokens_ok(const std::optional<torch::Tensor>& t, int64_t rows) {
+  return !t || (plain(*t, torch::kInt32, t->dim()) && t->numel() == rows);
+}
+
+// generate.logprobs: as int8_fast
+pybind11::object logprobs_fast(const torch::Tensor& l, const std::optional<torch::Tensor>& tokens, int64_t top,
+                               int64_t stream) {
+  const bool bf16 = l.scalar_type() == torch::kBFloat16;
+  if (l.dim() < 1 || l.dim() > 2 || !l.is_cuda() || l.layout() != torch::kStrided ||
+      (!bf16 && l.scalar_type() != torch::kFloat32) || l.numel() == 0 || l.stride(-1) != 1)
+    return pybind11::none();
+  const int64_t vocab = l.size(-1), rows = l.dim() == 2 ? l.size(0) : 1, stride = l.dim() == 2 ? l.stride(0) : vocab;
+  if (rows > INT32_MAX || vocab > INT32_MAX || top < 0 || top > INT32_MAX || (rows > 1 && stride < vocab) ||
+      !tokens_ok(tokens, rows) || !here(l, {tokens ? &*tokens : &l}))
+    return pybind11::none();
+  int64_t need = 0;
+  if (fl_logprobs_workspace((int32_t)rows, (int32_t)vocab, (int32_t)top, &need) != FL_OK) return pybind11::none();
+  LogprobOut o;
+  int rc = FL_E_HIP;
+  try {
+    pybind11::gil_scoped_release nogil;
+    o.make(rows, top, tokens.has_value(), l);
+    const torch::Tensor work = bytes_of(need, l);
+    rc = fl_logprobs(l.data_ptr(), bf16, stride, (int32_t)rows, (int32_t)vocab,
+                     tokens ? static_cast<const int32_t*>(tokens->data_ptr()) : nullptr, (int32_t)top,
+                     static_cast<float*>(data_of(o.logprob)), static_cast<float*>(data_of(o.entropy)),
+                     static_cast<int32_t*>(data_of(o.rank)), static_cast<int32_t*>(data_of(o.ids)),
+                     static_cast<float*>(data_of(o.top)), data_of(work), stream_of(stream));
+  } catch (const c10::OutOfMemoryError&) {
+  }
+  return rc == FL_OK ? o.cast() : pybind11::object(pybind11::none());
+}
+
+// generate.head_logprobs: as int8_fast
+pybind11::object head_logprobs_fast(const torch::Tensor& x, const torch::Tensor& wq, const torch::Tensor& ws,
+                                    const std::optional<torch::Tensor>& tokens, int64_t top, int64_t stream) {
+  if (!plain(wq, torch::kInt8, 2) || !plain(ws, torch::kFloat32, 1) || ws.size(0) != wq.size(0) || x.dim() < 1 ||
+      !plain(x, torch::kBFloat16, x.dim()) || x.numel() == 0 || wq.numel() == 0 || x.size(-1) != wq.size(1))
+    return pybind11::none();
+  const int64_t n = wq.size(0), k = wq.size(1), m = x.numel() / k;
+  if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX || top < 0 || top > INT32_MAX || !on16(x) || !on16(wq) ||
+      !tokens_ok(tokens, m) || !here(x, {&wq, &ws, tokens ? &*tokens : &x}))
+    return pybind11::none();
+  int64_t need = 0;
+  if (fl_head_logprobs_workspace((int32_t)m, (int32_t)n, (int32_t)k, (int32_t)top, &need) != FL_OK)
+    return pybind11::none();
+  LogprobOut o;
+  int rc = FL_E_HIP;
+  try {
+    pybind11::gil_scoped_release nogil;
+    o.make(m, top, tokens.has_value(), x);
+    const torch::Tensor work = bytes_of(need, x);
+    rc = fl_head_logprobs(static_cast<const uint16_t*>(x.data_ptr()), static_cast<const int8_t*>(wq.data_ptr()),
+                          static_cast<const float*>(ws.data_ptr()),
+                          tokens ? static_cast<const int32_t*>(tokens->data_ptr()) : nullptr, (int32_t)top,
+                          static_cast<float*>(data_of(o.logprob)), static_cast<float*>(data_of(o.entropy)),
+                          static_cast<int32_t*>(data_of(o.rank)), static_cast<int32_t*>(data_of(o.ids)),
+                          static_cast<float*>(data_of(o.top)), data_of(work), (int32_t)m, (int32_t)n, (int32_t)k,
+                          stream_of(stream));
+  } catch (const c10::OutOfMemoryError&) {
+  }
+  return rc == FL_OK ? o.cast() : pybind11::object(pybind11::none());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -238,5 +378,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("check", &Engine::check);
   m.def("int4_linear", &int4_linear);
   m.def("linear_fast", &linear_fast);
+  m.def("int8_fast", &int8_fast);
+  m.def("logprobs_fast", &logprobs_fast);
+  m.def("head_logprobs_fast", &head_logprobs_fast);
   m.def("version", []() { return fl_version(); });
 }

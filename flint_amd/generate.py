@@ -6,7 +6,19 @@ the device between steps: step i reads the token step i-1 wrote, so the loop iss
 back-to-back with no host synchronisation (gpt-fast's decode loop has none either). The prompt
 runs as GEMM passes over up to 1024 tokens (fl_prefill), a short one through the verify kernel.
 """
+import os
+from collections import namedtuple
+
 import torch
+
+# the whole of logprobs / head_logprobs as one call of the torch extension, as quantize's linears
+_logprobs_fast = _head_logprobs_fast = None
+if "FLINT_AMD_LIB" not in os.environ:
+    try:
+        from ._torch_ops import head_logprobs_fast as _head_logprobs_fast
+        from ._torch_ops import logprobs_fast as _logprobs_fast
+    except ImportError:
+        pass
 
 # prompts of more tokens than this run as fl_prefill passes: up to 16 tokens are one token pass of the verify
 # launch (flint-3b, 40 layers: 16 tokens 1.8 ms against 2.6 in a pass, 24 tokens 2.8 against 2.6)
@@ -79,6 +91,126 @@ def logits_to_probs(logits, temperature=1.0, top_k=None):
     return pr.view(logits.shape)
 
 
+# What logprobs and head_logprobs return, for R rows of logits: logprob fp32 [R] and rank int32 [R] of the tokens
+# given (None without tokens), entropy fp32 [R], top_ids int32 and top_logprobs fp32 [R, top] (None for top = 0).
+TokenLogprobs = namedtuple("TokenLogprobs", "logprob entropy rank top_ids top_logprobs")
+
+TOP_MAX = 32  # alternatives at most
+
+
+def _logprob_outputs(rows, tokens, top, dev):
+    f32, i32 = dict(dtype=torch.float32, device=dev), dict(dtype=torch.int32, device=dev)
+    return TokenLogprobs(torch.empty(rows, **f32) if tokens is not None else None, torch.empty(rows, **f32),
+                         torch.empty(rows, **i32) if tokens is not None else None,
+                         torch.empty(rows, top, **i32) if top else None, torch.empty(rows, top, **f32) if top else None)
+
+
+def _check_logprob_args(rows, vocab, tokens, top, dev):
+    """tokens as the kernels take them: int32 [rows] or None."""
+    if not 0 <= top <= min(TOP_MAX, vocab):
+        raise ValueError(f"top must be 0..{min(TOP_MAX, vocab)}")
+    if rows > 1 << 17 or not 1 <= vocab <= 1 << 20:
+        raise ValueError("at most 2^17 rows and a vocabulary of 1..2^20")
+    if tokens is None:
+        return None
+    if tokens.device != dev or tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("tokens must be int32 or int64, on the logits' device")
+    if tokens.numel() != rows:
+        raise ValueError(f"tokens: {tokens.numel()} ids for {rows} rows")
+    if tokens.dtype == torch.int64:
+        tokens = tokens.clamp(-1, 2 ** 31 - 1)  # ids outside the vocabulary stay outside it
+    return tokens.reshape(-1).to(torch.int32).contiguous()
+
+
+def logprobs(logits, tokens=None, top=0):
+    """Log probabilities of rows of logits (fp32 or bf16 device [V] or [..., V], strided rows too) on the GPU, in one
+    pass over them (fl_logprobs): of tokens (int, one per row; an id outside the vocabulary, as a padded row has,
+    gives NaN and rank -1) the log probability and the rank (0: the most likely; equal logits rank by
+    index), of every row the entropy in nats and the `top` (up to 32) most likely ids with their log probabilities. A
+    logit of -inf (a masked token) has probability 0; a row with nothing but -inf, or with a NaN or a +inf, gives NaN.
+    Returns TokenLogprobs over the flattened rows."""
+    from . import _lib
+    from .quantize import workspace
+    top = int(top)
+    if _logprobs_fast is not None and logits.is_cuda:
+        r = _logprobs_fast(logits, tokens, top, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+        if r is not None:
+            return TokenLogprobs(*r)
+    if not logits.is_cuda or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("logits must be an fp32 or bf16 CUDA (HIP) tensor")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits must be [..., V]")
+    vocab = logits.shape[-1]
+    lg = logits.detach()
+    lg = lg.reshape(-1, vocab) if lg.dim() != 2 else lg
+    rows = lg.shape[0]
+    if rows and (lg.stride(1) != 1 or (rows > 1 and lg.stride(0) < vocab)):
+        lg = lg.contiguous()
+    tokens = _check_logprob_args(rows, vocab, tokens, top, lg.device)
+    out = _logprob_outputs(rows, tokens, top, lg.device)
+    if rows:
+        with torch.cuda.device(lg.device):
+            work = workspace("fl_logprobs_workspace", rows, vocab, top, device=lg.device)
+            _lib.call("fl_logprobs", _lib.ptr(lg), int(lg.dtype == torch.bfloat16), lg.stride(0), rows, vocab,
+                      _lib.ptr(tokens), top, *map(_lib.ptr, out), _lib.ptr(work), _lib.stream_ptr())
+    return out
+
+
+def head_logprobs(feat, weight, scales, tokens=None, top=0):
+    """logprobs of the logits that an 8-bit vocabulary head (weight int8 [V, K], scales fp32 [V], as of
+    quantize.DynamicInt8Linear) gives for features (bf16 device [..., K], as of verify, prefill or decode), without
+    all of those logits in memory (fl_head_logprobs). The logits are fp32 and exact integer sums behind two scales, so
+    a row's ranks and ids do not depend on the batch it is scored in."""
+    from . import _lib
+    from .quantize import _check_weight, aligned16, workspace
+    top = int(top)
+    if _head_logprobs_fast is not None and feat.is_cuda:
+        r = _head_logprobs_fast(feat, weight, scales, tokens, top,
+                                torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+        if r is not None:
+            return TokenLogprobs(*r)
+    _check_weight(weight, scales)
+    n, k = weight.shape
+    if not feat.is_cuda or feat.dtype != torch.bfloat16:
+        raise ValueError("feat must be a torch.bfloat16 CUDA (HIP) tensor")
+    if feat.dim() < 1 or feat.shape[-1] != k or feat.device != weight.device:
+        raise ValueError(f"feat must be [..., {k}], on the weight's device")
+    x = aligned16(feat.detach().reshape(-1, k).contiguous())
+    rows = x.shape[0]
+    tokens = _check_logprob_args(rows, n, tokens, top, x.device)
+    out = _logprob_outputs(rows, tokens, top, x.device)
+    if rows:
+        with torch.cuda.device(x.device):
+            work = workspace("fl_head_logprobs_workspace", rows, n, k, top, device=x.device)
+            _lib.call("fl_head_logprobs", _lib.ptr(x), _lib.ptr(aligned16(weight)), _lib.ptr(scales), _lib.ptr(tokens),
+                      top, *map(_lib.ptr, out), _lib.ptr(work), rows, n, k, _lib.stream_ptr())
+    return out
+
+
+@torch.no_grad()
+def score(model, tokens, top=0, head=None):
+    """How likely a text is to the model: TokenLogprobs of tokens[1:] (int device [T], T >= 2), row i of the
+    distribution after tokens[:i + 1] at tokens[i + 1]. The tokens' K/V rows are in the cache afterwards.
+
+    head None: the model's own bf16 LM head, through the verify kernel's logits, 32 tokens at a time. head a
+    quantize.DynamicInt8Linear (Transformer.int8_head): one pass over the prompt and its features through the
+    8-bit head."""
+    from . import _lib
+    x = tokens.reshape(-1).to(device=model.device, dtype=torch.int32)
+    n = x.numel() - 1
+    if n < 1:
+        raise ValueError("score needs two tokens or more")
+    model.setup_caches(1, n + 1)
+    if head is not None:
+        return head_logprobs(model.prefill_features(x[:n], 0), head.weight, head.scales, x[1:], top)
+    parts = []
+    for s in range(0, n, _lib.MAX_VERIFY):
+        e = min(n, s + _lib.MAX_VERIFY)
+        _, logits, _ = model.verify(x[s:e], s, feat=False)
+        parts.append(logprobs(logits, x[s + 1:e + 1], top))
+    return TokenLogprobs(*(None if f[0] is None else torch.cat(f) for f in zip(*parts)))
+
+
 def decode_one_token(model, x, input_pos, logits=None, temperature=None, top_k=None, seed=0):
     """(next_token int32 device [1], logits) for one token at input_pos: greedy, or sampled when
     temperature or top_k is given (reference generate.py:62-66, sample at :52-55), with the
@@ -111,11 +243,13 @@ def decode_n_tokens(model, cur_token, input_pos, num_new_tokens, out=None):
 
 
 @torch.no_grad()
-def generate(model, prompt, max_new_tokens, temperature=None, top_k=None, seed=0):
+def generate(model, prompt, max_new_tokens, temperature=None, top_k=None, seed=0, logprobs=None):
     """Generate: returns int32 device [T + max_new_tokens] = prompt + new tokens. Greedy (the
     argmax fused into the decode kernel) unless temperature or top_k is given; then each step
     samples in the decode launch itself (fl_decode_sample) with the step's position as the noise
-    counter. Tokens stay on the device either way (no host synchronisation in the loop)."""
+    counter. Tokens stay on the device either way (no host synchronisation in the loop).
+    logprobs = n (0..32): (tokens, TokenLogprobs of the new ones with n alternatives each) of the
+    model's own distribution, before temperature and top_k."""
     prompt = prompt.reshape(-1).to(device=model.device, dtype=torch.int32)
     T = prompt.numel()
     model.setup_caches(1, T + max_new_tokens)
@@ -125,11 +259,25 @@ def generate(model, prompt, max_new_tokens, temperature=None, top_k=None, seed=0
         prefill(model, prompt[:-1], 0)
     sampled = temperature is not None or top_k is not None
     t = 1.0 if temperature is None else temperature
+    said, logits = [], None
+    if logprobs is not None:
+        _check_logprob_args(max_new_tokens, model.config.vocab_size, None, int(logprobs), seq.device)
+        logits = torch.empty(model.config.vocab_size, dtype=torch.float32, device=model.device)
     # the last prompt token produces the first new token
     for i in range(max_new_tokens):
         p = T - 1 + i
+        out = seq[p + 1:p + 2]
         if sampled:
-            model.decode_sample(seq[p:p + 1], p, t, top_k, seed=seed, offset=p, token_out=seq[p + 1:p + 2])
+            model.decode_sample(seq[p:p + 1], p, t, top_k, seed=seed, offset=p, token_out=out, logits=logits)
         else:
-            model.decode_step(seq[p:p + 1], p, token_out=seq[p + 1:p + 2])
-    return seq
+            model.decode_step(seq[p:p + 1], p, token_out=out, logits=logits)
+        if logits is not None:
+            said.append(_logprobs(logits, out, logprobs))
+    if logits is None:
+        return seq
+    if not said:
+        return seq, _logprob_outputs(0, seq[:0], int(logprobs), seq.device)
+    return seq, TokenLogprobs(*(None if f[0] is None else torch.cat(f) for f in zip(*said)))
+
+
+_logprobs = logprobs  # generate's argument of that name hides it there

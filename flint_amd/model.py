@@ -8,7 +8,7 @@ bf16 tensor, and one decode step is ONE cooperative kernel launch (fl_decode_ste
 import torch
 
 from . import _lib
-from .quantize import quantize_int4, tile_int4
+from .quantize import DynamicInt8Linear, quantize_int4, tile_int4
 from .synth import ModelArgs, freqs_cis_table
 
 
@@ -285,18 +285,37 @@ class Transformer:
         """A prompt (int32 device [n]) at cache slots pos..pos+n-1 in passes of up to 1024 tokens
         (fl_prefill): fills the cache and writes the greedy next token to token_out (int32 device
         [1]), which it returns. The workspace (80 MB for 1024 tokens of flint-3b) is torch's."""
+        tokens, n, ws = self._prefill_args(tokens, token_out)
+        _lib.call("fl_prefill", _lib.ctypes.byref(self._cw), self._state, _lib.ptr(tokens), n, int(pos),
+                  _lib.ptr(token_out), _lib.ptr(ws), _lib.stream_ptr())
+        return token_out
+
+    def _prefill_args(self, tokens, token_out):
         if self._state is None:
             raise RuntimeError("call setup_caches first")
         tokens = tokens.contiguous()
         for t, nm in ((tokens, "tokens"), (token_out, "token_out")):
-            if not t.is_cuda or t.dtype != torch.int32:
+            if t is not None and (not t.is_cuda or t.dtype != torch.int32):
                 raise ValueError(f"{nm} must be a {torch.int32} device tensor")
         n, need = tokens.numel(), _lib.ctypes.c_int64()
         _lib.call("fl_prefill_workspace", self._state, n, _lib.ctypes.byref(need))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=self.device)
-        _lib.call("fl_prefill", _lib.ctypes.byref(self._cw), self._state, _lib.ptr(tokens), n, int(pos),
-                  _lib.ptr(token_out), _lib.ptr(ws), _lib.stream_ptr())
-        return token_out
+        return tokens, n, torch.empty(need.value, dtype=torch.uint8, device=self.device)
+
+    def prefill_features(self, tokens, pos, token_out=None):
+        """prefill that returns the features of every token, bf16 [n, D] after the final norm
+        (fl_prefill_feat); the greedy next token is computed only where token_out is given."""
+        tokens, n, ws = self._prefill_args(tokens, token_out)
+        feat = torch.empty(n, self.config.dim, dtype=torch.bfloat16, device=self.device)
+        _lib.call("fl_prefill_feat", _lib.ctypes.byref(self._cw), self._state, _lib.ptr(tokens), n, int(pos),
+                  _lib.ptr(token_out), _lib.ptr(feat), _lib.ptr(ws), _lib.stream_ptr())
+        return feat
+
+    def int8_head(self):
+        """The tied LM head with 8-bit weights (quantize.DynamicInt8Linear, 126 MB for flint-3b), its scales
+        divided by logits_scaling: for generate.score and generate.head_logprobs. Made anew on every call."""
+        head = DynamicInt8Linear.from_float(self.packed.embed)
+        head.scales /= self.config.logits_scaling
+        return head
 
     def kv_move(self, src, dst):
         """Move the K/V rows of cache slots src[i] to dst[i] in every layer (host int lists, at most

@@ -1,5 +1,6 @@
 """Host side of the int4 weight path: quantise / dequantise / M=1 and M=k GEMV, all on the GPU
-through the C ABI, plus a drop-in for gpt-fast's WeightOnlyInt4Linear.
+through the C ABI, plus a drop-in for gpt-fast's WeightOnlyInt4Linear. Beside it 8-bit integers for
+weights and activations both (DynamicInt8Linear): one scale per output channel and per token.
 
 Mirrors reference engine/quantize.py:359-525 (prepare_int4_weight_and_scales_and_zeros,
 linear_forward_int4, WeightOnlyInt4Linear): same groupsize (128), same quantised values,
@@ -15,10 +16,11 @@ GROUP = _lib.GROUP
 
 # the whole forward of WeightOnlyInt4Linear as one call of the torch extension, over the library
 # beside it (not over another one that FLINT_AMD_LIB names)
-_linear_fast = None
+_linear_fast = _int8_fast = None
 if "FLINT_AMD_LIB" not in os.environ:
     try:
         from ._torch_ops import linear_fast as _linear_fast
+        from ._torch_ops import int8_fast as _int8_fast
     except ImportError:
         pass
 
@@ -198,3 +200,143 @@ class WeightOnlyInt4Linear(torch.nn.Module):
         else:
             y = gemm_int4(self.weight, self.scales_and_zeros, x2)
         return y.view(*shape[:-1], self.out_features)
+
+
+# ---- 8-bit integers ------------------------------------------------------------------------------
+
+def _check_int8(k):
+    if k % 16 or not 16 <= k <= 65536:
+        raise ValueError("K must be a multiple of 16, at most 65536")
+
+
+def _check_weight(wq, ws):
+    _check_dev(wq, torch.int8, "weight")
+    _check_dev(ws, torch.float32, "scales")
+    if wq.dim() != 2 or ws.shape != wq.shape[:1]:
+        raise ValueError("weight must be [N, K] and scales [N]")
+    _check_int8(wq.shape[1])
+    if ws.device != wq.device:
+        raise ValueError("weight and scales must be on one device")
+
+
+def aligned16(t):
+    """t, or a copy of it where its data does not start on 16 bytes (a view into a tensor may not)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def workspace(name, *sizes, device):
+    """Device bytes for a call, of what the C entry `name` asks for (None where that is 0)."""
+    need = _lib.ctypes.c_int64()
+    _lib.call(name, *sizes, _lib.ctypes.byref(need))
+    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+
+
+def quantize_int8(x, q=None, scale=None):
+    """Rows of a bf16 [M, K] device matrix in 8 bits: (q int8 [M, K], scale fp32 [M]), scale = max|row| times
+    fp32(1 / 127) and q = row / scale rounded to the nearest, ties to even (fl_quantize_int8). For a weight matrix these are its
+    output channels, for activations the tokens."""
+    _check_dev(x, torch.bfloat16, "x")
+    if x.dim() != 2:
+        raise ValueError("x must be [M, K]")
+    m, k = x.shape
+    _check_int8(k)
+    if q is None:
+        q = torch.empty(m, k, dtype=torch.int8, device=x.device)
+    if scale is None:
+        scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    _check_dev(q, torch.int8, "q")
+    _check_dev(scale, torch.float32, "scale")
+    if q.shape != x.shape or scale.shape != x.shape[:1] or q.device != x.device or scale.device != x.device:
+        raise ValueError("q must be [M, K] and scale [M], on x's device")
+    if m:
+        with torch.cuda.device(x.device):
+            _lib.call("fl_quantize_int8", _lib.ptr(aligned16(x)), _lib.ptr(q), _lib.ptr(scale), m, k, _lib.stream_ptr())
+    return q, scale
+
+
+def _check_out_dtype(out_dtype):
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("out_dtype must be torch.bfloat16 or torch.float32")
+
+
+def gemm_int8(xq, xs, wq, ws, out_dtype=torch.bfloat16):
+    """Y[M, N] = (xq . wq^T) * xs[:, None] * ws for 8-bit rows xq [M, K] and weights wq [N, K] with one fp32 scale
+    per row (quantize_int8's). The integer sums are exact, so a row's result does not depend on the batch
+    it is in. out_dtype: bf16, or fp32 (logits)."""
+    f32 = out_dtype is torch.float32
+    if _int8_fast is not None and xq.is_cuda and (f32 or out_dtype is torch.bfloat16):
+        y = _int8_fast(xq, xs, wq, ws, f32, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+        if y is not None:
+            return y
+    _check_out_dtype(out_dtype)
+    _check_weight(wq, ws)
+    _check_dev(xq, torch.int8, "xq")
+    _check_dev(xs, torch.float32, "xs")
+    n, k = wq.shape
+    if xq.dim() != 2 or xq.shape[1] != k or xs.shape != xq.shape[:1]:
+        raise ValueError("xq must be [M, K] and xs [M]")
+    if xq.device != wq.device or xs.device != wq.device:
+        raise ValueError("xq, xs and weight must be on one device")
+    m = xq.shape[0]
+    y = torch.empty(m, n, dtype=out_dtype, device=xq.device)
+    if m and n:
+        with torch.cuda.device(xq.device):
+            work = workspace("fl_gemm_int8_workspace", m, n, k, device=xq.device)
+            _lib.call("fl_gemm_int8", _lib.ptr(aligned16(xq)), _lib.ptr(xs), _lib.ptr(aligned16(wq)), _lib.ptr(ws),
+                      _lib.ptr(y), int(f32), _lib.ptr(work), m, n, k, _lib.stream_ptr())
+    return y
+
+
+def linear_int8(x, wq, ws, out_dtype=torch.bfloat16):
+    """x [..., K] bf16 -> [..., N]: quantize_int8 of x's rows (tokens) and gemm_int8 with the weights, in one call
+    (fl_linear_int8)."""
+    f32 = out_dtype is torch.float32
+    if _int8_fast is not None and x.is_cuda and (f32 or out_dtype is torch.bfloat16):
+        y = _int8_fast(x, None, wq, ws, f32, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+        if y is not None:
+            return y
+    _check_out_dtype(out_dtype)
+    _check_weight(wq, ws)
+    n, k = wq.shape
+    if not x.is_cuda or x.dtype != torch.bfloat16:
+        raise ValueError("x must be a torch.bfloat16 CUDA (HIP) tensor")
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"x's last dimension must be {k}")
+    if x.device != wq.device:
+        raise ValueError("x and weight must be on one device")
+    x2 = aligned16(x.detach().reshape(-1, k).contiguous())
+    m = x2.shape[0]
+    y = torch.empty(m, n, dtype=out_dtype, device=x.device)
+    if m and n:
+        with torch.cuda.device(x.device):
+            work = workspace("fl_linear_int8_workspace", m, n, k, device=x.device)
+            _lib.call("fl_linear_int8", _lib.ptr(x2), _lib.ptr(aligned16(wq)), _lib.ptr(ws), _lib.ptr(y), int(f32),
+                      _lib.ptr(work), m, n, k, _lib.stream_ptr())
+    return y.view(*x.shape[:-1], n)
+
+
+class DynamicInt8Linear(torch.nn.Module):
+    """A linear with 8-bit integer weights (one scale per output channel) whose input rows are quantised on the
+    way, one scale per token: the product runs on the integer matrix cores. For inference.
+
+    forward(x [..., K] bf16) -> [..., N] bf16, K a multiple of 16. For a vocabulary head whose logits are wanted in
+    fp32 or as log probabilities: linear_int8(..., out_dtype=torch.float32), generate.head_logprobs.
+    """
+
+    def __init__(self, in_features, out_features, bias=False, device=None):
+        super().__init__()
+        if bias:
+            raise ValueError("require bias=False")
+        _check_int8(in_features)
+        self.in_features, self.out_features = in_features, out_features
+        self.register_buffer("weight", torch.zeros(out_features, in_features, dtype=torch.int8, device=device))
+        self.register_buffer("scales", torch.zeros(out_features, dtype=torch.float32, device=device))
+
+    @classmethod
+    def from_float(cls, w):
+        m = cls(w.shape[1], w.shape[0], device=w.device)
+        quantize_int8(w.detach().to(torch.bfloat16).contiguous(), m.weight, m.scales)
+        return m
+
+    def forward(self, x):
+        return linear_int8(x.to(torch.bfloat16), self.weight, self.scales)

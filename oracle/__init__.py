@@ -8,6 +8,9 @@ Contents (each function cites the reference file:line it restates):
   model.py  - gpt-fast forward on dequantised weights with the reference's bf16 rounding points
               (engine/model.py), NEOX RoPE, fp32 attention, greedy decode (engine/generate.py)
 
+  scoring.py - 8-bit integer linears bit for bit, and log probabilities in float64 (no counterpart in the
+              reference; definitions in include/flint_amd.h)
+
 How each part is pinned (see tests/test_oracle.py):
   quant      closed-form invariants, brute force on tiny groups, and torch's independent CPU int4
              library kernel (aten::_weight_int4pack_mm_for_cpu) on the oracle's q / scales / zeros

@@ -1,0 +1,111 @@
+"""Refusals of the 8-bit linears and of the log probabilities, before anything reaches a device."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from flint_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    return _lib.load()
+
+
+P = ctypes.c_void_p(256)
+ODD = ctypes.c_void_p(264)  # not on 16 bytes
+
+
+@pytest.mark.parametrize("rows,k", [(0, 64), (-1, 64), (1, 0), (1, 8), (1, 24), (1, 65552), ((1 << 23) + 1, 64)])
+def test_shapes_that_8_bit_rows_do_not_take(lib, rows, k):
+    need = ctypes.c_int64()
+    assert lib.fl_quantize_int8(P, P, P, rows, k, None) == -1
+    for m, n in ((rows, 64), (64, rows)) if rows != 1 else ((1, 64),):
+        assert lib.fl_gemm_int8_workspace(m, n, k, ctypes.byref(need)) == -1
+        assert lib.fl_linear_int8_workspace(m, n, k, ctypes.byref(need)) == -1
+        assert lib.fl_gemm_int8(P, P, P, P, P, 0, P, m, n, k, None) == -1
+        assert lib.fl_linear_int8(P, P, P, P, 0, P, m, n, k, None) == -1
+        assert lib.fl_head_logprobs_workspace(m, n, k, 0, ctypes.byref(need)) == -1
+        assert lib.fl_head_logprobs(P, P, P, None, 0, None, P, None, None, None, P, m, n, k, None) == -1
+
+
+def test_pointers_that_8_bit_rows_do_not_take(lib):
+    for i in range(3):
+        a = [P, P, P]
+        a[i] = None
+        assert lib.fl_quantize_int8(*a, 4, 64, None) == -1
+    assert lib.fl_quantize_int8(ODD, P, P, 4, 64, None) == -1
+    assert lib.fl_quantize_int8(P, ODD, P, 4, 64, None) == -1
+    for bad in (None, ODD):
+        for i in (0, 2, 4):
+            a = [P, P, P, P, P, 0, P]
+            a[i] = bad
+            assert lib.fl_gemm_int8(*a, 4, 64, 64, None) == -1
+        for i in (0, 1, 3, 5):
+            a = [P, P, P, P, 0, P]
+            a[i] = bad
+            assert lib.fl_linear_int8(*a, 4, 64, 64, None) == -1
+    for i in (1, 3):
+        a = [P, P, P, P, P, 0, P]
+        a[i] = None
+        assert lib.fl_gemm_int8(*a, 4, 64, 64, None) == -1
+    assert lib.fl_gemm_int8_workspace(4, 64, 64, None) == -1
+    assert lib.fl_linear_int8_workspace(4, 64, 64, None) == -1
+
+
+def test_log_probabilities_that_are_refused(lib):
+    need = ctypes.c_int64()
+
+    def call(logits=P, stride=1000, rows=4, vocab=1000, tokens=P, top=5, outs=(P, P, P, P, P), work=P):
+        return lib.fl_logprobs(logits, 0, stride, rows, vocab, tokens, top, *outs, work, None)
+
+    for rows, vocab, top in ((0, 1000, 5), (4, 0, 0), (4, 1000, 33), (4, 1000, -1), (4, 7, 8), (4, (1 << 20) + 1, 5),
+                             ((1 << 17) + 1, 1000, 5)):
+        assert call(rows=rows, vocab=vocab, top=top, stride=1 << 21) == -1
+        assert lib.fl_logprobs_workspace(rows, vocab, top, ctypes.byref(need)) == -1
+    assert call(logits=None) == -1
+    assert call(stride=999) == -1                      # rows that overlap
+    assert call(outs=(None, P, P, P, P)) == -1         # tokens without a place for their log probabilities
+    assert call(outs=(P, None, P, P, P)) == -1
+    assert call(outs=(P, P, None, P, P)) == -1
+    assert call(outs=(P, P, P, None, P)) == -1
+    assert call(outs=(P, P, P, P, None)) == -1
+    assert lib.fl_logprobs_workspace(1, 49152, 5, ctypes.byref(need)) == 0 and need.value > 0
+    assert call(rows=1, vocab=49152, work=None) == -1  # several chunks of a row need it
+    assert call(rows=1, vocab=49152, work=ODD) == -1
+    assert lib.fl_head_logprobs_workspace(4, 1000, 64, 33, ctypes.byref(need)) == -1
+    for bad in (None, ODD):
+        for i in (0, 1, 10):
+            a = [P, P, P, P, 5, P, P, P, P, P, P]
+            a[i] = bad
+            assert lib.fl_head_logprobs(*a, 4, 1000, 64, None) == -1
+
+
+def test_a_prompt_with_features_needs_its_arguments(lib):
+    assert lib.fl_prefill_feat(None, None, P, 4, 0, None, P, P, None) == -1
+    assert lib.fl_prefill_feat(None, None, P, 4, 0, None, None, P, None) == -1
+    assert lib.fl_prefill_feat(None, None, P, 4, 0, None, ODD, P, None) == -1
+
+
+def test_host_layer_refuses():
+    from flint_amd import generate, quantize
+    w, s = torch.zeros(8, 32, dtype=torch.int8), torch.zeros(8)
+    x = torch.zeros(2, 32, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        quantize.quantize_int8(x)                      # not on a device
+    with pytest.raises(ValueError):
+        quantize.linear_int8(x, w, s)
+    with pytest.raises(ValueError):
+        quantize.gemm_int8(w, s, w, s)
+    with pytest.raises(ValueError):
+        quantize.gemm_int8(w, s, w, s, out_dtype=torch.float16)
+    with pytest.raises(ValueError):
+        generate.logprobs(torch.zeros(3, 10))
+    with pytest.raises(ValueError):
+        generate.head_logprobs(x, w, s)
+    with pytest.raises(ValueError):
+        quantize.DynamicInt8Linear(40, 8)              # K not a multiple of 16
+    with pytest.raises(ValueError):
+        quantize.DynamicInt8Linear(32, 8, bias=True)

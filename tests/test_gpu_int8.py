@@ -1,0 +1,231 @@
+"""8-bit integer rows, products and linears. Every bit is defined: the quotients and sums are exact, two fp32
+products and one rounding follow, so results are compared for equality with the oracle's."""
+import math
+
+import pytest
+import torch
+
+from flint_amd import _lib, quantize
+from oracle import scoring
+
+pytestmark = pytest.mark.gpu
+
+
+def rows_of(m, k, seed, kind="normal"):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g)
+    if kind == "outliers":
+        x[:, torch.randint(0, k, (max(1, k // 100),), generator=g)] *= 30.0
+    if kind == "ties":  # every value a multiple of half a scale step: max = 127 / 128
+        x = torch.randint(-254, 255, (m, k), generator=g).float() / 256.0
+        x[:, 0] = 254.0 / 256.0
+    if kind == "halves":  # the largest value halved again and again
+        x = x.abs().amax(1, keepdim=True) * 2.0 ** -torch.randint(0, 9, (m, k), generator=g).float()
+        x[:, 0] *= 2.0
+    if kind == "tiny":
+        x = x * 2.0 ** -torch.randint(120, 134, (m, 1), generator=g).float()
+    if kind == "huge":
+        x = x.sign() * torch.rand(m, k, generator=g) * 3.3e38
+    return x.to(torch.bfloat16)
+
+
+def same(a, b):
+    a, b = a.cpu(), b.cpu()
+    return a.dtype == b.dtype and torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+@pytest.mark.parametrize("kind", ["normal", "outliers", "ties", "halves", "tiny", "huge"])
+@pytest.mark.parametrize("m,k", [(1, 16), (5, 48), (3, 2560), (2, 8192), (2, 8208), (1, 65536)])
+def test_quantized_rows_are_the_oracles(dev, m, k, kind):
+    x = rows_of(m, k, 7 * m + k, kind)
+    q, s = quantize.quantize_int8(x.to(dev))
+    qr, sr = scoring.quantize_rows(x)
+    assert torch.equal(s.cpu(), sr)
+    assert torch.equal(q.cpu(), qr)
+    # half a step, and the half ulp that the scale may be off, of 127 steps
+    live = sr > 2.0 ** -100
+    off = (q.cpu().double() * sr.double()[:, None] - x.double()).abs().amax(1)
+    assert bool((off[live] <= sr.double()[live] * (0.5 + 127 * 2.0 ** -22)).all())
+
+
+def test_quantized_rows_at_every_mantissa_and_quotient(dev):
+    """All bf16 mantissas as the row's maximum, against every smaller bf16 value of nine octaves."""
+    top = torch.arange(128, 256).float()
+    small = torch.cat([torch.arange(128, 256).float() * 2.0 ** -e for e in range(1, 10)])
+    small = torch.cat([small, -small, top, -top])
+    x = small.repeat(128, 1)
+    x = torch.where(x.abs() > top[:, None], torch.zeros(()), x)
+    x = torch.cat([top[:, None], x, torch.zeros(128, (-(x.shape[1] + 1)) % 16)], 1).to(torch.bfloat16)
+    q, s = quantize.quantize_int8(x.to(dev))
+    qr, sr = scoring.quantize_rows(x)
+    assert torch.equal(s.cpu(), sr) and torch.equal(q.cpu(), qr)
+
+
+def test_rows_of_zeros_nan_and_infinities(dev):
+    x = rows_of(6, 96, 3)
+    x[1] = 0.0
+    x[2, 95] = math.nan
+    x[3, 0] = -math.inf
+    x[4] = -0.0
+    q, s = quantize.quantize_int8(x.to(dev))
+    qr, sr = scoring.quantize_rows(x)
+    assert torch.equal(q.cpu(), qr) and same(s, sr)
+    assert s[1] == 0 and s[4] == 0 and s[2].isnan() and s[3].isnan()
+    w = quantize.DynamicInt8Linear.from_float(rows_of(40, 96, 4).to(dev))
+    y, clean = w(x.to(dev)).cpu(), w(rows_of(6, 96, 3).to(dev)).cpu()
+    assert bool(y[2].isnan().all()) and bool(y[3].isnan().all()) and bool((y[1] == 0).all())
+    for r in (0, 5):  # the other rows are what they were
+        assert torch.equal(y[r], clean[r])
+
+
+M_SIZES = [1, 2, 3, 5, 8, 15, 16, 17, 31, 32, 33, 47, 48, 63, 64, 65, 96, 127, 128, 129, 200, 256, 257, 333, 520]
+SHAPES = [(1, 16), (17, 48), (70, 64), (64, 128), (129, 144), (257, 272), (500, 1040), (2570, 2560), (96, 8192)]
+
+
+def ints(m, k, seed, extreme=False):
+    g = torch.Generator().manual_seed(seed)
+    if extreme:
+        return torch.where(torch.rand(m, k, generator=g) < 0.97, -128, 127).to(torch.int8)
+    return torch.randint(-128, 128, (m, k), generator=g).to(torch.int8)
+
+
+@pytest.mark.parametrize("n,k", SHAPES)
+def test_products_are_exact(dev, n, k):
+    wq = ints(n, k, n + k)
+    ws = torch.rand(n, generator=torch.Generator().manual_seed(k)) * 1e-3
+    wd, sd = wq.to(dev), ws.to(dev)
+    xq = ints(max(M_SIZES), k, n)
+    xs = torch.rand(max(M_SIZES), generator=torch.Generator().manual_seed(n)) * 0.05
+    ref = scoring.product(xq, xs, wq, ws)
+    for m in M_SIZES:
+        y = quantize.gemm_int8(xq[:m].to(dev), xs[:m].to(dev), wd, sd, out_dtype=torch.float32)
+        assert torch.equal(y.cpu(), ref[:m]), m
+        y = quantize.gemm_int8(xq[:m].to(dev), xs[:m].to(dev), wd, sd)
+        assert torch.equal(y.cpu(), ref[:m].to(torch.bfloat16)), m
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 130, 300])
+def test_sums_of_the_largest_values(dev, m):
+    n, k = 72, 65536  # 128 * 128 * 65536 = 2^30
+    xq, wq = ints(m, k, 1, True), ints(n, k, 2, True)
+    one = torch.ones(max(m, n))
+    y = quantize.gemm_int8(xq.to(dev), one[:m].to(dev), wq.to(dev), one[:n].to(dev), out_dtype=torch.float32)
+    ref = scoring.product(xq, one[:m], wq, one[:n])
+    assert float(ref.abs().max()) > 2.0 ** 29
+    assert torch.equal(y.cpu(), ref)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 2560, 2560), (4, 3584, 2560), (12, 5003, 1408), (20, 16384, 2560), (32, 2560, 8192),
+                                   (33, 2560, 8192), (100, 1000, 4112), (1024, 3584, 2560), (300, 16384, 2560),
+                                   (1, 49152, 2560), (7, 49152, 2560)])
+def test_linear_is_quantising_and_the_product(dev, m, n, k):
+    w, x = rows_of(n, k, m), rows_of(m, k, n, "outliers")
+    lin = quantize.DynamicInt8Linear.from_float(w.to(dev))
+    wq, ws = lin.weight.cpu(), lin.scales.cpu()
+    xq, xs = scoring.quantize_rows(x)
+    ref = scoring.product(xq, xs, wq, ws)
+    assert torch.equal(lin(x.to(dev)).cpu(), ref.to(torch.bfloat16))
+    y = quantize.linear_int8(x.to(dev), lin.weight, lin.scales, out_dtype=torch.float32)
+    assert torch.equal(y.cpu(), ref)
+    # a row alone gives the bits that it gives in the batch
+    for r in {0, m // 2, m - 1}:
+        assert torch.equal(quantize.linear_int8(x[r:r + 1].to(dev), lin.weight, lin.scales, torch.float32).cpu(),
+                           ref[r:r + 1])
+
+
+def test_linear_takes_the_inputs_that_linears_take(dev):
+    lin = quantize.DynamicInt8Linear.from_float(rows_of(48, 64, 1).to(dev))
+    x = rows_of(6, 64, 2).to(dev)
+    y = lin(x)
+    assert torch.equal(lin(x.view(2, 3, 64)), y.view(2, 3, 48))
+    assert torch.equal(lin(x[0]), y[0])
+    assert torch.equal(lin(x.float()), y)
+    wide = torch.zeros(6, 80, dtype=torch.bfloat16, device=dev)
+    wide[:, :64] = x
+    assert torch.equal(lin(wide[:, :64]), y)                      # strided rows
+    assert torch.equal(lin(x.t().contiguous().t()), y)            # another order
+    shifted = torch.zeros(6 * 64 + 1, dtype=torch.bfloat16, device=dev)[1:].view(6, 64)
+    shifted.copy_(x)
+    assert shifted.data_ptr() % 16 and torch.equal(lin(shifted), y)
+    w2 = torch.zeros(48 * 64 + 1, dtype=torch.int8, device=dev)[1:].view(48, 64)
+    w2.copy_(lin.weight)
+    assert torch.equal(quantize.linear_int8(x, w2, lin.scales), y)
+    xq, xs = quantize.quantize_int8(x)
+    q2 = torch.zeros(6 * 64 + 1, dtype=torch.int8, device=dev)[1:].view(6, 64)
+    q2.copy_(xq)
+    assert torch.equal(quantize.gemm_int8(q2, xs, lin.weight, lin.scales), y)
+    assert lin(x[:0]).shape == (0, 48) and lin(x.view(2, 3, 64)[:, :0]).shape == (2, 0, 48)
+    assert quantize.gemm_int8(xq[:0], xs[:0], lin.weight, lin.scales).shape == (0, 48)
+    assert not lin(x.detach().requires_grad_()).requires_grad
+
+
+def test_refusals(dev):
+    lin = quantize.DynamicInt8Linear.from_float(rows_of(48, 64, 1).to(dev))
+    x = rows_of(6, 64, 2).to(dev)
+    xq, xs = quantize.quantize_int8(x)
+    w, s = lin.weight, lin.scales
+    for bad in (lambda: quantize.linear_int8(x.float(), w, s), lambda: quantize.linear_int8(x[:, :48], w, s),
+                lambda: quantize.linear_int8(x, w.t(), s), lambda: quantize.linear_int8(x, w, s[:40]),
+                lambda: quantize.linear_int8(x, w, s.double()), lambda: quantize.linear_int8(x, w, s, torch.float16),
+                lambda: quantize.linear_int8(x, w.cpu(), s), lambda: quantize.gemm_int8(xq, xs[:5], w, s),
+                lambda: quantize.gemm_int8(x, xs, w, s), lambda: quantize.gemm_int8(xq[:, :48], xs, w, s),
+                lambda: quantize.quantize_int8(x[:, :40].contiguous()), lambda: quantize.quantize_int8(x.float()),
+                lambda: quantize.quantize_int8(x, q=xq[:5]), lambda: quantize.quantize_int8(x, scale=xs[:5])):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 33, 80), (7, 100, 2560), (40, 77, 208), (130, 131, 336), (300, 259, 272)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_writes_its_outputs_and_nothing_else(dev, m, n, k, f32):
+    xq, wq = ints(m, k, 1).to(dev), ints(n, k, 2).to(dev)
+    xs, ws = torch.rand(m, device=dev), torch.rand(n, device=dev)
+    y = torch.full((m * n + 4096,), -7.0, dtype=torch.float32 if f32 else torch.bfloat16, device=dev)
+    need = _lib.ctypes.c_int64()
+    _lib.call("fl_gemm_int8_workspace", m, n, k, _lib.ctypes.byref(need))
+    work = torch.full((need.value + 4096,), 0x5A, dtype=torch.uint8, device=dev)
+    _lib.call("fl_gemm_int8", _lib.ptr(xq), _lib.ptr(xs), _lib.ptr(wq), _lib.ptr(ws), _lib.ptr(y), int(f32),
+              _lib.ptr(work), m, n, k, _lib.stream_ptr())
+    ref = scoring.product(xq.cpu(), xs.cpu(), wq.cpu(), ws.cpu()).to(y.dtype)
+    assert torch.equal(y[:m * n].view(m, n).cpu(), ref)
+    assert bool((y[m * n:] == -7.0).all()) and bool((work[need.value:] == 0x5A).all())
+
+
+@pytest.mark.parametrize("m", [1, 9, 40, 100, 400])
+def test_captured_and_replayed(dev, m):
+    n, k = 520, 1296
+    lin = quantize.DynamicInt8Linear.from_float(rows_of(n, k, 1).to(dev))
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=dev)
+    lin(x)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # two graphs, each with workspaces of its own
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = lin(x)
+        graphs.append((g, y))
+    for seed in range(4):
+        new = rows_of(m, k, seed)
+        x.copy_(new)
+        for g, y in graphs:
+            g.replay()
+            assert torch.equal(y.cpu(), lin(x).cpu())
+            torch.cuda.synchronize()
+        xq, xs = scoring.quantize_rows(new)
+        ref = scoring.product(xq, xs, lin.weight.cpu(), lin.scales.cpu()).to(torch.bfloat16)
+        assert torch.equal(graphs[0][1].cpu(), ref)
+
+
+def test_two_streams_at_once(dev):
+    lin = quantize.DynamicInt8Linear.from_float(rows_of(2560, 2560, 1).to(dev))
+    xs = [rows_of(m, 2560, m).to(dev) for m in (1, 16, 64, 300)]
+    ref = [lin(x).cpu() for x in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in xs], []
+    for _ in range(3):
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                got.append(lin(x))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y.cpu(), ref[i % len(xs)])
