@@ -7,10 +7,12 @@
 // whatever the batch.
 #include "fl_int8.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
 typedef int i8_x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t i8_u32x4 __attribute__((ext_vector_type(4)));
 
 // ---- quantisation -------------------------------------------------------------------------------
 
@@ -148,6 +150,235 @@ __global__ __launch_bounds__(64 * KW) void k_i8_rows(const int8_t* __restrict__ 
   }
 }
 
+// ---- tiles ------------------------------------------------------------------------------------------
+// A workgroup of WM x WN waves computes BM rows of x against BN weight rows over one part of K, in steps of 128
+// bytes of K. Both tiles of a step go straight from memory into LDS (buffer_load ... lds, 1 KB = 8 rows of 128
+// bytes per wave instruction), ST stages deep: a step's loads are issued ST - 1 steps before it. In LDS the 16-byte
+// piece c of row r sits at c ^ (r % 8), so that the 8 lanes of a read phase, on one piece of 8 rows, take all
+// banks; the lanes of the load fetch the pieces in that order. Waves use 32x32x32 MFMAs: a lane (r = l % 32, h = l /
+// 32) holds piece 2 j + h of row r at sub-step j. Weights are operand A: a lane ends with x row l % 32 and weight
+// rows 8 (i / 4) + 4 h + i % 4.
+
+typedef int i8_x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+
+// buf_rsrc's four words
+__device__ __forceinline__ i8_u32x4 buffer_words(const void* base, uint32_t bytes) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(base);
+  return i8_u32x4{(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, bytes, 0x00020000u};
+}
+// 64 lanes x 16 bytes from the buffer at voff + soff into LDS from `at` on, in lane order. In asm: the builtin's LDS
+// write would make the compiler wait for every load in flight before it reads any LDS. No register waits for it.
+__device__ __forceinline__ void dma_1k(i8_u32x4 rsrc, uint32_t at, uint32_t voff, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :: "s"(at), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // until at most N of this wave's loads are in flight
+  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+
+struct I8Tile {
+  const int8_t *xq, *wq;
+  const float *xs, *ws;
+  void* y;       // bf16 or fp32 [m, n]; with splits int32 [splits, m, n] part sums
+  int m, n, k;
+  int mblk, nblk, splits, sps;  // tiles along m and n; parts of K and their steps of 128
+};
+
+template <int BM, int BN, int WM, int WN, int ST, int OUT>  // OUT: 0 bf16, 1 fp32, 2 int32 part sums
+__global__ __launch_bounds__(64 * WM * WN, BM * BN >= 65536 ? 2 : 1) void k_i8_tile(I8Tile a) {
+  constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+  constexpr int UNITS = (BM + BN) / 8, PER = UNITS / NW, STAGE = (BM + BN) * 128;
+  static_assert(UNITS % NW == 0 && BN % 8 == 0 && TM % 32 == 0 && TN % 32 == 0, "whole units");
+  constexpr int SLAB = 32 * (TN + 4) * 4;  // a wave's 32 rows of x by TN sums, in the stages' place at the end
+  constexpr int SMEM = ST * STAGE > NW * SLAB ? ST * STAGE : NW * SLAB;
+  __shared__ __align__(1024) unsigned char smem[SMEM];
+  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
+  // an XCD's workgroups (blockIdx % 8) take neighbouring tiles: up to 8 along m, then along n
+  const int tiles = a.mblk * a.nblk * a.splits, share = (tiles + 7) >> 3;
+  const int t = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= share || t >= tiles) return;
+  const int split = t / (a.mblk * a.nblk), tt = t - split * (a.mblk * a.nblk);
+  const int grp = tt / (8 * a.nblk), gm = min(8, a.mblk - grp * 8), in = tt - grp * 8 * a.nblk;
+  const int m0 = (grp * 8 + in % gm) * BM, n0 = (in / gm) * BN;
+  const int steps = (a.k + 127) >> 7, s0 = split * a.sps, s1 = min(steps, s0 + a.sps);
+  const int rows_n = min(BN, a.n - n0), rows_m = min(BM, a.m - m0);
+  const i8_u32x4 wv = buffer_words(a.wq + (int64_t)n0 * a.k, (uint32_t)rows_n * (uint32_t)a.k);
+  const i8_u32x4 xv = buffer_words(a.xq + (int64_t)m0 * a.k, (uint32_t)rows_m * (uint32_t)a.k);
+  // this lane's piece of the wave's units; the buffers' range check makes rows past the end zeros
+  const int piece = (lane & 7) ^ (lane >> 3);
+  uint32_t off[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int row = (wave * PER + i) * 8 + (lane >> 3);
+    off[i] = (uint32_t)(row < BN ? row : row - BN) * (uint32_t)a.k + (uint32_t)piece * 16u;
+  }
+  const uint32_t base = (uint32_t)(uintptr_t)(lds_byte*)smem;
+  const int tail = a.k & 127;  // bytes of the last step, if it is not whole
+  auto load = [&](int s, int stage) {
+    const uint32_t k0 = (uint32_t)s * 128u;
+    // pieces past the end of a row are zeros too
+    const bool past = s == steps - 1 && tail != 0 && piece * 16 >= tail;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = wave * PER + i;
+      dma_1k(u * 8 < BN ? wv : xv, base + (uint32_t)(stage * STAGE + u * 1024), past ? 0x80000000u : off[i], k0);
+    }
+  };
+  i8_x16 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+#pragma unroll
+  for (int p = 0; p < ST - 1; ++p)
+    if (s0 + p < s1) load(s0 + p, p);
+  int stage = 0;
+  for (int s = s0; s < s1; ++s) {
+    // this step's loads have landed (fewer are in flight in the last steps: all of them, then)
+    if (ST > 2 && s + ST - 2 < s1) wait_loads<(ST - 2) * PER>();
+    else wait_loads<0>();
+    __builtin_amdgcn_s_barrier();
+    if (s + ST - 1 < s1) load(s + ST - 1, stage == 0 ? ST - 1 : stage - 1);
+    const unsigned char* wt = smem + stage * STAGE + (wn * TN + r) * 128;
+    const unsigned char* xt = smem + stage * STAGE + (BN + wm * TM + r) * 128;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      i8_x4 w[FN], x[FM];
+      const int at = ((2 * j + h) ^ (r & 7)) * 16;
+#pragma unroll
+      for (int f = 0; f < FN; ++f) w[f] = *reinterpret_cast<const i8_x4*>(wt + f * 32 * 128 + at);
+#pragma unroll
+      for (int f = 0; f < FM; ++f) x[f] = *reinterpret_cast<const i8_x4*>(xt + f * 32 * 128 + at);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int f = 0; f < FN; ++f) acc[i][f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[f], x[i], acc[i][f], 0, 0, 0);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is read: others may load into it
+    stage = stage == ST - 1 ? 0 : stage + 1;
+  }
+  // out through LDS, 32 rows of x at a time, so that a wave stores whole lines
+  __syncthreads();
+  int* slab = reinterpret_cast<int*>(smem + wave * SLAB);
+  constexpr int V = OUT == 0 ? 8 : 4, LR = TN / V, RI = 64 / LR;  // values of a lane's store; lanes of a row, rows at once
+  const int lc = (lane % LR) * V, nn = n0 + wn * TN + lc;
+  float sw[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) sw[e] = OUT < 2 && nn + e < a.n ? a.ws[nn + e] : 0.0f;
+  const bool wide = nn + V <= a.n && (a.n % V) == 0;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+#pragma unroll
+    for (int f = 0; f < FN; ++f)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<i8_x4*>(slab + r * (TN + 4) + f * 32 + 8 * q + 4 * h) =
+            i8_x4{acc[i][f][4 * q], acc[i][f][4 * q + 1], acc[i][f][4 * q + 2], acc[i][f][4 * q + 3]};
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int p = 0; p < 32 / RI; ++p) {
+      const int row = p * RI + lane / LR, mm = m0 + wm * TM + i * 32 + row;
+      int v[V];
+#pragma unroll
+      for (int e = 0; e < V; e += 4)
+        *reinterpret_cast<i8_x4*>(v + e) = *reinterpret_cast<const i8_x4*>(slab + row * (TN + 4) + lc + e);
+      if (mm >= a.m) continue;
+      const int64_t at = ((int64_t)split * a.m + mm) * a.n + nn;
+      if (OUT == 2) {
+        int* y = static_cast<int*>(a.y) + at;
+        if (wide) *reinterpret_cast<i8_x4*>(y) = i8_x4{v[0], v[1], v[2], v[3]};
+        else
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (nn + e < a.n) y[e] = v[e];
+      } else {
+        const float sx = a.xs[mm];
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = (float)v[e] * (sx * sw[e]);
+        if (OUT == 1) {
+          float* y = static_cast<float*>(a.y) + at;
+          if (wide) *reinterpret_cast<float4*>(y) = make_float4(o[0], o[1], o[2], o[3]);
+          else
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+              if (nn + e < a.n) y[e] = o[e];
+        } else {
+          uint16_t* y = static_cast<uint16_t*>(a.y) + at;
+          if (wide)
+            *reinterpret_cast<uint4*>(y) = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]),
+                                                      pack_bf16x2(o[4 % V], o[5 % V]), pack_bf16x2(o[6 % V], o[7 % V]));
+          else
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+              if (nn + e < a.n) y[e] = (uint16_t)f2bf(o[e]);
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// y = the sum of the part sums, scaled: four values a thread
+template <bool F32>
+__global__ __launch_bounds__(256) void k_i8_join(const int* __restrict__ part, int splits, const float* __restrict__ xs,
+                                                 const float* __restrict__ ws, void* __restrict__ y, int m, int n) {
+  const int64_t mn = (int64_t)m * n, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= mn) return;
+  if ((n & 3) == 0) {
+    i8_x4 v = *reinterpret_cast<const i8_x4*>(part + at);
+    for (int p = 1; p < splits; ++p) v += *reinterpret_cast<const i8_x4*>(part + p * mn + at);
+    const int64_t row = at / n;
+    const int c = (int)(at - row * n);
+    const float sx = xs[row];
+    const float4 w = *reinterpret_cast<const float4*>(ws + c);
+    const float o[4] = {(float)v[0] * (sx * w.x), (float)v[1] * (sx * w.y), (float)v[2] * (sx * w.z), (float)v[3] * (sx * w.w)};
+    if (F32) *reinterpret_cast<float4*>(static_cast<float*>(y) + at) = make_float4(o[0], o[1], o[2], o[3]);
+    else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(y) + at) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+  } else {
+    for (int64_t i = at; i < at + 4 && i < mn; ++i) {
+      int v = 0;
+      for (int p = 0; p < splits; ++p) v += part[p * mn + i];
+      const int64_t row = i / n;
+      i8_store<F32>(y, i, v, xs[row] * ws[i - row * n]);
+    }
+  }
+}
+
+// How a product is cut
+struct I8Plan {
+  int kind;        // 0: k_i8_rows; else the tile: 1: 256 x 256, 2: 128 x 128, 3: 64 x 64
+  int mblk, nblk, splits, sps;
+};
+I8Plan i8_plan(int m, int n, int k) {
+  I8Plan p{0, 0, 0, 1, 0};
+  const int steps = (k + 127) / 128;
+  auto tiles = [&](int b) { return (int64_t)((m + b - 1) / b) * ((n + b - 1) / b); };
+  if (m <= 32) return p;
+  p.kind = tiles(256) >= 192 ? 1 : tiles(128) >= 160 ? 2 : 3;
+  const int b = p.kind == 1 ? 256 : p.kind == 2 ? 128 : 64;
+  p.mblk = (m + b - 1) / b;
+  p.nblk = (n + b - 1) / b;
+  if (p.kind == 3) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 8, 384 / tiles(64)));
+  p.sps = (steps + p.splits - 1) / p.splits;
+  p.splits = (steps + p.sps - 1) / p.sps;
+  return p;
+}
+
+template <int BM, int BN, int WM, int WN, int ST>
+void i8_tiles(const I8Tile& a, bool f32, hipStream_t s) {
+  const unsigned grid = 8u * (unsigned)((a.mblk * a.nblk * a.splits + 7) / 8);
+  const dim3 nt(64 * WM * WN);
+  if (a.splits > 1) hipLaunchKernelGGL((k_i8_tile<BM, BN, WM, WN, ST, 2>), dim3(grid), nt, 0, s, a);
+  else if (f32) hipLaunchKernelGGL((k_i8_tile<BM, BN, WM, WN, ST, 1>), dim3(grid), nt, 0, s, a);
+  else hipLaunchKernelGGL((k_i8_tile<BM, BN, WM, WN, ST, 0>), dim3(grid), nt, 0, s, a);
+}
+
 }  // namespace
 
 int i8_quantize(const uint16_t* x, int8_t* q, float* scale, int32_t rows, int32_t k, hipStream_t s) {
@@ -155,17 +386,28 @@ int i8_quantize(const uint16_t* x, int8_t* q, float* scale, int32_t rows, int32_
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
 }
 
-int64_t i8_gemm_bytes(int32_t, int32_t, int32_t) { return 0; }
+int64_t i8_gemm_bytes(int32_t m, int32_t n, int32_t k) {
+  const I8Plan p = i8_plan(m, n, k);
+  return p.splits > 1 ? i8_pad((int64_t)p.splits * m * n * 4) : 0;
+}
 
-int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, void* y, bool y_fp32, void*,
+int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, void* y, bool y_fp32, void* work,
             int32_t m, int32_t n, int32_t k, hipStream_t s) {
-  constexpr int Y = 32768 * 32;  // rows per launch (the grid's second dimension)
-  for (int64_t m0 = 0; m0 < m; m0 += Y) {
-    const int mm = (int)std::min<int64_t>(Y, m - m0);
-    void* yy = static_cast<char*>(y) + m0 * n * (y_fp32 ? 4 : 2);
-    const dim3 grid((n + 15) / 16, (mm + 31) / 32);
-    if (y_fp32) hipLaunchKernelGGL((k_i8_rows<2, 4, true>), grid, dim3(256), 0, s, xq + m0 * k, xs + m0, wq, ws, yy, mm, n, k);
-    else hipLaunchKernelGGL((k_i8_rows<2, 4, false>), grid, dim3(256), 0, s, xq + m0 * k, xs + m0, wq, ws, yy, mm, n, k);
+  const I8Plan p = i8_plan(m, n, k);
+  if (p.kind == 0) {
+    const dim3 grid((n + 15) / 16, (m + 31) / 32);
+    if (y_fp32) hipLaunchKernelGGL((k_i8_rows<2, 4, true>), grid, dim3(256), 0, s, xq, xs, wq, ws, y, m, n, k);
+    else hipLaunchKernelGGL((k_i8_rows<2, 4, false>), grid, dim3(256), 0, s, xq, xs, wq, ws, y, m, n, k);
+  } else {
+    const I8Tile a{xq, wq, xs, ws, p.splits > 1 ? work : y, m, n, k, p.mblk, p.nblk, p.splits, p.sps};
+    if (p.kind == 1) i8_tiles<256, 256, 2, 4, 2>(a, y_fp32, s);
+    else if (p.kind == 2) i8_tiles<128, 128, 2, 2, 2>(a, y_fp32, s);
+    else i8_tiles<64, 64, 2, 2, 4>(a, y_fp32, s);
+    if (p.splits > 1) {
+      const dim3 grid((unsigned)(((int64_t)m * n + 1023) / 1024));
+      if (y_fp32) hipLaunchKernelGGL(k_i8_join<true>, grid, dim3(256), 0, s, static_cast<const int*>(work), p.splits, xs, ws, y, m, n);
+      else hipLaunchKernelGGL(k_i8_join<false>, grid, dim3(256), 0, s, static_cast<const int*>(work), p.splits, xs, ws, y, m, n);
+    }
   }
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
 }
