@@ -7,23 +7,25 @@
 // 0). Everything in fp32. A row without a finite maximum (all -inf, or with a +inf) or with a NaN has no
 // distribution: its log probabilities and entropy are NaN, its order is what it is.
 //
-// One pass over the logits: a workgroup holds a chunk of a row in registers, finds its maximum, then its
-// sums, its rank count and its first `top` indices. Rows of several chunks end in a merge launch of one
-// workgroup per row.
+// One pass over the logits: a workgroup streams a row, or a chunk of one, through registers; every thread keeps the
+// running maximum and sums of its values. Rows of several chunks end in a merge launch of one workgroup per row.
 #include "fl_int8.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
 typedef unsigned long long u64;
 
-constexpr int LP_NT = 512, LP_NW = LP_NT / FL_WAVE;
+constexpr float LP_LOG2E = 1.4426950408889634f;
+constexpr int LP_NT = 256, LP_NW = LP_NT / FL_WAVE;
+constexpr int LP_E = 16;                // values of a thread in a step
+constexpr int LP_STEP = LP_NT * LP_E;   // of a workgroup
 constexpr int LP_TOP = 32;     // alternatives at most
 constexpr int LP_CHUNKS = 32;  // of a row at most
 constexpr int LP_CAP = 1024;   // candidates kept in LDS
 constexpr int LP_MAXV = 1 << 20;
 static_assert(LP_CHUNKS * LP_TOP <= LP_CAP, "a merge's candidates always fit");
-static_assert(LP_MAXV <= LP_CHUNKS * LP_NT * 64, "every vocabulary fits its chunks");
 
 // Keys that order as the values do, as unsigned numbers (NaN, made positive, above +inf), with the index below
 // them: all keys of a row differ, and none is 0.
@@ -36,6 +38,10 @@ __device__ __forceinline__ float lp_value(u64 key) {
   const uint32_t o = (uint32_t)(key >> 32);
   return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
+
+// 16 bytes of a row, which starts where its type may
+typedef uint32_t lp_raw_f32 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t lp_raw_bf16 __attribute__((ext_vector_type(4), aligned(2)));
 
 struct LpArgs {
   const void* logits;
@@ -53,6 +59,7 @@ struct LpArgs {
 struct LpShared {
   float red[5][LP_NW];
   int count;
+  int place[LP_NW][FL_WAVE];
   u64 cand[LP_CAP], first[LP_TOP];
 };
 
@@ -74,19 +81,47 @@ __device__ __forceinline__ LpToken lp_token(const LpArgs& a, int64_t row) {
   return k;
 }
 
-// The first a.top of the sh.count (<= LP_CAP) keys in sh.cand, in order, into sh.first: a key's place is the
-// number of larger ones.
+// The first `top` of the sh.count (<= LP_CAP) keys in sh.cand, in order, into sh.first: a key's place is the number of
+// larger ones. Lanes take candidates, each wave counts over its share of them.
 __device__ __forceinline__ void lp_sort(LpShared& sh, int top) {
-  const int tid = threadIdx.x, c = sh.count;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = sh.count;
+  const int share = (c + LP_NW - 1) / LP_NW, c0 = min(c, wave * share), c1 = min(c, c0 + share);
   if (tid < top) sh.first[tid] = 0;
-  __syncthreads();
-  for (int i = tid; i < c; i += LP_NT) {
-    const u64 key = sh.cand[i];
-    int at = 0;
-    for (int j = 0; j < c; ++j) at += sh.cand[j] > key;
-    if (at < top) sh.first[at] = key;
+  for (int b = 0; b < c; b += FL_WAVE) {
+    const u64 key = b + lane < c ? sh.cand[b + lane] : 0;
+    int larger = 0;
+#pragma unroll 4
+    for (int j = c0; j < c1; ++j) larger += sh.cand[j] > key;
+    sh.place[wave][lane] = larger;
+    __syncthreads();
+    if (wave == 0 && key != 0) {
+      int at = 0;
+#pragma unroll
+      for (int w = 0; w < LP_NW; ++w) at += sh.place[w][lane];
+      if (at < top) sh.first[at] = key;
+    }
+    __syncthreads();
   }
   __syncthreads();
+}
+
+// A value that at least LP_NW q of the workgroup's values reach, if all lanes hold one: the smallest over the waves of
+// the q-th largest in the wave, stored for others to read at any time (rising values only make it rise)
+__device__ __forceinline__ void lp_publish(float* red, float mine, int q) {
+  const int lane = threadIdx.x & 63;
+  float w = -INFINITY;
+  for (int r = 0; r < q; ++r) {
+    w = wave_max(mine);
+    if (lane == __builtin_ctzll(__ballot(mine == w) | (1ull << 63))) mine = -INFINITY;
+  }
+  if (lane == 0) __hip_atomic_store(red + (threadIdx.x >> 6), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+__device__ __forceinline__ float lp_least(float* red, int waves) {
+  float t = waves > 0 ? INFINITY : -INFINITY;
+#pragma unroll
+  for (int k = 0; k < LP_NW; ++k)
+    if (k < waves) t = fminf(t, __hip_atomic_load(red + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+  return t;
 }
 
 // what the whole row says, from its maximum, sums and rank count, and sh.first
@@ -111,105 +146,137 @@ __device__ __forceinline__ void lp_write(const LpArgs& a, int64_t row, const LpT
   }
 }
 
-// One chunk of a row per workgroup, E values per thread in registers. VEC: rows are 16-byte aligned.
-template <bool BF16, bool VEC, int E>
-__global__ __launch_bounds__(LP_NT, E <= 64 ? 4 : 2) void k_logprobs(LpArgs a) {
-  constexpr int V = !VEC ? 1 : BF16 ? 8 : 4;  // consecutive values of a load
+// v_max3_f32 without the operation per operand that makes a loaded value canonical
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// how many lanes of the wave
+__device__ __forceinline__ int lp_count(bool is) { return __builtin_popcountll(__ballot(is)); }
+
+// (maximum, s, u) of a wave's lanes joined, in every lane
+__device__ __forceinline__ void lp_join(float& m, float& s, float& u) {
+  const float mm = wave_max(m), mu = mm == -INFINITY ? 0.0f : mm;
+  const float d = fmaxf(m - mu, -1000.0f), e = __builtin_amdgcn_exp2f(d * LP_LOG2E);  // nothing seen: s = u = 0
+  u = wave_sum((u + s * d) * e);
+  s = wave_sum(s * e);
+  m = mm;
+}
+
+// One chunk of a row per workgroup, in steps of LP_E values per thread; the next step's loads are in flight meanwhile.
+template <bool BF16>
+__global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
+  constexpr int V = BF16 ? 8 : 4;  // consecutive values of a load (16 bytes, aligned to the type only)
+  using raw4 = std::conditional_t<BF16, lp_raw_bf16, lp_raw_f32>;
   __shared__ LpShared sh;
-  const int tid = threadIdx.x, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / a.chunks;
   const int chunk = (int)(blockIdx.x % a.chunks);
-  const int j0 = chunk * a.per, j1 = min(a.vocab, j0 + a.per), len = j1 - j0;
-  const LpToken tok = lp_token<BF16>(a, row);
+  const int j0 = chunk * a.per, j1 = min(a.vocab, j0 + a.per);
   const float* lf = reinterpret_cast<const float*>(a.logits) + row * a.stride;
   const uint16_t* lh = reinterpret_cast<const uint16_t*>(a.logits) + row * a.stride;
-  auto index = [&](int e) { return j0 + ((e / V) * LP_NT + tid) * V + e % V; };
-  float x[E];
+  auto load = [&](int jb, float (&x)[LP_E]) {
+    if (jb + LP_STEP <= j1) {
 #pragma unroll
-  for (int i = 0; i < E / V; ++i) {
-    const int j = index(i * V);
-    if (V > 1 && j + V <= j1) {
-      if constexpr (BF16) {
-        const uint4 w = *reinterpret_cast<const uint4*>(lh + j);
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+      for (int i = 0; i < LP_E / V; ++i) {
+        const int j = jb + (i * LP_NT + tid) * V;
+        const raw4 w = *reinterpret_cast<const raw4*>(BF16 ? (const void*)(lh + j) : (const void*)(lf + j));
 #pragma unroll
-        for (int k = 0; k < V; ++k) x[i * V + k] = k & 1 ? bfhi(ww[(k / 2) & 3]) : bflo(ww[(k / 2) & 3]);
-      } else {
-        const float4 w = *reinterpret_cast<const float4*>(lf + j);
-        const float ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int k = 0; k < V; ++k) x[i * V + k] = ww[k & 3];
+        for (int k = 0; k < V; ++k)
+          x[i * V + k] = !BF16 ? __uint_as_float(w[k & 3]) : k & 1 ? bfhi(w[(k / 2) & 3]) : bflo(w[(k / 2) & 3]);
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < V; ++k) x[i * V + k] = j + k < j1 ? (BF16 ? bf2f(lh[j + k]) : lf[j + k]) : -INFINITY;
+      for (int e = 0; e < LP_E; ++e) {
+        const int j = jb + ((e / V) * LP_NT + tid) * V + e % V;
+        x[e] = j < j1 ? (BF16 ? bf2f(lh[j]) : lf[j]) : -INFINITY;
+      }
     }
-  }
-  float mine = -INFINITY;  // NaN is passed over here; it comes back through s
-#pragma unroll
-  for (int e = 0; e < E; ++e) mine = fmaxf(mine, x[e]);
-  // A value that at least `top` of the chunk reach: of each of the waves whose lanes all hold values, the q-th
-  // largest of its lanes' maxima; the smallest of these. Few others reach it.
-  const int full = min(LP_NW, len / (FL_WAVE * V)), q = full > 0 ? (a.top + full - 1) / full : 0;
-  float left = mine, wm = -INFINITY, wq = -INFINITY;
-  for (int i = 0; i < max(q, 1); ++i) {
-    wq = wave_max(left);
-    if (i == 0) wm = wq;
-    const int first = __builtin_ctzll(__ballot(left == wq) | (1ull << 63));
-    if ((tid & 63) == first) left = -INFINITY;
-  }
-  if ((tid & 63) == 0) sh.red[0][wave] = wm, sh.red[1][wave] = wq;
+  };
+  float x[LP_E];
+  load(j0, x);
+  const LpToken tok = lp_token<BF16>(a, row);
+  // Candidates for the first `top` places: of each of the waves whose lanes all hold values, the q-th largest of
+  // its lanes' maxima so far; at least `top` values of the chunk reach the smallest of these, T, and few others do. T
+  // only rises, so what is collected with an earlier T is too much at worst.
+  const int full = min(LP_NW, (j1 - j0) / (FL_WAVE * V)), q = full > 0 ? (a.top + full - 1) / full : 0;
   if (tid == 0) sh.count = 0;
-  __syncthreads();
-  float m = -INFINITY, T = full > 0 ? INFINITY : -INFINITY;
+  if (lane == 0) sh.red[0][wave] = -INFINITY;
+  float m = -INFINITY, s = 0.0f, u = 0.0f, T = -INFINITY;
+  int before = 0, i = 0;  // `before` of the wave
+  for (int jb = j0; jb < j1; jb += LP_STEP, ++i) {
+    float y[LP_E];
+    if (jb + LP_STEP < j1) load(jb + LP_STEP, y);
+    float top = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), x[5], x[6]);  // NaN is passed over; it comes back through s
+    top = max3(max3(max3(max3(top, x[7], x[8]), x[9], x[10]), x[11], x[12]), x[13], x[14]);
+    top = max3(top, x[15], x[15]);
+    const float old = m;
+    m = fmaxf(m, top);
+    // sums over the maximum so far; values past the chunk are -inf and add nothing
+    const float mu = m == -INFINITY ? 0.0f : m;
+    const float d0 = fmaxf(old - mu, -1000.0f), e0 = __builtin_amdgcn_exp2f(d0 * LP_LOG2E);
+    u = (u + s * d0) * e0;
+    s *= e0;
 #pragma unroll
-  for (int w = 0; w < LP_NW; ++w) {
-    m = fmaxf(m, sh.red[0][w]);
-    if (w < full) T = fminf(T, sh.red[1][w]);
-  }
-  // sums and rank count; values past the chunk are -inf and add nothing
-  const float mu = m == -INFINITY ? 0.0f : m;
-  float s = 0.0f, u = 0.0f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    float d = x[e] - mu;
-    d = d < -1000.0f ? -1000.0f : d;  // e = 0, and 0 * d = 0 for masked values; NaN stays
-    const float p = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
-    s += p;
-    u += p * d;
-  }
-  const bool odd = s != s;  // this thread holds a NaN, or the +inf that is the maximum
-  int before = 0;
-  if (tok.in) {
-    const int tm = min(tok.t, j1);
-    if (tok.l == tok.l) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) before += !(x[e] <= tok.l) || (x[e] == tok.l && index(e) < tm);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) before += x[e] != x[e] && index(e) < tm;
+    for (int e = 0; e < LP_E; ++e) {
+      const float d = x[e] - mu, p = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+      s += p;
+      u = __builtin_fmaf(p, fmaxf(d, -1000.0f), u);  // 0 times -1000 for masked values
     }
-  }
-  if (a.top > 0 && (odd || mine >= T)) {
+    const int jt = jb + tid * V;  // e's index: jt + (e / V) * LP_NT * V + e % V
+    if (tok.in) {
+      if (tok.l != tok.l || jb + LP_STEP > j1 || (tok.t >= jb && tok.t < jb + LP_STEP)) {
+        const int tm = min(tok.t, j1) - jt;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int j = index(e);
-      // over -inf alone: its first values by index besides whatever is larger
-      const bool is = T == -INFINITY ? !(x[e] <= T) || j < j0 + a.top : !(x[e] < T);
-      if (is && j < j1) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < LP_CAP) sh.cand[at] = lp_key(x[e], j);
+        for (int e = 0; e < LP_E; ++e) {
+          const bool lower = (e / V) * LP_NT * V + e % V < tm;
+          before += lp_count(tok.l == tok.l ? !(x[e] <= tok.l) || (x[e] == tok.l && lower) : x[e] != x[e] && lower);
+        }
+      } else if (tok.t < jb) {  // all of the step is behind the token: what is larger comes before it
+#pragma unroll
+        for (int e = 0; e < LP_E; ++e) before += lp_count(!(x[e] <= tok.l));
+      } else {  // a whole step before it: equal values, too
+#pragma unroll
+        for (int e = 0; e < LP_E; ++e) before += lp_count(!(x[e] < tok.l));
       }
     }
-  }
-  s = wave_sum(s);
-  u = wave_sum(u);
-  const float bf = wave_sum((float)before);  // at most 64 x 96: exact
-  if ((tid & 63) == 0) sh.red[2][wave] = s, sh.red[3][wave] = u, sh.red[4][wave] = bf;
-  __syncthreads();
-  s = u = 0.0f, before = 0;
+    if (a.top > 0) {
+      if ((i & (i + 1)) == 0) {  // steps 0, 1, 3, 7, ...
+        lp_publish(sh.red[0], m, q);
+        if (i == 0) __syncthreads();
+        T = lp_least(sh.red[0], full);
+      }
+      auto take = [&](float v, int j) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < LP_CAP) sh.cand[at] = lp_key(v, j);
+      };
+      if (T == -INFINITY) {  // all that is larger, and the chunk's first values by index
 #pragma unroll
-  for (int w = 0; w < LP_NW; ++w) s += sh.red[2][w], u += sh.red[3][w], before += (int)sh.red[4][w];
+        for (int e = 0; e < LP_E; ++e) {
+          const int j = jt + (e / V) * LP_NT * V + e % V;
+          if (j < j1 && (!(x[e] <= T) || j < j0 + a.top)) take(x[e], j);
+        }
+      } else if (s != s || top >= T) {
+#pragma unroll
+        for (int e = 0; e < LP_E; ++e)
+          if (!(x[e] < T)) take(x[e], jt + (e / V) * LP_NT * V + e % V);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < LP_E; ++e) x[e] = y[e];
+  }
+  lp_join(m, s, u);
+  if (lane == 0) sh.red[1][wave] = m, sh.red[2][wave] = s, sh.red[3][wave] = u, sh.red[4][wave] = (float)before;
+  __syncthreads();
+  const bool one = lane < LP_NW;
+  m = one ? sh.red[1][lane % LP_NW] : -INFINITY;
+  s = one ? sh.red[2][lane % LP_NW] : 0.0f;
+  u = one ? sh.red[3][lane % LP_NW] : 0.0f;
+  lp_join(m, s, u);
+  before = 0;
+#pragma unroll
+  for (int w = 0; w < LP_NW; ++w) before += (int)sh.red[4][w];
   if (a.top > 0) {
     if (sh.count <= LP_CAP) {
       lp_sort(sh, a.top);
@@ -223,7 +290,7 @@ __global__ __launch_bounds__(LP_NT, E <= 64 ? 4 : 2) void k_logprobs(LpArgs a) {
         }
         best = wave_max_u64(best);
         __syncthreads();
-        if ((tid & 63) == 0) sh.cand[wave] = best;
+        if (lane == 0) sh.cand[wave] = best;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < LP_NW; ++w) best = u64max(best, sh.cand[w]);
@@ -242,60 +309,55 @@ __global__ __launch_bounds__(LP_NT, E <= 64 ? 4 : 2) void k_logprobs(LpArgs a) {
   if (tid < a.top) a.cand[at * a.top + tid] = sh.first[tid];
 }
 
-// The chunks of a row in order: one workgroup per row
+// The chunks of a row joined: one workgroup per row, lane = chunk
 template <bool BF16>
 __global__ __launch_bounds__(LP_NT) void k_logprobs_merge(LpArgs a) {
   __shared__ LpShared sh;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int64_t row = blockIdx.x;
-  const LpToken tok = lp_token<BF16>(a, row);
-  const float4* part = a.part + row * a.chunks;
-  float m = -INFINITY, s = 0.0f, u = 0.0f;
-  int before = 0;
-  for (int c = 0; c < a.chunks; ++c) m = fmaxf(m, part[c].x);
-  for (int c = 0; c < a.chunks; ++c) {
-    const float4 p = part[c];
-    before += __float_as_int(p.w);
-    if (p.y == 0.0f) continue;  // nothing but -inf
-    // a NaN (or +inf) chunk has s = NaN, whatever its maximum
-    const float d = fmaxf(p.x - m, -1000.0f), e = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
-    s += p.y * e;
-    u += (p.z + p.y * d) * e;
-  }
+  const u64* cand = a.cand + row * a.chunks * a.top;
+  const bool one = lane < a.chunks;
+  const float4 p = one ? a.part[row * a.chunks + lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+  u64 mine[LP_CAP / LP_NT], T = 0;
   if (a.top > 0) {
-    const u64* cand = a.cand + row * a.chunks * a.top;
+#pragma unroll
+    for (int i = 0; i < LP_CAP / LP_NT; ++i) mine[i] = i * LP_NT + tid < a.chunks * a.top ? cand[i * LP_NT + tid] : 0;
+    if (one) T = cand[(lane + 1) * a.top - 1];
+  }
+  const LpToken tok = lp_token<BF16>(a, row);
+  float m = p.x, s = p.y, u = p.z;
+  lp_join(m, s, u);
+  const int before = (int)wave_sum((float)__float_as_int(p.w));
+  if (a.top > 0) {
     if (tid == 0) sh.count = 0;
-    // at least `top` keys reach the largest of the chunks' last ones
-    u64 T = 0;
-    for (int c = 0; c < a.chunks; ++c) T = u64max(T, cand[(c + 1) * a.top - 1]);
+    // at least `top` keys reach the largest of the chunks' last ones; and, as in a chunk, a value from the threads' largest
+    T = wave_max_u64(T);
+    u64 largest = 0;
+#pragma unroll
+    for (int i = 0; i < LP_CAP / LP_NT; ++i) largest = u64max(largest, mine[i]);
+    const int full = min(LP_NW, a.chunks * a.top / FL_WAVE), q = full > 0 ? (a.top + full - 1) / full : 0;
+    lp_publish(sh.red[0], largest != 0 ? lp_value(largest) : -INFINITY, q);
     __syncthreads();
-    for (int i = tid; i < a.chunks * a.top; i += LP_NT) {
-      const u64 k = cand[i];
-      if (k >= T && k != 0) sh.cand[atomicAdd(&sh.count, 1)] = k;
-    }
+    const float t = lp_least(sh.red[0], full);
+#pragma unroll
+    for (int i = 0; i < LP_CAP / LP_NT; ++i)
+      if (mine[i] != 0 && mine[i] >= T && !(lp_value(mine[i]) < t)) sh.cand[atomicAdd(&sh.count, 1)] = mine[i];
     __syncthreads();
     lp_sort(sh, a.top);
   }
   lp_write(a, row, tok, m, s, u, before, sh);
 }
 
-// Chunks of a row: one, or as many as give `want` workgroups in all, of 4096 values at least.
+// Chunks of a row: one, or as many as give 512 workgroups in all, of 2048 values at least.
 void lp_plan(LpArgs& a, int rows) {
-  const int most = std::min(LP_CHUNKS, std::max(1, a.vocab / 4096)), least = (a.vocab + LP_NT * 96 - 1) / (LP_NT * 96);
-  a.chunks = std::max(least, std::min(most, std::max(1, 512 / rows)));
+  a.chunks = std::max(1, std::min({LP_CHUNKS, a.vocab / 2048, 512 / rows}));
   a.per = ((a.vocab + a.chunks - 1) / a.chunks + 7) / 8 * 8;
   a.chunks = (a.vocab + a.per - 1) / a.per;
 }
 
-template <bool BF16, bool VEC>
+template <bool BF16>
 void lp_launch(const LpArgs& a, int rows, hipStream_t s) {
-  const dim3 grid((unsigned)rows * (unsigned)a.chunks);
-  const int e = (a.per + LP_NT - 1) / LP_NT;
-  if (e <= 8) hipLaunchKernelGGL((k_logprobs<BF16, VEC, 8>), grid, dim3(LP_NT), 0, s, a);
-  else if (e <= 16) hipLaunchKernelGGL((k_logprobs<BF16, VEC, 16>), grid, dim3(LP_NT), 0, s, a);
-  else if (e <= 32) hipLaunchKernelGGL((k_logprobs<BF16, VEC, 32>), grid, dim3(LP_NT), 0, s, a);
-  else if (e <= 64) hipLaunchKernelGGL((k_logprobs<BF16, VEC, 64>), grid, dim3(LP_NT), 0, s, a);
-  else hipLaunchKernelGGL((k_logprobs<BF16, VEC, 96>), grid, dim3(LP_NT), 0, s, a);
+  hipLaunchKernelGGL(k_logprobs<BF16>, dim3((unsigned)rows * (unsigned)a.chunks), dim3(LP_NT), 0, s, a);
   if (a.chunks > 1) hipLaunchKernelGGL(k_logprobs_merge<BF16>, dim3(rows), dim3(LP_NT), 0, s, a);
 }
 
@@ -304,7 +366,7 @@ int64_t lp_bytes(const LpArgs& a, int rows) {
   return a.chunks > 1 ? lp_part_bytes(a, rows) + i8_pad((int64_t)rows * a.chunks * a.top * 8) : 0;
 }
 
-constexpr int LP_MAXROWS = 1 << 17;  // rows x LP_CHUNKS workgroups of 512 threads in one grid
+constexpr int LP_MAXROWS = 1 << 17;  // rows x LP_CHUNKS workgroups of 256 threads in one grid
 
 bool lp_shape_ok(int rows, int vocab, int top) {
   return rows >= 1 && rows <= LP_MAXROWS && vocab >= 1 && vocab <= LP_MAXV && top >= 0 && top <= LP_TOP && top <= vocab;
@@ -318,12 +380,8 @@ int lp_run(LpArgs a, bool bf16, int rows, void* work, hipStream_t s) {
   lp_plan(a, rows);
   a.part = static_cast<float4*>(work);
   a.cand = reinterpret_cast<u64*>(static_cast<char*>(work) + lp_part_bytes(a, rows));
-  const int esize = bf16 ? 2 : 4;
-  const bool vec = i8_aligned(a.logits) && (a.stride * esize) % 16 == 0;
-  if (bf16 && vec) lp_launch<true, true>(a, rows, s);
-  else if (bf16) lp_launch<true, false>(a, rows, s);
-  else if (vec) lp_launch<false, true>(a, rows, s);
-  else lp_launch<false, false>(a, rows, s);
+  if (bf16) lp_launch<true>(a, rows, s);
+  else lp_launch<false>(a, rows, s);
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
 }
 

@@ -167,8 +167,7 @@ int fl_linear_int8(const uint16_t* x, const int8_t* wq, const float* ws, void* y
  * probabilities. fp32 throughout. A logit of -inf has probability 0. A row that is all -inf, or holds a +inf or a NaN,
  * has no distribution: its log probabilities and entropy are NaN, its rank and top_ids as defined. A token id outside the
  * vocabulary (a padded row): logprob NaN, rank -1. tokens may be NULL (then logprob and rank may be too and are not
- * written), top_ids and top_logprobs where top = 0. All pointers are device pointers; logits aligned to their type (rows
- * that are 16-byte aligned are read faster). work: 16-byte aligned, of fl_logprobs_workspace's bytes (0: may be NULL),
+ * written), top_ids and top_logprobs where top = 0. All pointers are device pointers; logits aligned to their type. work: 16-byte aligned, of fl_logprobs_workspace's bytes (0: may be NULL),
  * free for reuse once the call's work on the stream is done.
  * No counterpart in the reference, whose sample (engine/generate.py:36-55) returns tokens and probabilities. */
 int fl_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top, int64_t* bytes);
