@@ -19,3 +19,7 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
             int32_t m, int32_t n, int32_t k, hipStream_t s);
 // rows of x [rows, k] (bf16) in 8 bits; arguments already checked
 int i8_quantize(const uint16_t* x, int8_t* q, float* scale, int32_t rows, int32_t k, hipStream_t s);
+// the same from bf16 rows x, quantised on the way
+int64_t i8_linear_bytes(int32_t m, int32_t n, int32_t k);
+int i8_linear(const uint16_t* x, const int8_t* wq, const float* ws, void* y, bool y_fp32, void* work, int32_t m,
+              int32_t n, int32_t k, hipStream_t s);

@@ -31,12 +31,21 @@ __device__ __forceinline__ Q8Row q8_row(float amax) {
   return r;
 }
 __device__ __forceinline__ int q8_of(float x, const Q8Row& row) {
-  float q = __builtin_rintf(x * row.up * row.inv);
-  const float r = __builtin_fmaf(-q, row.s, x), two = r + r;
-  const bool odd = ((int)q & 1) != 0;
-  if (two > row.s || (two == row.s && odd)) q += 1.0f;
-  if (two < -row.s || (two == -row.s && odd)) q -= 1.0f;
-  return row.inv != 0.0f ? (int)fminf(fmaxf(q, -127.0f), 127.0f) : 0;
+  const float q = __builtin_rintf(x * row.up * row.inv), r = __builtin_fmaf(-q, row.s, x), two = fabsf(r + r);
+  const int i = (int)q;
+  return two > row.s || (two == row.s && (i & 1)) ? i + (r > 0.0f ? 1 : -1) : i;
+}
+// eight bf16 values
+__device__ __forceinline__ uint2 q8_pack(const uint4& p, const Q8Row& r) {
+  const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+  uint32_t o[2] = {0, 0};
+  if (!(r.inv != 0.0f)) return make_uint2(0, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = (uint32_t)q8_of(bflo(w[i]), r) & 0xFFu, b = (uint32_t)q8_of(bfhi(w[i]), r) & 0xFFu;
+    o[i >> 1] |= (a | b << 8) << (16 * (i & 1));
+  }
+  return make_uint2(o[0], o[1]);
 }
 
 constexpr int Q8_NT = 256, Q8_KEEP = 4;  // threads of a row; 8-value pieces that a thread keeps in registers
@@ -71,22 +80,12 @@ __global__ __launch_bounds__(Q8_NT) void k_quantize_i8(const uint16_t* __restric
   const Q8Row r = q8_row(bf2f(m));
   if (tid == 0) scale[row] = r.s;
   uint2* qr = reinterpret_cast<uint2*>(qo + row * k);
-  auto put = [&](int c, const uint4& p) {
-    const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-    uint32_t o[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t a = (uint32_t)q8_of(bflo(w[i]), r) & 0xFFu, b = (uint32_t)q8_of(bfhi(w[i]), r) & 0xFFu;
-      o[i >> 1] |= (a | b << 8) << (16 * (i & 1));
-    }
-    qr[c] = make_uint2(o[0], o[1]);
-  };
 #pragma unroll
   for (int i = 0; i < Q8_KEEP; ++i) {
     const int c = tid + i * Q8_NT;
-    if (c < nc) put(c, v[i]);
+    if (c < nc) qr[c] = q8_pack(v[i], r);
   }
-  for (int c = tid + Q8_KEEP * Q8_NT; c < nc; c += Q8_NT) put(c, xr[c]);
+  for (int c = tid + Q8_KEEP * Q8_NT; c < nc; c += Q8_NT) qr[c] = q8_pack(xr[c], r);
 }
 
 // ---- the product ----------------------------------------------------------------------------------
@@ -98,55 +97,191 @@ __device__ __forceinline__ void i8_store(void* y, int64_t at, int acc, float s) 
   else reinterpret_cast<uint16_t*>(y)[at] = (uint16_t)f2bf(v);
 }
 
-// Up to 16 MB rows of x against 16 weight rows per workgroup, whose KW waves each take a part of K. Lane
-// (r = l % 16, c = l / 16) of a wave holds 16 values of weight row r, and of x row r, at 64 step + 16 c: A and B
-// of v_mfma_i32_16x16x64_i8, which sums over k in any order as long as both operands use the same. D: x row
-// l % 16, weight rows 4 (l / 16) + 0..3.
-template <int MB, int KW, bool F32>
-__global__ __launch_bounds__(64 * KW) void k_i8_rows(const int8_t* __restrict__ xq, const float* __restrict__ xs,
-                                                     const int8_t* __restrict__ wq, const float* __restrict__ ws,
-                                                     void* __restrict__ y, int m, int n, int k) {
-  __shared__ i8_x4 part[KW > 1 ? KW - 1 : 1][MB][64];
+// Up to 16 MB rows of x against all weights, 16 weight rows (a block) at a time: the eight waves of a workgroup
+// each take a part of K. Lane (r = l % 16, c = l / 16) of a wave holds 16 values of weight row r, and of x row r, at
+// 64 step + 16 c: A and B of v_mfma_i32_16x16x64_i8, which sums over k in any order as long as both operands use
+// the same. D: x row l % 16, weight rows 4 (l / 16) + 0..3. Weights go from memory to registers, U steps at once and
+// the waves' sums meet in LDS.
+// XKB = 0: one block per workgroup, x from memory beside the weights. XKB > 0: the workgroups that fit the chip at
+// once take blocks in turn, two sets of registers in turn across them, x in XKB KB of LDS: every block reading x again would cost as much as the weights at 16
+// rows. QUANT: x is bf16 and the workgroup quantises the rows for itself into LDS, behind its first weight loads.
+constexpr int FEW_KW = 8;
+constexpr int QF_MOST = 16384, QF_KEEP = 8;  // values that a workgroup quantises; 8-value pieces of a lane
+__host__ __device__ inline int qf_slots(int m) {
+  int slots = 1;
+  while (slots < m && slots < FEW_KW) slots *= 2;
+  return slots;
+}
+// whether the waves hold the rows in QF_KEEP pieces a lane
+inline bool qf_fits(int m, int k) {
+  const int slots = qf_slots(m), w = 64 * (FEW_KW / slots);
+  return m <= 16 && m * (int64_t)k <= QF_MOST && (m + slots - 1) / slots * ((k / 8 + w - 1) / w) <= QF_KEEP;
+}
+__host__ __device__ inline int few_pitch(int k) { return ((k + 63) >> 6) * 64 + 16; }  // of x rows in LDS: r and r + 8 on the same banks
+struct I8Few {
+  const void* x;     // int8 [m, k], or (QUANT) bf16
+  const float* xs;   // not with QUANT
+  const int8_t* wq;
+  const float* ws;
+  void* y;
+  int m, n, k;
+};
+template <int MB, int XKB, bool QUANT, bool F32>
+__global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
+  constexpr int KW = FEW_KW, U = 5;
+  static_assert(!QUANT || (MB == 1 && XKB * 1024 >= QF_MOST + 16 * 64), "rows that are quantised here");
+  __shared__ __align__(16) int part[XKB ? 2 : 1][KW][MB][256];
+  __shared__ __align__(16) unsigned char xl[XKB ? XKB * 1024 : 16];
+  __shared__ float most[16][KW], sx[16];
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MB;
-  const int steps = (k + 63) >> 6, per = (steps + KW - 1) / KW;
+  const int m = a.m, k = a.k;
+  const int steps = (k + 63) >> 6, per = (steps + KW - 1) / KW, turns = (per + U - 1) / U;
   const int s0 = wave * per, s1 = min(steps, s0 + per);
-  // range-checked from the first row of the block: rows past the end read as zeros
-  const auto wr = buf_rsrc(wq + (int64_t)n0 * k, (uint32_t)min(16, n - n0) * (uint32_t)k);
-  const auto xr = buf_rsrc(xq + (int64_t)m0 * k, (uint32_t)min(16 * MB, m - m0) * (uint32_t)k);
+  const int blocks = (a.n + 15) >> 4;
+  const auto xr = buf_rsrc(a.x, (uint32_t)m * (uint32_t)k);
+  const int pitch = few_pitch(k);
+  // this thread's outputs: x row `row`, weight row tn of a block
+  const int tn = threadIdx.x & 15, row = threadIdx.x >> 4;
+  struct Set {
+    i8_x4 w[U], x[U][XKB ? 1 : MB];
+    float s;  // the scale of weight row tn
+  };
+  // the U steps of block b from turn t on; range-checked: rows past the end, steps past the wave's part: zeros
+  auto load = [&](int b, int t, Set& v) {
+    const bool live = b < blocks;  // wave-uniform
+    const int n0 = b * 16;
+    const auto wr = buf_rsrc(a.wq + (int64_t)(live ? n0 : 0) * k, live ? (uint32_t)min(16, a.n - n0) * (uint32_t)k : 0u);
+    if (t == turns - 1) v.s = live ? a.ws[min(n0 + tn, a.n - 1)] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int s = s0 + t * U + i, at = s * 64 + c * 16;
+      const bool in = s < s1 && at < k;
+      v.w[i] = __builtin_bit_cast(i8_x4, buf_ld128(wr, in ? (uint32_t)(r * k + at) : 0x80000000u));
+      if constexpr (XKB == 0) {
+#pragma unroll
+        for (int j = 0; j < MB; ++j)
+          v.x[i][j] = __builtin_bit_cast(i8_x4, buf_ld128(xr, in ? (uint32_t)((16 * j + r) * k + at) : 0x80000000u));
+      }
+    }
+  };
   i8_x4 acc[MB];
-#pragma unroll
-  for (int b = 0; b < MB; ++b) acc[b] = i8_x4{0, 0, 0, 0};
-#pragma unroll 4
-  for (int s = s0; s < s1; ++s) {
-    const int at = s * 64 + c * 16;
-    const uint32_t off = at < k ? (uint32_t)(r * k + at) : 0xFFFFFFF0u;  // past the row: zeros
-    const i8_x4 w = __builtin_bit_cast(i8_x4, buf_ld128(wr, off));
-#pragma unroll
-    for (int b = 0; b < MB; ++b) {
-      const i8_x4 x = __builtin_bit_cast(i8_x4, buf_ld128(xr, at < k ? off + (uint32_t)(16 * b * k) : 0xFFFFFFF0u));
-      acc[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, acc[b], 0, 0, 0);
-    }
+  Set A, B;
+  int b = blockIdx.x;
+  load(b, 0, A);
+  if constexpr (XKB > 0 && !QUANT) {  // a row per wave; beyond k of the last step: what LDS holds, times zeros
+    const uint4* xb = static_cast<const uint4*>(a.x);
+    for (int i = wave; i < m; i += KW)
+      for (int p = lane; p < (k >> 4); p += 64) *reinterpret_cast<uint4*>(xl + i * pitch + p * 16) = xb[(int64_t)i * (k >> 4) + p];
+    __syncthreads();
   }
-  if (wave > 0) {
+  if constexpr (QUANT) {
+    // Waves in `slots` groups of W: a group takes rows slot, slot + slots, ..., its waves 64 W pieces of 8 values at a
+    // time; the pieces (QF_KEEP a lane at most, by the rule of who comes here) stay in registers between the maximum
+    // and the quotients.
+    const int slots = qf_slots(m), W = KW / slots, slot = wave / W, sub = wave % W;
+    const int nc = k >> 3, cpr = (nc + 64 * W - 1) / (64 * W);
+    const uint4* xb = static_cast<const uint4*>(a.x);
+    uint4 v[QF_KEEP];
+    int qr = slot, j = 0;  // of piece i
 #pragma unroll
-    for (int b = 0; b < MB; ++b) part[wave - 1][b][lane] = acc[b];
-  }
-  __syncthreads();
-  if (wave > 0) return;
-#pragma unroll
-  for (int b = 0; b < MB; ++b) {
-#pragma unroll
-    for (int p = 0; p < KW - 1; ++p) acc[b] += part[p][b][lane];
-    const int mm = m0 + 16 * b + r;
-    if (mm >= m) continue;
-    const float sx = xs[mm];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int nn = n0 + 4 * c + i;
-      if (nn < n) i8_store<F32>(y, (int64_t)mm * n + nn, acc[b][i], sx * ws[nn]);
+    for (int i = 0; i < QF_KEEP; ++i) {
+      const int ch = (j * W + sub) * 64 + lane;
+      v[i] = qr < m && ch < nc ? xb[qr * nc + ch] : make_uint4(0, 0, 0, 0);
+      if (++j == cpr) j = 0, qr += slots;
     }
+    uint32_t mx = 0;
+    qr = slot, j = 0;
+#pragma unroll
+    for (int i = 0; i < QF_KEEP; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = max(mx, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));
+      if (++j == cpr) {
+        if (qr < m) {  // wave-uniform
+          const float wm = wave_max((float)mx);
+          if (lane == 0) most[qr][sub] = wm;
+        }
+        mx = 0, j = 0, qr += slots;
+      }
+    }
+    __syncthreads();
+    Q8Row q{};
+    qr = slot, j = 0;
+#pragma unroll
+    for (int i = 0; i < QF_KEEP; ++i) {
+      const int ch = (j * W + sub) * 64 + lane;
+      if (qr < m) {
+        if (j == 0) {
+          float am = most[qr][0];
+          for (int p = 1; p < W; ++p) am = fmaxf(am, most[qr][p]);
+          q = q8_row(bf2f((uint32_t)am));
+          if (lane == 0) sx[qr] = q.s;
+        }
+        if (ch < nc) *reinterpret_cast<uint2*>(xl + qr * pitch + ch * 8) = q8_pack(v[i], q);
+      }
+      if (++j == cpr) j = 0, qr += slots;
+    }
+    __syncthreads();
+  }
+  const float sr = row < 16 * MB && row < m ? (QUANT ? sx[row & 15] : a.xs[row]) : 0.0f;
+  int buf = 0;
+  // one turn of a block; the last one ends it
+  auto turn = [&](int t, const Set& v) {
+    if (t == 0) {
+#pragma unroll
+      for (int j = 0; j < MB; ++j) acc[j] = i8_x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+#pragma unroll
+      for (int j = 0; j < MB; ++j) {
+        i8_x4 x;
+        if constexpr (XKB == 0) x = v.x[i][j];
+        else  // the last row again for lanes behind it (not stored); a step within the row
+          x = *reinterpret_cast<const i8_x4*>(xl + min(16 * j + r, m - 1) * pitch + min(s0 + t * U + i, steps - 1) * 64 + c * 16);
+        acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v.w[i], x, acc[j], 0, 0, 0);
+      }
+    }
+    if (t < turns - 1) return;
+#pragma unroll
+    for (int j = 0; j < MB; ++j) *reinterpret_cast<i8_x4*>(&part[buf][wave][j][lane * 4]) = acc[j];
+    lds_barrier();
+    // a thread adds up and stores one value, 16 weight rows side by side. The next block's sums go to the other
+    // buffer, and a wave that is there has passed this barrier: the one after is enough for this buffer.
+    const int nn = b * 16 + tn;
+    if (row < 16 * MB && row < m && nn < a.n) {
+      int sum = 0;
+#pragma unroll
+      for (int p = 0; p < KW; ++p) sum += part[buf][p][row >> 4][((tn >> 2) * 16 + (row & 15)) * 4 + (tn & 3)];
+      i8_store<F32>(a.y, (int64_t)row * a.n + nn, sum, sr * v.s);
+    }
+    if (XKB) buf ^= 1;
+  };
+  // (block, turn) pairs in order, the next pair's loads in flight during one
+  int t = 0;
+  auto next = [&](int& nb, int& nt) {
+    nt = t + 1, nb = b;
+    if (nt == turns) nt = 0, nb = b + (int)gridDim.x;
+  };
+  if constexpr (XKB == 0) {
+    for (; t < turns; ++t) {
+      turn(t, A);
+      if (t + 1 < turns) load(b, t + 1, A);
+    }
+    return;
+  }
+  while (b < blocks) {
+    int nb, nt;
+    next(nb, nt);
+    load(nb, nt, B);
+    turn(t, A);
+    b = nb, t = nt;
+    if (b >= blocks) break;
+    next(nb, nt);
+    load(nb, nt, A);
+    turn(t, B);
+    b = nb, t = nt;
   }
 }
 
@@ -370,6 +505,14 @@ I8Plan i8_plan(int m, int n, int k) {
   return p;
 }
 
+template <int MB, int XKB, bool QUANT>
+void i8_few(const I8Few& a, int per_cu, bool f32, hipStream_t s) {
+  const int blocks = (a.n + 15) / 16;
+  const dim3 grid(XKB ? std::min(blocks, 256 * per_cu) : blocks), nt(64 * FEW_KW);
+  if (f32) hipLaunchKernelGGL((k_i8_few<MB, XKB, QUANT, true>), grid, nt, 0, s, a);
+  else hipLaunchKernelGGL((k_i8_few<MB, XKB, QUANT, false>), grid, nt, 0, s, a);
+}
+
 template <int BM, int BN, int WM, int WN, int ST>
 void i8_tiles(const I8Tile& a, bool f32, hipStream_t s) {
   const unsigned grid = 8u * (unsigned)((a.mblk * a.nblk * a.splits + 7) / 8);
@@ -395,9 +538,14 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
             int32_t m, int32_t n, int32_t k, hipStream_t s) {
   const I8Plan p = i8_plan(m, n, k);
   if (p.kind == 0) {
-    const dim3 grid((n + 15) / 16, (m + 31) / 32);
-    if (y_fp32) hipLaunchKernelGGL((k_i8_rows<2, 4, true>), grid, dim3(256), 0, s, xq, xs, wq, ws, y, m, n, k);
-    else hipLaunchKernelGGL((k_i8_rows<2, 4, false>), grid, dim3(256), 0, s, xq, xs, wq, ws, y, m, n, k);
+    const I8Few a{xq, xs, wq, ws, y, m, n, k};
+    const int64_t lds = (int64_t)m * few_pitch(k);
+    if (n < 8192) m <= 16 ? i8_few<1, 0, false>(a, 0, y_fp32, s) : i8_few<2, 0, false>(a, 0, y_fp32, s);
+    else if (m <= 16 && lds <= 48 << 10) i8_few<1, 48, false>(a, 2, y_fp32, s);
+    else if (m <= 16 && lds <= 132 << 10) i8_few<1, 132, false>(a, 1, y_fp32, s);
+    else if (m <= 16) i8_few<1, 0, false>(a, 0, y_fp32, s);
+    else if (lds <= 112 << 10) i8_few<2, 112, false>(a, 1, y_fp32, s);
+    else i8_few<2, 0, false>(a, 0, y_fp32, s);
   } else {
     const I8Tile a{xq, wq, xs, ws, p.splits > 1 ? work : y, m, n, k, p.mblk, p.nblk, p.splits, p.sps};
     if (p.kind == 1) i8_tiles<256, 256, 2, 4, 2>(a, y_fp32, s);
@@ -410,6 +558,23 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
     }
   }
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
+}
+
+int64_t i8_linear_bytes(int32_t m, int32_t n, int32_t k) {
+  return i8_pad((int64_t)m * k) + i8_pad((int64_t)m * 4) + i8_gemm_bytes(m, n, k);
+}
+
+int i8_linear(const uint16_t* x, const int8_t* wq, const float* ws, void* y, bool y_fp32, void* work, int32_t m,
+              int32_t n, int32_t k, hipStream_t s) {
+  if (qf_fits(m, k)) {
+    i8_few<1, 20, true>(I8Few{x, nullptr, wq, ws, y, m, n, k}, 2, y_fp32, s);
+    return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
+  }
+  int8_t* xq = static_cast<int8_t*>(work);
+  float* xs = reinterpret_cast<float*>(xq + i8_pad((int64_t)m * k));
+  const int rc = i8_quantize(x, xq, xs, m, k, s);
+  if (rc != FL_OK) return rc;
+  return i8_gemm(xq, xs, wq, ws, y, y_fp32, reinterpret_cast<char*>(xs) + i8_pad((int64_t)m * 4), m, n, k, s);
 }
 
 extern "C" {
@@ -435,7 +600,7 @@ int fl_gemm_int8(const int8_t* xq, const float* xs, const int8_t* wq, const floa
 
 int fl_linear_int8_workspace(int32_t m, int32_t n, int32_t k, int64_t* bytes) {
   if (!bytes || !i8_shape_ok(m, n, k)) return FL_E_ARG;
-  *bytes = i8_pad((int64_t)m * k) + i8_pad((int64_t)m * 4) + i8_gemm_bytes(m, n, k);
+  *bytes = i8_linear_bytes(m, n, k);
   return FL_OK;
 }
 
@@ -444,11 +609,7 @@ int fl_linear_int8(const uint16_t* x, const int8_t* wq, const float* ws, void* y
   if (!i8_shape_ok(m, n, k) || !i8_aligned(x) || !i8_aligned(wq) || !ws || !i8_aligned(y) || !i8_aligned(work))
     return FL_E_ARG;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  int8_t* xq = static_cast<int8_t*>(work);
-  float* xs = reinterpret_cast<float*>(xq + i8_pad((int64_t)m * k));
-  const int rc = i8_quantize(x, xq, xs, m, k, s);
-  if (rc != FL_OK) return rc;
-  return i8_gemm(xq, xs, wq, ws, y, y_fp32 != 0, reinterpret_cast<char*>(xs) + i8_pad((int64_t)m * 4), m, n, k, s);
+  return i8_linear(x, wq, ws, y, y_fp32 != 0, work, m, n, k, s);
 }
 
 }  // extern "C"

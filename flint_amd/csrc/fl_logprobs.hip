@@ -385,11 +385,11 @@ int lp_run(LpArgs a, bool bf16, int rows, void* work, hipStream_t s) {
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
 }
 
-// Features -> log probabilities: the rows of x in 8 bits, then blocks of rows through the head, whose fp32
-// logits stay in the workspace (up to 128 MB of them, half of what the last-level cache holds).
+// Features -> log probabilities: blocks of rows through the 8-bit head, whose fp32 logits stay in the workspace (up to
+// 128 MB of them, half of what the last-level cache holds).
 struct HeadPlan {
   int rows;  // of a block
-  int64_t xq, xs, logits, gemm, lp, bytes;
+  int64_t logits, linear, lp, bytes;
 };
 HeadPlan head_plan(int m, int n, int k, int top) {
   HeadPlan p{};
@@ -398,19 +398,16 @@ HeadPlan head_plan(int m, int n, int k, int top) {
   LpArgs a{};
   a.vocab = n;
   a.top = top;
-  int64_t lp = 0;
-  for (const int r : {p.rows, m % p.rows}) {
+  int64_t lp = 0, linear = 0;
+  for (const int r : {p.rows, m % p.rows}) {  // whole blocks and the last one
     if (r == 0) continue;
     lp_plan(a, r);
     lp = std::max(lp, lp_bytes(a, r));
-    p.gemm = std::max(p.gemm, i8_gemm_bytes(r, n, k));
+    linear = std::max(linear, i8_linear_bytes(r, n, k));
   }
-  const int64_t gemm = p.gemm;
-  p.xq = 0;
-  p.xs = i8_pad((int64_t)m * k);
-  p.logits = p.xs + i8_pad((int64_t)m * 4);
-  p.gemm = p.logits + i8_pad((int64_t)p.rows * n * 4);
-  p.lp = p.gemm + i8_pad(gemm);
+  p.logits = 0;
+  p.linear = i8_pad((int64_t)p.rows * n * 4);
+  p.lp = p.linear + i8_pad(linear);
   p.bytes = p.lp + lp;
   return p;
 }
@@ -457,20 +454,18 @@ int fl_head_logprobs(const uint16_t* x, const int8_t* wq, const float* ws, const
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const HeadPlan p = head_plan(m, n, k, top);
   char* base = static_cast<char*>(work);
-  int8_t* xq = reinterpret_cast<int8_t*>(base + p.xq);
-  float* xs = reinterpret_cast<float*>(base + p.xs);
-  int rc = i8_quantize(x, xq, xs, m, k, s);
-  for (int r0 = 0; r0 < m && rc == FL_OK; r0 += p.rows) {
+  for (int r0 = 0; r0 < m; r0 += p.rows) {
     const int r = std::min(p.rows, m - r0);
-    rc = i8_gemm(xq + (int64_t)r0 * k, xs + r0, wq, ws, base + p.logits, true, base + p.gemm, r, n, k, s);
-    if (rc != FL_OK) break;
+    int rc = i8_linear(x + (int64_t)r0 * k, wq, ws, base + p.logits, true, base + p.linear, r, n, k, s);
+    if (rc != FL_OK) return rc;
     const int64_t t0 = (int64_t)r0 * top;
     LpArgs a{base + p.logits, n, n, top, 0, 0, tokens ? tokens + r0 : nullptr, tokens ? logprob + r0 : nullptr,
              entropy + r0, tokens ? rank + r0 : nullptr, top ? top_ids + t0 : nullptr, top ? top_logprobs + t0 : nullptr,
              nullptr, nullptr};
     rc = lp_run(a, false, r, base + p.lp, s);
+    if (rc != FL_OK) return rc;
   }
-  return rc;
+  return FL_OK;
 }
 
 }  // extern "C"
