@@ -288,7 +288,7 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
 // ---- tiles ------------------------------------------------------------------------------------------
 // A workgroup of WM x WN waves computes BM rows of x against BN weight rows over one part of K, in steps of 128
 // bytes of K. Both tiles of a step go straight from memory into LDS (buffer_load ... lds, 1 KB = 8 rows of 128
-// bytes per wave instruction), ST stages deep: a step's loads are issued ST - 1 steps before it. In LDS the 16-byte
+// bytes per wave instruction), ST stages deep. In LDS the 16-byte
 // piece c of row r sits at c ^ (r % 8), so that the 8 lanes of a read phase, on one piece of 8 rows, take all
 // banks; the lanes of the load fetch the pieces in that order. Waves use 32x32x32 MFMAs: a lane (r = l % 32, h = l /
 // 32) holds piece 2 j + h of row r at sub-step j. Weights are operand A: a lane ends with x row l % 32 and weight
@@ -343,23 +343,23 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 65536 ? 2 : 1) void k_i8_t
   const i8_u32x4 wv = buffer_words(a.wq + (int64_t)n0 * a.k, (uint32_t)rows_n * (uint32_t)a.k);
   const i8_u32x4 xv = buffer_words(a.xq + (int64_t)m0 * a.k, (uint32_t)rows_m * (uint32_t)a.k);
   // this lane's piece of the wave's units; the buffers' range check makes rows past the end zeros
-  const int piece = (lane & 7) ^ (lane >> 3);
+  auto piece = [&](int i) { return (lane & 7) ^ (((wave * PER + i) & 1) * 4 + (lane >> 4)); };
   uint32_t off[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int row = (wave * PER + i) * 8 + (lane >> 3);
-    off[i] = (uint32_t)(row < BN ? row : row - BN) * (uint32_t)a.k + (uint32_t)piece * 16u;
+    off[i] = (uint32_t)(row < BN ? row : row - BN) * (uint32_t)a.k + (uint32_t)piece(i) * 16u;
   }
   const uint32_t base = (uint32_t)(uintptr_t)(lds_byte*)smem;
   const int tail = a.k & 127;  // bytes of the last step, if it is not whole
   auto load = [&](int s, int stage) {
     const uint32_t k0 = (uint32_t)s * 128u;
     // pieces past the end of a row are zeros too
-    const bool past = s == steps - 1 && tail != 0 && piece * 16 >= tail;
+    const bool cut = s == steps - 1 && tail != 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int u = wave * PER + i;
-      dma_1k(u * 8 < BN ? wv : xv, base + (uint32_t)(stage * STAGE + u * 1024), past ? 0x80000000u : off[i], k0);
+      dma_1k(u * 8 < BN ? wv : xv, base + (uint32_t)(stage * STAGE + u * 1024), cut && piece(i) * 16 >= tail ? 0x80000000u : off[i], k0);
     }
   };
   i8_x16 acc[FM][FN];
@@ -369,33 +369,55 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 65536 ? 2 : 1) void k_i8_t
     for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+  // Sub-step j of a step: fragments of 32 bytes of K. They are read one sub-step ahead; the last one of a step reads
+  // the next step's first, behind the step's one barrier, when the next stage has landed for every wave and
+  // this one has been read by every wave, so that it can be loaded again.
+  struct Frag {
+    i8_x4 w[FN], x[FM];
+  };
+  auto read = [&](int stage, int j, Frag& f) {
+    const int at = ((2 * j + h) ^ ((r >> 1) & 7)) * 16;
+    const unsigned char* wt = smem + stage * STAGE + (wn * TN + r) * 128 + at;
+    const unsigned char* xt = smem + stage * STAGE + (BN + wm * TM + r) * 128 + at;
 #pragma unroll
-  for (int p = 0; p < ST - 1; ++p)
+    for (int i = 0; i < FN; ++i) f.w[i] = *reinterpret_cast<const i8_x4*>(wt + i * 32 * 128);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) f.x[i] = *reinterpret_cast<const i8_x4*>(xt + i * 32 * 128);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](const Frag& f) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[j], f.x[i], acc[i][j], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll
+  for (int p = 0; p < ST; ++p)
     if (s0 + p < s1) load(s0 + p, p);
+  if (s0 + ST - 1 < s1) wait_loads<(ST - 1) * PER>();
+  else wait_loads<0>();
+  __builtin_amdgcn_s_barrier();
+  Frag A, B;
+  read(0, 0, A);
   int stage = 0;
   for (int s = s0; s < s1; ++s) {
-    // this step's loads have landed (fewer are in flight in the last steps: all of them, then)
-    if (ST > 2 && s + ST - 2 < s1) wait_loads<(ST - 2) * PER>();
+    const int then = stage == ST - 1 ? 0 : stage + 1;
+    read(stage, 1, B);
+    multiply(A);
+    read(stage, 2, A);
+    multiply(B);
+    read(stage, 3, B);
+    multiply(A);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): B is here, this stage is read
+    // in flight behind the next stage's loads: those of the stages after it, fewer in the last steps
+    if (s + ST - 1 < s1) wait_loads<(ST - 2) * PER>();
     else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
-    if (s + ST - 1 < s1) load(s + ST - 1, stage == 0 ? ST - 1 : stage - 1);
-    const unsigned char* wt = smem + stage * STAGE + (wn * TN + r) * 128;
-    const unsigned char* xt = smem + stage * STAGE + (BN + wm * TM + r) * 128;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      i8_x4 w[FN], x[FM];
-      const int at = ((2 * j + h) ^ (r & 7)) * 16;
-#pragma unroll
-      for (int f = 0; f < FN; ++f) w[f] = *reinterpret_cast<const i8_x4*>(wt + f * 32 * 128 + at);
-#pragma unroll
-      for (int f = 0; f < FM; ++f) x[f] = *reinterpret_cast<const i8_x4*>(xt + f * 32 * 128 + at);
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int f = 0; f < FN; ++f) acc[i][f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[f], x[i], acc[i][f], 0, 0, 0);
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is read: others may load into it
-    stage = stage == ST - 1 ? 0 : stage + 1;
+    if (s + ST < s1) load(s + ST, stage);
+    read(then, 0, A);  // (after the last step: what is there, not used)
+    multiply(B);
+    stage = then;
   }
   // out through LDS, 32 rows of x at a time, so that a wave stores whole lines
   __syncthreads();
@@ -499,7 +521,7 @@ I8Plan i8_plan(int m, int n, int k) {
   const int b = p.kind == 1 ? 256 : p.kind == 2 ? 128 : 64;
   p.mblk = (m + b - 1) / b;
   p.nblk = (n + b - 1) / b;
-  if (p.kind == 3) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 8, 384 / tiles(64)));
+  if (p.kind == 3) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 8, 256 / tiles(64)));
   p.sps = (steps + p.splits - 1) / p.splits;
   p.splits = (steps + p.sps - 1) / p.sps;
   return p;
@@ -548,9 +570,10 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
     else i8_few<2, 0, false>(a, 0, y_fp32, s);
   } else {
     const I8Tile a{xq, wq, xs, ws, p.splits > 1 ? work : y, m, n, k, p.mblk, p.nblk, p.splits, p.sps};
+    const bool one = p.mblk * p.nblk * p.splits <= 256;  // a CU holds one workgroup: it may have all of its LDS
     if (p.kind == 1) i8_tiles<256, 256, 2, 4, 2>(a, y_fp32, s);
-    else if (p.kind == 2) i8_tiles<128, 128, 2, 2, 2>(a, y_fp32, s);
-    else i8_tiles<64, 64, 2, 2, 4>(a, y_fp32, s);
+    else if (p.kind == 2) one ? i8_tiles<128, 128, 2, 2, 4>(a, y_fp32, s) : i8_tiles<128, 128, 2, 2, 2>(a, y_fp32, s);
+    else one ? i8_tiles<64, 64, 2, 2, 8>(a, y_fp32, s) : i8_tiles<64, 64, 2, 2, 4>(a, y_fp32, s);
     if (p.splits > 1) {
       const dim3 grid((unsigned)(((int64_t)m * n + 1023) / 1024));
       if (y_fp32) hipLaunchKernelGGL(k_i8_join<true>, grid, dim3(256), 0, s, static_cast<const int*>(work), p.splits, xs, ws, y, m, n);
