@@ -286,11 +286,11 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
 }
 
 // ---- tiles ------------------------------------------------------------------------------------------
-// A workgroup of WM x WN waves computes BM rows of x against BN weight rows over one part of K, in steps of 128
-// bytes of K. Both tiles of a step go straight from memory into LDS (buffer_load ... lds, 1 KB = 8 rows of 128
-// bytes per wave instruction), ST stages deep. In LDS the 16-byte
-// piece c of row r sits at c ^ (r % 8), so that the 8 lanes of a read phase, on one piece of 8 rows, take all
-// banks; the lanes of the load fetch the pieces in that order. Waves use 32x32x32 MFMAs: a lane (r = l % 32, h = l /
+// A workgroup of WM x WN waves computes T rows of x against T weight rows over one part of K, in steps of 128
+// bytes of K. The two units of a step, weights and x, go straight from memory into LDS (buffer_load ... lds, 1 KB = 8
+// rows of 128 bytes per wave instruction), into a ring of NR units. In LDS the 16-byte
+// piece c of row r sits at c ^ (r / 2 % 8), so that 16 lanes on one piece of 16 rows take all 64 banks once
+// (c ^ r % 8: 8.5 M conflict cycles in 90 us); the lanes of the load fetch the pieces in that order. Waves use 32x32x32 MFMAs: a lane (r = l % 32, h = l /
 // 32) holds piece 2 j + h of row r at sub-step j. Weights are operand A: a lane ends with x row l % 32 and weight
 // rows 8 (i / 4) + 4 h + i % 4.
 
@@ -321,13 +321,13 @@ struct I8Tile {
   int mblk, nblk, splits, sps;  // tiles along m and n; parts of K and their steps of 128
 };
 
-template <int BM, int BN, int WM, int WN, int ST, int OUT>  // OUT: 0 bf16, 1 fp32, 2 int32 part sums
-__global__ __launch_bounds__(64 * WM * WN, BM * BN >= 65536 ? 2 : 1) void k_i8_tile(I8Tile a) {
-  constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
-  constexpr int UNITS = (BM + BN) / 8, PER = UNITS / NW, STAGE = (BM + BN) * 128;
-  static_assert(UNITS % NW == 0 && BN % 8 == 0 && TM % 32 == 0 && TN % 32 == 0, "whole units");
-  constexpr int SLAB = 32 * (TN + 4) * 4;  // a wave's 32 rows of x by TN sums, in the stages' place at the end
-  constexpr int SMEM = ST * STAGE > NW * SLAB ? ST * STAGE : NW * SLAB;
+template <int T, int WM, int WN, int NR, int OUT>  // OUT: 0 bf16, 1 fp32, 2 int32 part sums
+__global__ __launch_bounds__(64 * WM * WN, T == 256 ? 2 : 1) void k_i8_tile(I8Tile a) {
+  constexpr int NW = WM * WN, TM = T / WM, TN = T / WN, FM = TM / 32, FN = TN / 32;
+  constexpr int PER = T / 8 / NW, UNIT = T * 128;  // loads of a wave for a unit; its bytes
+  static_assert(T % (8 * NW) == 0 && TM % 32 == 0 && TN % 32 == 0 && NR >= 4, "whole loads, two steps");
+  constexpr int SLAB = 32 * (TN + 4) * 4;  // a wave's 32 rows of x by TN sums, in the units' place at the end
+  constexpr int SMEM = NR * UNIT > NW * SLAB ? NR * UNIT : NW * SLAB;
   __shared__ __align__(1024) unsigned char smem[SMEM];
   const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
@@ -337,30 +337,27 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 65536 ? 2 : 1) void k_i8_t
   if ((int)(blockIdx.x >> 3) >= share || t >= tiles) return;
   const int split = t / (a.mblk * a.nblk), tt = t - split * (a.mblk * a.nblk);
   const int grp = tt / (8 * a.nblk), gm = min(8, a.mblk - grp * 8), in = tt - grp * 8 * a.nblk;
-  const int m0 = (grp * 8 + in % gm) * BM, n0 = (in / gm) * BN;
+  const int m0 = (grp * 8 + in % gm) * T, n0 = (in / gm) * T;
   const int steps = (a.k + 127) >> 7, s0 = split * a.sps, s1 = min(steps, s0 + a.sps);
-  const int rows_n = min(BN, a.n - n0), rows_m = min(BM, a.m - m0);
+  const int rows_n = min(T, a.n - n0), rows_m = min(T, a.m - m0);
   const i8_u32x4 wv = buffer_words(a.wq + (int64_t)n0 * a.k, (uint32_t)rows_n * (uint32_t)a.k);
   const i8_u32x4 xv = buffer_words(a.xq + (int64_t)m0 * a.k, (uint32_t)rows_m * (uint32_t)a.k);
-  // this lane's piece of the wave's units; the buffers' range check makes rows past the end zeros
+  // this lane's piece of the wave's loads of a unit; the buffers' range check makes rows past the end zeros
   auto piece = [&](int i) { return (lane & 7) ^ (((wave * PER + i) & 1) * 4 + (lane >> 4)); };
   uint32_t off[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int row = (wave * PER + i) * 8 + (lane >> 3);
-    off[i] = (uint32_t)(row < BN ? row : row - BN) * (uint32_t)a.k + (uint32_t)piece(i) * 16u;
-  }
-  const uint32_t base = (uint32_t)(uintptr_t)(lds_byte*)smem;
+  for (int i = 0; i < PER; ++i) off[i] = (uint32_t)((wave * PER + i) * 8 + (lane >> 3)) * (uint32_t)a.k + (uint32_t)piece(i) * 16u;
+  const uint32_t base = (uint32_t)(uintptr_t)(lds_byte*)smem + (uint32_t)(wave * PER) * 1024u;
   const int tail = a.k & 127;  // bytes of the last step, if it is not whole
-  auto load = [&](int s, int stage) {
-    const uint32_t k0 = (uint32_t)s * 128u;
-    // pieces past the end of a row are zeros too
-    const bool cut = s == steps - 1 && tail != 0;
+  // unit u of this part of K (2 s: weights of step s0 + s, 2 s + 1: x) into its slot, if there is such a step
+  auto load = [&](int u, int slot) {
+    const int s = s0 + (u >> 1);
+    if (s >= s1) return;
+    const bool cut = s == steps - 1 && tail != 0;  // pieces past the end of a row are zeros too
+    const i8_u32x4 v = u & 1 ? xv : wv;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = wave * PER + i;
-      dma_1k(u * 8 < BN ? wv : xv, base + (uint32_t)(stage * STAGE + u * 1024), cut && piece(i) * 16 >= tail ? 0x80000000u : off[i], k0);
-    }
+    for (int i = 0; i < PER; ++i)
+      dma_1k(v, base + (uint32_t)(slot * UNIT + i * 1024), cut && piece(i) * 16 >= tail ? 0x80000000u : off[i], (uint32_t)s * 128u);
   };
   i8_x16 acc[FM][FN];
 #pragma unroll
@@ -370,15 +367,15 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 65536 ? 2 : 1) void k_i8_t
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
   // Sub-step j of a step: fragments of 32 bytes of K. They are read one sub-step ahead; the last one of a step reads
-  // the next step's first, behind the step's one barrier, when the next stage has landed for every wave and
-  // this one has been read by every wave, so that it can be loaded again.
+  // the next step's first, behind the step's one barrier, when the next step's units have landed for every wave
+  // and this step's have been read by every wave, so that their slots can be loaded again.
   struct Frag {
     i8_x4 w[FN], x[FM];
   };
-  auto read = [&](int stage, int j, Frag& f) {
+  auto read = [&](int ws, int xs, int j, Frag& f) {
     const int at = ((2 * j + h) ^ ((r >> 1) & 7)) * 16;
-    const unsigned char* wt = smem + stage * STAGE + (wn * TN + r) * 128 + at;
-    const unsigned char* xt = smem + stage * STAGE + (BN + wm * TM + r) * 128 + at;
+    const unsigned char* wt = smem + ws * UNIT + (wn * TN + r) * 128 + at;
+    const unsigned char* xt = smem + xs * UNIT + (wm * TM + r) * 128 + at;
 #pragma unroll
     for (int i = 0; i < FN; ++i) f.w[i] = *reinterpret_cast<const i8_x4*>(wt + i * 32 * 128);
 #pragma unroll
@@ -393,31 +390,33 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 65536 ? 2 : 1) void k_i8_t
     __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll
-  for (int p = 0; p < ST; ++p)
-    if (s0 + p < s1) load(s0 + p, p);
-  if (s0 + ST - 1 < s1) wait_loads<(ST - 1) * PER>();
+  for (int u = 0; u < NR; ++u) load(u, u);
+  if (s0 + (NR - 1) / 2 < s1) wait_loads<(NR - 2) * PER>();
   else wait_loads<0>();
   __builtin_amdgcn_s_barrier();
   Frag A, B;
-  read(0, 0, A);
-  int stage = 0;
-  for (int s = s0; s < s1; ++s) {
-    const int then = stage == ST - 1 ? 0 : stage + 1;
-    read(stage, 1, B);
+  read(0, 1, 0, A);
+  int ws = 0, xs = 1;  // this step's slots
+  for (int s = 0; s < s1 - s0; ++s) {
+    const int wn_ = ws + 2 >= NR ? ws + 2 - NR : ws + 2, xn_ = xs + 2 >= NR ? xs + 2 - NR : xs + 2;
+    read(ws, xs, 1, B);
+    // the second of the two units that follow the last step's, whose slots are free since its barrier: not both at
+    // once, a load instruction takes 16 cycles
+    if (s > 0) load(2 * s - 1 + NR, xs >= 2 ? xs - 2 : xs - 2 + NR);
     multiply(A);
-    read(stage, 2, A);
+    read(ws, xs, 2, A);
     multiply(B);
-    read(stage, 3, B);
+    read(ws, xs, 3, B);
     multiply(A);
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): B is here, this stage is read
-    // in flight behind the next stage's loads: those of the stages after it, fewer in the last steps
-    if (s + ST - 1 < s1) wait_loads<(ST - 2) * PER>();
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): B is here, this step's units are read
+    // in flight behind the next step's units: those after them, NR - 4, fewer in the last steps
+    if (s0 + s + (NR - 1) / 2 < s1) wait_loads<(NR - 4) * PER>();
     else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
-    if (s + ST < s1) load(s + ST, stage);
-    read(then, 0, A);  // (after the last step: what is there, not used)
+    load(2 * s + NR, ws);
+    read(wn_, xn_, 0, A);  // (after the last step: what is there, not used)
     multiply(B);
-    stage = then;
+    ws = wn_, xs = xn_;
   }
   // out through LDS, 32 rows of x at a time, so that a wave stores whole lines
   __syncthreads();
@@ -535,13 +534,13 @@ void i8_few(const I8Few& a, int per_cu, bool f32, hipStream_t s) {
   else hipLaunchKernelGGL((k_i8_few<MB, XKB, QUANT, false>), grid, nt, 0, s, a);
 }
 
-template <int BM, int BN, int WM, int WN, int ST>
+template <int T, int WM, int WN, int NR>
 void i8_tiles(const I8Tile& a, bool f32, hipStream_t s) {
   const unsigned grid = 8u * (unsigned)((a.mblk * a.nblk * a.splits + 7) / 8);
   const dim3 nt(64 * WM * WN);
-  if (a.splits > 1) hipLaunchKernelGGL((k_i8_tile<BM, BN, WM, WN, ST, 2>), dim3(grid), nt, 0, s, a);
-  else if (f32) hipLaunchKernelGGL((k_i8_tile<BM, BN, WM, WN, ST, 1>), dim3(grid), nt, 0, s, a);
-  else hipLaunchKernelGGL((k_i8_tile<BM, BN, WM, WN, ST, 0>), dim3(grid), nt, 0, s, a);
+  if (a.splits > 1) hipLaunchKernelGGL((k_i8_tile<T, WM, WN, NR, 2>), dim3(grid), nt, 0, s, a);
+  else if (f32) hipLaunchKernelGGL((k_i8_tile<T, WM, WN, NR, 1>), dim3(grid), nt, 0, s, a);
+  else hipLaunchKernelGGL((k_i8_tile<T, WM, WN, NR, 0>), dim3(grid), nt, 0, s, a);
 }
 
 }  // namespace
@@ -571,9 +570,9 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
   } else {
     const I8Tile a{xq, wq, xs, ws, p.splits > 1 ? work : y, m, n, k, p.mblk, p.nblk, p.splits, p.sps};
     const bool one = p.mblk * p.nblk * p.splits <= 256;  // a CU holds one workgroup: it may have all of its LDS
-    if (p.kind == 1) i8_tiles<256, 256, 2, 4, 2>(a, y_fp32, s);
-    else if (p.kind == 2) one ? i8_tiles<128, 128, 2, 2, 4>(a, y_fp32, s) : i8_tiles<128, 128, 2, 2, 2>(a, y_fp32, s);
-    else one ? i8_tiles<64, 64, 2, 2, 8>(a, y_fp32, s) : i8_tiles<64, 64, 2, 2, 4>(a, y_fp32, s);
+    if (p.kind == 1) i8_tiles<256, 2, 4, 5>(a, y_fp32, s);
+    else if (p.kind == 2) one ? i8_tiles<128, 2, 2, 8>(a, y_fp32, s) : i8_tiles<128, 2, 2, 4>(a, y_fp32, s);
+    else one ? i8_tiles<64, 2, 2, 16>(a, y_fp32, s) : i8_tiles<64, 2, 2, 8>(a, y_fp32, s);
     if (p.splits > 1) {
       const dim3 grid((unsigned)(((int64_t)m * n + 1023) / 1024));
       if (y_fp32) hipLaunchKernelGGL(k_i8_join<true>, grid, dim3(256), 0, s, static_cast<const int*>(work), p.splits, xs, ws, y, m, n);
