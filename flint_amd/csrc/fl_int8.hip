@@ -321,16 +321,21 @@ struct I8Tile {
   int mblk, nblk, splits, sps;  // tiles along m and n; parts of K and their steps of 128
 };
 
-template <int T, int WM, int WN, int NR, int OUT>  // OUT: 0 bf16, 1 fp32, 2 int32 part sums
-__global__ __launch_bounds__(64 * WM * WN, T == 256 ? 2 : 1) void k_i8_tile(I8Tile a) {
+// KW > 1: the waves are KW ways of WM x WN, each over its own steps with a ring of its own, for calls of few tiles, where
+// a step's latency counts: a way of one wave needs no barrier, and its products are four times those of a wave
+// that shares the tile with three others. The ways' sums meet in LDS.
+template <int T, int KW, int WM, int WN, int NR, int Q, int OUT>  // OUT: 0 bf16, 1 fp32, 2 int32 part sums
+__global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k_i8_tile(I8Tile a) {
   constexpr int NW = WM * WN, TM = T / WM, TN = T / WN, FM = TM / 32, FN = TN / 32;
   constexpr int PER = T / 8 / NW, UNIT = T * 128;  // loads of a wave for a unit; its bytes
   static_assert(T % (8 * NW) == 0 && TM % 32 == 0 && TN % 32 == 0 && NR >= 4, "whole loads, two steps");
-  constexpr int SLAB = 32 * (TN + 4) * 4;  // a wave's 32 rows of x by TN sums, in the units' place at the end
-  constexpr int SMEM = NR * UNIT > NW * SLAB ? NR * UNIT : NW * SLAB;
+  // at the end, in the units' place: 32 rows of x by TN sums of a wave at a time; with ways all sums of each
+  constexpr int LD = KW == 1 ? TN + 4 : T + 4, SLAB = (KW == 1 ? 32 : T) * LD * 4, SLABS = KW == 1 ? NW : KW;
+  constexpr int SMEM = KW * NR * UNIT > SLABS * SLAB ? KW * NR * UNIT : SLABS * SLAB;
   __shared__ __align__(1024) unsigned char smem[SMEM];
   const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
+  const int wv0 = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int way = wv0 / NW, wave = wv0 % NW, wm = wave % WM, wn = wave / WM;
   // an XCD's workgroups (blockIdx % 8) take neighbouring tiles: up to 8 along m, then along n
   const int tiles = a.mblk * a.nblk * a.splits, share = (tiles + 7) >> 3;
   const int t = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
@@ -338,7 +343,10 @@ __global__ __launch_bounds__(64 * WM * WN, T == 256 ? 2 : 1) void k_i8_tile(I8Ti
   const int split = t / (a.mblk * a.nblk), tt = t - split * (a.mblk * a.nblk);
   const int grp = tt / (8 * a.nblk), gm = min(8, a.mblk - grp * 8), in = tt - grp * 8 * a.nblk;
   const int m0 = (grp * 8 + in % gm) * T, n0 = (in / gm) * T;
-  const int steps = (a.k + 127) >> 7, s0 = split * a.sps, s1 = min(steps, s0 + a.sps);
+  const int steps = (a.k + 127) >> 7;
+  // the workgroup's part of K, the way's of that; every way passes as many barriers
+  const int p0 = split * a.sps, p1 = min(steps, p0 + a.sps), per = (p1 - p0 + KW - 1) / KW;
+  const int s0 = p0 + way * per, s1 = min(p1, s0 + per);
   const int rows_n = min(T, a.n - n0), rows_m = min(T, a.m - m0);
   const i8_u32x4 wv = buffer_words(a.wq + (int64_t)n0 * a.k, (uint32_t)rows_n * (uint32_t)a.k);
   const i8_u32x4 xv = buffer_words(a.xq + (int64_t)m0 * a.k, (uint32_t)rows_m * (uint32_t)a.k);
@@ -347,7 +355,8 @@ __global__ __launch_bounds__(64 * WM * WN, T == 256 ? 2 : 1) void k_i8_tile(I8Ti
   uint32_t off[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) off[i] = (uint32_t)((wave * PER + i) * 8 + (lane >> 3)) * (uint32_t)a.k + (uint32_t)piece(i) * 16u;
-  const uint32_t base = (uint32_t)(uintptr_t)(lds_byte*)smem + (uint32_t)(wave * PER) * 1024u;
+  unsigned char* const ring = smem + way * (NR * UNIT);
+  const uint32_t base = (uint32_t)(uintptr_t)(lds_byte*)smem + (uint32_t)(way * NR * UNIT + wave * PER * 1024);
   const int tail = a.k & 127;  // bytes of the last step, if it is not whole
   // unit u of this part of K (2 s: weights of step s0 + s, 2 s + 1: x) into its slot, if there is such a step
   auto load = [&](int u, int slot) {
@@ -358,6 +367,9 @@ __global__ __launch_bounds__(64 * WM * WN, T == 256 ? 2 : 1) void k_i8_tile(I8Ti
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       dma_1k(v, base + (uint32_t)(slot * UNIT + i * 1024), cut && piece(i) * 16 >= tail ? 0x80000000u : off[i], (uint32_t)s * 128u);
+  };
+  auto meet = [&] {  // one wave's loads and reads are its own
+    if (NW > 1) __builtin_amdgcn_s_barrier();
   };
   i8_x16 acc[FM][FN];
 #pragma unroll
@@ -370,30 +382,36 @@ __global__ __launch_bounds__(64 * WM * WN, T == 256 ? 2 : 1) void k_i8_tile(I8Ti
   // the next step's first, behind the step's one barrier, when the next step's units have landed for every wave
   // and this step's have been read by every wave, so that their slots can be loaded again.
   struct Frag {
-    i8_x4 w[FN], x[FM];
+    i8_x4 w[Q][FN], x[Q][FM];
   };
   auto read = [&](int ws, int xs, int j, Frag& f) {
-    const int at = ((2 * j + h) ^ ((r >> 1) & 7)) * 16;
-    const unsigned char* wt = smem + ws * UNIT + (wn * TN + r) * 128 + at;
-    const unsigned char* xt = smem + xs * UNIT + (wm * TM + r) * 128 + at;
+    const unsigned char* wt = ring + ws * UNIT + (wn * TN + r) * 128;
+    const unsigned char* xt = ring + xs * UNIT + (wm * TM + r) * 128;
 #pragma unroll
-    for (int i = 0; i < FN; ++i) f.w[i] = *reinterpret_cast<const i8_x4*>(wt + i * 32 * 128);
+    for (int q = 0; q < Q; ++q) {
+      const int at = ((2 * (j * Q + q) + h) ^ ((r >> 1) & 7)) * 16;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) f.x[i] = *reinterpret_cast<const i8_x4*>(xt + i * 32 * 128);
+      for (int i = 0; i < FN; ++i) f.w[q][i] = *reinterpret_cast<const i8_x4*>(wt + i * 32 * 128 + at);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) f.x[q][i] = *reinterpret_cast<const i8_x4*>(xt + i * 32 * 128 + at);
+    }
     __builtin_amdgcn_sched_barrier(0);
   };
   auto multiply = [&](const Frag& f) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+    for (int q = 0; q < Q; ++q)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[j], f.x[i], acc[i][j], 0, 0, 0);
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[q][j], f.x[q][i], acc[i][j], 0, 0, 0);
     __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll
   for (int u = 0; u < NR; ++u) load(u, u);
   if (s0 + (NR - 1) / 2 < s1) wait_loads<(NR - 2) * PER>();
   else wait_loads<0>();
-  __builtin_amdgcn_s_barrier();
+  meet();
   Frag A, B;
   read(0, 1, 0, A);
   int ws = 0, xs = 1;  // this step's slots
@@ -404,79 +422,97 @@ __global__ __launch_bounds__(64 * WM * WN, T == 256 ? 2 : 1) void k_i8_tile(I8Ti
     // once, a load instruction takes 16 cycles
     if (s > 0) load(2 * s - 1 + NR, xs >= 2 ? xs - 2 : xs - 2 + NR);
     multiply(A);
-    read(ws, xs, 2, A);
-    multiply(B);
-    read(ws, xs, 3, B);
-    multiply(A);
+    if constexpr (Q == 1) {
+      read(ws, xs, 2, A);
+      multiply(B);
+      read(ws, xs, 3, B);
+      multiply(A);
+    }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): B is here, this step's units are read
     // in flight behind the next step's units: those after them, NR - 4, fewer in the last steps
     if (s0 + s + (NR - 1) / 2 < s1) wait_loads<(NR - 4) * PER>();
     else wait_loads<0>();
-    __builtin_amdgcn_s_barrier();
+    meet();
     load(2 * s + NR, ws);
     read(wn_, xn_, 0, A);  // (after the last step: what is there, not used)
     multiply(B);
     ws = wn_, xs = xn_;
   }
-  // out through LDS, 32 rows of x at a time, so that a wave stores whole lines
+  if (NW > 1)  // a way with fewer steps (or none) than the others
+    for (int s = max(s1 - s0, 0); s < per; ++s) __builtin_amdgcn_s_barrier();
+  // out through LDS, so that a wave stores whole lines
   __syncthreads();
-  int* slab = reinterpret_cast<int*>(smem + wave * SLAB);
-  constexpr int V = OUT == 0 ? 8 : 4, LR = TN / V, RI = 64 / LR;  // values of a lane's store; lanes of a row, rows at once
-  const int lc = (lane % LR) * V, nn = n0 + wn * TN + lc;
+  constexpr int V = OUT == 0 ? 8 : 4;  // values of a lane's store
+  const bool wide = (a.n % V) == 0;
+  auto put = [&](const int* v, int mm, int nn, float sx, const float* sw) {  // V sums of x row mm from weight row nn on
+    const int64_t at = ((int64_t)split * a.m + mm) * a.n + nn;
+    float o[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = OUT == 2 ? 0.0f : (float)v[e] * (sx * sw[e]);
+    if (wide && nn < a.n) {
+      if (OUT == 2) *reinterpret_cast<i8_x4*>(static_cast<int*>(a.y) + at) = i8_x4{v[0], v[1], v[2], v[3]};
+      else if (OUT == 1) *reinterpret_cast<float4*>(static_cast<float*>(a.y) + at) = make_float4(o[0], o[1], o[2], o[3]);
+      else
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + at) =
+            make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4 % V], o[5 % V]),
+                       pack_bf16x2(o[6 % V], o[7 % V]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (nn + e >= a.n) break;
+        if (OUT == 2) static_cast<int*>(a.y)[at + e] = v[e];
+        else if (OUT == 1) static_cast<float*>(a.y)[at + e] = o[e];
+        else static_cast<uint16_t*>(a.y)[at + e] = (uint16_t)f2bf(o[e]);
+      }
+    }
+  };
+  constexpr int COLS = KW == 1 ? TN : T, LR = COLS / V;  // lanes of a row
+  const int lc = (lane % LR) * V, nn = n0 + (KW == 1 ? wn * TN : 0) + lc;
   float sw[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) sw[e] = OUT < 2 && nn + e < a.n ? a.ws[nn + e] : 0.0f;
-  const bool wide = nn + V <= a.n && (a.n % V) == 0;
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
+  auto keep = [&](int* slab, int i, int row) {  // sums of x rows 32 i + r of the wave
 #pragma unroll
     for (int f = 0; f < FN; ++f)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<i8_x4*>(slab + r * (TN + 4) + f * 32 + 8 * q + 4 * h) =
+        *reinterpret_cast<i8_x4*>(slab + row * LD + f * 32 + 8 * q + 4 * h) =
             i8_x4{acc[i][f][4 * q], acc[i][f][4 * q + 1], acc[i][f][4 * q + 2], acc[i][f][4 * q + 3]};
-    __builtin_amdgcn_wave_barrier();
+  };
+  if constexpr (KW == 1) {
+    int* slab = reinterpret_cast<int*>(smem + wave * SLAB);
 #pragma unroll
-    for (int p = 0; p < 32 / RI; ++p) {
-      const int row = p * RI + lane / LR, mm = m0 + wm * TM + i * 32 + row;
+    for (int i = 0; i < FM; ++i) {
+      keep(slab, i, r);
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int p = 0; p < 32 * LR / 64; ++p) {
+        const int row = (p * 64 + lane) / LR, mm = m0 + wm * TM + i * 32 + row;
+        int v[V];
+#pragma unroll
+        for (int e = 0; e < V; e += 4) *reinterpret_cast<i8_x4*>(v + e) = *reinterpret_cast<const i8_x4*>(slab + row * LD + lc + e);
+        if (mm < a.m) put(v, mm, nn, OUT < 2 ? a.xs[mm] : 0.0f, sw);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  } else {
+    int* slab = reinterpret_cast<int*>(smem);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) keep(slab + way * (T * LD) + wn * TN, i, wm * TM + i * 32 + r);
+    __syncthreads();
+    for (int at = threadIdx.x; at < T * LR; at += 64 * KW * NW) {  // at % LR is lane % LR
+      const int row = at / LR, mm = m0 + row;
+      if (mm >= a.m) break;
       int v[V];
 #pragma unroll
-      for (int e = 0; e < V; e += 4)
-        *reinterpret_cast<i8_x4*>(v + e) = *reinterpret_cast<const i8_x4*>(slab + row * (TN + 4) + lc + e);
-      if (mm >= a.m) continue;
-      const int64_t at = ((int64_t)split * a.m + mm) * a.n + nn;
-      if (OUT == 2) {
-        int* y = static_cast<int*>(a.y) + at;
-        if (wide) *reinterpret_cast<i8_x4*>(y) = i8_x4{v[0], v[1], v[2], v[3]};
-        else
+      for (int e = 0; e < V; e += 4) {
+        i8_x4 z = *reinterpret_cast<const i8_x4*>(slab + row * LD + lc + e);
 #pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (nn + e < a.n) y[e] = v[e];
-      } else {
-        const float sx = a.xs[mm];
-        float o[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = (float)v[e] * (sx * sw[e]);
-        if (OUT == 1) {
-          float* y = static_cast<float*>(a.y) + at;
-          if (wide) *reinterpret_cast<float4*>(y) = make_float4(o[0], o[1], o[2], o[3]);
-          else
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-              if (nn + e < a.n) y[e] = o[e];
-        } else {
-          uint16_t* y = static_cast<uint16_t*>(a.y) + at;
-          if (wide)
-            *reinterpret_cast<uint4*>(y) = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]),
-                                                      pack_bf16x2(o[4 % V], o[5 % V]), pack_bf16x2(o[6 % V], o[7 % V]));
-          else
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-              if (nn + e < a.n) y[e] = (uint16_t)f2bf(o[e]);
-        }
+        for (int w = 1; w < KW; ++w) z += *reinterpret_cast<const i8_x4*>(slab + w * (T * LD) + row * LD + lc + e);
+        *reinterpret_cast<i8_x4*>(v + e) = z;
       }
+      put(v, mm, nn, OUT < 2 ? a.xs[mm] : 0.0f, sw);
     }
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -534,13 +570,13 @@ void i8_few(const I8Few& a, int per_cu, bool f32, hipStream_t s) {
   else hipLaunchKernelGGL((k_i8_few<MB, XKB, QUANT, false>), grid, nt, 0, s, a);
 }
 
-template <int T, int WM, int WN, int NR>
+template <int T, int KW, int WM, int WN, int NR, int Q>
 void i8_tiles(const I8Tile& a, bool f32, hipStream_t s) {
   const unsigned grid = 8u * (unsigned)((a.mblk * a.nblk * a.splits + 7) / 8);
-  const dim3 nt(64 * WM * WN);
-  if (a.splits > 1) hipLaunchKernelGGL((k_i8_tile<T, WM, WN, NR, 2>), dim3(grid), nt, 0, s, a);
-  else if (f32) hipLaunchKernelGGL((k_i8_tile<T, WM, WN, NR, 1>), dim3(grid), nt, 0, s, a);
-  else hipLaunchKernelGGL((k_i8_tile<T, WM, WN, NR, 0>), dim3(grid), nt, 0, s, a);
+  const dim3 nt(64 * KW * WM * WN);
+  if (a.splits > 1) hipLaunchKernelGGL((k_i8_tile<T, KW, WM, WN, NR, Q, 2>), dim3(grid), nt, 0, s, a);
+  else if (f32) hipLaunchKernelGGL((k_i8_tile<T, KW, WM, WN, NR, Q, 1>), dim3(grid), nt, 0, s, a);
+  else hipLaunchKernelGGL((k_i8_tile<T, KW, WM, WN, NR, Q, 0>), dim3(grid), nt, 0, s, a);
 }
 
 }  // namespace
@@ -570,9 +606,9 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
   } else {
     const I8Tile a{xq, wq, xs, ws, p.splits > 1 ? work : y, m, n, k, p.mblk, p.nblk, p.splits, p.sps};
     const bool one = p.mblk * p.nblk * p.splits <= 256;  // a CU holds one workgroup: it may have all of its LDS
-    if (p.kind == 1) i8_tiles<256, 2, 4, 5>(a, y_fp32, s);
-    else if (p.kind == 2) one ? i8_tiles<128, 2, 2, 8>(a, y_fp32, s) : i8_tiles<128, 2, 2, 4>(a, y_fp32, s);
-    else one ? i8_tiles<64, 2, 2, 16>(a, y_fp32, s) : i8_tiles<64, 2, 2, 8>(a, y_fp32, s);
+    if (p.kind == 1) i8_tiles<256, 1, 2, 4, 5, 1>(a, y_fp32, s);
+    else if (p.kind == 2) one ? i8_tiles<128, 1, 2, 4, 8, 1>(a, y_fp32, s) : i8_tiles<128, 1, 2, 2, 4, 1>(a, y_fp32, s);
+    else one ? i8_tiles<64, 4, 1, 1, 4, 1>(a, y_fp32, s) : i8_tiles<64, 1, 2, 2, 8, 1>(a, y_fp32, s);
     if (p.splits > 1) {
       const dim3 grid((unsigned)(((int64_t)m * n + 1023) / 1024));
       if (y_fp32) hipLaunchKernelGGL(k_i8_join<true>, grid, dim3(256), 0, s, static_cast<const int*>(work), p.splits, xs, ws, y, m, n);
