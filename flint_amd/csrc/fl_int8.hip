@@ -16,46 +16,58 @@ typedef uint32_t i8_u32x4 __attribute__((ext_vector_type(4)));
 
 // ---- quantisation -------------------------------------------------------------------------------
 
-// x / s rounded to the nearest whole number, ties to even, for |x| <= 127 s (1 + 2^-22). The product with
-// 1 / s is off by a few ulp, which matters next to a half (x = max / 2 gives 63.5, often), so the remainder
-// r = x - q s decides. It is exact in one fma: q s has at most 31 bits and |r| <= s, a multiple of an ulp
-// of the smaller of x and s.
+// x / s rounded to the nearest whole number, ties to even, for |x| <= 127 s (1 + 2^-22). t = x (1 / s) is off by at
+// most 127 * 2^-22, so its nearest whole number q may be one off next to a half, and x = max / 2, which gives 63.5,
+// is frequent: the remainder r = x - q s decides. It is exact in one fma: q s has at most 31 bits and |r| <= s is a
+// multiple of an ulp of the smaller of x and s. An exact half needs s to be a power of two (x has 8 bits, and max / 127
+// to 24 bits has few only if 127 divides max's), and then t is exact and its rounding went to the even side.
 struct Q8Row {
-  float s, inv, up;  // scale; 1 / (s up); up: a power of two that keeps 1 / s of tiny rows finite
+  float s;           // the scale
+  float w, h, inv;   // s, half of it and 1 / s; of tiny rows, whose 1 / s is not finite, of s times 2^80
+  bool tiny;
 };
+constexpr float Q8_UP = 0x1p80f;
 __device__ __forceinline__ Q8Row q8_row(float amax) {
   Q8Row r;
   r.s = amax < INFINITY ? amax * (1.0f / 127.0f) : __builtin_nanf("");
-  r.up = amax < 0x1p-64f ? 0x1p80f : 1.0f;
-  r.inv = r.s > 0.0f ? 1.0f / (r.s * r.up) : 0.0f;  // zero rows and rows with a NaN or an infinity: q = 0
+  r.tiny = amax < 0x1p-64f;
+  r.w = r.tiny ? r.s * Q8_UP : r.s;
+  r.h = 0.5f * r.w;
+  r.inv = r.s > 0.0f ? __builtin_amdgcn_rcpf(r.w) : 0.0f;  // zero rows and rows with a NaN or an infinity: q = 0
   return r;
 }
-__device__ __forceinline__ int q8_of(float x, const Q8Row& row) {
-  const float q = __builtin_rintf(x * row.up * row.inv), r = __builtin_fmaf(-q, row.s, x), two = fabsf(r + r);
-  const int i = (int)q;
-  return two > row.s || (two == row.s && (i & 1)) ? i + (r > 0.0f ? 1 : -1) : i;
-}
 // eight bf16 values
-__device__ __forceinline__ uint2 q8_pack(const uint4& p, const Q8Row& r) {
+__device__ __forceinline__ uint2 q8_pack(const uint4& p, const Q8Row& row) {
+  if (!(row.inv != 0.0f)) return make_uint2(0, 0);
   const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-  uint32_t o[2] = {0, 0};
-  if (!(r.inv != 0.0f)) return make_uint2(0, 0);
+  float x[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t a = (uint32_t)q8_of(bflo(w[i]), r) & 0xFFu, b = (uint32_t)q8_of(bfhi(w[i]), r) & 0xFFu;
-    o[i >> 1] |= (a | b << 8) << (16 * (i & 1));
+  for (int i = 0; i < 4; ++i) x[2 * i] = bflo(w[i]), x[2 * i + 1] = bfhi(w[i]);
+  if (row.tiny) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= Q8_UP;
   }
-  return make_uint2(o[0], o[1]);
+  uint32_t o[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = __builtin_rintf(x[i] * row.inv), r = __builtin_fmaf(-q, row.w, x[i]);
+    const float one = fabsf(r) > row.h ? __builtin_copysignf(1.0f, r) : 0.0f;
+    o[i >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(q + 128.0f + one, i & 3, o[i >> 2]);  // 1..255
+  }
+  return make_uint2(o[0] ^ 0x80808080u, o[1] ^ 0x80808080u);
 }
 
-constexpr int Q8_NT = 256, Q8_KEEP = 4;  // threads of a row; 8-value pieces that a thread keeps in registers
+constexpr int Q8_NT = 256, Q8_KEEP = 5;  // threads of a workgroup; 8-value pieces that a lane keeps in registers
 
-// One workgroup per row; rows of up to 8192 values are read once.
+// WR waves per row, 4 / WR rows per workgroup; rows of up to 2560 WR values are read once
+template <int WR>
 __global__ __launch_bounds__(Q8_NT) void k_quantize_i8(const uint16_t* __restrict__ x, int8_t* __restrict__ qo,
-                                                       float* __restrict__ scale, int k) {
+                                                       float* __restrict__ scale, int rows, int k) {
+  constexpr int LANES = 64 * WR;
   __shared__ float red[Q8_NT / FL_WAVE];
-  const int tid = threadIdx.x, nc = k >> 3;
-  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x % LANES, nc = k >> 3;
+  const int64_t row = (int64_t)blockIdx.x * (Q8_NT / LANES) + threadIdx.x / LANES;
+  if (WR < 4 && row >= rows) return;
   const uint4* xr = reinterpret_cast<const uint4*>(x + row * k);
   uint4 v[Q8_KEEP];
   // the largest magnitude as its bf16 bits: a NaN's are above an infinity's, and both win
@@ -67,28 +79,50 @@ __global__ __launch_bounds__(Q8_NT) void k_quantize_i8(const uint16_t* __restric
   };
 #pragma unroll
   for (int i = 0; i < Q8_KEEP; ++i) {
-    const int c = tid + i * Q8_NT;
+    const int c = tid + i * LANES;
     v[i] = c < nc ? xr[c] : make_uint4(0, 0, 0, 0);
-    look(v[i]);
   }
-  for (int c = tid + Q8_KEEP * Q8_NT; c < nc; c += Q8_NT) look(xr[c]);
+#pragma unroll
+  for (int i = 0; i < Q8_KEEP; ++i) look(v[i]);
+  for (int c = tid + Q8_KEEP * LANES; c < nc; c += LANES) look(xr[c]);
   // integers below 2^15 are exact floats, and larger ones stay larger
-  const float wm = wave_max((float)mx);
-  if ((tid & 63) == 0) red[tid >> 6] = wm;
-  __syncthreads();
-  const uint32_t m = (uint32_t)fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const Q8Row r = q8_row(bf2f(m));
+  float am = wave_max((float)mx);
+  if constexpr (WR > 1) {
+    if ((tid & 63) == 0) red[threadIdx.x >> 6] = am;
+    __syncthreads();
+    am = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    static_assert(WR == 4, "all waves on one row");
+  }
+  const Q8Row r = q8_row(bf2f((uint32_t)am));
   if (tid == 0) scale[row] = r.s;
   uint2* qr = reinterpret_cast<uint2*>(qo + row * k);
 #pragma unroll
   for (int i = 0; i < Q8_KEEP; ++i) {
-    const int c = tid + i * Q8_NT;
+    const int c = tid + i * LANES;
     if (c < nc) qr[c] = q8_pack(v[i], r);
   }
-  for (int c = tid + Q8_KEEP * Q8_NT; c < nc; c += Q8_NT) qr[c] = q8_pack(xr[c], r);
+  for (int c = tid + Q8_KEEP * LANES; c < nc; c += LANES) qr[c] = q8_pack(xr[c], r);
 }
 
 // ---- the product ----------------------------------------------------------------------------------
+
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+
+// buf_rsrc's four words
+__device__ __forceinline__ i8_u32x4 buffer_words(const void* base, uint32_t bytes) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(base);
+  return i8_u32x4{(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, bytes, 0x00020000u};
+}
+// 64 lanes x 16 bytes from the buffer at voff + soff into LDS from `at` on, in lane order. In asm: the builtin's LDS
+// write would make the compiler wait for every load in flight before it reads any LDS. No register waits for it.
+__device__ __forceinline__ void dma_1k(i8_u32x4 rsrc, uint32_t at, uint32_t voff, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :: "s"(at), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // until at most N of this wave's loads are in flight
+  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
 
 template <bool F32>
 __device__ __forceinline__ void i8_store(void* y, int64_t at, int acc, float s) {
@@ -107,14 +141,11 @@ __device__ __forceinline__ void i8_store(void* y, int64_t at, int acc, float s) 
 // rows. QUANT: x is bf16 and the workgroup quantises the rows for itself into LDS, behind its first weight loads.
 constexpr int FEW_KW = 8;
 constexpr int QF_MOST = 16384, QF_KEEP = 8;  // values that a workgroup quantises; 8-value pieces of a lane
-__host__ __device__ inline int qf_slots(int m) {
-  int slots = 1;
-  while (slots < m && slots < FEW_KW) slots *= 2;
-  return slots;
-}
+// log2 of the waves of a row, so that the eight hold as many rows at once as there are (all eight one row at most)
+__host__ __device__ inline int qf_log_waves(int m) { return m > 4 ? 0 : m > 2 ? 1 : m > 1 ? 2 : 3; }
 // whether the waves hold the rows in QF_KEEP pieces a lane
 inline bool qf_fits(int m, int k) {
-  const int slots = qf_slots(m), w = 64 * (FEW_KW / slots);
+  const int lw = qf_log_waves(m), slots = FEW_KW >> lw, w = 64 << lw;
   return m <= 16 && m * (int64_t)k <= QF_MOST && (m + slots - 1) / slots * ((k / 8 + w - 1) / w) <= QF_KEEP;
 }
 __host__ __device__ inline int few_pitch(int k) { return ((k + 63) >> 6) * 64 + 16; }  // of x rows in LDS: r and r + 8 on the same banks
@@ -167,20 +198,35 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
   };
   i8_x4 acc[MB];
   Set A, B;
-  int b = blockIdx.x;
-  load(b, 0, A);
+  int b = blockIdx.x, t = 0;
+  // (block, turn) pairs in order
+  auto next = [&](int& nb, int& nt) {
+    nt = t + 1, nb = b;
+    if (nt == turns) nt = 0, nb = b + (int)gridDim.x;
+  };
   if constexpr (XKB > 0 && !QUANT) {  // a row per wave; beyond k of the last step: what LDS holds, times zeros
-    const uint4* xb = static_cast<const uint4*>(a.x);
+    const uint32_t at = (uint32_t)(uintptr_t)(lds_byte*)xl;
+    const i8_u32x4 xv = buffer_words(a.x, (uint32_t)m * (uint32_t)k);
     for (int i = wave; i < m; i += KW)
-      for (int p = lane; p < (k >> 4); p += 64) *reinterpret_cast<uint4*>(xl + i * pitch + p * 16) = xb[(int64_t)i * (k >> 4) + p];
-    __syncthreads();
+      for (int p = 0; p < k; p += 1024)
+        if (p + lane * 16 < k) dma_1k(xv, at + (uint32_t)(i * pitch + p), (uint32_t)(lane * 16), (uint32_t)(i * k + p));
+  }
+  load(b, 0, A);
+  if constexpr (XKB > 0) {
+    int nb, nt;
+    next(nb, nt);
+    load(nb, nt, B);
+    if constexpr (!QUANT) {
+      wait_loads<2 * U>();  // x is here; the weights, requested after it, need not be
+      __syncthreads();
+    }
   }
   if constexpr (QUANT) {
     // Waves in `slots` groups of W: a group takes rows slot, slot + slots, ..., its waves 64 W pieces of 8 values at a
     // time; the pieces (QF_KEEP a lane at most, by the rule of who comes here) stay in registers between the maximum
     // and the quotients.
-    const int slots = qf_slots(m), W = KW / slots, slot = wave / W, sub = wave % W;
-    const int nc = k >> 3, cpr = (nc + 64 * W - 1) / (64 * W);
+    const int lw = qf_log_waves(m), W = 1 << lw, slots = KW >> lw, slot = wave >> lw, sub = wave & (W - 1);
+    const int nc = k >> 3, cpr = (nc + 64 * W - 1) >> (6 + lw);
     const uint4* xb = static_cast<const uint4*>(a.x);
     uint4 v[QF_KEEP];
     int qr = slot, j = 0;  // of piece i
@@ -213,9 +259,7 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
       const int ch = (j * W + sub) * 64 + lane;
       if (qr < m) {
         if (j == 0) {
-          float am = most[qr][0];
-          for (int p = 1; p < W; ++p) am = fmaxf(am, most[qr][p]);
-          q = q8_row(bf2f((uint32_t)am));
+          q = q8_row(bf2f((uint32_t)wave_max(most[qr][lane & (W - 1)])));
           if (lane == 0) sx[qr] = q.s;
         }
         if (ch < nc) *reinterpret_cast<uint2*>(xl + qr * pitch + ch * 8) = q8_pack(v[i], q);
@@ -258,12 +302,6 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
     }
     if (XKB) buf ^= 1;
   };
-  // (block, turn) pairs in order, the next pair's loads in flight during one
-  int t = 0;
-  auto next = [&](int& nb, int& nt) {
-    nt = t + 1, nb = b;
-    if (nt == turns) nt = 0, nb = b + (int)gridDim.x;
-  };
   if constexpr (XKB == 0) {
     for (; t < turns; ++t) {
       turn(t, A);
@@ -271,17 +309,19 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
     }
     return;
   }
-  while (b < blocks) {
+  // the loads of the two pairs after the one at work are in flight
+  auto go = [&](Set& v) {
+    turn(t, v);
     int nb, nt;
     next(nb, nt);
-    load(nb, nt, B);
-    turn(t, A);
     b = nb, t = nt;
-    if (b >= blocks) break;
     next(nb, nt);
-    load(nb, nt, A);
-    turn(t, B);
-    b = nb, t = nt;
+    load(nb, nt, v);
+  };
+  while (b < blocks) {
+    go(A);
+    if (b >= blocks) break;
+    go(B);
   }
 }
 
@@ -295,23 +335,8 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
 // rows 8 (i / 4) + 4 h + i % 4.
 
 typedef int i8_x16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) unsigned char lds_byte;
-
-// buf_rsrc's four words
-__device__ __forceinline__ i8_u32x4 buffer_words(const void* base, uint32_t bytes) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(base);
-  return i8_u32x4{(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, bytes, 0x00020000u};
-}
-// 64 lanes x 16 bytes from the buffer at voff + soff into LDS from `at` on, in lane order. In asm: the builtin's LDS
-// write would make the compiler wait for every load in flight before it reads any LDS. No register waits for it.
-__device__ __forceinline__ void dma_1k(i8_u32x4 rsrc, uint32_t at, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :: "s"(at), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void wait_loads() {  // until at most N of this wave's loads are in flight
-  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
-}
+typedef int i8_out32 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t i8_out16 __attribute__((ext_vector_type(4), aligned(2)));
 
 struct I8Tile {
   const int8_t *xq, *wq;
@@ -443,19 +468,20 @@ __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k
   // out through LDS, so that a wave stores whole lines
   __syncthreads();
   constexpr int V = OUT == 0 ? 8 : 4;  // values of a lane's store
-  const bool wide = (a.n % V) == 0;
   auto put = [&](const int* v, int mm, int nn, float sx, const float* sw) {  // V sums of x row mm from weight row nn on
     const int64_t at = ((int64_t)split * a.m + mm) * a.n + nn;
     float o[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) o[e] = OUT == 2 ? 0.0f : (float)v[e] * (sx * sw[e]);
-    if (wide && nn < a.n) {
-      if (OUT == 2) *reinterpret_cast<i8_x4*>(static_cast<int*>(a.y) + at) = i8_x4{v[0], v[1], v[2], v[3]};
-      else if (OUT == 1) *reinterpret_cast<float4*>(static_cast<float*>(a.y) + at) = make_float4(o[0], o[1], o[2], o[3]);
+    if (nn + V <= a.n) {  // 16 bytes, aligned to the type only where n is odd
+      if (OUT == 2) *reinterpret_cast<i8_out32*>(static_cast<int*>(a.y) + at) = i8_out32{v[0], v[1], v[2], v[3]};
+      else if (OUT == 1)
+        *reinterpret_cast<i8_out32*>(static_cast<float*>(a.y) + at) =
+            i8_out32{__float_as_int(o[0]), __float_as_int(o[1]), __float_as_int(o[2]), __float_as_int(o[3])};
       else
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + at) =
-            make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4 % V], o[5 % V]),
-                       pack_bf16x2(o[6 % V], o[7 % V]));
+        *reinterpret_cast<i8_out16*>(static_cast<uint16_t*>(a.y) + at) =
+            i8_out16{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4 % V], o[5 % V]),
+                     pack_bf16x2(o[6 % V], o[7 % V])};
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -543,20 +569,42 @@ __global__ __launch_bounds__(256) void k_i8_join(const int* __restrict__ part, i
 }
 
 // How a product is cut
+enum I8Kind { I8_FEW, I8_T64, I8_T128, I8_T256 };
 struct I8Plan {
-  int kind;        // 0: k_i8_rows; else the tile: 1: 256 x 256, 2: 128 x 128, 3: 64 x 64
-  int mblk, nblk, splits, sps;
+  I8Kind kind;
+  int mblk, nblk, splits, sps;  // of tiles
 };
+
+// Whether x of up to 32 rows goes through k_i8_few. It reads x once per 16 weight rows (from LDS where a workgroup takes
+// several blocks, n >= 8192), tiles once per 64, but a tile has less in flight: us, few and tiles of 64,
+// - 8 / 16 / 32 rows x 2560 x 2560 4.1 / 4.4 / 5.5 and 6.8 / 6.9 / 7.1; x 2560 x 8192 7.6 / 9.9 / 13.7 and 10.2 / 10.2 / 10.6; 16
+//   x 5003 x 8192 17.9 and 14.7;
+// - 32 rows x 16384 x 2560 11.8 and 10.9, 8 rows 9.8 and 10.3; x 49152 x 2560, weights from HBM, 30 and 37, 27 and 34;
+// - short rows, whose K is too little for eight waves: 16 x 16384 x 512 6.1 and 4.7.
+bool i8_few_rows(int m, int n, int k) {
+  if (m > 32 || (int64_t)m * k >= 131072 || (k <= 1024 && n >= 8192)) return false;
+  if (m <= 16) return true;
+  return n < 8192 ? n <= 4096 && k < 4096 : n >= 32768 && m * few_pitch(k) <= 112 << 10;
+}
+
 I8Plan i8_plan(int m, int n, int k) {
-  I8Plan p{0, 0, 0, 1, 0};
+  I8Plan p{I8_FEW, 0, 0, 1, 0};
+  if (i8_few_rows(m, n, k)) return p;
   const int steps = (k + 127) / 128;
   auto tiles = [&](int b) { return (int64_t)((m + b - 1) / b) * ((n + b - 1) / b); };
-  if (m <= 32) return p;
-  p.kind = tiles(256) >= 192 ? 1 : tiles(128) >= 160 ? 2 : 3;
-  const int b = p.kind == 1 ? 256 : p.kind == 2 ? 128 : 64;
+  // us of a round of 256 tiles: its start and end and each step, as measured over m 33..2048, n 512..16384 and k 512..8192
+  // (252 products: 1% over the best kind for each in the mean, 30% at most)
+  auto rounds = [&](int b, double ends, double step) { return (double)((tiles(b) + 255) / 256) * (ends + step * steps); };
+  double t64 = rounds(64, 1.0, 0.19);
+  const double t128 = rounds(128, 2.0, 0.48), t256 = rounds(256, 4.0, 1.4);
+  // few tiles: K in parts of twelve steps at least, 2.5 us to join them (64 x 2560 x 8192: 11.0 in five parts, 17 in one)
+  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 12, 256 / tiles(64)));
+  if (parts > 1) t64 = 3.5 + 0.19 * steps / parts;
+  p.kind = t64 <= t128 && t64 <= t256 ? I8_T64 : t128 <= t256 ? I8_T128 : I8_T256;
+  const int b = p.kind == I8_T256 ? 256 : p.kind == I8_T128 ? 128 : 64;
   p.mblk = (m + b - 1) / b;
   p.nblk = (n + b - 1) / b;
-  if (p.kind == 3) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 8, 256 / tiles(64)));
+  p.splits = p.kind == I8_T64 ? parts : 1;
   p.sps = (steps + p.splits - 1) / p.splits;
   p.splits = (steps + p.sps - 1) / p.sps;
   return p;
@@ -572,7 +620,7 @@ void i8_few(const I8Few& a, int per_cu, bool f32, hipStream_t s) {
 
 template <int T, int KW, int WM, int WN, int NR, int Q>
 void i8_tiles(const I8Tile& a, bool f32, hipStream_t s) {
-  const unsigned grid = 8u * (unsigned)((a.mblk * a.nblk * a.splits + 7) / 8);
+  const unsigned grid = 8u * (unsigned)(((int64_t)a.mblk * a.nblk * a.splits + 7) / 8);
   const dim3 nt(64 * KW * WM * WN);
   if (a.splits > 1) hipLaunchKernelGGL((k_i8_tile<T, KW, WM, WN, NR, Q, 2>), dim3(grid), nt, 0, s, a);
   else if (f32) hipLaunchKernelGGL((k_i8_tile<T, KW, WM, WN, NR, Q, 1>), dim3(grid), nt, 0, s, a);
@@ -582,7 +630,10 @@ void i8_tiles(const I8Tile& a, bool f32, hipStream_t s) {
 }  // namespace
 
 int i8_quantize(const uint16_t* x, int8_t* q, float* scale, int32_t rows, int32_t k, hipStream_t s) {
-  hipLaunchKernelGGL(k_quantize_i8, dim3(rows), dim3(Q8_NT), 0, s, x, q, scale, k);
+  // us, wave per row and workgroup per row: 32 x 2560 3.5 and 3.0, 1024 x 2560 3.9 and 4.0, 2048 x 2560 5.3 and 5.8; 1024 x
+  // 8192, which a wave reads twice, 12.0 and 7.5
+  if (rows >= 1024 && k <= 64 * 8 * Q8_KEEP) hipLaunchKernelGGL(k_quantize_i8<1>, dim3((rows + 3) / 4), dim3(Q8_NT), 0, s, x, q, scale, rows, k);
+  else hipLaunchKernelGGL(k_quantize_i8<4>, dim3(rows), dim3(Q8_NT), 0, s, x, q, scale, rows, k);
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
 }
 
@@ -594,20 +645,18 @@ int64_t i8_gemm_bytes(int32_t m, int32_t n, int32_t k) {
 int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, void* y, bool y_fp32, void* work,
             int32_t m, int32_t n, int32_t k, hipStream_t s) {
   const I8Plan p = i8_plan(m, n, k);
-  if (p.kind == 0) {
+  if (p.kind == I8_FEW) {
     const I8Few a{xq, xs, wq, ws, y, m, n, k};
-    const int64_t lds = (int64_t)m * few_pitch(k);
+    const int lds = m * few_pitch(k);
     if (n < 8192) m <= 16 ? i8_few<1, 0, false>(a, 0, y_fp32, s) : i8_few<2, 0, false>(a, 0, y_fp32, s);
-    else if (m <= 16 && lds <= 48 << 10) i8_few<1, 48, false>(a, 2, y_fp32, s);
-    else if (m <= 16 && lds <= 132 << 10) i8_few<1, 132, false>(a, 1, y_fp32, s);
-    else if (m <= 16) i8_few<1, 0, false>(a, 0, y_fp32, s);
-    else if (lds <= 112 << 10) i8_few<2, 112, false>(a, 1, y_fp32, s);
-    else i8_few<2, 0, false>(a, 0, y_fp32, s);
+    else if (m > 16) i8_few<2, 112, false>(a, 1, y_fp32, s);
+    else if (lds <= 48 << 10) i8_few<1, 48, false>(a, 2, y_fp32, s);
+    else i8_few<1, 132, false>(a, 1, y_fp32, s);
   } else {
     const I8Tile a{xq, wq, xs, ws, p.splits > 1 ? work : y, m, n, k, p.mblk, p.nblk, p.splits, p.sps};
-    const bool one = p.mblk * p.nblk * p.splits <= 256;  // a CU holds one workgroup: it may have all of its LDS
-    if (p.kind == 1) i8_tiles<256, 1, 2, 4, 5, 1>(a, y_fp32, s);
-    else if (p.kind == 2) one ? i8_tiles<128, 1, 2, 4, 8, 1>(a, y_fp32, s) : i8_tiles<128, 1, 2, 2, 4, 1>(a, y_fp32, s);
+    const bool one = (int64_t)p.mblk * p.nblk * p.splits <= 256;  // a CU holds one workgroup: it may have all of its LDS
+    if (p.kind == I8_T256) i8_tiles<256, 1, 2, 4, 5, 1>(a, y_fp32, s);
+    else if (p.kind == I8_T128) one ? i8_tiles<128, 1, 2, 4, 8, 1>(a, y_fp32, s) : i8_tiles<128, 1, 2, 2, 4, 1>(a, y_fp32, s);
     else one ? i8_tiles<64, 4, 1, 1, 4, 1>(a, y_fp32, s) : i8_tiles<64, 1, 2, 2, 8, 1>(a, y_fp32, s);
     if (p.splits > 1) {
       const dim3 grid((unsigned)(((int64_t)m * n + 1023) / 1024));

@@ -385,15 +385,16 @@ int lp_run(LpArgs a, bool bf16, int rows, void* work, hipStream_t s) {
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
 }
 
-// Features -> log probabilities: blocks of rows through the 8-bit head, whose fp32 logits stay in the workspace (up to
-// 128 MB of them, half of what the last-level cache holds).
+// Features -> log probabilities: blocks of rows through the 8-bit head, whose fp32 logits stay in the workspace, up to
+// 256 MB of them. 1024 rows of 49152 in one block are three whole rounds of 256 x 256 tiles, 512 one and a half, which
+// take two: 199 us in one block, 248 in two, though the last-level cache holds the logits of the smaller ones.
 struct HeadPlan {
   int rows;  // of a block
   int64_t logits, linear, lp, bytes;
 };
 HeadPlan head_plan(int m, int n, int k, int top) {
   HeadPlan p{};
-  const int64_t fit = std::max<int64_t>(1, (128ll << 20) / ((int64_t)n * 4));
+  const int64_t fit = std::max<int64_t>(1, (256ll << 20) / ((int64_t)n * 4));
   p.rows = (int)std::min<int64_t>(m, fit >= 256 ? fit / 256 * 256 : fit);
   LpArgs a{};
   a.vocab = n;

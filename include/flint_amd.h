@@ -175,7 +175,7 @@ int fl_logprobs(const void* logits, int32_t bf16, int64_t stride, int32_t rows, 
                 int32_t top, float* logprob, float* entropy, int32_t* rank, int32_t* top_ids, float* top_logprobs,
                 void* work, void* stream);
 /* The same from features x (bf16 [M, K]) through an 8-bit vocabulary head wq [N, K], ws [N]: fl_linear_int8's product in
- * fp32 and fl_logprobs of it, without M x N logits in memory at once (up to 128 MB of them in work). Limits of both. A
+ * fp32 and fl_logprobs of it, without M x N logits in memory at once (up to 256 MB of them in work, or one row's). Limits of both. A
  * row's logits, ranks and top_ids do not depend on the other rows; the order of its fp32 sums does. */
 int fl_head_logprobs_workspace(int32_t m, int32_t n, int32_t k, int32_t top, int64_t* bytes);
 int fl_head_logprobs(const uint16_t* x, const int8_t* wq, const float* ws, const int32_t* tokens, int32_t top,
