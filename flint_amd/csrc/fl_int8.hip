@@ -668,6 +668,7 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
 }
 
 int64_t i8_linear_bytes(int32_t m, int32_t n, int32_t k) {
+  if (qf_fits(m, k)) return 0;
   return i8_pad((int64_t)m * k) + i8_pad((int64_t)m * 4) + i8_gemm_bytes(m, n, k);
 }
 
@@ -713,7 +714,8 @@ int fl_linear_int8_workspace(int32_t m, int32_t n, int32_t k, int64_t* bytes) {
 
 int fl_linear_int8(const uint16_t* x, const int8_t* wq, const float* ws, void* y, int32_t y_fp32, void* work,
                    int32_t m, int32_t n, int32_t k, void* stream) {
-  if (!i8_shape_ok(m, n, k) || !i8_aligned(x) || !i8_aligned(wq) || !ws || !i8_aligned(y) || !i8_aligned(work))
+  if (!i8_shape_ok(m, n, k) || !i8_aligned(x) || !i8_aligned(wq) || !ws || !i8_aligned(y) ||
+      (i8_linear_bytes(m, n, k) > 0 && !i8_aligned(work)))
     return FL_E_ARG;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return i8_linear(x, wq, ws, y, y_fp32 != 0, work, m, n, k, s);

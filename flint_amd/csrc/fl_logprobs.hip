@@ -23,9 +23,9 @@ constexpr int LP_E = 16;                // values of a thread in a step
 constexpr int LP_STEP = LP_NT * LP_E;   // of a workgroup
 constexpr int LP_TOP = 32;     // alternatives at most
 constexpr int LP_CHUNKS = 32;  // of a row at most
-constexpr int LP_CAP = 1024;   // candidates kept in LDS
+constexpr int LP_KEEP = 256;   // candidates that a wave keeps in LDS
 constexpr int LP_MAXV = 1 << 20;
-static_assert(LP_CHUNKS * LP_TOP <= LP_CAP, "a merge's candidates always fit");
+static_assert(LP_CHUNKS * LP_TOP <= LP_NW * LP_KEEP, "a merge's candidates always fit");
 
 // Keys that order as the values do, as unsigned numbers (NaN, made positive, above +inf), with the index below
 // them: all keys of a row differ, and none is 0.
@@ -57,10 +57,11 @@ struct LpArgs {
 };
 
 struct LpShared {
-  float red[5][LP_NW];
-  int count;
+  uint32_t bound[LP_NW];
+  float red[4][LP_NW];
+  int kept[LP_NW];  // candidates of each wave
   int place[LP_NW][FL_WAVE];
-  u64 cand[LP_CAP], first[LP_TOP];
+  u64 cand[LP_NW][LP_KEEP], first[LP_TOP];
 };
 
 // the row's token and its logit; in = false (no token asked for, or an id outside the vocabulary): NaN
@@ -81,47 +82,72 @@ __device__ __forceinline__ LpToken lp_token(const LpArgs& a, int64_t row) {
   return k;
 }
 
-// The first `top` of the sh.count (<= LP_CAP) keys in sh.cand, in order, into sh.first: a key's place is the number of
-// larger ones. Lanes take candidates, each wave counts over its share of them.
+// The first `top` of the waves' candidates (sh.kept of them each, <= LP_KEEP), in order, into sh.first: a key's place is
+// the number of larger ones. Lanes take candidates, each wave counts over its own.
 __device__ __forceinline__ void lp_sort(LpShared& sh, int top) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = sh.count;
-  const int share = (c + LP_NW - 1) / LP_NW, c0 = min(c, wave * share), c1 = min(c, c0 + share);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mine = sh.kept[wave];
   if (tid < top) sh.first[tid] = 0;
+  int n[LP_NW], c = 0;
+#pragma unroll
+  for (int w = 0; w < LP_NW; ++w) c += n[w] = sh.kept[w];
   for (int b = 0; b < c; b += FL_WAVE) {
-    const u64 key = b + lane < c ? sh.cand[b + lane] : 0;
+    int i = b + lane, w = 0;
+#pragma unroll
+    for (int v = 0; v < LP_NW - 1; ++v)
+      if (w == v && i >= n[v]) i -= n[v], ++w;
+    const u64 key = b + lane < c ? sh.cand[w][i] : 0;
     int larger = 0;
 #pragma unroll 4
-    for (int j = c0; j < c1; ++j) larger += sh.cand[j] > key;
+    for (int j = 0; j < mine; ++j) larger += sh.cand[wave][j] > key;
     sh.place[wave][lane] = larger;
     __syncthreads();
     if (wave == 0 && key != 0) {
       int at = 0;
 #pragma unroll
-      for (int w = 0; w < LP_NW; ++w) at += sh.place[w][lane];
+      for (int v = 0; v < LP_NW; ++v) at += sh.place[v][lane];
       if (at < top) sh.first[at] = key;
     }
     __syncthreads();
   }
-  __syncthreads();
+  if (c == 0) __syncthreads();
 }
 
 // A value that at least LP_NW q of the workgroup's values reach, if all lanes hold one: the smallest over the waves of
-// the q-th largest in the wave, stored for others to read at any time (rising values only make it rise)
-__device__ __forceinline__ void lp_publish(float* red, float mine, int q) {
-  const int lane = threadIdx.x & 63;
-  float w = -INFINITY;
-  for (int r = 0; r < q; ++r) {
-    w = wave_max(mine);
-    if (lane == __builtin_ctzll(__ballot(mine == w) | (1ull << 63))) mine = -INFINITY;
-  }
-  if (lane == 0) __hip_atomic_store(red + (threadIdx.x >> 6), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+// the q-th largest in the wave, stored for others to read at any time (rising values only make it rise). On ordered
+// whole numbers, whose maximum is one DPP instruction a step.
+__device__ __forceinline__ uint32_t lp_ord(float x) {  // not of NaN
+  const uint32_t b = __float_as_uint(x + 0.0f);         // -0 becomes 0
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float lp_least(float* red, int waves) {
-  float t = waves > 0 ? INFINITY : -INFINITY;
+__device__ __forceinline__ float lp_unord(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+template <int CTRL>
+__device__ __forceinline__ uint32_t umax_dpp(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_umax32(uint32_t v) {
+  v = umax_dpp<0xB1>(v);   // lane ^ 1
+  v = umax_dpp<0x4E>(v);   // lane ^ 2
+  v = umax_dpp<0x141>(v);  // the other four of 8
+  v = umax_dpp<0x140>(v);  // the other eight of 16
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(r[0], r[1]);
+  const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(q[0], q[1]);
+}
+__device__ __forceinline__ void lp_publish(uint32_t* red, float mine, int q) {
+  uint32_t v = mine == mine ? lp_ord(mine) : 0u, w = lp_ord(-INFINITY);
+  for (int r = 0; r < q; ++r) {
+    w = wave_umax32(v);
+    if ((threadIdx.x & 63) == __builtin_ctzll(__ballot(v == w) | (1ull << 63))) v = 0;
+  }
+  if ((threadIdx.x & 63) == 0) __hip_atomic_store(red + (threadIdx.x >> 6), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+__device__ __forceinline__ float lp_least(uint32_t* red, int waves) {
+  uint32_t t = waves > 0 ? ~0u : lp_ord(-INFINITY);
 #pragma unroll
   for (int k = 0; k < LP_NW; ++k)
-    if (k < waves) t = fminf(t, __hip_atomic_load(red + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
-  return t;
+    if (k < waves) t = min(t, __hip_atomic_load(red + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+  return t <= lp_ord(-INFINITY) ? -INFINITY : lp_unord(t);
 }
 
 // what the whole row says, from its maximum, sums and rank count, and sh.first
@@ -176,38 +202,44 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
   const int j0 = chunk * a.per, j1 = min(a.vocab, j0 + a.per);
   const float* lf = reinterpret_cast<const float*>(a.logits) + row * a.stride;
   const uint16_t* lh = reinterpret_cast<const uint16_t*>(a.logits) + row * a.stride;
-  auto load = [&](int jb, float (&x)[LP_E]) {
-    if (jb + LP_STEP <= j1) {
+  constexpr uint32_t NINF = BF16 ? 0xFF80FF80u : 0xFF800000u;
+  // kept as loaded until used: anything done to a value here would wait for it
+  auto load = [&](int jb, raw4 (&x)[LP_E / V]) {
 #pragma unroll
-      for (int i = 0; i < LP_E / V; ++i) {
-        const int j = jb + (i * LP_NT + tid) * V;
-        const raw4 w = *reinterpret_cast<const raw4*>(BF16 ? (const void*)(lh + j) : (const void*)(lf + j));
+    for (int i = 0; i < LP_E / V; ++i) {
+      const int j = jb + (i * LP_NT + tid) * V;
+      x[i] = raw4{NINF, NINF, NINF, NINF};
+      if (jb + (i + 1) * LP_NT * V <= j1 || j + V <= j1)
+        x[i] = *reinterpret_cast<const raw4*>(BF16 ? (const void*)(lh + j) : (const void*)(lf + j));
+      else if (j < j1) {  // the one lane where the row ends inside 16 bytes
+        uint32_t v[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-          x[i * V + k] = !BF16 ? __uint_as_float(w[k & 3]) : k & 1 ? bfhi(w[(k / 2) & 3]) : bflo(w[(k / 2) & 3]);
-      }
-    } else {
+        for (int k = 0; k < V; ++k) v[k] = BF16 ? lh[min(j + k, j1 - 1)] : __float_as_uint(lf[min(j + k, j1 - 1)]);
 #pragma unroll
-      for (int e = 0; e < LP_E; ++e) {
-        const int j = jb + ((e / V) * LP_NT + tid) * V + e % V;
-        x[e] = j < j1 ? (BF16 ? bf2f(lh[j]) : lf[j]) : -INFINITY;
+        for (int k = 0; k < V; ++k) v[k] = j + k < j1 ? v[k] : NINF & (BF16 ? 0xFFFFu : ~0u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[i][k] = BF16 ? v[(2 * k) % V] | v[(2 * k + 1) % V] << 16 : v[k % V];
       }
     }
   };
-  float x[LP_E];
-  load(j0, x);
+  raw4 cur[LP_E / V];
+  load(j0, cur);
   const LpToken tok = lp_token<BF16>(a, row);
   // Candidates for the first `top` places: of each of the waves whose lanes all hold values, the q-th largest of
   // its lanes' maxima so far; at least `top` values of the chunk reach the smallest of these, T, and few others do. T
   // only rises, so what is collected with an earlier T is too much at worst.
   const int full = min(LP_NW, (j1 - j0) / (FL_WAVE * V)), q = full > 0 ? (a.top + full - 1) / full : 0;
-  if (tid == 0) sh.count = 0;
-  if (lane == 0) sh.red[0][wave] = -INFINITY;
   float m = -INFINITY, s = 0.0f, u = 0.0f, T = -INFINITY;
-  int before = 0, i = 0;  // `before` of the wave
+  int before = 0, kept = 0, i = 0;  // `before` and kept: of the wave
   for (int jb = j0; jb < j1; jb += LP_STEP, ++i) {
-    float y[LP_E];
-    if (jb + LP_STEP < j1) load(jb + LP_STEP, y);
+    raw4 ahead[LP_E / V];
+    if (jb + LP_STEP < j1) load(jb + LP_STEP, ahead);
+    float x[LP_E];
+#pragma unroll
+    for (int e = 0; e < LP_E; ++e) {
+      const uint32_t w = cur[e / V][(BF16 ? e / 2 : e) & 3];
+      x[e] = !BF16 ? __uint_as_float(w) : e & 1 ? bfhi(w) : bflo(w);
+    }
     float top = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), x[5], x[6]);  // NaN is passed over; it comes back through s
     top = max3(max3(max3(max3(top, x[7], x[8]), x[9], x[10]), x[11], x[12]), x[13], x[14]);
     top = max3(top, x[15], x[15]);
@@ -225,7 +257,31 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
       u = __builtin_fmaf(p, fmaxf(d, -1000.0f), u);  // 0 times -1000 for masked values
     }
     const int jt = jb + tid * V;  // e's index: jt + (e / V) * LP_NT * V + e % V
-    if (tok.in) {
+    if (a.top > 0) {
+      if ((i & (i + 1)) == 0) {  // steps 0, 1, 3, 7, ...
+        lp_publish(sh.bound, m, q);
+        if (i == 0) __syncthreads();
+        T = lp_least(sh.bound, full);
+      }
+      auto take = [&](bool is, float v, int j) {
+        const u64 lanes = __ballot(is);
+        if (lanes == 0) return;
+        const int at = kept + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+        if (is && at < LP_KEEP) sh.cand[wave][at] = lp_key(v, j);
+        kept += __builtin_popcountll(lanes);
+      };
+      if (T == -INFINITY) {  // all that is larger, and the chunk's first values by index
+#pragma unroll
+        for (int e = 0; e < LP_E; ++e) {
+          const int j = jt + (e / V) * LP_NT * V + e % V;
+          take(j < j1 && (!(x[e] <= T) || j < j0 + a.top), x[e], j);
+        }
+      } else if (__ballot(s != s || top >= T) != 0) {
+#pragma unroll
+        for (int e = 0; e < LP_E; ++e) take(!(x[e] < T), x[e], jt + (e / V) * LP_NT * V + e % V);
+      }
+    }
+    if (tok.in) {  // last: the token's logit comes from two loads in a row
       if (tok.l != tok.l || jb + LP_STEP > j1 || (tok.t >= jb && tok.t < jb + LP_STEP)) {
         const int tm = min(tok.t, j1) - jt;
 #pragma unroll
@@ -241,44 +297,25 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
         for (int e = 0; e < LP_E; ++e) before += lp_count(!(x[e] < tok.l));
       }
     }
-    if (a.top > 0) {
-      if ((i & (i + 1)) == 0) {  // steps 0, 1, 3, 7, ...
-        lp_publish(sh.red[0], m, q);
-        if (i == 0) __syncthreads();
-        T = lp_least(sh.red[0], full);
-      }
-      auto take = [&](float v, int j) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < LP_CAP) sh.cand[at] = lp_key(v, j);
-      };
-      if (T == -INFINITY) {  // all that is larger, and the chunk's first values by index
 #pragma unroll
-        for (int e = 0; e < LP_E; ++e) {
-          const int j = jt + (e / V) * LP_NT * V + e % V;
-          if (j < j1 && (!(x[e] <= T) || j < j0 + a.top)) take(x[e], j);
-        }
-      } else if (s != s || top >= T) {
-#pragma unroll
-        for (int e = 0; e < LP_E; ++e)
-          if (!(x[e] < T)) take(x[e], jt + (e / V) * LP_NT * V + e % V);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < LP_E; ++e) x[e] = y[e];
+    for (int v = 0; v < LP_E / V; ++v) cur[v] = ahead[v];
   }
   lp_join(m, s, u);
-  if (lane == 0) sh.red[1][wave] = m, sh.red[2][wave] = s, sh.red[3][wave] = u, sh.red[4][wave] = (float)before;
+  if (lane == 0) sh.red[0][wave] = m, sh.red[1][wave] = s, sh.red[2][wave] = u, sh.red[3][wave] = (float)before, sh.kept[wave] = kept;
   __syncthreads();
   const bool one = lane < LP_NW;
-  m = one ? sh.red[1][lane % LP_NW] : -INFINITY;
-  s = one ? sh.red[2][lane % LP_NW] : 0.0f;
-  u = one ? sh.red[3][lane % LP_NW] : 0.0f;
+  m = one ? sh.red[0][lane % LP_NW] : -INFINITY;
+  s = one ? sh.red[1][lane % LP_NW] : 0.0f;
+  u = one ? sh.red[2][lane % LP_NW] : 0.0f;
   lp_join(m, s, u);
   before = 0;
 #pragma unroll
-  for (int w = 0; w < LP_NW; ++w) before += (int)sh.red[4][w];
+  for (int w = 0; w < LP_NW; ++w) before += (int)sh.red[3][w];
   if (a.top > 0) {
-    if (sh.count <= LP_CAP) {
+    int most = 0;
+#pragma unroll
+    for (int w = 0; w < LP_NW; ++w) most = max(most, sh.kept[w]);
+    if (most <= LP_KEEP) {
       lp_sort(sh, a.top);
     } else {  // a crowd of equal values: one after the other, from memory
       u64 last = ~0ull;
@@ -290,10 +327,10 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
         }
         best = wave_max_u64(best);
         __syncthreads();
-        if (lane == 0) sh.cand[wave] = best;
+        if (lane == 0) sh.cand[0][wave] = best;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < LP_NW; ++w) best = u64max(best, sh.cand[w]);
+        for (int w = 0; w < LP_NW; ++w) best = u64max(best, sh.cand[0][w]);
         if (tid == 0) sh.first[r] = best;
         last = best;
       }
@@ -318,10 +355,10 @@ __global__ __launch_bounds__(LP_NT) void k_logprobs_merge(LpArgs a) {
   const u64* cand = a.cand + row * a.chunks * a.top;
   const bool one = lane < a.chunks;
   const float4 p = one ? a.part[row * a.chunks + lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-  u64 mine[LP_CAP / LP_NT], T = 0;
+  u64 mine[LP_KEEP / FL_WAVE], T = 0;
   if (a.top > 0) {
 #pragma unroll
-    for (int i = 0; i < LP_CAP / LP_NT; ++i) mine[i] = i * LP_NT + tid < a.chunks * a.top ? cand[i * LP_NT + tid] : 0;
+    for (int i = 0; i < LP_KEEP / FL_WAVE; ++i) mine[i] = i * LP_NT + tid < a.chunks * a.top ? cand[i * LP_NT + tid] : 0;
     if (one) T = cand[(lane + 1) * a.top - 1];
   }
   const LpToken tok = lp_token<BF16>(a, row);
@@ -329,28 +366,34 @@ __global__ __launch_bounds__(LP_NT) void k_logprobs_merge(LpArgs a) {
   lp_join(m, s, u);
   const int before = (int)wave_sum((float)__float_as_int(p.w));
   if (a.top > 0) {
-    if (tid == 0) sh.count = 0;
     // at least `top` keys reach the largest of the chunks' last ones; and, as in a chunk, a value from the threads' largest
     T = wave_max_u64(T);
     u64 largest = 0;
 #pragma unroll
-    for (int i = 0; i < LP_CAP / LP_NT; ++i) largest = u64max(largest, mine[i]);
+    for (int i = 0; i < LP_KEEP / FL_WAVE; ++i) largest = u64max(largest, mine[i]);
     const int full = min(LP_NW, a.chunks * a.top / FL_WAVE), q = full > 0 ? (a.top + full - 1) / full : 0;
-    lp_publish(sh.red[0], largest != 0 ? lp_value(largest) : -INFINITY, q);
+    lp_publish(sh.bound, largest != 0 ? lp_value(largest) : -INFINITY, q);
     __syncthreads();
-    const float t = lp_least(sh.red[0], full);
+    const float t = lp_least(sh.bound, full);
+    int kept = 0;
 #pragma unroll
-    for (int i = 0; i < LP_CAP / LP_NT; ++i)
-      if (mine[i] != 0 && mine[i] >= T && !(lp_value(mine[i]) < t)) sh.cand[atomicAdd(&sh.count, 1)] = mine[i];
+    for (int i = 0; i < LP_KEEP / FL_WAVE; ++i) {
+      const bool is = mine[i] != 0 && mine[i] >= T && !(lp_value(mine[i]) < t);
+      const u64 lanes = __ballot(is);
+      const int at = kept + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+      if (is) sh.cand[tid >> 6][at] = mine[i];
+      kept += __builtin_popcountll(lanes);
+    }
+    if (lane == 0) sh.kept[tid >> 6] = kept;
     __syncthreads();
     lp_sort(sh, a.top);
   }
   lp_write(a, row, tok, m, s, u, before, sh);
 }
 
-// Chunks of a row: one, or as many as give 512 workgroups in all, of 2048 values at least.
+// Chunks of a row: one, or as many as give 1024 workgroups in all, of 4096 values (a step) at least.
 void lp_plan(LpArgs& a, int rows) {
-  a.chunks = std::max(1, std::min({LP_CHUNKS, a.vocab / 2048, 512 / rows}));
+  a.chunks = std::max(1, std::min({LP_CHUNKS, (a.vocab + LP_STEP - 1) / LP_STEP, 1024 / rows}));
   a.per = ((a.vocab + a.chunks - 1) / a.chunks + 7) / 8 * 8;
   a.chunks = (a.vocab + a.per - 1) / a.per;
 }

@@ -282,15 +282,30 @@ pybind11::object int8_fast(const torch::Tensor& x, const std::optional<torch::Te
   return pybind11::cast(y);
 }
 
-// Outputs of generate.logprobs and generate.head_logprobs, rows of them
+// A contiguous tensor over part of base's storage, without the dispatcher's view machinery (0.2 us instead of 0.7;
+// an allocation takes 1.3)
+torch::Tensor piece(const torch::Tensor& base, int64_t byte, torch::IntArrayRef sizes, torch::ScalarType dt) {
+  auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(dt));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  t.unsafeGetTensorImpl()->set_storage_offset(byte / (int64_t)c10::elementSize(dt));
+  return t;
+}
+
+// Outputs of generate.logprobs and generate.head_logprobs, rows of them, in one allocation
 struct LogprobOut {
   torch::Tensor logprob, entropy, rank, ids, top;
   void make(int64_t rows, int64_t n, bool tokens, const torch::Tensor& like) {
-    const auto f = like.options().dtype(torch::kFloat32).requires_grad(false);
-    const auto i = f.dtype(torch::kInt32);
-    if (tokens) logprob = torch::empty({rows}, f), rank = torch::empty({rows}, i);
-    entropy = torch::empty({rows}, f);
-    if (n > 0) ids = torch::empty({rows, n}, i), top = torch::empty({rows, n}, f);
+    const int64_t words = rows * ((tokens ? 3 : 1) + 2 * n);
+    const torch::Tensor all = bytes_of(4 * words, like);
+    int64_t at = 0;
+    auto next = [&](torch::IntArrayRef sizes, torch::ScalarType dt) {
+      torch::Tensor t = piece(all, at, sizes, dt);
+      at += 4 * t.numel();
+      return t;
+    };
+    entropy = next({rows}, torch::kFloat32);
+    if (tokens) logprob = next({rows}, torch::kFloat32), rank = next({rows}, torch::kInt32);
+    if (n > 0) ids = next({rows, n}, torch::kInt32), top = next({rows, n}, torch::kFloat32);
   }
   pybind11::object cast() const {
     auto one = [](const torch::Tensor& t) -> pybind11::object {

@@ -153,7 +153,7 @@ int fl_gemm_int8_workspace(int32_t m, int32_t n, int32_t k, int64_t* bytes);
 int fl_gemm_int8(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, void* y, int32_t y_fp32,
                  void* work, int32_t m, int32_t n, int32_t k, void* stream);
 /* The same from bf16 rows x [M, K] (16-byte aligned): fl_quantize_int8 of x, then the product. work as above, of
- * fl_linear_int8_workspace's bytes (never 0). */
+ * fl_linear_int8_workspace's bytes. */
 int fl_linear_int8_workspace(int32_t m, int32_t n, int32_t k, int64_t* bytes);
 int fl_linear_int8(const uint16_t* x, const int8_t* wq, const float* ws, void* y, int32_t y_fp32, void* work,
                    int32_t m, int32_t n, int32_t k, void* stream);

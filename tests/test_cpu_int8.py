@@ -46,7 +46,7 @@ def test_pointers_that_8_bit_rows_do_not_take(lib):
         for i in (0, 1, 3, 5):
             a = [P, P, P, P, 0, P]
             a[i] = bad
-            assert lib.fl_linear_int8(*a, 4, 64, 64, None) == -1
+            assert lib.fl_linear_int8(*a, 400, 64, 64, None) == -1
     for i in (1, 3):
         a = [P, P, P, P, P, 0, P]
         a[i] = None
