@@ -52,16 +52,19 @@ struct LpArgs {
   int32_t* rank;                // [rows]
   int32_t* top_ids;             // [rows, top]
   float* top_lp;                // [rows, top]
-  float4* part;                 // chunks > 1: per (row, chunk) maximum, s, u, rank count (its bits) ...
-  u64* cand;                    // ... and its first `top` keys, in order, then zeros
+  // chunks > 1: per (row, chunk) maximum, s, u, rank count (its bits) and the first `top` keys, in order, then zeros; per
+  // row the token's logit and whether there is one
+  float4* part;
+  u64* cand;
+  float2* given;
 };
 
 struct LpShared {
   uint32_t bound[LP_NW];
-  float red[4][LP_NW];
-  int kept[LP_NW];  // candidates of each wave
+  float4 red[LP_NW];  // maximum, s, u, rank count of each wave
+  int kept[LP_NW];    // candidates of each wave
   int place[LP_NW][FL_WAVE];
-  u64 cand[LP_NW][LP_KEEP], first[LP_TOP];
+  u64 cand[LP_NW][LP_KEEP];  // their keys
 };
 
 // the row's token and its logit; in = false (no token asked for, or an id outside the vocabulary): NaN
@@ -82,14 +85,17 @@ __device__ __forceinline__ LpToken lp_token(const LpArgs& a, int64_t row) {
   return k;
 }
 
-// The first `top` of the waves' candidates (sh.kept of them each, <= LP_KEEP), in order, into sh.first: a key's place is
-// the number of larger ones. Lanes take candidates, each wave counts over its own.
-__device__ __forceinline__ void lp_sort(LpShared& sh, int top) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, mine = sh.kept[wave];
-  if (tid < top) sh.first[tid] = 0;
+// The first `top` of the waves' candidates (sh.kept of them each, <= LP_KEEP; a barrier lies behind them), in order: out(
+// place, key) in wave 0, key 0 past the last. A key's place is the number of larger ones: lanes take candidates, each
+// wave counts over its own.
+template <class F>
+__device__ __forceinline__ void lp_sort(LpShared& sh, int top, F out) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int n[LP_NW], c = 0;
 #pragma unroll
   for (int w = 0; w < LP_NW; ++w) c += n[w] = sh.kept[w];
+  const int own = sh.kept[wave];
+  if (wave == 0 && lane >= c && lane < top) out(lane, (u64)0);
   for (int b = 0; b < c; b += FL_WAVE) {
     int i = b + lane, w = 0;
 #pragma unroll
@@ -97,29 +103,23 @@ __device__ __forceinline__ void lp_sort(LpShared& sh, int top) {
       if (w == v && i >= n[v]) i -= n[v], ++w;
     const u64 key = b + lane < c ? sh.cand[w][i] : 0;
     int larger = 0;
-#pragma unroll 4
-    for (int j = 0; j < mine; ++j) larger += sh.cand[wave][j] > key;
+#pragma unroll 8
+    for (int j = 0; j < own; ++j) larger += sh.cand[wave][j] > key;
     sh.place[wave][lane] = larger;
     __syncthreads();
     if (wave == 0 && key != 0) {
       int at = 0;
 #pragma unroll
       for (int v = 0; v < LP_NW; ++v) at += sh.place[v][lane];
-      if (at < top) sh.first[at] = key;
+      if (at < top) out(at, key);
     }
-    __syncthreads();
+    if (b + FL_WAVE < c) __syncthreads();
   }
-  if (c == 0) __syncthreads();
 }
 
-// A value that at least LP_NW q of the workgroup's values reach, if all lanes hold one: the smallest over the waves of
-// the q-th largest in the wave, stored for others to read at any time (rising values only make it rise). On ordered
-// whole numbers, whose maximum is one DPP instruction a step.
-__device__ __forceinline__ uint32_t lp_ord(float x) {  // not of NaN
-  const uint32_t b = __float_as_uint(x + 0.0f);         // -0 becomes 0
-  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-}
-__device__ __forceinline__ float lp_unord(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+// Of values with a lane each, the q-th largest of the wave, which q reach; stored for others to read at any time (rising
+// values only make it rise). On ordered whole numbers, whose maximum is one DPP instruction a step: 190 cycles a
+// place; a ballot for each of 16 bits instead takes 1300.
 template <int CTRL>
 __device__ __forceinline__ uint32_t umax_dpp(uint32_t v) {
   return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
@@ -134,42 +134,42 @@ __device__ __forceinline__ uint32_t wave_umax32(uint32_t v) {
   const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   return max(q[0], q[1]);
 }
-__device__ __forceinline__ void lp_publish(uint32_t* red, float mine, int q) {
-  uint32_t v = mine == mine ? lp_ord(mine) : 0u, w = lp_ord(-INFINITY);
+__device__ __forceinline__ void lp_publish(uint32_t* bound, float mine, int q) {
+  const uint32_t b = __float_as_uint(mine + 0.0f);  // -0 becomes 0
+  uint32_t v = mine == mine ? b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u) : 0u, t = 0;
   for (int r = 0; r < q; ++r) {
-    w = wave_umax32(v);
-    if ((threadIdx.x & 63) == __builtin_ctzll(__ballot(v == w) | (1ull << 63))) v = 0;
+    t = wave_umax32(v);
+    if ((threadIdx.x & 63) == __builtin_ctzll(__ballot(v == t) | (1ull << 63))) v = 0;
   }
-  if ((threadIdx.x & 63) == 0) __hip_atomic_store(red + (threadIdx.x >> 6), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  if ((threadIdx.x & 63) == 0)
+    __hip_atomic_store(bound + (threadIdx.x >> 6), t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
-__device__ __forceinline__ float lp_least(uint32_t* red, int waves) {
-  uint32_t t = waves > 0 ? ~0u : lp_ord(-INFINITY);
+// the smallest of the first waves' bounds: a value that LP_NW q reach
+__device__ __forceinline__ float lp_least(uint32_t* bound, int waves) {
+  uint32_t t = waves > 0 ? ~0u : 0u;
 #pragma unroll
   for (int k = 0; k < LP_NW; ++k)
-    if (k < waves) t = min(t, __hip_atomic_load(red + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
-  return t <= lp_ord(-INFINITY) ? -INFINITY : lp_unord(t);
+    if (k < waves) t = min(t, __hip_atomic_load(bound + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+  return t <= 0x007FFFFFu ? -INFINITY : lp_value((u64)t << 32);  // -inf's ordered bits
 }
 
-// what the whole row says, from its maximum, sums and rank count, and sh.first
-__device__ __forceinline__ void lp_write(const LpArgs& a, int64_t row, const LpToken& tok, float m, float s, float u,
-                                         int before, const LpShared& sh) {
-  const float nan = __builtin_nanf("");
-  const bool fine = fabsf(m) < INFINITY;
-  const float logs = fine ? logf(s) : nan;  // s is NaN if a value is
-  const int tid = threadIdx.x;
-  if (tid == 0) {
-    if (a.tokens) {
-      a.logprob[row] = tok.in ? (tok.l - m) - logs : nan;
-      a.rank[row] = tok.in ? before : -1;
-    }
-    const float h = logs - u / s;
-    a.entropy[row] = h < 0.0f ? 0.0f : h;  // rounding
+// what the whole row says, from its maximum, sums and rank count: by wave 1, beside wave 0's sort
+__device__ __forceinline__ float lp_logsum(float m, float s) {  // NaN without a distribution; s is NaN if a value is
+  return fabsf(m) < INFINITY ? logf(s) : __builtin_nanf("");
+}
+__device__ __forceinline__ void lp_write(const LpArgs& a, int64_t row, const LpToken& tok, float m, float logs, float s,
+                                         float u, int before) {
+  if (threadIdx.x != FL_WAVE) return;
+  if (a.tokens) {
+    a.logprob[row] = tok.in ? (tok.l - m) - logs : __builtin_nanf("");
+    a.rank[row] = tok.in ? before : -1;
   }
-  if (tid < a.top) {
-    const u64 key = sh.first[tid];
-    a.top_ids[row * a.top + tid] = (int32_t)(0xFFFFFFFFu - (uint32_t)key);
-    a.top_lp[row * a.top + tid] = (lp_value(key) - m) - logs;
-  }
+  const float h = logs - u / s;
+  a.entropy[row] = h < 0.0f ? 0.0f : h;  // rounding
+}
+__device__ __forceinline__ void lp_place(const LpArgs& a, int64_t row, float m, float logs, int place, u64 key) {
+  a.top_ids[row * a.top + place] = (int32_t)(0xFFFFFFFFu - (uint32_t)key);
+  a.top_lp[row * a.top + place] = (lp_value(key) - m) - logs;
 }
 
 // v_max3_f32 without the operation per operand that makes a loaded value canonical
@@ -301,94 +301,104 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
     for (int v = 0; v < LP_E / V; ++v) cur[v] = ahead[v];
   }
   lp_join(m, s, u);
-  if (lane == 0) sh.red[0][wave] = m, sh.red[1][wave] = s, sh.red[2][wave] = u, sh.red[3][wave] = (float)before, sh.kept[wave] = kept;
+  if (lane == 0) sh.red[wave] = make_float4(m, s, u, __int_as_float(before)), sh.kept[wave] = kept;
   __syncthreads();
-  const bool one = lane < LP_NW;
-  m = one ? sh.red[0][lane % LP_NW] : -INFINITY;
-  s = one ? sh.red[1][lane % LP_NW] : 0.0f;
-  u = one ? sh.red[2][lane % LP_NW] : 0.0f;
-  lp_join(m, s, u);
+  int most = 0;
   before = 0;
+  {
+    float4 w[LP_NW];
 #pragma unroll
-  for (int w = 0; w < LP_NW; ++w) before += (int)sh.red[3][w];
-  if (a.top > 0) {
-    int most = 0;
+    for (int k = 0; k < LP_NW; ++k) {
+      w[k] = sh.red[k];
+      m = fmaxf(m, w[k].x);
+      before += __float_as_int(w[k].w);
+      most = max(most, sh.kept[k]);
+    }
+    const float mu = m == -INFINITY ? 0.0f : m;
+    s = u = 0.0f;
 #pragma unroll
-    for (int w = 0; w < LP_NW; ++w) most = max(most, sh.kept[w]);
-    if (most <= LP_KEEP) {
-      lp_sort(sh, a.top);
-    } else {  // a crowd of equal values: one after the other, from memory
-      u64 last = ~0ull;
-      for (int r = 0; r < a.top; ++r) {
-        u64 best = 0;
-        for (int j = j0 + tid; j < j1; j += LP_NT) {
-          const u64 k = lp_key(BF16 ? bf2f(lh[j]) : lf[j], j);
-          if (k < last) best = u64max(best, k);
-        }
-        best = wave_max_u64(best);
-        __syncthreads();
-        if (lane == 0) sh.cand[0][wave] = best;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < LP_NW; ++w) best = u64max(best, sh.cand[0][w]);
-        if (tid == 0) sh.first[r] = best;
-        last = best;
-      }
-      __syncthreads();
+    for (int k = 0; k < LP_NW; ++k) {
+      const float d = fmaxf(w[k].x - mu, -1000.0f), e = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+      s += w[k].y * e;
+      u += (w[k].z + w[k].y * d) * e;
     }
   }
-  if (a.chunks == 1) {
-    lp_write(a, row, tok, m, s, u, before, sh);
+  const float logs = lp_logsum(m, s);
+  const int64_t at = row * a.chunks + chunk;
+  auto out = [&](int place, u64 key) {
+    if (a.chunks == 1) lp_place(a, row, m, logs, place, key);
+    else a.cand[at * a.top + place] = key;
+  };
+  if (a.chunks == 1) lp_write(a, row, tok, m, logs, s, u, before);
+  else if (tid == FL_WAVE) {
+    a.part[at] = make_float4(m, s, u, __int_as_float(before));
+    if (chunk == 0) a.given[row] = make_float2(tok.l, tok.in ? 1.0f : 0.0f);
+  }
+  if (a.top == 0) return;
+  if (most <= LP_KEEP) {
+    lp_sort(sh, a.top, out);
     return;
   }
-  const int64_t at = row * a.chunks + chunk;
-  if (tid == 0) a.part[at] = make_float4(m, s, u, __int_as_float(before));
-  if (tid < a.top) a.cand[at * a.top + tid] = sh.first[tid];
+  u64 last = ~0ull;  // a crowd of equal values: one after the other, from memory
+  for (int r = 0; r < a.top; ++r) {
+    u64 best = 0;
+    for (int j = j0 + tid; j < j1; j += LP_NT) {
+      const u64 k = lp_key(BF16 ? bf2f(lh[j]) : lf[j], j);
+      if (k < last) best = u64max(best, k);
+    }
+    best = wave_max_u64(best);
+    __syncthreads();
+    if (lane == 0) sh.cand[0][wave] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < LP_NW; ++w) best = u64max(best, sh.cand[0][w]);
+    if (tid == 0) out(r, best);
+    last = best;
+  }
 }
 
 // The chunks of a row joined: one workgroup per row, lane = chunk
-template <bool BF16>
 __global__ __launch_bounds__(LP_NT) void k_logprobs_merge(LpArgs a) {
+  constexpr int E = LP_CHUNKS * LP_TOP / LP_NT;  // keys of a thread
   __shared__ LpShared sh;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, keys = a.chunks * a.top;
   const int64_t row = blockIdx.x;
-  const u64* cand = a.cand + row * a.chunks * a.top;
-  const bool one = lane < a.chunks;
-  const float4 p = one ? a.part[row * a.chunks + lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-  u64 mine[LP_KEEP / FL_WAVE], T = 0;
+  const u64* cand = a.cand + row * keys;
+  const float4 p = lane < a.chunks ? a.part[row * a.chunks + lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+  u64 mine[E];
+  float largest = -INFINITY;  // NaN is passed over
   if (a.top > 0) {
 #pragma unroll
-    for (int i = 0; i < LP_KEEP / FL_WAVE; ++i) mine[i] = i * LP_NT + tid < a.chunks * a.top ? cand[i * LP_NT + tid] : 0;
-    if (one) T = cand[(lane + 1) * a.top - 1];
-  }
-  const LpToken tok = lp_token<BF16>(a, row);
-  float m = p.x, s = p.y, u = p.z;
-  lp_join(m, s, u);
-  const int before = (int)wave_sum((float)__float_as_int(p.w));
-  if (a.top > 0) {
-    // at least `top` keys reach the largest of the chunks' last ones; and, as in a chunk, a value from the threads' largest
-    T = wave_max_u64(T);
-    u64 largest = 0;
+    for (int i = 0; i < E; ++i) mine[i] = i * LP_NT + tid < keys ? cand[i * LP_NT + tid] : 0;
 #pragma unroll
-    for (int i = 0; i < LP_KEEP / FL_WAVE; ++i) largest = u64max(largest, mine[i]);
-    const int full = min(LP_NW, a.chunks * a.top / FL_WAVE), q = full > 0 ? (a.top + full - 1) / full : 0;
-    lp_publish(sh.bound, largest != 0 ? lp_value(largest) : -INFINITY, q);
+    for (int i = 0; i < E; ++i) largest = fmaxf(largest, mine[i] != 0 ? lp_value(mine[i]) : -INFINITY);
+    const int full = min(LP_NW, keys / FL_WAVE), q = full > 0 ? (a.top + full - 1) / full : 0;
+    lp_publish(sh.bound, largest, q);
     __syncthreads();
     const float t = lp_least(sh.bound, full);
     int kept = 0;
 #pragma unroll
-    for (int i = 0; i < LP_KEEP / FL_WAVE; ++i) {
-      const bool is = mine[i] != 0 && mine[i] >= T && !(lp_value(mine[i]) < t);
+    for (int i = 0; i < E; ++i) {
+      const bool is = mine[i] != 0 && !(lp_value(mine[i]) < t);
       const u64 lanes = __ballot(is);
       const int at = kept + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
-      if (is) sh.cand[tid >> 6][at] = mine[i];
+      if (is) sh.cand[wave][at] = mine[i];
       kept += __builtin_popcountll(lanes);
     }
-    if (lane == 0) sh.kept[tid >> 6] = kept;
-    __syncthreads();
-    lp_sort(sh, a.top);
+    if (lane == 0) sh.kept[wave] = kept;
   }
-  lp_write(a, row, tok, m, s, u, before, sh);
+  LpToken tok{-1, false, 0.0f};
+  if (a.tokens) {
+    const float2 g = a.given[row];
+    tok.l = g.x, tok.in = g.y != 0.0f;
+  }
+  float m = p.x, s = p.y, u = p.z;
+  lp_join(m, s, u);
+  const float logs = lp_logsum(m, s);
+  lp_write(a, row, tok, m, logs, s, u, (int)wave_sum((float)__float_as_int(p.w)));  // below 2^24: exact
+  if (a.top == 0) return;
+  __syncthreads();
+  lp_sort(sh, a.top, [&](int place, u64 key) { lp_place(a, row, m, logs, place, key); });
 }
 
 // Chunks of a row: one, or as many as give 1024 workgroups in all, of 4096 values (a step) at least.
@@ -401,12 +411,13 @@ void lp_plan(LpArgs& a, int rows) {
 template <bool BF16>
 void lp_launch(const LpArgs& a, int rows, hipStream_t s) {
   hipLaunchKernelGGL(k_logprobs<BF16>, dim3((unsigned)rows * (unsigned)a.chunks), dim3(LP_NT), 0, s, a);
-  if (a.chunks > 1) hipLaunchKernelGGL(k_logprobs_merge<BF16>, dim3(rows), dim3(LP_NT), 0, s, a);
+  if (a.chunks > 1) hipLaunchKernelGGL(k_logprobs_merge, dim3(rows), dim3(LP_NT), 0, s, a);
 }
 
-int64_t lp_part_bytes(const LpArgs& a, int rows) { return a.chunks > 1 ? i8_pad((int64_t)rows * a.chunks * 16) : 0; }
+int64_t lp_part_bytes(const LpArgs& a, int rows) { return i8_pad((int64_t)rows * a.chunks * 16); }
+int64_t lp_cand_bytes(const LpArgs& a, int rows) { return i8_pad((int64_t)rows * a.chunks * a.top * 8); }
 int64_t lp_bytes(const LpArgs& a, int rows) {
-  return a.chunks > 1 ? lp_part_bytes(a, rows) + i8_pad((int64_t)rows * a.chunks * a.top * 8) : 0;
+  return a.chunks > 1 ? lp_part_bytes(a, rows) + lp_cand_bytes(a, rows) + (int64_t)rows * 8 : 0;
 }
 
 constexpr int LP_MAXROWS = 1 << 17;  // rows x LP_CHUNKS workgroups of 256 threads in one grid
@@ -421,8 +432,10 @@ bool lp_outputs_ok(const int32_t* tokens, int top, const float* logprob, const f
 
 int lp_run(LpArgs a, bool bf16, int rows, void* work, hipStream_t s) {
   lp_plan(a, rows);
-  a.part = static_cast<float4*>(work);
-  a.cand = reinterpret_cast<u64*>(static_cast<char*>(work) + lp_part_bytes(a, rows));
+  char* const base = static_cast<char*>(work);
+  a.part = reinterpret_cast<float4*>(base);
+  a.cand = reinterpret_cast<u64*>(base + lp_part_bytes(a, rows));
+  a.given = reinterpret_cast<float2*>(base + lp_part_bytes(a, rows) + lp_cand_bytes(a, rows));
   if (bf16) lp_launch<true>(a, rows, s);
   else lp_launch<false>(a, rows, s);
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
@@ -477,7 +490,7 @@ int fl_logprobs(const void* logits, int32_t bf16, int64_t stride, int32_t rows, 
       !lp_outputs_ok(tokens, top, logprob, entropy, rank, top_ids, top_logprobs))
     return FL_E_ARG;
   LpArgs a{logits, rows > 1 ? stride : 0, vocab, top, 0, 0, tokens, logprob, entropy, rank, top_ids, top_logprobs,
-           nullptr, nullptr};
+           nullptr, nullptr, nullptr};
   lp_plan(a, rows);
   if (lp_bytes(a, rows) > 0 && !i8_aligned(work)) return FL_E_ARG;
   return lp_run(a, bf16 != 0, rows, work, reinterpret_cast<hipStream_t>(stream));
@@ -505,7 +518,7 @@ int fl_head_logprobs(const uint16_t* x, const int8_t* wq, const float* ws, const
     const int64_t t0 = (int64_t)r0 * top;
     LpArgs a{base + p.logits, n, n, top, 0, 0, tokens ? tokens + r0 : nullptr, tokens ? logprob + r0 : nullptr,
              entropy + r0, tokens ? rank + r0 : nullptr, top ? top_ids + t0 : nullptr, top ? top_logprobs + t0 : nullptr,
-             nullptr, nullptr};
+             nullptr, nullptr, nullptr};
     rc = lp_run(a, false, r, base + p.lp, s);
     if (rc != FL_OK) return rc;
   }
