@@ -575,16 +575,19 @@ struct I8Plan {
   int mblk, nblk, splits, sps;  // of tiles
 };
 
-// Whether x of up to 32 rows goes through k_i8_few. It reads x once per 16 weight rows (from LDS where a workgroup takes
-// several blocks, n >= 8192), tiles once per 64, but a tile has less in flight: us, few and tiles of 64,
-// - 8 / 16 / 32 rows x 2560 x 2560 4.1 / 4.4 / 5.5 and 6.8 / 6.9 / 7.1; x 2560 x 8192 7.6 / 9.9 / 13.7 and 10.2 / 10.2 / 10.6; 16
-//   x 5003 x 8192 17.9 and 14.7;
-// - 32 rows x 16384 x 2560 11.8 and 10.9, 8 rows 9.8 and 10.3; x 49152 x 2560, weights from HBM, 30 and 37, 27 and 34;
+// Whether x of up to 32 rows goes through k_i8_few, which reads x once per 16 weight rows (from LDS where a workgroup
+// takes several blocks) and has more weights in flight than tiles, which read x once per 64. us, few and tiles of 64:
+// - 8 / 16 / 32 rows x 2560 x 2560 4.1 / 4.4 / 5.5 and 6.8 / 6.9 / 7.1; x 2560 x 8192 7.6 / 9.9 / 13.7 and 10.2 / 10.2 / 10.6;
+//   16 x 5003 x 8192 17.9 and 14.7;
+// - 16 rows x 49152 x 2560, the weights from HBM, 27.7 and 29.2; 8 x 16384 x 2560 9.8 and 10.3; beyond 48 KB of x in LDS
+//   16 x 49152 x 4096 42.9 and 42.7, 16 x 16384 x 4096 15.8 and 15.1;
+// - 32 rows x 16384 x 2560 11.8 and 10.9, 24 x 32768 x 2560 20.8 and 18.0, 32 x 49152 x 2560 29.9 and 31.4;
 // - short rows, whose K is too little for eight waves: 16 x 16384 x 512 6.1 and 4.7.
+constexpr int FEW_LDS_KB = 48;
 bool i8_few_rows(int m, int n, int k) {
-  if (m > 32 || (int64_t)m * k >= 131072 || (k <= 1024 && n >= 8192)) return false;
-  if (m <= 16) return true;
-  return n < 8192 ? n <= 4096 && k < 4096 : n >= 32768 && m * few_pitch(k) <= 112 << 10;
+  if (m > 16) return m <= 32 && n <= 4096 && k < 4096;
+  if (n >= 8192) return k > 1024 && (m <= 2 || m * few_pitch(k) <= FEW_LDS_KB << 10);
+  return (int64_t)m * k < 131072;
 }
 
 I8Plan i8_plan(int m, int n, int k) {
@@ -647,14 +650,15 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
   const I8Plan p = i8_plan(m, n, k);
   if (p.kind == I8_FEW) {
     const I8Few a{xq, xs, wq, ws, y, m, n, k};
-    const int lds = m * few_pitch(k);
-    if (n < 8192) m <= 16 ? i8_few<1, 0, false>(a, 0, y_fp32, s) : i8_few<2, 0, false>(a, 0, y_fp32, s);
-    else if (m > 16) i8_few<2, 112, false>(a, 1, y_fp32, s);
-    else if (lds <= 48 << 10) i8_few<1, 48, false>(a, 2, y_fp32, s);
-    else i8_few<1, 132, false>(a, 1, y_fp32, s);
+    if (m > 16) i8_few<2, 0, false>(a, 0, y_fp32, s);
+    // x in LDS and blocks in turn, 8 / 16 rows x 49152 x 2560: 27 / 28 us, 31 / 38 without; one row 25 and 23
+    else if (n < 8192 || m <= 2) i8_few<1, 0, false>(a, 0, y_fp32, s);
+    else i8_few<1, FEW_LDS_KB, false>(a, 2, y_fp32, s);
   } else {
     const I8Tile a{xq, wq, xs, ws, p.splits > 1 ? work : y, m, n, k, p.mblk, p.nblk, p.splits, p.sps};
-    const bool one = (int64_t)p.mblk * p.nblk * p.splits <= 256;  // a CU holds one workgroup: it may have all of its LDS
+    // up to 256 tiles a CU holds one workgroup, which may have all of its LDS; beyond, two that take turns at waiting: us,
+    // two and one, 128 x 128 tiles of 1500 x 5003 x 2560 (480) 27 and 31, 64 x 64 of 2048 x 2560 x 512 (1280) 11 and 17
+    const bool one = (int64_t)p.mblk * p.nblk * p.splits <= 256;
     if (p.kind == I8_T256) i8_tiles<256, 1, 2, 4, 5, 1>(a, y_fp32, s);
     else if (p.kind == I8_T128) one ? i8_tiles<128, 1, 2, 4, 8, 1>(a, y_fp32, s) : i8_tiles<128, 1, 2, 2, 4, 1>(a, y_fp32, s);
     else one ? i8_tiles<64, 4, 1, 1, 4, 1>(a, y_fp32, s) : i8_tiles<64, 1, 2, 2, 8, 1>(a, y_fp32, s);
