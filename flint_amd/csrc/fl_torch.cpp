@@ -291,21 +291,26 @@ torch::Tensor piece(const torch::Tensor& base, int64_t byte, torch::IntArrayRef 
   return t;
 }
 
-// Outputs of generate.logprobs and generate.head_logprobs, rows of them, in one allocation
+// Outputs of generate.logprobs and generate.head_logprobs, rows of them: the floats in one allocation, the integers in
+// another (torch.save refuses types that share one)
 struct LogprobOut {
   torch::Tensor logprob, entropy, rank, ids, top;
   void make(int64_t rows, int64_t n, bool tokens, const torch::Tensor& like) {
-    const int64_t words = rows * ((tokens ? 3 : 1) + 2 * n);
-    const torch::Tensor all = bytes_of(4 * words, like);
+    torch::Tensor all;
     int64_t at = 0;
+    auto open = [&](int64_t words) { all = bytes_of(4 * words, like), at = 0; };
     auto next = [&](torch::IntArrayRef sizes, torch::ScalarType dt) {
       torch::Tensor t = piece(all, at, sizes, dt);
       at += 4 * t.numel();
       return t;
     };
+    open(rows * ((tokens ? 2 : 1) + n));
     entropy = next({rows}, torch::kFloat32);
-    if (tokens) logprob = next({rows}, torch::kFloat32), rank = next({rows}, torch::kInt32);
-    if (n > 0) ids = next({rows, n}, torch::kInt32), top = next({rows, n}, torch::kFloat32);
+    if (tokens) logprob = next({rows}, torch::kFloat32);
+    if (n > 0) top = next({rows, n}, torch::kFloat32);
+    open(rows * ((tokens ? 1 : 0) + n));
+    if (tokens) rank = next({rows}, torch::kInt32);
+    if (n > 0) ids = next({rows, n}, torch::kInt32);
   }
   pybind11::object cast() const {
     auto one = [](const torch::Tensor& t) -> pybind11::object {

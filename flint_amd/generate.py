@@ -250,6 +250,8 @@ def generate(model, prompt, max_new_tokens, temperature=None, top_k=None, seed=0
     counter. Tokens stay on the device either way (no host synchronisation in the loop).
     logprobs = n (0..32): (tokens, TokenLogprobs of the new ones with n alternatives each) of the
     model's own distribution, before temperature and top_k."""
+    if logprobs is not None:
+        _check_logprob_args(1, model.config.vocab_size, None, int(logprobs), model.device)
     prompt = prompt.reshape(-1).to(device=model.device, dtype=torch.int32)
     T = prompt.numel()
     model.setup_caches(1, T + max_new_tokens)
@@ -261,7 +263,6 @@ def generate(model, prompt, max_new_tokens, temperature=None, top_k=None, seed=0
     t = 1.0 if temperature is None else temperature
     said, logits = [], None
     if logprobs is not None:
-        _check_logprob_args(max_new_tokens, model.config.vocab_size, None, int(logprobs), seq.device)
         logits = torch.empty(model.config.vocab_size, dtype=torch.float32, device=model.device)
     # the last prompt token produces the first new token
     for i in range(max_new_tokens):

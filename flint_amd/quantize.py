@@ -264,7 +264,7 @@ def gemm_int8(xq, xs, wq, ws, out_dtype=torch.bfloat16):
     per row (quantize_int8's). The integer sums are exact, so a row's result does not depend on the batch
     it is in. out_dtype: bf16, or fp32 (logits)."""
     f32 = out_dtype is torch.float32
-    if _int8_fast is not None and xq.is_cuda and (f32 or out_dtype is torch.bfloat16):
+    if _int8_fast is not None and xs is not None and xq.is_cuda and (f32 or out_dtype is torch.bfloat16):
         y = _int8_fast(xq, xs, wq, ws, f32, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
         if y is not None:
             return y

@@ -197,6 +197,58 @@ def test_refusals(dev):
             bad()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(1, 4095), (1, 4096), (1, 4097), (2, 8191), (1, 8193), (3, 12296), (1, 131072),
+                                        (1, 131073), (40, 65537), (1100, 4095), (1100, 4097), (1100, 8200)])
+def test_where_steps_and_chunks_meet(dev, rows, vocab, dtype):
+    """Few values, so that equal ones lie on both sides of every boundary; the tokens at the boundaries themselves."""
+    g = torch.Generator().manual_seed(vocab)
+    logits = torch.randint(0, 5, (rows, vocab), generator=g).to(dtype)
+    logits[torch.rand(rows, vocab, generator=g) < 0.01] = -math.inf
+    chunks = max(1, min(32, -(-vocab // 4096), 1024 // rows))
+    per = -(-(-(-vocab // chunks)) // 8) * 8
+    at = [0, vocab - 1, min(per, vocab) - 1, min(per, vocab - 1), min(4095, vocab - 1), min(4096, vocab - 1), vocab // 2]
+    logits, some = logits.to(dev), sorted({0, rows - 1, rows // 2})
+    for t in at:
+        tokens = torch.full((rows,), t, dtype=torch.int32)
+        out = host(generate.logprobs(logits, tokens.to(dev), 7))
+        check(generate.TokenLogprobs(*(f[some] for f in out)), logits.cpu()[some], tokens[some], 7)
+
+
+def test_results_can_be_saved(dev):
+    import io
+    lg, tok = rows_of(3, 100, 1, torch.float32)
+    for tokens, top in ((tok.to(dev), 5), (tok.to(dev), 0), (None, 5), (None, 0)):
+        out = generate.logprobs(lg.to(dev), tokens, top)
+        buf = io.BytesIO()
+        torch.save(list(out), buf)
+        buf.seek(0)
+        for a, b in zip(torch.load(buf, weights_only=True), out):
+            assert (a is None and b is None) or torch.equal(a, b)
+
+
+def test_two_streams_at_once(dev):
+    lg, tok = rows_of(4, 49152, 1, torch.float32)
+    logits, tokens = lg.to(dev), tok.to(dev)
+    w = (torch.randn(9001, 256, generator=torch.Generator().manual_seed(2)) * 0.1).to(torch.bfloat16)
+    head = quantize.DynamicInt8Linear.from_float(w.to(dev))
+    feat = torch.randn(70, 256, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(dev)
+    calls = [lambda: generate.logprobs(logits, tokens, 5), lambda: generate.logprobs(logits[:1], tokens[:1], 20),
+             lambda: generate.head_logprobs(feat, head.weight, head.scales, None, 8),
+             lambda: generate.head_logprobs(feat[:3], head.weight, head.scales, tokens[:3], 8)]
+    want = [host(f()) for f in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in calls], []
+    for _ in range(3):
+        for s, f in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(f())
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        for a, b in zip(host(out), want[i % len(calls)]):  # NaN: an id outside the smaller vocabulary
+            assert (a is None and b is None) or torch.equal(a.nan_to_num(9.0), b.nan_to_num(9.0))
+
+
 # ---- from features -----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("m,n,k,top", [(1, 49152, 2560, 5), (8, 49152, 2560, 20), (1, 1000, 64, 3), (33, 1003, 1040, 32),
@@ -347,3 +399,12 @@ def test_generate_with_log_probabilities(dev, model, sampled):
     assert len(seq) == 20 and out.logprob.shape == (0,) and out.top_ids.shape == (0, 2)
     with pytest.raises(ValueError):
         generate.generate(model, prompt, 2, logprobs=33)
+
+
+def test_generate_refuses_log_probabilities_it_has_not(dev, model):
+    prompt = torch.tensor([3, 5], dtype=torch.int32, device=dev)
+    for n in (-1, 33):
+        with pytest.raises(ValueError):
+            generate.generate(model, prompt, 2, logprobs=n)
+    seq, said = generate.generate(model, prompt, 0, logprobs=2)
+    assert seq.tolist() == [3, 5] and said.logprob.shape == (0,) and said.top_ids.shape == (0, 2)
