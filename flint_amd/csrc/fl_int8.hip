@@ -336,6 +336,7 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
 
 typedef int i8_x16 __attribute__((ext_vector_type(16)));
 typedef int i8_out32 __attribute__((ext_vector_type(4), aligned(4)));
+typedef float i8_scale4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t i8_out16 __attribute__((ext_vector_type(4), aligned(2)));
 
 struct I8Tile {
@@ -349,11 +350,12 @@ struct I8Tile {
 // KW > 1: the waves are KW ways of WM x WN, each over its own steps with a ring of its own, for calls of few tiles, where
 // a step's latency counts: a way of one wave needs no barrier, and its products are four times those of a wave
 // that shares the tile with three others. The ways' sums meet in LDS.
-template <int T, int KW, int WM, int WN, int NR, int Q, int OUT>  // OUT: 0 bf16, 1 fp32, 2 int32 part sums
+template <int T, int KW, int WM, int WN, int NR, int OUT>  // OUT: 0 bf16, 1 fp32, 2 int32 part sums
 __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k_i8_tile(I8Tile a) {
   constexpr int NW = WM * WN, TM = T / WM, TN = T / WN, FM = TM / 32, FN = TN / 32;
   constexpr int PER = T / 8 / NW, UNIT = T * 128;  // loads of a wave for a unit; its bytes
   static_assert(T % (8 * NW) == 0 && TM % 32 == 0 && TN % 32 == 0 && NR >= 4, "whole loads, two steps");
+  static_assert(KW == 1 || NW == 1, "ways take their own numbers of steps: no barrier between them");
   // at the end, in the units' place: 32 rows of x by TN sums of a wave at a time; with ways all sums of each
   constexpr int LD = KW == 1 ? TN + 4 : T + 4, SLAB = (KW == 1 ? 32 : T) * LD * 4, SLABS = KW == 1 ? NW : KW;
   constexpr int SMEM = KW * NR * UNIT > SLABS * SLAB ? KW * NR * UNIT : SLABS * SLAB;
@@ -369,7 +371,7 @@ __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k
   const int grp = tt / (8 * a.nblk), gm = min(8, a.mblk - grp * 8), in = tt - grp * 8 * a.nblk;
   const int m0 = (grp * 8 + in % gm) * T, n0 = (in / gm) * T;
   const int steps = (a.k + 127) >> 7;
-  // the workgroup's part of K, the way's of that; every way passes as many barriers
+  // the workgroup's part of K, the way's of that
   const int p0 = split * a.sps, p1 = min(steps, p0 + a.sps), per = (p1 - p0 + KW - 1) / KW;
   const int s0 = p0 + way * per, s1 = min(p1, s0 + per);
   const int rows_n = min(T, a.n - n0), rows_m = min(T, a.m - m0);
@@ -407,29 +409,24 @@ __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k
   // the next step's first, behind the step's one barrier, when the next step's units have landed for every wave
   // and this step's have been read by every wave, so that their slots can be loaded again.
   struct Frag {
-    i8_x4 w[Q][FN], x[Q][FM];
+    i8_x4 w[FN], x[FM];
   };
   auto read = [&](int ws, int xs, int j, Frag& f) {
     const unsigned char* wt = ring + ws * UNIT + (wn * TN + r) * 128;
     const unsigned char* xt = ring + xs * UNIT + (wm * TM + r) * 128;
+    const int at = ((2 * j + h) ^ ((r >> 1) & 7)) * 16;
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int at = ((2 * (j * Q + q) + h) ^ ((r >> 1) & 7)) * 16;
+    for (int i = 0; i < FN; ++i) f.w[i] = *reinterpret_cast<const i8_x4*>(wt + i * 32 * 128 + at);
 #pragma unroll
-      for (int i = 0; i < FN; ++i) f.w[q][i] = *reinterpret_cast<const i8_x4*>(wt + i * 32 * 128 + at);
-#pragma unroll
-      for (int i = 0; i < FM; ++i) f.x[q][i] = *reinterpret_cast<const i8_x4*>(xt + i * 32 * 128 + at);
-    }
+    for (int i = 0; i < FM; ++i) f.x[i] = *reinterpret_cast<const i8_x4*>(xt + i * 32 * 128 + at);
     __builtin_amdgcn_sched_barrier(0);
   };
   auto multiply = [&](const Frag& f) {
 #pragma unroll
-    for (int q = 0; q < Q; ++q)
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[q][j], f.x[q][i], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < FN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[j], f.x[i], acc[i][j], 0, 0, 0);
     __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll
@@ -447,12 +444,10 @@ __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k
     // once, a load instruction takes 16 cycles
     if (s > 0) load(2 * s - 1 + NR, xs >= 2 ? xs - 2 : xs - 2 + NR);
     multiply(A);
-    if constexpr (Q == 1) {
-      read(ws, xs, 2, A);
-      multiply(B);
-      read(ws, xs, 3, B);
-      multiply(A);
-    }
+    read(ws, xs, 2, A);
+    multiply(B);
+    read(ws, xs, 3, B);
+    multiply(A);
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): B is here, this step's units are read
     // in flight behind the next step's units: those after them, NR - 4, fewer in the last steps
     if (s0 + s + (NR - 1) / 2 < s1) wait_loads<(NR - 4) * PER>();
@@ -463,8 +458,6 @@ __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k
     multiply(B);
     ws = wn_, xs = xn_;
   }
-  if (NW > 1)  // a way with fewer steps (or none) than the others
-    for (int s = max(s1 - s0, 0); s < per; ++s) __builtin_amdgcn_s_barrier();
   // out through LDS, so that a wave stores whole lines
   __syncthreads();
   constexpr int V = OUT == 0 ? 8 : 4;  // values of a lane's store
@@ -554,7 +547,7 @@ __global__ __launch_bounds__(256) void k_i8_join(const int* __restrict__ part, i
     const int64_t row = at / n;
     const int c = (int)(at - row * n);
     const float sx = xs[row];
-    const float4 w = *reinterpret_cast<const float4*>(ws + c);
+    const i8_scale4 w = *reinterpret_cast<const i8_scale4*>(ws + c);
     const float o[4] = {(float)v[0] * (sx * w.x), (float)v[1] * (sx * w.y), (float)v[2] * (sx * w.z), (float)v[3] * (sx * w.w)};
     if (F32) *reinterpret_cast<float4*>(static_cast<float*>(y) + at) = make_float4(o[0], o[1], o[2], o[3]);
     else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(y) + at) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
@@ -621,13 +614,18 @@ void i8_few(const I8Few& a, int per_cu, bool f32, hipStream_t s) {
   else hipLaunchKernelGGL((k_i8_few<MB, XKB, QUANT, false>), grid, nt, 0, s, a);
 }
 
-template <int T, int KW, int WM, int WN, int NR, int Q>
+template <int T, int KW, int WM, int WN, int NR>
 void i8_tiles(const I8Tile& a, bool f32, hipStream_t s) {
   const unsigned grid = 8u * (unsigned)(((int64_t)a.mblk * a.nblk * a.splits + 7) / 8);
   const dim3 nt(64 * KW * WM * WN);
-  if (a.splits > 1) hipLaunchKernelGGL((k_i8_tile<T, KW, WM, WN, NR, Q, 2>), dim3(grid), nt, 0, s, a);
-  else if (f32) hipLaunchKernelGGL((k_i8_tile<T, KW, WM, WN, NR, Q, 1>), dim3(grid), nt, 0, s, a);
-  else hipLaunchKernelGGL((k_i8_tile<T, KW, WM, WN, NR, Q, 0>), dim3(grid), nt, 0, s, a);
+  if constexpr (KW > 1) {  // parts of K come with few tiles only
+    if (a.splits > 1) {
+      hipLaunchKernelGGL((k_i8_tile<T, KW, WM, WN, NR, 2>), dim3(grid), nt, 0, s, a);
+      return;
+    }
+  }
+  if (f32) hipLaunchKernelGGL((k_i8_tile<T, KW, WM, WN, NR, 1>), dim3(grid), nt, 0, s, a);
+  else hipLaunchKernelGGL((k_i8_tile<T, KW, WM, WN, NR, 0>), dim3(grid), nt, 0, s, a);
 }
 
 }  // namespace
@@ -659,9 +657,9 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
     // up to 256 tiles a CU holds one workgroup, which may have all of its LDS; beyond, two that take turns at waiting: us,
     // two and one, 128 x 128 tiles of 1500 x 5003 x 2560 (480) 27 and 31, 64 x 64 of 2048 x 2560 x 512 (1280) 11 and 17
     const bool one = (int64_t)p.mblk * p.nblk * p.splits <= 256;
-    if (p.kind == I8_T256) i8_tiles<256, 1, 2, 4, 5, 1>(a, y_fp32, s);
-    else if (p.kind == I8_T128) one ? i8_tiles<128, 1, 2, 4, 8, 1>(a, y_fp32, s) : i8_tiles<128, 1, 2, 2, 4, 1>(a, y_fp32, s);
-    else one ? i8_tiles<64, 4, 1, 1, 4, 1>(a, y_fp32, s) : i8_tiles<64, 1, 2, 2, 8, 1>(a, y_fp32, s);
+    if (p.kind == I8_T256) i8_tiles<256, 1, 2, 4, 5>(a, y_fp32, s);
+    else if (p.kind == I8_T128) one ? i8_tiles<128, 1, 2, 4, 8>(a, y_fp32, s) : i8_tiles<128, 1, 2, 2, 4>(a, y_fp32, s);
+    else one ? i8_tiles<64, 4, 1, 1, 4>(a, y_fp32, s) : i8_tiles<64, 1, 2, 2, 8>(a, y_fp32, s);
     if (p.splits > 1) {
       const dim3 grid((unsigned)(((int64_t)m * n + 1023) / 1024));
       if (y_fp32) hipLaunchKernelGGL(k_i8_join<true>, grid, dim3(256), 0, s, static_cast<const int*>(work), p.splits, xs, ws, y, m, n);

@@ -229,3 +229,61 @@ def test_two_streams_at_once(dev):
     torch.cuda.synchronize()
     for i, y in enumerate(got):
         assert torch.equal(y.cpu(), ref[i % len(xs)])
+
+
+@pytest.mark.parametrize("m,n,k", [
+    (33, 90, 4112), (70, 1003, 4112), (64, 1000, 8208),        # few tiles of 64: K in parts, joined
+    (333, 2571, 1104), (64, 2570, 16),                         # up to 256 tiles of 64
+    (600, 2571, 272), (333, 4003, 400),                        # more of them
+    (1000, 3999, 1104), (1021, 4000, 2064),                    # up to 256 tiles of 128
+    (1500, 5003, 1104), (1501, 5000, 144),                     # more of them
+    (1900, 8003, 400), (2048, 8192, 528), (2049, 16130, 144),  # tiles of 256
+    (19, 1001, 2064), (32, 4095, 1040),                        # up to 32 rows without LDS
+    (1, 8195, 9616), (2, 16390, 1040), (9, 8191, 1040),        # up to 16 rows without, of long and of short matrices
+    (3, 8209, 1040), (8, 16400, 2576), (16, 9001, 2832), (5, 8209, 9600), (4, 24577, 2576)])  # in LDS, blocks in turn
+@pytest.mark.parametrize("f32", [False, True])
+def test_every_way_to_cut_a_product(dev, m, n, k, f32):
+    """Ragged rows, weights and K; scales that start on 4 bytes only; rows behind the last are left as they were."""
+    xq, wq = ints(m, k, m + k), ints(n, k, n)
+    g = torch.Generator().manual_seed(k)
+    xs, ws = torch.rand(m, generator=g) * 0.05, torch.rand(n, generator=g) * 1e-3
+    y = torch.full((m * n + 4096,), -7.0, dtype=torch.float32 if f32 else torch.bfloat16, device=dev)
+    need = _lib.ctypes.c_int64()
+    _lib.call("fl_gemm_int8_workspace", m, n, k, _lib.ctypes.byref(need))
+    work = torch.full((need.value + 4096,), 0x5A, dtype=torch.uint8, device=dev)
+    a, b = xq.to(dev), wq.to(dev)
+    s = torch.cat([torch.full((1,), math.nan), xs, torch.full((2,), math.nan), ws]).to(dev)
+    off = s[1:], s[1 + m + 2:]
+    _lib.call("fl_gemm_int8", _lib.ptr(a), _lib.ptr(off[0]), _lib.ptr(b), _lib.ptr(off[1]), _lib.ptr(y), int(f32),
+              _lib.ptr(work), m, n, k, _lib.stream_ptr())
+    ref = scoring.product(xq, xs, wq, ws).to(y.dtype)
+    assert torch.equal(y[:m * n].view(m, n).cpu(), ref)
+    assert bool((y[m * n:] == -7.0).all()) and bool((work[need.value:] == 0x5A).all())
+
+
+@pytest.mark.parametrize("kind", ["normal", "halves", "tiny"])
+@pytest.mark.parametrize("m,k", [(1024, 16), (1025, 2560), (1027, 1040), (1030, 2576)])
+def test_quantized_rows_of_large_batches(dev, m, k, kind):
+    x = rows_of(m, k, m + k, kind)
+    x[m - 1] = 0.0
+    x[m - 2, k - 1] = math.inf
+    q = torch.full((m + 2, k), 99, dtype=torch.int8, device=dev)
+    s = torch.full((m + 2,), 99.0, device=dev)
+    quantize.quantize_int8(x.to(dev), q[:m], s[:m])
+    qr, sr = scoring.quantize_rows(x)
+    assert torch.equal(q[:m].cpu(), qr) and same(s[:m], sr)
+    assert bool((q[m:] == 99).all()) and bool((s[m:] == 99.0).all())
+
+
+@pytest.mark.parametrize("m", list(range(1, 18)))
+def test_linears_that_quantise_on_the_way(dev, m):
+    """As long rows as 16384 values in all allow, one step longer, and short ones; more blocks than workgroups."""
+    n = 8225
+    for k in {16384 // m // 16 * 16, 16384 // m // 16 * 16 + 16, 528}:
+        x = rows_of(m, k, k, "outliers")
+        if m > 2:
+            x[1] = 0.0
+            x[2, k - 1] = math.nan
+        wq, ws = ints(n, k, m), torch.rand(n, generator=torch.Generator().manual_seed(m)) * 1e-3
+        y = quantize.linear_int8(x.to(dev), wq.to(dev), ws.to(dev), torch.float32)
+        assert same(y, scoring.product(*scoring.quantize_rows(x), wq, ws)), k
