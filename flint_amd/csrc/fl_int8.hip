@@ -2,9 +2,10 @@
 // channel), and the quantisation of bf16 rows that feeds them.
 //
 // A row r in 8 bits: scale s = max|r| times fp32(1 / 127), rounded to fp32 (within an ulp of max|r| / 127, without
-// a division), q = r / s rounded to nearest, ties to even, exactly (below). y[m, n] = fp32(sum_k xq[m, k] wq[n, k]) * fp32(xs[m] * ws[n]): the sum is a whole number and
-// exact in int32 whatever the order (|sum| <= 2^30), so every kernel and every split here gives the same bits,
-// whatever the batch.
+// a division), q = r / s rounded to nearest, ties to even, exactly (below).
+// y[m, n] = fp32(sum_k xq[m, k] wq[n, k]) * fp32(xs[m] * ws[n]): the sum is a whole number and exact in int32 whatever
+// the order (|sum| <= 2^30), so every kernel and every split here gives the same bits, whatever the batch. Rounded: the
+// sum to fp32 (24 bits of at most 30), the scales' product, theirs with the sum, and that to bf16 where y is.
 #include "fl_int8.h"
 #include <algorithm>
 #include <type_traits>
@@ -59,7 +60,8 @@ __device__ __forceinline__ uint2 q8_pack(const uint4& p, const Q8Row& row) {
 
 constexpr int Q8_NT = 256, Q8_KEEP = 5;  // threads of a workgroup; 8-value pieces that a lane keeps in registers
 
-// WR waves per row, 4 / WR rows per workgroup; rows of up to 2560 WR values are read once
+// WR waves per row, 4 / WR rows per workgroup; rows of up to 2560 WR values are read once. Bound by the launch up to some
+// hundred rows (32 x 2560 3.0 us), then by memory: 2048 x 2560 5.3 us, 3 TB/s, with 11 vector instructions a value beside.
 template <int WR>
 __global__ __launch_bounds__(Q8_NT) void k_quantize_i8(const uint16_t* __restrict__ x, int8_t* __restrict__ qo,
                                                        float* __restrict__ scale, int rows, int k) {
@@ -134,11 +136,15 @@ __device__ __forceinline__ void i8_store(void* y, int64_t at, int acc, float s) 
 // Up to 16 MB rows of x against all weights, 16 weight rows (a block) at a time: the eight waves of a workgroup
 // each take a part of K. Lane (r = l % 16, c = l / 16) of a wave holds 16 values of weight row r, and of x row r, at
 // 64 step + 16 c: A and B of v_mfma_i32_16x16x64_i8, which sums over k in any order as long as both operands use
-// the same. D: x row l % 16, weight rows 4 (l / 16) + 0..3. Weights go from memory to registers, U steps at once and
+// the same. D: x row l % 16, weight rows 4 (l / 16) + 0..3. Weights go from memory to registers, U steps at once, and
 // the waves' sums meet in LDS.
 // XKB = 0: one block per workgroup, x from memory beside the weights. XKB > 0: the workgroups that fit the chip at
-// once take blocks in turn, two sets of registers in turn across them, x in XKB KB of LDS: every block reading x again would cost as much as the weights at 16
-// rows. QUANT: x is bf16 and the workgroup quantises the rows for itself into LDS, behind its first weight loads.
+// once take blocks in turn, with two sets of registers in turn across them and x in XKB KB of LDS: every block reading x
+// again would cost as much as the weights at 16 rows. QUANT: x is bf16 and the workgroup quantises the rows for itself
+// into LDS, behind its first weight loads.
+// Bound by the weights' way from memory: 8 x 49152 x 2560 26.6 us, 4.7 TB/s (matrix pipes 1% busy; a wave per block,
+// without the sums' meeting, is no faster); below some 10 MB of weights by one launch's start, a memory latency and the end:
+// 2560 x 2560 with one row quantised here 5.1 us.
 constexpr int FEW_KW = 8;
 constexpr int QF_MOST = 16384, QF_KEEP = 8;  // values that a workgroup quantises; 8-value pieces of a lane
 // log2 of the waves of a row, so that the eight hold as many rows at once as there are (all eight one row at most)
@@ -148,7 +154,8 @@ inline bool qf_fits(int m, int k) {
   const int lw = qf_log_waves(m), slots = FEW_KW >> lw, w = 64 << lw;
   return m <= 16 && m * (int64_t)k <= QF_MOST && (m + slots - 1) / slots * ((k / 8 + w - 1) / w) <= QF_KEEP;
 }
-__host__ __device__ inline int few_pitch(int k) { return ((k + 63) >> 6) * 64 + 16; }  // of x rows in LDS: r and r + 8 on the same banks
+// of x rows in LDS: r and r + 8 on the same banks
+__host__ __device__ inline int few_pitch(int k) { return ((k + 63) >> 6) * 64 + 16; }
 struct I8Few {
   const void* x;     // int8 [m, k], or (QUANT) bf16
   const float* xs;   // not with QUANT
@@ -182,7 +189,8 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
   auto load = [&](int b, int t, Set& v) {
     const bool live = b < blocks;  // wave-uniform
     const int n0 = b * 16;
-    const auto wr = buf_rsrc(a.wq + (int64_t)(live ? n0 : 0) * k, live ? (uint32_t)min(16, a.n - n0) * (uint32_t)k : 0u);
+    const uint32_t rows = live ? (uint32_t)min(16, a.n - n0) : 0u;
+    const auto wr = buf_rsrc(a.wq + (int64_t)(live ? n0 : 0) * k, rows * (uint32_t)k);
     if (t == turns - 1) v.s = live ? a.ws[min(n0 + tn, a.n - 1)] : 0.0f;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -283,7 +291,8 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
         i8_x4 x;
         if constexpr (XKB == 0) x = v.x[i][j];
         else  // the last row again for lanes behind it (not stored); a step within the row
-          x = *reinterpret_cast<const i8_x4*>(xl + min(16 * j + r, m - 1) * pitch + min(s0 + t * U + i, steps - 1) * 64 + c * 16);
+          x = *reinterpret_cast<const i8_x4*>(xl + min(16 * j + r, m - 1) * pitch + min(s0 + t * U + i, steps - 1) * 64 +
+                                              c * 16);
         acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v.w[i], x, acc[j], 0, 0, 0);
       }
     }
@@ -328,11 +337,16 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
 // ---- tiles ------------------------------------------------------------------------------------------
 // A workgroup of WM x WN waves computes T rows of x against T weight rows over one part of K, in steps of 128
 // bytes of K. The two units of a step, weights and x, go straight from memory into LDS (buffer_load ... lds, 1 KB = 8
-// rows of 128 bytes per wave instruction), into a ring of NR units. In LDS the 16-byte
-// piece c of row r sits at c ^ (r / 2 % 8), so that 16 lanes on one piece of 16 rows take all 64 banks once
-// (c ^ r % 8: 8.5 M conflict cycles in 90 us); the lanes of the load fetch the pieces in that order. Waves use 32x32x32 MFMAs: a lane (r = l % 32, h = l /
+// rows of 128 bytes per wave instruction), into a ring of NR units. In LDS the 16-byte piece c of row r sits at
+// c ^ (r / 2 % 8), so that 16 lanes on one piece of 16 rows take all 64 banks once (c ^ r % 8: 8.5 M conflict cycles in
+// 90 us); the lanes of the load fetch the pieces in that order. Waves use 32x32x32 MFMAs: a lane (r = l % 32, h = l /
 // 32) holds piece 2 j + h of row r at sub-step j. Weights are operand A: a lane ends with x row l % 32 and weight
 // rows 8 (i / 4) + 4 h + i % 4.
+// What bounds the tiles of 256, at 2048 x 16384 x 2560 (two rounds of 256 tiles, 84 us, 2.0 POPS, the matrix pipes busy in
+// 0.48 of the cycles at 2.04 GHz): 1.59 us a step, of which the MFMAs and their reads of LDS alone take 1.39, at the clock
+// that the card then keeps; 6 us a round for its start and end, 5.5 for bf16 results (8.3 for fp32). Hiding the ends does
+// not pay, the time goes with the work done: tiles started 0 to 8 us apart, so that few store at a time, take 85 to 86, and
+// two workgroups a CU of 192 x 128, with 1.7 times the reads from L2, 97.
 
 typedef int i8_x16 __attribute__((ext_vector_type(16)));
 typedef int i8_out32 __attribute__((ext_vector_type(4), aligned(4)));
@@ -347,9 +361,9 @@ struct I8Tile {
   int mblk, nblk, splits, sps;  // tiles along m and n; parts of K and their steps of 128
 };
 
-// KW > 1: the waves are KW ways of WM x WN, each over its own steps with a ring of its own, for calls of few tiles, where
-// a step's latency counts: a way of one wave needs no barrier, and its products are four times those of a wave
-// that shares the tile with three others. The ways' sums meet in LDS.
+// KW > 1: the waves are KW ways of one wave, each over its own steps with a ring of its own, for calls of few tiles,
+// where a step's latency counts: a way needs no barrier, and its products are four times those of a wave that shares the
+// tile with three others (333 x 2570 x 2560 11 -> 8.8 us). The ways' sums meet in LDS.
 template <int T, int KW, int WM, int WN, int NR, int OUT>  // OUT: 0 bf16, 1 fp32, 2 int32 part sums
 __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k_i8_tile(I8Tile a) {
   constexpr int NW = WM * WN, TM = T / WM, TN = T / WN, FM = TM / 32, FN = TN / 32;
@@ -381,7 +395,8 @@ __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k
   auto piece = [&](int i) { return (lane & 7) ^ (((wave * PER + i) & 1) * 4 + (lane >> 4)); };
   uint32_t off[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) off[i] = (uint32_t)((wave * PER + i) * 8 + (lane >> 3)) * (uint32_t)a.k + (uint32_t)piece(i) * 16u;
+  for (int i = 0; i < PER; ++i)
+    off[i] = (uint32_t)((wave * PER + i) * 8 + (lane >> 3)) * (uint32_t)a.k + (uint32_t)piece(i) * 16u;
   unsigned char* const ring = smem + way * (NR * UNIT);
   const uint32_t base = (uint32_t)(uintptr_t)(lds_byte*)smem + (uint32_t)(way * NR * UNIT + wave * PER * 1024);
   const int tail = a.k & 127;  // bytes of the last step, if it is not whole
@@ -393,7 +408,8 @@ __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k
     const i8_u32x4 v = u & 1 ? xv : wv;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      dma_1k(v, base + (uint32_t)(slot * UNIT + i * 1024), cut && piece(i) * 16 >= tail ? 0x80000000u : off[i], (uint32_t)s * 128u);
+      dma_1k(v, base + (uint32_t)(slot * UNIT + i * 1024), cut && piece(i) * 16 >= tail ? 0x80000000u : off[i],
+             (uint32_t)s * 128u);
   };
   auto meet = [&] {  // one wave's loads and reads are its own
     if (NW > 1) __builtin_amdgcn_s_barrier();
@@ -509,7 +525,8 @@ __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k
         const int row = (p * 64 + lane) / LR, mm = m0 + wm * TM + i * 32 + row;
         int v[V];
 #pragma unroll
-        for (int e = 0; e < V; e += 4) *reinterpret_cast<i8_x4*>(v + e) = *reinterpret_cast<const i8_x4*>(slab + row * LD + lc + e);
+        for (int e = 0; e < V; e += 4)
+          *reinterpret_cast<i8_x4*>(v + e) = *reinterpret_cast<const i8_x4*>(slab + row * LD + lc + e);
         if (mm < a.m) put(v, mm, nn, OUT < 2 ? a.xs[mm] : 0.0f, sw);
       }
       __builtin_amdgcn_wave_barrier();
@@ -535,7 +552,8 @@ __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k
   }
 }
 
-// y = the sum of the part sums, scaled: four values a thread
+// y = the sum of the part sums, scaled: four values a thread. A launch's time: the parts are those of a few tiles
+// (64 x 2560 in five parts 3.9 us)
 template <bool F32>
 __global__ __launch_bounds__(256) void k_i8_join(const int* __restrict__ part, int splits, const float* __restrict__ xs,
                                                  const float* __restrict__ ws, void* __restrict__ y, int m, int n) {
@@ -548,9 +566,13 @@ __global__ __launch_bounds__(256) void k_i8_join(const int* __restrict__ part, i
     const int c = (int)(at - row * n);
     const float sx = xs[row];
     const i8_scale4 w = *reinterpret_cast<const i8_scale4*>(ws + c);
-    const float o[4] = {(float)v[0] * (sx * w.x), (float)v[1] * (sx * w.y), (float)v[2] * (sx * w.z), (float)v[3] * (sx * w.w)};
+    float o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (float)v[e] * (sx * w[e]);
     if (F32) *reinterpret_cast<float4*>(static_cast<float*>(y) + at) = make_float4(o[0], o[1], o[2], o[3]);
-    else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(y) + at) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    else
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(y) + at) =
+          make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
   } else {
     for (int64_t i = at; i < at + 4 && i < mn; ++i) {
       int v = 0;
@@ -570,10 +592,10 @@ struct I8Plan {
 
 // Whether x of up to 32 rows goes through k_i8_few, which reads x once per 16 weight rows (from LDS where a workgroup
 // takes several blocks) and has more weights in flight than tiles, which read x once per 64. us, few and tiles of 64:
-// - 8 / 16 / 32 rows x 2560 x 2560 4.1 / 4.4 / 5.5 and 6.8 / 6.9 / 7.1; x 2560 x 8192 7.6 / 9.9 / 13.7 and 10.2 / 10.2 / 10.6;
-//   16 x 5003 x 8192 17.9 and 14.7;
-// - 16 rows x 49152 x 2560, the weights from HBM, 27.7 and 29.2; 8 x 16384 x 2560 9.8 and 10.3; beyond 48 KB of x in LDS
-//   16 x 49152 x 4096 42.9 and 42.7, 16 x 16384 x 4096 15.8 and 15.1;
+// - 8 / 16 / 32 rows x 2560 x 2560 4.1 / 4.4 / 5.5 and 6.8 / 6.9 / 7.1;
+//   x 2560 x 8192 7.6 / 9.9 / 13.7 and 10.2 / 10.2 / 10.6; 16 x 5003 x 8192 17.9 and 14.7;
+// - 16 rows x 49152 x 2560, the weights from HBM, 27.7 and 29.2; 8 x 16384 x 2560 9.8 and 10.3;
+//   beyond 48 KB of x in LDS 16 x 49152 x 4096 42.9 and 42.7, 16 x 16384 x 4096 15.8 and 15.1;
 // - 32 rows x 16384 x 2560 11.8 and 10.9, 24 x 32768 x 2560 20.8 and 18.0, 32 x 49152 x 2560 29.9 and 31.4;
 // - short rows, whose K is too little for eight waves: 16 x 16384 x 512 6.1 and 4.7.
 constexpr int FEW_LDS_KB = 48;
@@ -588,12 +610,15 @@ I8Plan i8_plan(int m, int n, int k) {
   if (i8_few_rows(m, n, k)) return p;
   const int steps = (k + 127) / 128;
   auto tiles = [&](int b) { return (int64_t)((m + b - 1) / b) * ((n + b - 1) / b); };
-  // us of a round of 256 tiles: its start and end and each step, as measured over m 33..2048, n 512..16384 and k 512..8192
-  // (252 products: 1% over the best kind for each in the mean, 30% at most)
-  auto rounds = [&](int b, double ends, double step) { return (double)((tiles(b) + 255) / 256) * (ends + step * steps); };
+  // us of a round of 256 tiles: its start and end and each step, as measured over m 33..2048, n 512..16384 and
+  // k 512..8192 (252 products: 1% over the best kind for each in the mean, 30% at most)
+  auto rounds = [&](int b, double ends, double step) {
+    return (double)((tiles(b) + 255) / 256) * (ends + step * steps);
+  };
   double t64 = rounds(64, 1.0, 0.19);
   const double t128 = rounds(128, 2.0, 0.48), t256 = rounds(256, 4.0, 1.4);
-  // few tiles: K in parts of twelve steps at least, 2.5 us to join them (64 x 2560 x 8192: 11.0 in five parts, 17 in one)
+  // few tiles: K in parts of twelve steps at least, 2.5 us to join them (64 x 2560 x 8192: 11.0 in five parts,
+  // 17 in one)
   const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 12, 256 / tiles(64)));
   if (parts > 1) t64 = 3.5 + 0.19 * steps / parts;
   p.kind = t64 <= t128 && t64 <= t256 ? I8_T64 : t128 <= t256 ? I8_T128 : I8_T256;
@@ -631,10 +656,13 @@ void i8_tiles(const I8Tile& a, bool f32, hipStream_t s) {
 }  // namespace
 
 int i8_quantize(const uint16_t* x, int8_t* q, float* scale, int32_t rows, int32_t k, hipStream_t s) {
-  // us, wave per row and workgroup per row: 32 x 2560 3.5 and 3.0, 1024 x 2560 3.9 and 4.0, 2048 x 2560 5.3 and 5.8; 1024 x
-  // 8192, which a wave reads twice, 12.0 and 7.5
-  if (rows >= 1024 && k <= 64 * 8 * Q8_KEEP) hipLaunchKernelGGL(k_quantize_i8<1>, dim3((rows + 3) / 4), dim3(Q8_NT), 0, s, x, q, scale, rows, k);
-  else hipLaunchKernelGGL(k_quantize_i8<4>, dim3(rows), dim3(Q8_NT), 0, s, x, q, scale, rows, k);
+  // us, wave per row and workgroup per row: 32 x 2560 3.5 and 3.0, 1024 x 2560 3.9 and 4.0, 2048 x 2560 5.3 and 5.8;
+  // 1024 x 8192, which a wave reads twice, 12.0 and 7.5
+  const dim3 nt(Q8_NT);
+  if (rows >= 1024 && k <= 64 * 8 * Q8_KEEP)
+    hipLaunchKernelGGL(k_quantize_i8<1>, dim3((rows + 3) / 4), nt, 0, s, x, q, scale, rows, k);
+  else
+    hipLaunchKernelGGL(k_quantize_i8<4>, dim3(rows), nt, 0, s, x, q, scale, rows, k);
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
 }
 
@@ -654,16 +682,18 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
     else i8_few<1, FEW_LDS_KB, false>(a, 2, y_fp32, s);
   } else {
     const I8Tile a{xq, wq, xs, ws, p.splits > 1 ? work : y, m, n, k, p.mblk, p.nblk, p.splits, p.sps};
-    // up to 256 tiles a CU holds one workgroup, which may have all of its LDS; beyond, two that take turns at waiting: us,
-    // two and one, 128 x 128 tiles of 1500 x 5003 x 2560 (480) 27 and 31, 64 x 64 of 2048 x 2560 x 512 (1280) 11 and 17
+    // up to 256 tiles a CU holds one workgroup, which may have all of its LDS; beyond, two that take turns at waiting:
+    // us, two and one, 128 x 128 tiles of 1500 x 5003 x 2560 (480) 27 and 31, 64 x 64 of 2048 x 2560 x 512 (1280) 11
+    // and 17
     const bool one = (int64_t)p.mblk * p.nblk * p.splits <= 256;
     if (p.kind == I8_T256) i8_tiles<256, 1, 2, 4, 5>(a, y_fp32, s);
     else if (p.kind == I8_T128) one ? i8_tiles<128, 1, 2, 4, 8>(a, y_fp32, s) : i8_tiles<128, 1, 2, 2, 4>(a, y_fp32, s);
     else one ? i8_tiles<64, 4, 1, 1, 4>(a, y_fp32, s) : i8_tiles<64, 1, 2, 2, 8>(a, y_fp32, s);
     if (p.splits > 1) {
-      const dim3 grid((unsigned)(((int64_t)m * n + 1023) / 1024));
-      if (y_fp32) hipLaunchKernelGGL(k_i8_join<true>, grid, dim3(256), 0, s, static_cast<const int*>(work), p.splits, xs, ws, y, m, n);
-      else hipLaunchKernelGGL(k_i8_join<false>, grid, dim3(256), 0, s, static_cast<const int*>(work), p.splits, xs, ws, y, m, n);
+      const dim3 grid((unsigned)(((int64_t)m * n + 1023) / 1024)), nt(256);
+      const int* part = static_cast<const int*>(work);
+      if (y_fp32) hipLaunchKernelGGL(k_i8_join<true>, grid, nt, 0, s, part, p.splits, xs, ws, y, m, n);
+      else hipLaunchKernelGGL(k_i8_join<false>, grid, nt, 0, s, part, p.splits, xs, ws, y, m, n);
     }
   }
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;

@@ -52,8 +52,8 @@ struct LpArgs {
   int32_t* rank;                // [rows]
   int32_t* top_ids;             // [rows, top]
   float* top_lp;                // [rows, top]
-  // chunks > 1: per (row, chunk) maximum, s, u, rank count (its bits) and the first `top` keys, in order, then zeros; per
-  // row the token's logit and whether there is one
+  // chunks > 1: per (row, chunk) maximum, s, u, rank count (its bits) and the first `top` keys, in order, then zeros;
+  // per row the token's logit and whether there is one
   float4* part;
   u64* cand;
   float2* given;
@@ -85,9 +85,9 @@ __device__ __forceinline__ LpToken lp_token(const LpArgs& a, int64_t row) {
   return k;
 }
 
-// The first `top` of the waves' candidates (sh.kept of them each, <= LP_KEEP; a barrier lies behind them), in order: out(
-// place, key) in wave 0, key 0 past the last. A key's place is the number of larger ones: lanes take candidates, each
-// wave counts over its own.
+// The first `top` of the waves' candidates (sh.kept of them each, <= LP_KEEP; a barrier lies behind them), in order:
+// out(place, key) in wave 0, key 0 past the last. A key's place is the number of larger ones: lanes take candidates,
+// each wave counts over its own.
 template <class F>
 __device__ __forceinline__ void lp_sort(LpShared& sh, int top, F out) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -178,6 +178,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
+// how many of these lanes are below this one
+__device__ __forceinline__ int lp_below(u64 lanes) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+}
 // how many lanes of the wave
 __device__ __forceinline__ int lp_count(bool is) { return __builtin_popcountll(__ballot(is)); }
 
@@ -191,6 +195,9 @@ __device__ __forceinline__ void lp_join(float& m, float& s, float& u) {
 }
 
 // One chunk of a row per workgroup, in steps of LP_E values per thread; the next step's loads are in flight meanwhile.
+// 1024 rows of 49152 (fp32, top 5) 39 us, 5.1 TB/s, the rate of a large copy here, with the vector ALUs busy in more than
+// half of the cycles (17 instructions a value); 34 without alternatives, two steps in flight no faster. One row of 49152,
+// twelve chunks, 6.1 us and 3.6 to merge them: a launch and a memory latency each, and the alternatives' places (1.8).
 template <bool BF16>
 __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
   constexpr int V = BF16 ? 8 : 4;  // consecutive values of a load (16 bytes, aligned to the type only)
@@ -240,7 +247,8 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
       const uint32_t w = cur[e / V][(BF16 ? e / 2 : e) & 3];
       x[e] = !BF16 ? __uint_as_float(w) : e & 1 ? bfhi(w) : bflo(w);
     }
-    float top = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), x[5], x[6]);  // NaN is passed over; it comes back through s
+    // NaN is passed over; it comes back through s
+    float top = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), x[5], x[6]);
     top = max3(max3(max3(max3(top, x[7], x[8]), x[9], x[10]), x[11], x[12]), x[13], x[14]);
     top = max3(top, x[15], x[15]);
     const float old = m;
@@ -266,7 +274,7 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
       auto take = [&](bool is, float v, int j) {
         const u64 lanes = __ballot(is);
         if (lanes == 0) return;
-        const int at = kept + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+        const int at = kept + lp_below(lanes);
         if (is && at < LP_KEEP) sh.cand[wave][at] = lp_key(v, j);
         kept += __builtin_popcountll(lanes);
       };
@@ -381,7 +389,7 @@ __global__ __launch_bounds__(LP_NT) void k_logprobs_merge(LpArgs a) {
     for (int i = 0; i < E; ++i) {
       const bool is = mine[i] != 0 && !(lp_value(mine[i]) < t);
       const u64 lanes = __ballot(is);
-      const int at = kept + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+      const int at = kept + lp_below(lanes);
       if (is) sh.cand[wave][at] = mine[i];
       kept += __builtin_popcountll(lanes);
     }
@@ -443,7 +451,7 @@ int lp_run(LpArgs a, bool bf16, int rows, void* work, hipStream_t s) {
 
 // Features -> log probabilities: blocks of rows through the 8-bit head, whose fp32 logits stay in the workspace, up to
 // 256 MB of them. 1024 rows of 49152 in one block are three whole rounds of 256 x 256 tiles, 512 one and a half, which
-// take two: 199 us in one block, 248 in two, though the last-level cache holds the logits of the smaller ones.
+// take two: 185 us in one block, 215 in two (2048 rows in blocks of 256 / 512 MB: 395 / 379).
 struct HeadPlan {
   int rows;  // of a block
   int64_t logits, linear, lp, bytes;

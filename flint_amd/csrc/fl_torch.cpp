@@ -285,17 +285,20 @@ pybind11::object int8_fast(const torch::Tensor& x, const std::optional<torch::Te
 // A contiguous tensor over part of base's storage, without the dispatcher's view machinery (0.2 us instead of 0.7;
 // an allocation takes 1.3)
 torch::Tensor piece(const torch::Tensor& base, int64_t byte, torch::IntArrayRef sizes, torch::ScalarType dt) {
-  auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(dt));
+  auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(),
+                                                    c10::scalarTypeToTypeMeta(dt));
   t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
   t.unsafeGetTensorImpl()->set_storage_offset(byte / (int64_t)c10::elementSize(dt));
   return t;
 }
 
-// Outputs of generate.logprobs and generate.head_logprobs, rows of them: the floats in one allocation, the integers in
-// another (torch.save refuses types that share one)
+// Outputs of generate.logprobs and generate.head_logprobs, rows of them, and the call's workspace: the floats in one
+// allocation, the integers in another (torch.save refuses types that share one). A workspace of up to 4 KB, a row's or
+// two's, lies behind the floats: an allocation is 1.3 of a call's 10 us, and no more than that stays with the results.
 struct LogprobOut {
-  torch::Tensor logprob, entropy, rank, ids, top;
-  void make(int64_t rows, int64_t n, bool tokens, const torch::Tensor& like) {
+  torch::Tensor logprob, entropy, rank, ids, top, own;
+  void* work = nullptr;
+  void make(int64_t rows, int64_t n, bool tokens, int64_t need, const torch::Tensor& like) {
     torch::Tensor all;
     int64_t at = 0;
     auto open = [&](int64_t words) { all = bytes_of(4 * words, like), at = 0; };
@@ -304,7 +307,10 @@ struct LogprobOut {
       at += 4 * t.numel();
       return t;
     };
-    open(rows * ((tokens ? 2 : 1) + n));
+    const int64_t floats = rows * ((tokens ? 2 : 1) + n), behind = (floats + 3) / 4 * 4;
+    open(need <= 4096 ? behind + (need + 3) / 4 : floats);
+    if (need <= 4096) work = need > 0 ? static_cast<char*>(all.data_ptr()) + 4 * behind : nullptr;
+    else own = bytes_of(need, like), work = own.data_ptr();
     entropy = next({rows}, torch::kFloat32);
     if (tokens) logprob = next({rows}, torch::kFloat32);
     if (n > 0) top = next({rows, n}, torch::kFloat32);
@@ -341,13 +347,12 @@ pybind11::object logprobs_fast(const torch::Tensor& l, const std::optional<torch
   int rc = FL_E_HIP;
   try {
     pybind11::gil_scoped_release nogil;
-    o.make(rows, top, tokens.has_value(), l);
-    const torch::Tensor work = bytes_of(need, l);
+    o.make(rows, top, tokens.has_value(), need, l);
     rc = fl_logprobs(l.data_ptr(), bf16, stride, (int32_t)rows, (int32_t)vocab,
                      tokens ? static_cast<const int32_t*>(tokens->data_ptr()) : nullptr, (int32_t)top,
                      static_cast<float*>(data_of(o.logprob)), static_cast<float*>(data_of(o.entropy)),
                      static_cast<int32_t*>(data_of(o.rank)), static_cast<int32_t*>(data_of(o.ids)),
-                     static_cast<float*>(data_of(o.top)), data_of(work), stream_of(stream));
+                     static_cast<float*>(data_of(o.top)), o.work, stream_of(stream));
   } catch (const c10::OutOfMemoryError&) {
   }
   return rc == FL_OK ? o.cast() : pybind11::object(pybind11::none());
@@ -370,14 +375,13 @@ pybind11::object head_logprobs_fast(const torch::Tensor& x, const torch::Tensor&
   int rc = FL_E_HIP;
   try {
     pybind11::gil_scoped_release nogil;
-    o.make(m, top, tokens.has_value(), x);
-    const torch::Tensor work = bytes_of(need, x);
+    o.make(m, top, tokens.has_value(), need, x);
     rc = fl_head_logprobs(static_cast<const uint16_t*>(x.data_ptr()), static_cast<const int8_t*>(wq.data_ptr()),
                           static_cast<const float*>(ws.data_ptr()),
                           tokens ? static_cast<const int32_t*>(tokens->data_ptr()) : nullptr, (int32_t)top,
                           static_cast<float*>(data_of(o.logprob)), static_cast<float*>(data_of(o.entropy)),
                           static_cast<int32_t*>(data_of(o.rank)), static_cast<int32_t*>(data_of(o.ids)),
-                          static_cast<float*>(data_of(o.top)), data_of(work), (int32_t)m, (int32_t)n, (int32_t)k,
+                          static_cast<float*>(data_of(o.top)), o.work, (int32_t)m, (int32_t)n, (int32_t)k,
                           stream_of(stream));
   } catch (const c10::OutOfMemoryError&) {
   }

@@ -233,8 +233,8 @@ def workspace(name, *sizes, device):
 
 def quantize_int8(x, q=None, scale=None):
     """Rows of a bf16 [M, K] device matrix in 8 bits: (q int8 [M, K], scale fp32 [M]), scale = max|row| times
-    fp32(1 / 127) and q = row / scale rounded to the nearest, ties to even (fl_quantize_int8). For a weight matrix these are its
-    output channels, for activations the tokens."""
+    fp32(1 / 127) and q = row / scale rounded to the nearest, ties to even (fl_quantize_int8). For a weight matrix the
+    rows are its output channels, for activations the tokens."""
     _check_dev(x, torch.bfloat16, "x")
     if x.dim() != 2:
         raise ValueError("x must be [M, K]")

@@ -136,15 +136,15 @@ int fl_gemv_int4_tiled(const uint32_t* qt, const uint32_t* sz, const uint16_t* x
 /* ---- 8-bit integer products ---------------------------------------------------------------- */
 
 /* Rows in 8 bits, one scale each: a row r (bf16, K % 16 == 0, K <= 65536) becomes scale = max|r| * fp32(1 / 127),
- * rounded to fp32, and q = r / scale rounded to the nearest whole number, ties to even (the quotient exact); a zero row: scale 0, q 0; a row
- * with a NaN or an infinity: scale NaN, q 0. Weights have one scale per output channel this way, activations one per
- * token. x and q 16-byte aligned, at most 2^23 rows.
+ * rounded to fp32, and q = r / scale rounded to the nearest whole number, ties to even (the quotient exact); a zero
+ * row: scale 0, q 0; a row with a NaN or an infinity: scale NaN, q 0. Weights have one scale per output channel this
+ * way, activations one per token. x and q 16-byte aligned, at most 2^23 rows.
  * No counterpart in the reference's engine, which has int4 weights only. */
 int fl_quantize_int8(const uint16_t* x, int8_t* q, float* scale, int32_t rows, int32_t k, void* stream);
 
 /* y[m, n] = fp32(sum_k xq[m, k] wq[n, k]) * fp32(xs[m] * ws[n]), rounded to bf16 (y_fp32 = 0, y uint16 [M, N]) or
- * left as it is (y_fp32 != 0, y float [M, N]). The sum is exact (int32, K <= 65536), so a row's result does not depend on
- * the other rows, on M or on how the work is cut. xq [M, K] and wq [N, K] row-major, any values of int8, K % 16 ==
+ * left as it is (y_fp32 != 0, y float [M, N]). The sum is exact (int32, K <= 65536), so a row's result does not depend
+ * on the other rows, on M or on how the work is cut. xq [M, K] and wq [N, K] row-major, any values of int8, K % 16 ==
  * 0; xq, wq, y and work 16-byte aligned; M, N at most 2^23. work: device memory of the bytes that
  * fl_gemm_int8_workspace gives (0: may be NULL), free for reuse once the call's work on the stream is done, not to be
  * shared by calls that may run at the same time.
@@ -165,18 +165,19 @@ int fl_linear_int8(const uint16_t* x, const int8_t* wq, const float* ws, void* y
  * indices come before tokens[row] when ordered by value, larger first, equal values by rising index (NaN first; -0
  * equals 0); top_ids / top_logprobs [rows, top] = the first `top` (0..32, <= vocab) of that order and their log
  * probabilities. fp32 throughout. A logit of -inf has probability 0. A row that is all -inf, or holds a +inf or a NaN,
- * has no distribution: its log probabilities and entropy are NaN, its rank and top_ids as defined. A token id outside the
- * vocabulary (a padded row): logprob NaN, rank -1. tokens may be NULL (then logprob and rank may be too and are not
- * written), top_ids and top_logprobs where top = 0. All pointers are device pointers; logits aligned to their type. work: 16-byte aligned, of fl_logprobs_workspace's bytes (0: may be NULL),
- * free for reuse once the call's work on the stream is done.
+ * has no distribution: its log probabilities and entropy are NaN, its rank and top_ids as defined. A token id outside
+ * the vocabulary (a padded row): logprob NaN, rank -1. tokens may be NULL (then logprob and rank may be too and are not
+ * written), top_ids and top_logprobs where top = 0. All pointers are device pointers; logits aligned to their type.
+ * work: 16-byte aligned, of fl_logprobs_workspace's bytes (0: may be NULL), free for reuse once the call's work on the
+ * stream is done, not to be shared by calls that may run at the same time.
  * No counterpart in the reference, whose sample (engine/generate.py:36-55) returns tokens and probabilities. */
 int fl_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top, int64_t* bytes);
 int fl_logprobs(const void* logits, int32_t bf16, int64_t stride, int32_t rows, int32_t vocab, const int32_t* tokens,
                 int32_t top, float* logprob, float* entropy, int32_t* rank, int32_t* top_ids, float* top_logprobs,
                 void* work, void* stream);
-/* The same from features x (bf16 [M, K]) through an 8-bit vocabulary head wq [N, K], ws [N]: fl_linear_int8's product in
- * fp32 and fl_logprobs of it, without M x N logits in memory at once (up to 256 MB of them in work, or one row's). Limits of both. A
- * row's logits, ranks and top_ids do not depend on the other rows; the order of its fp32 sums does. */
+/* The same from features x (bf16 [M, K]) through an 8-bit vocabulary head wq [N, K], ws [N]: fl_linear_int8's product
+ * in fp32 and fl_logprobs of it, without M x N logits in memory at once (up to 256 MB of them in work, or one row's).
+ * Limits of both. A row's logits, ranks and top_ids do not depend on the other rows; the order of its fp32 sums does. */
 int fl_head_logprobs_workspace(int32_t m, int32_t n, int32_t k, int32_t top, int64_t* bytes);
 int fl_head_logprobs(const uint16_t* x, const int8_t* wq, const float* ws, const int32_t* tokens, int32_t top,
                      float* logprob, float* entropy, int32_t* rank, int32_t* top_ids, float* top_logprobs, void* work,
