@@ -146,13 +146,24 @@ __device__ __forceinline__ void i8_store(void* y, int64_t at, int acc, float s) 
 // without the sums' meeting, is no faster); below some 10 MB of weights by one launch's start, a memory latency and the end:
 // 2560 x 2560 with one row quantised here 5.1 us.
 constexpr int FEW_KW = 8;
-constexpr int QF_MOST = 16384, QF_KEEP = 8;  // values that a workgroup quantises; 8-value pieces of a lane
+constexpr int QF_MOST = 32768, QF_KEEP = 8;  // values that a workgroup quantises; 8-value pieces of a lane
 // log2 of the waves of a row, so that the eight hold as many rows at once as there are (all eight one row at most)
 __host__ __device__ inline int qf_log_waves(int m) { return m > 4 ? 0 : m > 2 ? 1 : m > 1 ? 2 : 3; }
-// whether the waves hold the rows in QF_KEEP pieces a lane
-inline bool qf_fits(int m, int k) {
+// Whether the product's workgroups quantise the rows themselves: if the waves hold them in QF_KEEP pieces a lane, and if
+// it beats a launch of its own before the product. us, on the way and before it, of the kernels alone; called one by one
+// the two launches take 8 at least.
+// - up to 4 rows: 2 x 2560 x 2560 5.4 and 6.0, 4 x 5003 x 8192 15.7 and 17.4, 4 x 16384 x 4096 15.2 and 17.0; but
+//   4 x 49152 x 512 11.7 and 10.4, the rows again in every workgroup beside a short K;
+// - up to 8: 8 x 49152 x 2560 26.8 and 29.8; 8 x 16384 x 1600 10.5 and 9.8, 8 x 8192 x 2560 10.1 and 9.2; while two
+//   launches take longer to call than to run, 8 x 2560 x 2048 5.8 and 6.1, 8 x 5003 x 1600 7.7 and 6.4;
+// - up to 16 only then: 16 x 2560 x 1024 6.0 and 5.9; 16 x 5003 x 1024 8.4 and 7.2, 16 x 49152 x 2048 24.0 and 23.5.
+inline bool qf_pays(int m, int n, int k) {
   const int lw = qf_log_waves(m), slots = FEW_KW >> lw, w = 64 << lw;
-  return m <= 16 && m * (int64_t)k <= QF_MOST && (m + slots - 1) / slots * ((k / 8 + w - 1) / w) <= QF_KEEP;
+  const int64_t values = (int64_t)m * k;
+  if (m > 16 || values > QF_MOST || (m + slots - 1) / slots * ((k / 8 + w - 1) / w) > QF_KEEP) return false;
+  if (m <= 4) return k >= 1024 || n < 32768;
+  if (n < (m > 8 ? 4096 : 8192)) return values <= 16384;
+  return m <= 8 && n >= 32768 && k > 1024;
 }
 // of x rows in LDS: r and r + 8 on the same banks
 __host__ __device__ inline int few_pitch(int k) { return ((k + 63) >> 6) * 64 + 16; }
@@ -167,7 +178,7 @@ struct I8Few {
 template <int MB, int XKB, bool QUANT, bool F32>
 __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
   constexpr int KW = FEW_KW, U = 5;
-  static_assert(!QUANT || (MB == 1 && XKB * 1024 >= QF_MOST + 16 * 64), "rows that are quantised here");
+  static_assert(!QUANT || (MB == 1 && XKB * 1024 >= QF_MOST + 16 * 64), "the rows, each up to 64 bytes longer");
   __shared__ __align__(16) int part[XKB ? 2 : 1][KW][MB][256];
   __shared__ __align__(16) unsigned char xl[XKB ? XKB * 1024 : 16];
   __shared__ float most[16][KW], sx[16];
@@ -231,7 +242,7 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
   }
   if constexpr (QUANT) {
     // Waves in `slots` groups of W: a group takes rows slot, slot + slots, ..., its waves 64 W pieces of 8 values at a
-    // time; the pieces (QF_KEEP a lane at most, by the rule of who comes here) stay in registers between the maximum
+    // time; the pieces (QF_KEEP a lane at most, by qf_pays) stay in registers between the maximum
     // and the quotients.
     const int lw = qf_log_waves(m), W = 1 << lw, slots = KW >> lw, slot = wave >> lw, sub = wave & (W - 1);
     const int nc = k >> 3, cpr = (nc + 64 * W - 1) >> (6 + lw);
@@ -700,14 +711,14 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
 }
 
 int64_t i8_linear_bytes(int32_t m, int32_t n, int32_t k) {
-  if (qf_fits(m, k)) return 0;
+  if (qf_pays(m, n, k)) return 0;
   return i8_pad((int64_t)m * k) + i8_pad((int64_t)m * 4) + i8_gemm_bytes(m, n, k);
 }
 
 int i8_linear(const uint16_t* x, const int8_t* wq, const float* ws, void* y, bool y_fp32, void* work, int32_t m,
               int32_t n, int32_t k, hipStream_t s) {
-  if (qf_fits(m, k)) {
-    i8_few<1, 20, true>(I8Few{x, nullptr, wq, ws, y, m, n, k}, 2, y_fp32, s);
+  if (qf_pays(m, n, k)) {
+    i8_few<1, 36, true>(I8Few{x, nullptr, wq, ws, y, m, n, k}, 2, y_fp32, s);
     return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
   }
   int8_t* xq = static_cast<int8_t*>(work);

@@ -287,3 +287,16 @@ def test_linears_that_quantise_on_the_way(dev, m):
         wq, ws = ints(n, k, m), torch.rand(n, generator=torch.Generator().manual_seed(m)) * 1e-3
         y = quantize.linear_int8(x.to(dev), wq.to(dev), ws.to(dev), torch.float32)
         assert same(y, scoring.product(*scoring.quantize_rows(x), wq, ws)), k
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 2577, 32768), (2, 1001, 16384), (3, 2577, 8192), (3, 2577, 8208), (4, 4097, 8192),
+                                   (4, 40, 8208), (2, 32767, 512), (2, 32768, 512), (5, 32801, 1040), (8, 32801, 4096),
+                                   (8, 33000, 4112), (7, 49152, 2560), (5, 8191, 3264), (8, 8191, 2048), (9, 8191, 1040),
+                                   (16, 4095, 1024), (16, 4096, 1024), (15, 77, 1088), (9, 33000, 1040)])
+def test_linears_on_both_sides_of_the_rules_lines(dev, m, n, k):
+    x = rows_of(m, k, n, "outliers")
+    x[m // 2, k // 2:] = 0.0
+    wq, ws = ints(n, k, m), torch.rand(n, generator=torch.Generator().manual_seed(m)) * 1e-3
+    ref = scoring.product(*scoring.quantize_rows(x), wq, ws)
+    assert torch.equal(quantize.linear_int8(x.to(dev), wq.to(dev), ws.to(dev), torch.float32).cpu(), ref)
+    assert torch.equal(quantize.linear_int8(x.to(dev), wq.to(dev), ws.to(dev)).cpu(), ref.to(torch.bfloat16))
