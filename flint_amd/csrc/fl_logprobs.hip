@@ -64,7 +64,7 @@ struct LpShared {
   float4 red[LP_NW];  // maximum, s, u, rank count of each wave
   int kept[LP_NW];    // candidates of each wave
   int place[LP_NW][FL_WAVE];
-  u64 cand[LP_NW][LP_KEEP];  // their keys
+  u64 cand[LP_NW][LP_KEEP];  // their keys, zeros up to the next multiple of eight
 };
 
 // the row's token and its logit; in = false (no token asked for, or an id outside the vocabulary): NaN
@@ -103,8 +103,9 @@ __device__ __forceinline__ void lp_sort(LpShared& sh, int top, F out) {
       if (w == v && i >= n[v]) i -= n[v], ++w;
     const u64 key = b + lane < c ? sh.cand[w][i] : 0;
     int larger = 0;
-#pragma unroll 8
-    for (int j = 0; j < own; ++j) larger += sh.cand[wave][j] > key;
+    for (int j = 0; j < own; j += 8)  // zeros behind the last
+#pragma unroll
+      for (int i = 0; i < 8; ++i) larger += sh.cand[wave][j + i] > key;
     sh.place[wave][lane] = larger;
     __syncthreads();
     if (wave == 0 && key != 0) {
@@ -117,30 +118,45 @@ __device__ __forceinline__ void lp_sort(LpShared& sh, int top, F out) {
   }
 }
 
-// Of values with a lane each, the q-th largest of the wave, which q reach; stored for others to read at any time (rising
-// values only make it rise). On ordered whole numbers, whose maximum is one DPP instruction a step: 190 cycles a
-// place; a ballot for each of 16 bits instead takes 1300.
+// A value that q of G groups of lanes reach, close to the q-th largest of theirs: v orders as unsigned and agrees in the
+// 64 / G (or, with G = 32, the lower) lanes of a group. The last bits tell equal groups apart and are dropped from the
+// answer. Every group counts the larger ones: 16 groups 300 cycles, against 190 for each of q rounds of maxima.
+template <int G>
+__device__ __forceinline__ uint32_t lp_reached(uint32_t v, int q) {
+  constexpr int N = G == 32 ? 1 : FL_WAVE / G;  // lanes of a group
+  const int lane = threadIdx.x & 63;
+  v = (v & ~(uint32_t)(G - 1)) | (uint32_t)(lane / N % G);
+  int larger = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) larger += (uint32_t)__builtin_amdgcn_readlane((int)v, g * N) > v;
+  const u64 at = __ballot(larger == q - 1);  // q = 0: nowhere, any value will do
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, __builtin_ctzll(at | (1ull << 63))) & ~(uint32_t)(G - 1);
+}
 template <int CTRL>
 __device__ __forceinline__ uint32_t umax_dpp(uint32_t v) {
   return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
 }
 __device__ __forceinline__ uint32_t wave_umax32(uint32_t v) {
-  v = umax_dpp<0xB1>(v);   // lane ^ 1
-  v = umax_dpp<0x4E>(v);   // lane ^ 2
-  v = umax_dpp<0x141>(v);  // the other four of 8
-  v = umax_dpp<0x140>(v);  // the other eight of 16
+  v = umax_dpp<0x4E>(umax_dpp<0xB1>(v));  // of 4 lanes
+  v = umax_dpp<0x140>(umax_dpp<0x141>(v));  // of 16
   const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
   v = max(r[0], r[1]);
   const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   return max(q[0], q[1]);
 }
-__device__ __forceinline__ void lp_publish(uint32_t* bound, float mine, int q) {
+// Of values with a lane each, one that q of the wave's lanes reach, stored for the other waves to read at any time
+// (rising values only make it rise): close to the q-th largest where it is asked for once, the chunk being one step; else
+// the q-th largest, in q rounds, as a higher bound spares candidates in all the steps that follow (1024 rows of 49152,
+// top 32: 49 us, 55 without).
+__device__ __forceinline__ void lp_publish(uint32_t* bound, float mine, int q, bool once) {
   const uint32_t b = __float_as_uint(mine + 0.0f);  // -0 becomes 0
   uint32_t v = mine == mine ? b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u) : 0u, t = 0;
-  for (int r = 0; r < q; ++r) {
-    t = wave_umax32(v);
-    if ((threadIdx.x & 63) == __builtin_ctzll(__ballot(v == t) | (1ull << 63))) v = 0;
-  }
+  if (once && q <= 16) t = lp_reached<16>(umax_dpp<0x4E>(umax_dpp<0xB1>(v)), q);
+  else
+    for (int r = 0; r < q; ++r) {
+      t = wave_umax32(v);
+      if ((threadIdx.x & 63) == __builtin_ctzll(__ballot(v == t) | (1ull << 63))) v = 0;
+    }
   if ((threadIdx.x & 63) == 0)
     __hip_atomic_store(bound + (threadIdx.x >> 6), t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
@@ -267,26 +283,49 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
     const int jt = jb + tid * V;  // e's index: jt + (e / V) * LP_NT * V + e % V
     if (a.top > 0) {
       if ((i & (i + 1)) == 0) {  // steps 0, 1, 3, 7, ...
-        lp_publish(sh.bound, m, q);
+        lp_publish(sh.bound, m, q, j1 - j0 <= LP_STEP);
         if (i == 0) __syncthreads();
         T = lp_least(sh.bound, full);
       }
-      auto take = [&](bool is, float v, int j) {
-        const u64 lanes = __ballot(is);
-        if (lanes == 0) return;
-        const int at = kept + lp_below(lanes);
-        if (is && at < LP_KEEP) sh.cand[wave][at] = lp_key(v, j);
-        kept += __builtin_popcountll(lanes);
-      };
-      if (T == -INFINITY) {  // all that is larger, and the chunk's first values by index
+      if (i == 0) {
+        // The first step has most of them, in any of a lane's values: a candidate of every lane that has one at a time
+        // (16 ballots in a row take twice as long). T = -inf: all that is larger, and the chunk's first values by index.
+        uint32_t mask = 0;  // value e: bit 15 - e
+        if (T == -INFINITY) {
 #pragma unroll
-        for (int e = 0; e < LP_E; ++e) {
-          const int j = jt + (e / V) * LP_NT * V + e % V;
-          take(j < j1 && (!(x[e] <= T) || j < j0 + a.top), x[e], j);
+          for (int e = 0; e < LP_E; ++e) {
+            const int j = jt + (e / V) * LP_NT * V + e % V;
+            mask = mask << 1 | (uint32_t)(j < j1 && (!(x[e] <= T) || j < j0 + a.top));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < LP_E; ++e) mask = mask << 1 | (uint32_t)!(x[e] < T);
         }
-      } else if (__ballot(s != s || top >= T) != 0) {
+        for (u64 lanes; (lanes = __ballot(mask != 0)) != 0; mask &= mask - 1) {
+          const int b = __builtin_ctz(mask | 1u << LP_E), e = LP_E - 1 - b;
+          float half[LP_E];
 #pragma unroll
-        for (int e = 0; e < LP_E; ++e) take(!(x[e] < T), x[e], jt + (e / V) * LP_NT * V + e % V);
+          for (int i = 0; i < LP_E; ++i) half[i] = x[LP_E - 1 - i];
+#pragma unroll
+          for (int w = LP_E / 2, bit = 1; w > 0; w /= 2, bit *= 2)
+#pragma unroll
+            for (int i = 0; i < w; ++i) half[i] = b & bit ? half[2 * i + 1] : half[2 * i];
+          const int at = kept + lp_below(lanes);
+          if (mask != 0 && at < LP_KEEP) sh.cand[wave][at] = lp_key(half[0], jt + e / V * (LP_NT * V) + e % V);
+          kept += __builtin_popcountll(lanes);
+        }
+      } else {
+        const float least = fmaxf(T, -3.4028235e38f);  // -inf counts among the chunk's first values only
+        if (__ballot(s != s || top >= least) != 0) {
+#pragma unroll
+          for (int e = 0; e < LP_E; ++e) {
+            const u64 lanes = __ballot(!(x[e] < least));
+            if (lanes == 0) continue;
+            const int at = kept + lp_below(lanes);
+            if (!(x[e] < least) && at < LP_KEEP) sh.cand[wave][at] = lp_key(x[e], jt + (e / V) * LP_NT * V + e % V);
+            kept += __builtin_popcountll(lanes);
+          }
+        }
       }
     }
     if (tok.in) {  // last: the token's logit comes from two loads in a row
@@ -310,6 +349,7 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
   }
   lp_join(m, s, u);
   if (lane == 0) sh.red[wave] = make_float4(m, s, u, __int_as_float(before)), sh.kept[wave] = kept;
+  if (lane < 8 && (kept & 7) + lane < 8 && kept + lane < LP_KEEP) sh.cand[wave][kept + lane] = 0;
   __syncthreads();
   int most = 0;
   before = 0;
@@ -331,7 +371,7 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
       u += (w[k].z + w[k].y * d) * e;
     }
   }
-  const float logs = lp_logsum(m, s);
+  const float logs = a.chunks == 1 ? lp_logsum(m, s) : 0.0f;
   const int64_t at = row * a.chunks + chunk;
   auto out = [&](int place, u64 key) {
     if (a.chunks == 1) lp_place(a, row, m, logs, place, key);
@@ -373,27 +413,24 @@ __global__ __launch_bounds__(LP_NT) void k_logprobs_merge(LpArgs a) {
   const int64_t row = blockIdx.x;
   const u64* cand = a.cand + row * keys;
   const float4 p = lane < a.chunks ? a.part[row * a.chunks + lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-  u64 mine[E];
-  float largest = -INFINITY;  // NaN is passed over
   if (a.top > 0) {
+    u64 mine[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) mine[i] = i * LP_NT + tid < keys ? cand[i * LP_NT + tid] : 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) largest = fmaxf(largest, mine[i] != 0 ? lp_value(mine[i]) : -INFINITY);
-    const int full = min(LP_NW, keys / FL_WAVE), q = full > 0 ? (a.top + full - 1) / full : 0;
-    lp_publish(sh.bound, largest, q);
-    __syncthreads();
-    const float t = lp_least(sh.bound, full);
+    // At least `top` keys reach what q chunks' keys at place `at` do, with at so that q is about half of the chunks.
+    const int at = min((2 * a.top + a.chunks - 1) / a.chunks, a.top) - 1, q = (a.top + at) / (at + 1);
+    const uint32_t t = lp_reached<LP_CHUNKS>(lane < a.chunks ? (uint32_t)(cand[lane * a.top + at] >> 32) : 0u, q);
     int kept = 0;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const bool is = mine[i] != 0 && !(lp_value(mine[i]) < t);
+      const bool is = mine[i] != 0 && (uint32_t)(mine[i] >> 32) >= t;
       const u64 lanes = __ballot(is);
       const int at = kept + lp_below(lanes);
       if (is) sh.cand[wave][at] = mine[i];
       kept += __builtin_popcountll(lanes);
     }
     if (lane == 0) sh.kept[wave] = kept;
+    if (lane < 8 && (kept & 7) + lane < 8 && kept + lane < LP_KEEP) sh.cand[wave][kept + lane] = 0;
   }
   LpToken tok{-1, false, 0.0f};
   if (a.tokens) {

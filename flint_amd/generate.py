@@ -129,13 +129,13 @@ def logprobs(logits, tokens=None, top=0):
     index), of every row the entropy in nats and the `top` (up to 32) most likely ids with their log probabilities. A
     logit of -inf (a masked token) has probability 0; a row with nothing but -inf, or with a NaN or a +inf, gives NaN.
     Returns TokenLogprobs over the flattened rows."""
-    from . import _lib
-    from .quantize import workspace
     top = int(top)
     if _logprobs_fast is not None and logits.is_cuda:
-        r = _logprobs_fast(logits, tokens, top, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+        r = _logprobs_fast(logits, tokens, top, torch._C._cuda_getCurrentRawStream(logits.get_device()))
         if r is not None:
             return TokenLogprobs(*r)
+    from . import _lib  # here: the two lines take 1.5 us
+    from .quantize import workspace
     if not logits.is_cuda or logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("logits must be an fp32 or bf16 CUDA (HIP) tensor")
     if logits.dim() < 1 or logits.shape[-1] < 1:
@@ -161,14 +161,14 @@ def head_logprobs(feat, weight, scales, tokens=None, top=0):
     quantize.DynamicInt8Linear) gives for features (bf16 device [..., K], as of verify, prefill or decode), without
     all of those logits in memory (fl_head_logprobs). The logits are fp32 and exact integer sums behind two scales, so
     a row's ranks and ids do not depend on the batch it is scored in."""
-    from . import _lib
-    from .quantize import _check_weight, aligned16, workspace
     top = int(top)
     if _head_logprobs_fast is not None and feat.is_cuda:
         r = _head_logprobs_fast(feat, weight, scales, tokens, top,
-                                torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+                                torch._C._cuda_getCurrentRawStream(feat.get_device()))
         if r is not None:
             return TokenLogprobs(*r)
+    from . import _lib
+    from .quantize import _check_weight, aligned16, workspace
     _check_weight(weight, scales)
     n, k = weight.shape
     if not feat.is_cuda or feat.dtype != torch.bfloat16:

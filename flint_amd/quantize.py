@@ -265,7 +265,7 @@ def gemm_int8(xq, xs, wq, ws, out_dtype=torch.bfloat16):
     it is in. out_dtype: bf16, or fp32 (logits)."""
     f32 = out_dtype is torch.float32
     if _int8_fast is not None and xs is not None and xq.is_cuda and (f32 or out_dtype is torch.bfloat16):
-        y = _int8_fast(xq, xs, wq, ws, f32, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+        y = _int8_fast(xq, xs, wq, ws, f32, torch._C._cuda_getCurrentRawStream(xq.get_device()))
         if y is not None:
             return y
     _check_out_dtype(out_dtype)
@@ -292,7 +292,7 @@ def linear_int8(x, wq, ws, out_dtype=torch.bfloat16):
     (fl_linear_int8)."""
     f32 = out_dtype is torch.float32
     if _int8_fast is not None and x.is_cuda and (f32 or out_dtype is torch.bfloat16):
-        y = _int8_fast(x, None, wq, ws, f32, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+        y = _int8_fast(x, None, wq, ws, f32, torch._C._cuda_getCurrentRawStream(x.get_device()))
         if y is not None:
             return y
     _check_out_dtype(out_dtype)
