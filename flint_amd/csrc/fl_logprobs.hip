@@ -329,8 +329,9 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
         }
       }
     }
-    if (tok.in) {  // last: the token's logit comes from two loads in a row
-      if (tok.l != tok.l || jb + LP_STEP > j1 || (tok.t >= jb && tok.t < jb + LP_STEP)) {
+    // last: the token's logit comes from two loads in a row; mostly a likely token's, which few steps have anything above
+    if (tok.in && (tok.l != tok.l || __ballot(s != s || !(top < tok.l)) != 0)) {
+      if (tok.l != tok.l || (tok.t >= jb && tok.t < jb + LP_STEP) || (tok.l == -INFINITY && jb + LP_STEP > j1)) {
         const int tm = min(tok.t, j1) - jt;
 #pragma unroll
         for (int e = 0; e < LP_E; ++e) {

@@ -215,6 +215,33 @@ def test_where_steps_and_chunks_meet(dev, rows, vocab, dtype):
         check(generate.TokenLogprobs(*(f[some] for f in out)), logits.cpu()[some], tokens[some], 7)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [4008, 5000, 20001])
+def test_ranks_of_every_kind_of_token(dev, vocab, dtype):
+    """The most likely token, the least likely, forbidden ones, NaN and its neighbours: everywhere in the row, in one row
+    and in more rows than are cut into chunks."""
+    g = torch.Generator().manual_seed(vocab)
+    base = (torch.randn(vocab, generator=g) * 3).to(torch.bfloat16)
+    rows, tokens = [], []
+    for at in (0, 1, vocab // 2, 4007, vocab - 1):
+        for value in (40.0, -40.0, -math.inf, math.nan, math.inf, float(base.max())):
+            for other in (None, -math.inf, math.nan):
+                r = base.clone()
+                if other is not None:
+                    r[torch.randint(0, vocab, (20,), generator=g)] = other
+                    r[vocab - 1] = other
+                r[at] = value
+                rows.append(r)
+                tokens.append(at)
+    logits, tokens = torch.stack(rows).to(dtype), torch.tensor(tokens, dtype=torch.int32)
+    check(host(generate.logprobs(logits.to(dev), tokens.to(dev), 3)), logits, tokens, 3)
+    for i in range(0, len(rows), 7):
+        check(host(generate.logprobs(logits[i].to(dev), tokens[i:i + 1].to(dev), 3)), logits[i:i + 1], tokens[i:i + 1], 3)
+    many = torch.cat([logits] * 12)
+    out = host(generate.logprobs(many.to(dev), tokens.repeat(12).to(dev), 3))
+    check(generate.TokenLogprobs(*(f[-90:] for f in out)), logits, tokens, 3)
+
+
 def test_results_can_be_saved(dev):
     import io
     lg, tok = rows_of(3, 100, 1, torch.float32)
