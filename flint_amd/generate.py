@@ -128,7 +128,7 @@ def logprobs(logits, tokens=None, top=0):
     gives NaN and rank -1) the log probability and the rank (0: the most likely; equal logits rank by
     index), of every row the entropy in nats and the `top` (up to 32) most likely ids with their log probabilities. A
     logit of -inf (a masked token) has probability 0; a row with nothing but -inf, or with a NaN or a +inf, gives NaN.
-    Returns TokenLogprobs over the flattened rows."""
+    Returns TokenLogprobs over the flattened rows; they carry no gradient."""
     top = int(top)
     if _logprobs_fast is not None and logits.is_cuda:
         r = _logprobs_fast(logits, tokens, top, torch._C._cuda_getCurrentRawStream(logits.get_device()))

@@ -300,3 +300,43 @@ def test_linears_on_both_sides_of_the_rules_lines(dev, m, n, k):
     ref = scoring.product(*scoring.quantize_rows(x), wq, ws)
     assert torch.equal(quantize.linear_int8(x.to(dev), wq.to(dev), ws.to(dev), torch.float32).cpu(), ref)
     assert torch.equal(quantize.linear_int8(x.to(dev), wq.to(dev), ws.to(dev)).cpu(), ref.to(torch.bfloat16))
+
+
+def scaled_sums(xq, xs, wq, ws):
+    """The definition on the device, for a few rows or columns of a large product."""
+    acc = xq.double() @ wq.double().T  # whole numbers below 2^53: exact in any order
+    return acc.float() * (xs[:, None] * ws[None, :])
+
+
+@pytest.mark.parametrize("n", [1, 3, 70])
+def test_as_many_rows_as_there_may_be(dev, n):
+    """2^23 rows of x, and of weights: offsets of the operand beyond 2^31."""
+    m, k = 1 << 23, 272
+    xq = torch.randint(-128, 128, (m, k), dtype=torch.int8, device=dev)
+    xs, ws = torch.rand(m, device=dev), torch.rand(n, device=dev)
+    wq = torch.randint(-128, 128, (n, k), dtype=torch.int8, device=dev)
+    at = torch.tensor([0, 1, 63, 64, 4095, (1 << 22) + 5, m - 65, m - 2, m - 1], device=dev)
+    y = quantize.gemm_int8(xq, xs, wq, ws, torch.float32)
+    assert torch.equal(y[at], scaled_sums(xq[at], xs[at], wq, ws))
+    y = quantize.gemm_int8(wq, ws, xq, xs, torch.float32)  # the other way round
+    assert torch.equal(y[:, at], scaled_sums(wq, ws, xq[at], xs[at]))
+    with pytest.raises(ValueError):
+        quantize.gemm_int8(xq[:, :264], xs, wq[:, :264], ws)
+
+
+def test_more_results_than_32_bits_count(dev):
+    m, n, k = 1 << 17, 33000, 16
+    xq, wq = (torch.randint(-128, 128, (r, k), dtype=torch.int8, device=dev) for r in (m, n))
+    xs, ws = torch.rand(m, device=dev), torch.rand(n, device=dev)
+    y = quantize.gemm_int8(xq, xs, wq, ws)
+    at = torch.tensor([0, 65535, 65536, 130156, 130157, m - 257, m - 1], device=dev)
+    assert y.numel() > 2 ** 32 and torch.equal(y[at], scaled_sums(xq[at], xs[at], wq, ws).to(torch.bfloat16))
+
+
+def test_as_many_rows_quantised_as_there_may_be(dev):
+    m = 1 << 23
+    x = torch.randn(m, 16, device=dev).to(torch.bfloat16)
+    q, s = quantize.quantize_int8(x)
+    at = torch.tensor([0, 3, 4, 1 << 22, m - 5, m - 1], device=dev)
+    qr, sr = scoring.quantize_rows(x[at].cpu())
+    assert torch.equal(q[at].cpu(), qr) and torch.equal(s[at].cpu(), sr)

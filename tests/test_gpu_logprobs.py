@@ -299,6 +299,35 @@ def test_head(dev, m, n, k, top):
     assert torch.equal(two.rank, out.rank) and (top == 0 or torch.equal(two.top_ids, out.top_ids))
 
 
+@pytest.mark.parametrize("top,given", [(6, True), (0, True), (3, False)])
+def test_head_of_more_logits_than_one_block_holds(dev, top, given):
+    """600000 logits a row, 111 rows of them in 256 MB: two whole blocks and a last one."""
+    m, n, k = 250, 600000, 32
+    g = torch.Generator().manual_seed(1)
+    w = torch.randint(-128, 128, (n, k), generator=g).to(torch.int8)
+    s = torch.rand(n, generator=g) * 1e-3
+    x = torch.randn(m, k, generator=g).to(torch.bfloat16)
+    tokens = torch.randint(0, n, (m,), generator=g, dtype=torch.int32)
+    call = lambda a, b: host(generate.head_logprobs(x[a:b].to(dev), w.to(dev), s.to(dev),  # noqa: E731
+                                                    tokens[a:b].to(dev) if given else None, top))
+    out = call(0, m)
+    some = [0, 110, 111, 221, 222, 249]
+    logits = scoring.product(*scoring.quantize_rows(x[some]), w, s)
+    pick = lambda f: None if f is None else f[some]  # noqa: E731
+    check(generate.TokenLogprobs(*map(pick, out)), logits, tokens[some] if given else None, top)
+    for a, b in zip(call(111, 222), out):
+        assert a is None or a.dtype != torch.int32 or torch.equal(a, b[111:222])
+
+
+def test_as_many_rows_as_there_may_be(dev):
+    rows, vocab = 1 << 17, 100
+    logits = torch.randn(rows, vocab, device=dev)
+    tokens = torch.randint(0, vocab, (rows,), dtype=torch.int32, device=dev)
+    out = host(generate.logprobs(logits, tokens, 4))
+    some = [0, 1, 255, 256, 65536, rows - 1]
+    check(generate.TokenLogprobs(*(f[some] for f in out)), logits[some].cpu(), tokens[some].cpu(), 4)
+
+
 def test_head_refusals_and_shapes(dev):
     w, s = torch.zeros(40, 64, dtype=torch.int8, device=dev), torch.ones(40, device=dev)
     x, t = torch.zeros(6, 64, dtype=torch.bfloat16, device=dev), torch.zeros(6, dtype=torch.int32, device=dev)
@@ -435,3 +464,24 @@ def test_generate_refuses_log_probabilities_it_has_not(dev, model):
             generate.generate(model, prompt, 2, logprobs=n)
     seq, said = generate.generate(model, prompt, 0, logprobs=2)
     assert seq.tolist() == [3, 5] and said.logprob.shape == (0,) and said.top_ids.shape == (0, 2)
+
+
+def test_features_of_a_prompt_of_several_passes(dev):
+    """2100 tokens, three passes: the same as one call for each, and as the greedy prefill."""
+    args = ModelArgs.from_name("tiny")
+    args.block_size = 2304
+    model = Transformer.from_weights(args, synth_weights(args, seed=0), "cuda:0")
+    g = torch.Generator().manual_seed(9)
+    tokens = torch.randint(0, model.config.vocab_size, (2100,), generator=g, dtype=torch.int32).to(dev)
+    model.setup_caches(1, 2200)
+    one, two = (torch.full((1,), -1, dtype=torch.int32, device=dev) for _ in range(2))
+    feat = model.prefill_features(tokens, 0, one)
+    parts = [model.prefill_features(tokens[:1024], 0), model.prefill_features(tokens[1024:2048], 1024),
+             model.prefill_features(tokens[2048:], 2048)]
+    assert torch.equal(feat, torch.cat(parts))
+    model.prefill(tokens, 0, two)
+    assert int(one) == int(two) >= 0
+    said = generate.score(model, tokens, 2, model.int8_head())
+    head = model.int8_head()
+    want = generate.head_logprobs(feat[:-1], head.weight, head.scales, tokens[1:], 2)
+    assert all(torch.equal(a, b) for a, b in zip(said, want))
