@@ -255,6 +255,7 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
   const int full = min(LP_NW, (j1 - j0) / (FL_WAVE * V)), q = full > 0 ? (a.top + full - 1) / full : 0;
   float m = -INFINITY, s = 0.0f, u = 0.0f, T = -INFINITY;
   int before = 0, kept = 0, i = 0;  // `before` and kept: of the wave
+  bool masked = false;              // whether the wave has met a -inf: without one its sums spare an operation a value
   for (int jb = j0; jb < j1; jb += LP_STEP, ++i) {
     raw4 ahead[LP_E / V];
     if (jb + LP_STEP < j1) load(jb + LP_STEP, ahead);
@@ -275,12 +276,22 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
     const float d0 = fmaxf(old - mu, -1000.0f), e0 = __builtin_amdgcn_exp2f(d0 * LP_LOG2E);
     u = (u + s * d0) * e0;
     s *= e0;
+    auto sums = [&](float& s, float& u, auto low) {
 #pragma unroll
-    for (int e = 0; e < LP_E; ++e) {
-      const float d = x[e] - mu, p = __builtin_amdgcn_exp2f(d * LP_LOG2E);
-      s += p;
-      u = __builtin_fmaf(p, fmaxf(d, -1000.0f), u);  // 0 times -1000 for masked values
+      for (int e = 0; e < LP_E; ++e) {
+        const float d = x[e] - mu, p = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+        s += p;
+        u = __builtin_fmaf(p, low(d), u);
+      }
+    };
+    float s1 = s, u1 = u;
+    masked = masked || jb + LP_STEP > j1;
+    if (!masked) {
+      sums(s1, u1, [](float d) { return d; });
+      masked = __ballot(u1 != u1) != 0;  // 0 times -inf
     }
+    if (masked) s1 = s, u1 = u, sums(s1, u1, [](float d) { return fmaxf(d, -1000.0f); });  // 0 times -1000
+    s = s1, u = u1;
     const int jt = jb + tid * V;  // e's index: jt + (e / V) * LP_NT * V + e % V
     if (a.top > 0) {
       if ((i & (i + 1)) == 0) {  // steps 0, 1, 3, 7, ...
