@@ -118,14 +118,13 @@ __device__ __forceinline__ void lp_sort(LpShared& sh, int top, F out) {
   }
 }
 
-// A value that q of G groups of lanes reach, close to the q-th largest of theirs: v orders as unsigned and agrees in the
-// 64 / G (or, with G = 32, the lower) lanes of a group. The last bits tell equal groups apart and are dropped from the
-// answer. Every group counts the larger ones: 16 groups 300 cycles, against 190 for each of q rounds of maxima.
-template <int G>
+// A value that q of G groups of N lanes reach (of the wave's first lanes), close to the q-th largest of theirs: v orders
+// as unsigned, agrees in a group and is 0 in the lanes behind. The last bits tell equal groups apart and are dropped from
+// the answer. Every group counts the larger ones: 16 groups 300 cycles, against 190 for each of q rounds of maxima; whole
+// 64-bit keys in a loop over the chunks there are: 0.7 us more than 32 chunks in 32 bits.
+template <int G, int N>
 __device__ __forceinline__ uint32_t lp_reached(uint32_t v, int q) {
-  constexpr int N = G == 32 ? 1 : FL_WAVE / G;  // lanes of a group
-  const int lane = threadIdx.x & 63;
-  v = (v & ~(uint32_t)(G - 1)) | (uint32_t)(lane / N % G);
+  v = (v & ~(uint32_t)(G - 1)) | (uint32_t)((threadIdx.x & 63) / N % G);
   int larger = 0;
 #pragma unroll
   for (int g = 0; g < G; ++g) larger += (uint32_t)__builtin_amdgcn_readlane((int)v, g * N) > v;
@@ -151,7 +150,7 @@ __device__ __forceinline__ uint32_t wave_umax32(uint32_t v) {
 __device__ __forceinline__ void lp_publish(uint32_t* bound, float mine, int q, bool once) {
   const uint32_t b = __float_as_uint(mine + 0.0f);  // -0 becomes 0
   uint32_t v = mine == mine ? b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u) : 0u, t = 0;
-  if (once && q <= 16) t = lp_reached<16>(umax_dpp<0x4E>(umax_dpp<0xB1>(v)), q);
+  if (once && q <= 16) t = lp_reached<16, 4>(umax_dpp<0x4E>(umax_dpp<0xB1>(v)), q);
   else
     for (int r = 0; r < q; ++r) {
       t = wave_umax32(v);
@@ -299,20 +298,13 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
         if (i == 0) __syncthreads();
         T = lp_least(sh.bound, full);
       }
+      const float least = fmaxf(T, -3.4028235e38f);
       if (i == 0) {
         // The first step has most of them, in any of a lane's values: a candidate of every lane that has one at a time
-        // (16 ballots in a row take twice as long). T = -inf: all that is larger, and the chunk's first values by index.
+        // (16 ballots in a row take twice as long).
         uint32_t mask = 0;  // value e: bit 15 - e
-        if (T == -INFINITY) {
 #pragma unroll
-          for (int e = 0; e < LP_E; ++e) {
-            const int j = jt + (e / V) * LP_NT * V + e % V;
-            mask = mask << 1 | (uint32_t)(j < j1 && (!(x[e] <= T) || j < j0 + a.top));
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < LP_E; ++e) mask = mask << 1 | (uint32_t)!(x[e] < T);
-        }
+        for (int e = 0; e < LP_E; ++e) mask = mask << 1 | (uint32_t)!(x[e] < least);
         for (u64 lanes; (lanes = __ballot(mask != 0)) != 0; mask &= mask - 1) {
           const int b = __builtin_ctz(mask | 1u << LP_E), e = LP_E - 1 - b;
           float half[LP_E];
@@ -326,17 +318,24 @@ __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
           if (mask != 0 && at < LP_KEEP) sh.cand[wave][at] = lp_key(half[0], jt + e / V * (LP_NT * V) + e % V);
           kept += __builtin_popcountll(lanes);
         }
-      } else {
-        const float least = fmaxf(T, -3.4028235e38f);  // -inf counts among the chunk's first values only
-        if (__ballot(s != s || top >= least) != 0) {
+        if (T == -INFINITY && wave == 0) {
+          // all that is larger may be too little: the values of -inf among the chunk's first `top`, which come next
+          const int j = j0 + lane;
+          float v = 0.0f;
+          if (lane < a.top && j < j1) v = BF16 ? bf2f(lh[j]) : lf[j];
+          const u64 lanes = __ballot(v == -INFINITY);
+          const int at = kept + lp_below(lanes);
+          if (v == -INFINITY && at < LP_KEEP) sh.cand[wave][at] = lp_key(v, j);
+          kept += __builtin_popcountll(lanes);
+        }
+      } else if (__ballot(s != s || top >= least) != 0) {
 #pragma unroll
-          for (int e = 0; e < LP_E; ++e) {
-            const u64 lanes = __ballot(!(x[e] < least));
-            if (lanes == 0) continue;
-            const int at = kept + lp_below(lanes);
-            if (!(x[e] < least) && at < LP_KEEP) sh.cand[wave][at] = lp_key(x[e], jt + (e / V) * LP_NT * V + e % V);
-            kept += __builtin_popcountll(lanes);
-          }
+        for (int e = 0; e < LP_E; ++e) {
+          const u64 lanes = __ballot(!(x[e] < least));
+          if (lanes == 0) continue;
+          const int at = kept + lp_below(lanes);
+          if (!(x[e] < least) && at < LP_KEEP) sh.cand[wave][at] = lp_key(x[e], jt + (e / V) * LP_NT * V + e % V);
+          kept += __builtin_popcountll(lanes);
         }
       }
     }
@@ -429,10 +428,13 @@ __global__ __launch_bounds__(LP_NT) void k_logprobs_merge(LpArgs a) {
   if (a.top > 0) {
     u64 mine[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) mine[i] = i * LP_NT + tid < keys ? cand[i * LP_NT + tid] : 0;
+    for (int i = 0; i < E; ++i) {  // neighbours to different waves: a chunk's first keys are the larger ones
+      const int k = i * LP_NT + lane * LP_NW + wave;
+      mine[i] = k < keys ? cand[k] : 0;
+    }
     // At least `top` keys reach what q chunks' keys at place `at` do, with at so that q is about half of the chunks.
     const int at = min((2 * a.top + a.chunks - 1) / a.chunks, a.top) - 1, q = (a.top + at) / (at + 1);
-    const uint32_t t = lp_reached<LP_CHUNKS>(lane < a.chunks ? (uint32_t)(cand[lane * a.top + at] >> 32) : 0u, q);
+    const uint32_t t = lp_reached<LP_CHUNKS, 1>(lane < a.chunks ? (uint32_t)(cand[lane * a.top + at] >> 32) : 0u, q);
     int kept = 0;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
