@@ -152,18 +152,19 @@ __host__ __device__ inline int qf_log_waves(int m) { return m > 4 ? 0 : m > 2 ? 
 // Whether the product's workgroups quantise the rows themselves: if the waves hold them in QF_KEEP pieces a lane, and if
 // it beats a launch of its own before the product. us, on the way and before it, of the kernels alone; called one by one
 // the two launches take 8 at least.
-// - up to 4 rows: 2 x 2560 x 2560 5.4 and 6.0, 4 x 5003 x 8192 15.7 and 17.4, 4 x 16384 x 4096 15.2 and 17.0; but
+// - up to 4 rows: 2 x 5003 x 2560 7.3 and 8.0, 4 x 8192 x 2560 8.4 and 9.3, 4 x 16384 x 4096 15.2 and 17.0; but
 //   4 x 49152 x 512 11.7 and 10.4, the rows again in every workgroup beside a short K;
-// - up to 8: 8 x 49152 x 2560 26.8 and 29.8; 8 x 16384 x 1600 10.5 and 9.8, 8 x 8192 x 2560 10.1 and 9.2; while two
-//   launches take longer to call than to run, 8 x 2560 x 2048 5.8 and 6.1, 8 x 5003 x 1600 7.7 and 6.4;
-// - up to 16 only then: 16 x 2560 x 1024 6.0 and 5.9; 16 x 5003 x 1024 8.4 and 7.2, 16 x 49152 x 2048 24.0 and 23.5.
+// - up to 8: 8 x 8192 x 1024 6.0 and 7.0, 8 x 5003 x 1600 6.5 and 6.5, 8 x 8192 x 2560 9.2 and 9.3, 8 x 49152 x 2560 26.8
+//   and 29.8; 8 x 4096 x 4096 9.4 and 8.7, 8 x 16384 x 1600 10.5 and 9.8;
+// - up to 16: 12 x 8192 x 1024 6.5 and 7.2, 16 x 5003 x 1024 7.1 and 7.2 (10 x 5003 x 1600 7.5 and 6.5: then the calls
+//   decide); 16 x 12000 x 1024 8.5 and 8.0, 16 x 49152 x 2048 24.0 and 23.5.
 inline bool qf_pays(int m, int n, int k) {
   const int lw = qf_log_waves(m), slots = FEW_KW >> lw, w = 64 << lw;
   const int64_t values = (int64_t)m * k;
   if (m > 16 || values > QF_MOST || (m + slots - 1) / slots * ((k / 8 + w - 1) / w) > QF_KEEP) return false;
   if (m <= 4) return k >= 1024 || n < 32768;
-  if (n < (m > 8 ? 4096 : 8192)) return values <= 16384;
-  return m <= 8 && n >= 32768 && k > 1024;
+  if (m <= 8) return n <= 12288 ? values <= 20480 : n >= 32768 && k > 1024;
+  return n <= 8192 && values <= 16384;
 }
 // of x rows in LDS: r and r + 8 on the same banks
 __host__ __device__ inline int few_pitch(int k) { return ((k + 63) >> 6) * 64 + 16; }
@@ -718,7 +719,11 @@ int64_t i8_linear_bytes(int32_t m, int32_t n, int32_t k) {
 int i8_linear(const uint16_t* x, const int8_t* wq, const float* ws, void* y, bool y_fp32, void* work, int32_t m,
               int32_t n, int32_t k, hipStream_t s) {
   if (qf_pays(m, n, k)) {
-    i8_few<1, 36, true>(I8Few{x, nullptr, wq, ws, y, m, n, k}, 2, y_fp32, s);
+    // one workgroup a CU, which quantises once for the blocks that it takes in turn, or two, which have more weights in
+    // flight: us, 7 x 5003 x 1408 6.5 and 7.5, 8 x 8000 x 2048 8.1 and 9.5, 8 x 12000 x 2560 10.9 and 11.6; 4 x 12000 x 4096
+    // 14.1 and 12.3, 4 x 16384 x 2560 12.0 and 11.8, 1 x 49152 x 2560 28.3 and 25.6
+    const bool one = n <= 8192 || (n <= 12288 && k < 4096);
+    i8_few<1, 36, true>(I8Few{x, nullptr, wq, ws, y, m, n, k}, one ? 1 : 2, y_fp32, s);
     return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
   }
   int8_t* xq = static_cast<int8_t*>(work);

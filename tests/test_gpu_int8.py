@@ -340,3 +340,14 @@ def test_as_many_rows_quantised_as_there_may_be(dev):
     at = torch.tensor([0, 3, 4, 1 << 22, m - 5, m - 1], device=dev)
     qr, sr = scoring.quantize_rows(x[at].cpu())
     assert torch.equal(q[at].cpu(), qr) and torch.equal(s[at].cpu(), sr)
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 12288, 2560), (8, 12289, 2560), (5, 12288, 4096), (5, 12288, 4112), (4, 12288, 4080),
+                                   (4, 12288, 4096), (4, 12289, 4080), (1, 8192, 8192), (1, 8193, 8192), (16, 8192, 1024),
+                                   (16, 8193, 1024), (9, 8192, 1808), (9, 8192, 1824), (7, 4097, 2912), (7, 4097, 2928)])
+def test_linears_whose_workgroups_take_blocks_in_turn(dev, m, n, k):
+    x = rows_of(m, k, n + k, "outliers")
+    wq, ws = ints(n, k, m), torch.rand(n, generator=torch.Generator().manual_seed(m)) * 1e-3
+    ref = scoring.product(*scoring.quantize_rows(x), wq, ws)
+    assert torch.equal(quantize.linear_int8(x.to(dev), wq.to(dev), ws.to(dev), torch.float32).cpu(), ref)
+    assert torch.equal(quantize.linear_int8(x.to(dev), wq.to(dev), ws.to(dev)).cpu(), ref.to(torch.bfloat16))
