@@ -210,10 +210,10 @@ __device__ __forceinline__ void lp_join(float& m, float& s, float& u) {
 }
 
 // One chunk of a row per workgroup, in steps of LP_E values per thread; the next step's loads are in flight meanwhile.
-// 1024 rows of 49152 (fp32, top 5) 39 us, 5.1 TB/s, the rate of a large copy here, with the vector ALUs busy in more than
-// half of the cycles (17 instructions a value); 34 without alternatives, two steps in flight no faster. One row of 49152,
-// top 20, twelve chunks, 5.4 us and 3.2 to merge them (5.8 in all without alternatives): a launch and a memory latency
-// each, then one dependent step after another.
+// 1024 rows of 49152 (fp32, top 5) 37 us, 5.4 TB/s with part of them in the last-level cache, the vector ALUs busy in more
+// than half of the cycles (16 instructions a value; bf16, 32 us, is bound by these); 34 without alternatives, two steps in
+// flight no faster. One row of 49152, top 20, twelve chunks, 5.5 us and 3.0 to merge them (5.8 in all without
+// alternatives): a launch and a memory latency each, then one dependent step after another.
 template <bool BF16>
 __global__ __launch_bounds__(LP_NT, 4) void k_logprobs(LpArgs a) {
   constexpr int V = BF16 ? 8 : 4;  // consecutive values of a load (16 bytes, aligned to the type only)
