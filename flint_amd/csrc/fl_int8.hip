@@ -689,9 +689,13 @@ int i8_gemm(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws
   if (p.kind == I8_FEW) {
     const I8Few a{xq, xs, wq, ws, y, m, n, k};
     if (m > 16) i8_few<2, 0, false>(a, 0, y_fp32, s);
-    // x in LDS and blocks in turn, 8 / 16 rows x 49152 x 2560: 27 / 28 us, 31 / 38 without; one row 25 and 23
-    else if (n < 8192 || m <= 2) i8_few<1, 0, false>(a, 0, y_fp32, s);
-    else i8_few<1, FEW_LDS_KB, false>(a, 2, y_fp32, s);
+    // x in LDS and blocks in turn, and x from memory with a block a workgroup: us, 8 / 16 x 49152 x 2560 27 / 28 and
+    // 31 / 38, 1 x 49152 x 2560 26 and 24, 8 x 5003 x 1600 4.4 and 4.0; 8 x 5003 x 4096 8.4 and 9.0, 2 x 6500 x 8192 11.9
+    // and 13.2, 1 x 10000 x 8192 17.1 and 18.3, 2 x 4096 x 4096 5.6 and 5.5. One workgroup a CU, and two: 4 x 5003 x 8192
+    // 12.3 and 12.9, 8 x 16384 x 2560 10.1 and 9.7
+    else if (m * few_pitch(k) <= FEW_LDS_KB << 10 && (k < 4096 ? n >= 8192 && m > 2 : n > 4096))
+      i8_few<1, FEW_LDS_KB, false>(a, n <= 8192 ? 1 : 2, y_fp32, s);
+    else i8_few<1, 0, false>(a, 0, y_fp32, s);
   } else {
     const I8Tile a{xq, wq, xs, ws, p.splits > 1 ? work : y, m, n, k, p.mblk, p.nblk, p.splits, p.sps};
     // up to 256 tiles a CU holds one workgroup, which may have all of its LDS; beyond, two that take turns at waiting:

@@ -351,3 +351,15 @@ def test_linears_whose_workgroups_take_blocks_in_turn(dev, m, n, k):
     ref = scoring.product(*scoring.quantize_rows(x), wq, ws)
     assert torch.equal(quantize.linear_int8(x.to(dev), wq.to(dev), ws.to(dev), torch.float32).cpu(), ref)
     assert torch.equal(quantize.linear_int8(x.to(dev), wq.to(dev), ws.to(dev)).cpu(), ref.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 4096, 4112), (2, 4097, 4112), (2, 4097, 4080), (1, 5003, 65536), (6, 8191, 8000),
+                                   (7, 8191, 8000), (11, 4500, 4400), (2, 8192, 4096), (1, 10007, 8208), (3, 8192, 4080)])
+def test_few_rows_with_and_without_lds(dev, m, n, k):
+    xq, wq = ints(m, k, m + k), ints(n, k, n)
+    g = torch.Generator().manual_seed(k)
+    xs, ws = torch.rand(m, generator=g) * 0.05, torch.rand(n, generator=g) * 1e-3
+    ref = scoring.product(xq, xs, wq, ws)
+    d = [t.to(dev) for t in (xq, xs, wq, ws)]
+    assert torch.equal(quantize.gemm_int8(*d, out_dtype=torch.float32).cpu(), ref)
+    assert torch.equal(quantize.gemm_int8(*d).cpu(), ref.to(torch.bfloat16))
