@@ -180,9 +180,10 @@ def head_logprobs(feat, weight, scales, tokens=None, top=0):
     tokens = _check_logprob_args(rows, n, tokens, top, x.device)
     out = _logprob_outputs(rows, tokens, top, x.device)
     if rows:
+        wa = aligned16(weight)
         with torch.cuda.device(x.device):
             work = workspace("fl_head_logprobs_workspace", rows, n, k, top, device=x.device)
-            _lib.call("fl_head_logprobs", _lib.ptr(x), _lib.ptr(aligned16(weight)), _lib.ptr(scales), _lib.ptr(tokens),
+            _lib.call("fl_head_logprobs", _lib.ptr(x), _lib.ptr(wa), _lib.ptr(scales), _lib.ptr(tokens),
                       top, *map(_lib.ptr, out), _lib.ptr(work), rows, n, k, _lib.stream_ptr())
     return out
 

@@ -220,7 +220,8 @@ def _check_weight(wq, ws):
 
 
 def aligned16(t):
-    """t, or a copy of it where its data does not start on 16 bytes (a view into a tensor may not)."""
+    """t, or a copy of it where its data does not start on 16 bytes (a view into a tensor may not). To be held in a
+    name until the launch: a copy freed before it may be given to the next one, or to another thread."""
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -249,8 +250,9 @@ def quantize_int8(x, q=None, scale=None):
     if q.shape != x.shape or scale.shape != x.shape[:1] or q.device != x.device or scale.device != x.device:
         raise ValueError("q must be [M, K] and scale [M], on x's device")
     if m:
+        xa = aligned16(x)
         with torch.cuda.device(x.device):
-            _lib.call("fl_quantize_int8", _lib.ptr(aligned16(x)), _lib.ptr(q), _lib.ptr(scale), m, k, _lib.stream_ptr())
+            _lib.call("fl_quantize_int8", _lib.ptr(xa), _lib.ptr(q), _lib.ptr(scale), m, k, _lib.stream_ptr())
     return q, scale
 
 
@@ -280,10 +282,11 @@ def gemm_int8(xq, xs, wq, ws, out_dtype=torch.bfloat16):
     m = xq.shape[0]
     y = torch.empty(m, n, dtype=out_dtype, device=xq.device)
     if m and n:
+        xa, wa = aligned16(xq), aligned16(wq)
         with torch.cuda.device(xq.device):
             work = workspace("fl_gemm_int8_workspace", m, n, k, device=xq.device)
-            _lib.call("fl_gemm_int8", _lib.ptr(aligned16(xq)), _lib.ptr(xs), _lib.ptr(aligned16(wq)), _lib.ptr(ws),
-                      _lib.ptr(y), int(f32), _lib.ptr(work), m, n, k, _lib.stream_ptr())
+            _lib.call("fl_gemm_int8", _lib.ptr(xa), _lib.ptr(xs), _lib.ptr(wa), _lib.ptr(ws), _lib.ptr(y), int(f32),
+                      _lib.ptr(work), m, n, k, _lib.stream_ptr())
     return y
 
 
@@ -308,9 +311,10 @@ def linear_int8(x, wq, ws, out_dtype=torch.bfloat16):
     m = x2.shape[0]
     y = torch.empty(m, n, dtype=out_dtype, device=x.device)
     if m and n:
+        wa = aligned16(wq)
         with torch.cuda.device(x.device):
             work = workspace("fl_linear_int8_workspace", m, n, k, device=x.device)
-            _lib.call("fl_linear_int8", _lib.ptr(x2), _lib.ptr(aligned16(wq)), _lib.ptr(ws), _lib.ptr(y), int(f32),
+            _lib.call("fl_linear_int8", _lib.ptr(x2), _lib.ptr(wa), _lib.ptr(ws), _lib.ptr(y), int(f32),
                       _lib.ptr(work), m, n, k, _lib.stream_ptr())
     return y.view(*x.shape[:-1], n)
 

@@ -109,3 +109,68 @@ def test_host_layer_refuses():
         quantize.DynamicInt8Linear(40, 8)              # K not a multiple of 16
     with pytest.raises(ValueError):
         quantize.DynamicInt8Linear(32, 8, bias=True)
+
+
+class _OnDevice(torch.Tensor):
+    """A CPU tensor that says it is a device's, so that the host layer runs up to the C call."""
+    is_cuda, off16 = True, False
+
+    def data_ptr(self):
+        return super().data_ptr() + (4 if self.off16 else 0)
+
+
+def _device_tensor(t, off16=False):
+    t = t.as_subclass(_OnDevice)
+    t.off16 = off16
+    return t
+
+
+@pytest.fixture
+def c_calls(monkeypatch):
+    """The host layer without a device: C calls end in a list of (name, whether each of the copies made for it on 16
+    bytes was still held when it was made)."""
+    import contextlib
+    import gc
+    import weakref
+    from flint_amd import _lib, generate, quantize
+    copies, calls = [], []
+    real = quantize.aligned16
+
+    def copying(t):
+        c = real(t)
+        if c is not t:
+            copies.append(weakref.ref(c))
+        return c
+
+    def call(name, *args):
+        if "workspace" in name:
+            return 0
+        gc.collect()
+        calls.append((name, [c() is not None for c in copies]))
+        return 0
+
+    monkeypatch.setattr(quantize, "aligned16", copying)
+    monkeypatch.setattr(quantize, "_int8_fast", None)
+    monkeypatch.setattr(generate, "_head_logprobs_fast", None)
+    monkeypatch.setattr(_lib, "call", call)
+    monkeypatch.setattr(_lib, "stream_ptr", lambda stream=None: None)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    return calls
+
+
+def test_copies_on_16_bytes_live_until_the_launch(c_calls):
+    """A copy that is freed before the launch can be given to the next one, which then overwrites what the kernel reads:
+    two operands of one size that both start off 16 bytes."""
+    from flint_amd import generate, quantize
+    w, s = _device_tensor(torch.zeros(8, 32, dtype=torch.int8), True), _device_tensor(torch.zeros(8))
+    xq = _device_tensor(torch.zeros(8, 32, dtype=torch.int8), True)
+    x = _device_tensor(torch.zeros(8, 32, dtype=torch.bfloat16), True)
+    quantize.gemm_int8(xq, s, w, s)
+    quantize.quantize_int8(x, _device_tensor(torch.zeros(8, 32, dtype=torch.int8)), s)
+    quantize.linear_int8(x, w, s)
+    generate.head_logprobs(x, w, s)
+    assert [n for n, _ in c_calls] == ["fl_gemm_int8", "fl_quantize_int8", "fl_linear_int8", "fl_head_logprobs"]
+    made = 0
+    for (name, held), n in zip(c_calls, (2, 1, 1, 1)):  # linear_int8's and head_logprobs' rows lose the mark on their way
+        assert held[made:] == [True] * n, name
+        made += n

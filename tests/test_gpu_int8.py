@@ -363,3 +363,20 @@ def test_few_rows_with_and_without_lds(dev, m, n, k):
     d = [t.to(dev) for t in (xq, xs, wq, ws)]
     assert torch.equal(quantize.gemm_int8(*d, out_dtype=torch.float32).cpu(), ref)
     assert torch.equal(quantize.gemm_int8(*d).cpu(), ref.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("m,n,k", [(72, 72, 96), (5, 5, 1040), (300, 300, 272)])
+def test_both_operands_off_16_bytes(dev, m, n, k):
+    """x and weights of one size in views that start on 1, 4 or 8 bytes: each is copied, and both copies have to live."""
+    xq, wq = ints(m, k, 1), ints(n, k, 2)
+    xs, ws = torch.rand(m), torch.rand(n)
+    ref = scoring.product(xq, xs, wq, ws)
+    for off in (1, 4, 8):
+        packed = torch.zeros(2 * m * k + 16 + off, dtype=torch.int8, device=dev)
+        a, b = packed[off:off + m * k].view(m, k), packed[off + 16 + m * k:].view(n, k)
+        a.copy_(xq)
+        b.copy_(wq)
+        assert a.data_ptr() % 16 == off and b.data_ptr() % 16 == off
+        y = quantize.gemm_int8(a, xs.to(dev), b, ws.to(dev), out_dtype=torch.float32)
+        assert torch.equal(y.cpu(), ref)
+        assert torch.equal(packed[:off].cpu(), torch.zeros(off, dtype=torch.int8))
