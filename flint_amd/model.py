@@ -276,9 +276,10 @@ class Transformer:
             feat = None
         if tokens_out is None:
             tokens_out = torch.empty(m, dtype=torch.int32, device=dev)
-        _lib.call("fl_verify", _lib.ctypes.byref(self._cw), self._state, _lib.ptr(tokens.int().contiguous()),
-                  m, _lib.ptr(depth.int().contiguous()), _lib.ptr(amask.to(torch.uint8).contiguous()), int(pos),
-                  _lib.ptr(tokens_out), _lib.ptr(logits), _lib.ptr(feat), _lib.stream_ptr())
+        # in names, so that none is freed, and its memory given to the next, before the launch
+        tokens, depth, amask = tokens.int().contiguous(), depth.int().contiguous(), amask.to(torch.uint8).contiguous()
+        _lib.call("fl_verify", _lib.ctypes.byref(self._cw), self._state, _lib.ptr(tokens), m, _lib.ptr(depth),
+                  _lib.ptr(amask), int(pos), _lib.ptr(tokens_out), _lib.ptr(logits), _lib.ptr(feat), _lib.stream_ptr())
         return tokens_out, logits, feat
 
     def prefill(self, tokens, pos, token_out):

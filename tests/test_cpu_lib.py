@@ -118,3 +118,34 @@ def test_torch_extension_loads():
     sz = torch.zeros(8, 2, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="device tensor"):
         ops.int4_linear(x, q, sz, 0)
+
+
+def test_verify_holds_what_it_converts(monkeypatch):
+    """int64 tokens and depths and a bool mask are converted for the launch. A conversion that is freed before it can be
+    given to the next one, which then overwrites what the kernel reads: all have to live until the C call."""
+    import gc
+    import weakref
+    from types import SimpleNamespace
+    from flint_amd import _lib
+    from flint_amd.model import Transformer
+    given, held = [], []
+
+    def ptr(t):
+        if t is not None:
+            given.append(weakref.ref(t))
+        return t if t is None else t.data_ptr()
+
+    def call(name, *args):
+        gc.collect()
+        held.extend(r() is not None for r in given)
+
+    monkeypatch.setattr(_lib, "ptr", ptr)
+    monkeypatch.setattr(_lib, "call", call)
+    monkeypatch.setattr(_lib, "stream_ptr", lambda stream=None: None)
+    eng = Transformer.__new__(Transformer)
+    eng._state, eng._cw, eng.device = 1, _lib.Weights(), torch.device("cpu")
+    eng.config = SimpleNamespace(vocab_size=16, dim=8)
+    tokens, depth = torch.tensor([3, 5, 7, 9]), torch.arange(4)
+    eng.verify(tokens, 0, depth=depth, amask=torch.ones(4, 4, dtype=torch.bool).tril())
+    eng._state = None
+    assert len(held) == 6 and all(held), held

@@ -157,3 +157,16 @@ def test_verify_rows_do_not_depend_on_width(dev, attn_mode, name, pos):
     d = (l5.float() - l8[:5].float()).abs().max().item()
     log(f"{name} pos={pos}: rows 0..4 at width 5 vs 8: max|d|={d:.3e}")
     assert torch.equal(l5, l8[:5]) and torch.equal(f5, f8[:5])
+
+
+def test_verify_takes_64_bit_tokens_and_depths(dev):
+    """int64 tokens and depths and a bool mask give what int32 and uint8 ones do."""
+    args, _, eng, _ = make_pair("tiny", seed=2)
+    eng.setup_caches(1, 64)
+    tokens = torch.randint(0, args.vocab_size, (12,), generator=torch.Generator().manual_seed(4)).to(dev)
+    depth = torch.arange(12, device=dev) // 2
+    amask = torch.ones(12, 12, dtype=torch.bool, device=dev).tril()
+    want = [t.clone() for t in eng.verify(tokens.int(), 5, depth.int(), amask.to(torch.uint8))]
+    for a, b in zip(eng.verify(tokens, 5, depth, amask), want):
+        assert torch.equal(a, b)
+    eng.check()
