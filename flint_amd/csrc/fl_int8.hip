@@ -1,8 +1,11 @@
 // Matrix products of 8-bit integers with one scale per row of either operand (per token and per
 // channel), and the quantisation of bf16 rows that feeds them.
 //
-// A row r in 8 bits: scale s = max|r| times fp32(1 / 127), rounded to fp32 (within an ulp of max|r| / 127, without
-// a division), q = r / s rounded to nearest, ties to even, exactly (below).
+// A row r in 8 bits: scale s = max|r| times fp32(1 / 127), rounded to fp32, q = r / s rounded to nearest, ties to even,
+// exactly (below). The product is the definition, as in the form that torch gives max / 127 on a device; it is not always
+// the rounded quotient: where the maximum's 8 bits are 143, 144, 175, 207, 208 or 239, s is an ulp below fp32(max / 127),
+// and a value of exactly max / 2 is a hair above 63.5 steps, so 64, where the quotient's scale would make it 63. No other
+// q differs. Either is within half a step.
 // y[m, n] = fp32(sum_k xq[m, k] wq[n, k]) * fp32(xs[m] * ws[n]): the sum is a whole number and exact in int32 whatever
 // the order (|sum| <= 2^30), so every kernel and every split here gives the same bits, whatever the batch. Rounded: the
 // sum to fp32 (24 bits of at most 30), the scales' product, theirs with the sum, and that to bf16 where y is.
@@ -17,8 +20,8 @@ typedef uint32_t i8_u32x4 __attribute__((ext_vector_type(4)));
 
 // ---- quantisation -------------------------------------------------------------------------------
 
-// x / s rounded to the nearest whole number, ties to even, for |x| <= 127 s (1 + 2^-22). t = x (1 / s) is off by at
-// most 127 * 2^-22, so its nearest whole number q may be one off next to a half, and x = max / 2, which gives 63.5,
+// x / s rounded to the nearest whole number, ties to even, for |x| <= 127 s (1 + 2^-22) (127.008 s where s is
+// subnormal and has few bits). t = x (1 / s) is off by at most 127.008 * 2^-22, so its nearest whole number q may be one off next to a half, and x = max / 2, which gives 63.5,
 // is frequent: the remainder r = x - q s decides. It is exact in one fma: q s has at most 31 bits and |r| <= s is a
 // multiple of an ulp of the smaller of x and s. An exact half needs s to be a power of two (x has 8 bits, and max / 127
 // to 24 bits has few only if 127 divides max's), and then t is exact and its rounding went to the even side.

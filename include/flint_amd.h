@@ -136,7 +136,9 @@ int fl_gemv_int4_tiled(const uint32_t* qt, const uint32_t* sz, const uint16_t* x
 /* ---- 8-bit integer products ---------------------------------------------------------------- */
 
 /* Rows in 8 bits, one scale each: a row r (bf16, K % 16 == 0, K <= 65536) becomes scale = max|r| * fp32(1 / 127),
- * rounded to fp32, and q = r / scale rounded to the nearest whole number, ties to even (the quotient exact); a zero
+ * rounded to fp32, and q = r / scale rounded to the nearest whole number, ties to even (the quotient exact). The scale
+ * is that product, not fp32(max|r| / 127), which is an ulp more where the maximum's bf16 significand is 143, 144, 175,
+ * 207, 208 or 239 (of 128..255) and would make a value of exactly half the maximum 63 instead of 64. A zero
  * row: scale 0, q 0; a row with a NaN or an infinity: scale NaN, q 0. Weights have one scale per output channel this
  * way, activations one per token. x and q 16-byte aligned, at most 2^23 rows.
  * No counterpart in the reference's engine, which has int4 weights only. */

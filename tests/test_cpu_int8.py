@@ -174,3 +174,33 @@ def test_copies_on_16_bytes_live_until_the_launch(c_calls):
     for (name, held), n in zip(c_calls, (2, 1, 1, 1)):  # linear_int8's and head_logprobs' rows lose the mark on their way
         assert held[made:] == [True] * n, name
         made += n
+
+
+def test_the_scale_is_the_product():
+    """At every bf16 significand: s = fp32(max fp32(1 / 127)), computed here in whole numbers; where that is an ulp below
+    fp32(max / 127), half the maximum is 64, and 63.5 steps to even, 64, elsewhere or 63."""
+    from fractions import Fraction
+    from oracle import scoring
+
+    def fp32(x):  # of a positive fraction, to nearest even
+        e = 0
+        while x >= 1 << 24:
+            x, e = x / 2, e + 1
+        while x < 1 << 23:
+            x, e = x * 2, e - 1
+        return Fraction(round(x)) * Fraction(2) ** e
+
+    rec, below = fp32(Fraction(1, 127)), []
+    for top in range(128, 256):
+        x = torch.tensor([[top, top / 2, -top / 2] + [0.0] * 13]).to(torch.bfloat16)
+        q, s = scoring.quantize_rows(x)
+        product, quotient = fp32(top * rec), fp32(Fraction(top, 127))
+        assert Fraction(float(s[0])) == product
+        half = round(Fraction(top, 2) / product)  # ties to even
+        assert q[0, :3].tolist() == [127, half, -half]
+        if product != quotient:
+            below.append(top)
+            assert product < quotient and half == 64 and round(Fraction(top, 2) / quotient) == 63
+        else:
+            assert half in (63, 64)
+    assert below == [143, 144, 175, 207, 208, 239]

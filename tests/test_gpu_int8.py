@@ -380,3 +380,23 @@ def test_both_operands_off_16_bytes(dev, m, n, k):
         y = quantize.gemm_int8(a, xs.to(dev), b, ws.to(dev), out_dtype=torch.float32)
         assert torch.equal(y.cpu(), ref)
         assert torch.equal(packed[:off].cpu(), torch.zeros(off, dtype=torch.int8))
+
+
+@pytest.mark.parametrize("rows", [128, 1024])
+def test_the_scale_is_the_product(dev, rows):
+    """Every bf16 significand as the maximum, with its half in the row: the scale is fp32(max fp32(1 / 127)), which torch's
+    max / 127 on the device is too, and not always fp32(max / 127); for six significands that makes the half 64."""
+    top = torch.arange(128, 256).repeat(rows // 128).float()
+    x = torch.zeros(rows, 32)
+    x[:, 3], x[:, 17], x[:, 31] = -top, top / 2, -top / 2
+    q, s = quantize.quantize_int8(x.to(torch.bfloat16).to(dev))
+    product = top.to(dev) * (torch.ones(()) / torch.full((), 127.0)).to(dev)
+    assert torch.equal(s, product) and torch.equal(s, top.to(dev) / 127)
+    quotient = (top.double() / 127).float()  # the nearest fp32: a quotient of 8 by 7 bits is no half of an ulp in fp64
+    six = torch.tensor([143.0, 144.0, 175.0, 207.0, 208.0, 239.0])
+    assert torch.equal(top[s.cpu() != quotient].unique(), six)
+    low = torch.isin(top, six)
+    assert bool((q[:, 3] == -127).all()) and torch.equal(q[:, 17], -q[:, 31])
+    assert bool((q.cpu()[low][:, 17] == 64).all())
+    ref = torch.round(top.double() / 2 / s.cpu().double())
+    assert torch.equal(q[:, 17].cpu().double(), ref)
