@@ -322,7 +322,8 @@ def linear_int8(x, wq, ws, out_dtype=torch.bfloat16):
 
 class DynamicInt8Linear(torch.nn.Module):
     """A linear with 8-bit integer weights (one scale per output channel) whose input rows are quantised on the
-    way, one scale per token: the product runs on the integer matrix cores. For inference.
+    way, one scale per token: the product runs on the integer matrix cores. For inference. The scales stay fp32 when a
+    model that holds it is cast to another type.
 
     forward(x [..., K] bf16) -> [..., N] bf16, K a multiple of 16. For a vocabulary head whose logits are wanted in
     fp32 or as log probabilities: linear_int8(..., out_dtype=torch.float32), generate.head_logprobs.
@@ -336,6 +337,13 @@ class DynamicInt8Linear(torch.nn.Module):
         self.in_features, self.out_features = in_features, out_features
         self.register_buffer("weight", torch.zeros(out_features, in_features, dtype=torch.int8, device=device))
         self.register_buffer("scales", torch.zeros(out_features, dtype=torch.float32, device=device))
+
+    def _apply(self, fn, recurse=True):
+        scales = self.scales
+        super()._apply(fn, recurse)
+        if self.scales.dtype != torch.float32:  # the whole model was cast (to(bfloat16), half()): the scales are not
+            self.scales = scales.to(self.scales.device)
+        return self
 
     @classmethod
     def from_float(cls, w):

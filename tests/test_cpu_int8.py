@@ -204,3 +204,19 @@ def test_the_scale_is_the_product():
         else:
             assert half in (63, 64)
     assert below == [143, 144, 175, 207, 208, 239]
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.bfloat16(), lambda m: m.half(),
+                                  lambda m: m.to("meta", torch.bfloat16), lambda m: m.double(),
+                                  lambda m: torch.nn.Sequential(m).to(device="cpu", dtype=torch.bfloat16)[0]])
+def test_scales_stay_fp32_when_the_model_is_cast(cast):
+    """A model is put into its precision as a whole; the scales are no activations' type."""
+    from flint_amd.quantize import DynamicInt8Linear
+    m = DynamicInt8Linear(32, 8)
+    m.scales.copy_(torch.arange(8) + 1 / 3)
+    m.weight.fill_(5)
+    scales = m.scales.clone()
+    m = cast(m)
+    assert m.scales.dtype == torch.float32 and m.weight.dtype == torch.int8
+    assert m.scales.device == m.weight.device and "scales" in m.state_dict()
+    assert m.scales.is_meta or torch.equal(m.scales, scales)

@@ -400,3 +400,12 @@ def test_the_scale_is_the_product(dev, rows):
     assert bool((q.cpu()[low][:, 17] == 64).all())
     ref = torch.round(top.double() / 2 / s.cpu().double())
     assert torch.equal(q[:, 17].cpu().double(), ref)
+
+
+def test_linear_in_a_model_that_is_cast(dev):
+    w, x = rows_of(48, 64, 1), rows_of(6, 64, 2).to(dev)
+    lin = quantize.DynamicInt8Linear.from_float(w.to(dev))
+    y = lin(x)
+    model = torch.nn.Sequential(lin).to(device=dev, dtype=torch.bfloat16)
+    assert torch.equal(model(x), y)
+    assert torch.equal(model.cpu().to(dev)(x), y)
