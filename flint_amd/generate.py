@@ -190,8 +190,8 @@ def head_logprobs(feat, weight, scales, tokens=None, top=0):
 
 @torch.no_grad()
 def score(model, tokens, top=0, head=None):
-    """How likely a text is to the model: TokenLogprobs of tokens[1:] (int device [T], T >= 2), row i of the
-    distribution after tokens[:i + 1] at tokens[i + 1]. The tokens' K/V rows are in the cache afterwards.
+    """How likely a text is to the model: TokenLogprobs of tokens[1:] (int device [T], T from 2 to block_size + 1),
+    row i of the distribution after tokens[:i + 1] at tokens[i + 1]. The tokens' K/V rows are in the cache afterwards.
 
     head None: the model's own bf16 LM head, through the verify kernel's logits, 32 tokens at a time. head a
     quantize.DynamicInt8Linear (Transformer.int8_head): one pass over the prompt and its features through the
@@ -201,7 +201,8 @@ def score(model, tokens, top=0, head=None):
     n = x.numel() - 1
     if n < 1:
         raise ValueError("score needs two tokens or more")
-    model.setup_caches(1, n + 1)
+    # the last token takes no position here; room for it, to decode on from it, where there is one (caches come in eights)
+    model.setup_caches(1, n + 1 if n + 1 <= model.packed.rope.shape[0] // 8 * 8 else n)
     if head is not None:
         return head_logprobs(model.prefill_features(x[:n], 0), head.weight, head.scales, x[1:], top)
     parts = []

@@ -485,3 +485,26 @@ def test_features_of_a_prompt_of_several_passes(dev):
     head = model.int8_head()
     want = generate.head_logprobs(feat[:-1], head.weight, head.scales, tokens[1:], 2)
     assert all(torch.equal(a, b) for a, b in zip(said, want))
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_score_of_a_text_that_fills_the_positions(dev, int8):
+    """128 positions, 129 tokens: the last one is only asked for."""
+    args = ModelArgs.from_name("tiny")
+    args.block_size = 128
+    model = Transformer.from_weights(args, synth_weights(args, seed=0), "cuda:0")
+    head = model.int8_head() if int8 else None
+    tokens = torch.randint(0, args.vocab_size, (129,), generator=torch.Generator().manual_seed(2), dtype=torch.int32).to(dev)
+    whole = host(generate.score(model, tokens, 3, head))
+    model.check()
+    part = host(generate.score(model, tokens[:128], 3, head))
+    for a, b in zip(whole, part):
+        assert a.shape[0] == 128 and torch.equal(a[:96], b[:96])
+    if int8:
+        logits = scoring.product(*scoring.quantize_rows(model.prefill_features(tokens[:128], 0).cpu()), head.weight.cpu(),
+                                 head.scales.cpu())
+    else:
+        logits = model.verify(tokens[96:128], 96)[1].cpu()
+    check(generate.TokenLogprobs(*(f[-len(logits):] for f in whole)), logits, tokens[-len(logits):].cpu(), 3)
+    with pytest.raises(ValueError):
+        generate.score(model, torch.cat([tokens, tokens[:1]]), 3, head)
