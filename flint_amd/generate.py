@@ -191,7 +191,8 @@ def head_logprobs(feat, weight, scales, tokens=None, top=0):
 @torch.no_grad()
 def score(model, tokens, top=0, head=None):
     """How likely a text is to the model: TokenLogprobs of tokens[1:] (int device [T], T from 2 to block_size + 1),
-    row i of the distribution after tokens[:i + 1] at tokens[i + 1]. The tokens' K/V rows are in the cache afterwards.
+    row i of the distribution after tokens[:i + 1] at tokens[i + 1]. The K/V rows of tokens[:-1] are in the cache
+    afterwards: to go on, feed tokens[-1] at position T - 1.
 
     head None: the model's own bf16 LM head, through the verify kernel's logits, 32 tokens at a time. head a
     quantize.DynamicInt8Linear (Transformer.int8_head): one pass over the prompt and its features through the

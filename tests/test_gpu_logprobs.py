@@ -508,3 +508,22 @@ def test_score_of_a_text_that_fills_the_positions(dev, int8):
     check(generate.TokenLogprobs(*(f[-len(logits):] for f in whole)), logits, tokens[-len(logits):].cpu(), 3)
     with pytest.raises(ValueError):
         generate.score(model, torch.cat([tokens, tokens[:1]]), 3, head)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_decoding_goes_on_from_a_scored_text(dev, model, int8):
+    """The cache holds the rows of all tokens but the last, which is fed at its own position; the slots from there on are
+    left as they were."""
+    n = 50
+    tokens = torch.randint(0, 1024, (n,), generator=torch.Generator().manual_seed(8), dtype=torch.int32).to(dev)
+    model.setup_caches(1, 64)
+    model.k_cache.fill_(7.0)
+    generate.score(model, tokens, head=model.int8_head() if int8 else None)
+    assert bool((model.k_cache[:, :, n - 1:] == 7.0).all()) and not bool((model.k_cache[:, :, :n - 1] == 7.0).all(3).any())
+    after = model.decode_step(tokens[-1:], n - 1).clone()
+    if int8:  # score's one pass over tokens[:-1], again
+        model.prefill_features(tokens[:-1], 0)
+    else:
+        for s in range(0, n - 1, 32):
+            model.verify(tokens[s:min(n - 1, s + 32)], s)
+    assert torch.equal(model.decode_step(tokens[-1:], n - 1), after)
