@@ -202,6 +202,10 @@ def score(model, tokens, top=0, head=None):
     n = x.numel() - 1
     if n < 1:
         raise ValueError("score needs two tokens or more")
+    if head is None:  # refusals before the model has run
+        _check_logprob_args(1, model.config.vocab_size, None, int(top), model.device)
+    else:
+        _check_logprob_args(n, head.weight.shape[0], None, int(top), model.device)
     # the last token takes no position here; room for it, to decode on from it, where there is one (caches come in eights)
     model.setup_caches(1, n + 1 if n + 1 <= model.packed.rope.shape[0] // 8 * 8 else n)
     if head is not None:

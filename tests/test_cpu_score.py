@@ -70,3 +70,13 @@ def test_a_longer_text_is_refused(given, head):
     with pytest.raises(ValueError):
         generate.score(model, torch.zeros(66, dtype=torch.int32), 0, head)
     assert model.fed == []
+
+
+@pytest.mark.parametrize("head", [None, HEAD])
+@pytest.mark.parametrize("top", [-1, 33, 51])
+def test_alternatives_that_are_refused_are_refused_first(given, head, top):
+    """Before the model has run, which takes the time of a prompt and overwrites its cache."""
+    model = Model(64)
+    with pytest.raises(ValueError):
+        generate.score(model, torch.zeros(40, dtype=torch.int32), top, head)
+    assert model.fed == [] and model.room == 0

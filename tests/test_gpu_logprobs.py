@@ -527,3 +527,14 @@ def test_decoding_goes_on_from_a_scored_text(dev, model, int8):
         for s in range(0, n - 1, 32):
             model.verify(tokens[s:min(n - 1, s + 32)], s)
     assert torch.equal(model.decode_step(tokens[-1:], n - 1), after)
+
+
+def test_score_refuses_before_it_runs(dev, model):
+    tokens = torch.zeros(40, dtype=torch.int32, device=dev)
+    model.setup_caches(1, 64)
+    model.k_cache.fill_(7.0)
+    for head in (None, model.int8_head()):
+        for top in (-1, 33):
+            with pytest.raises(ValueError):
+                generate.score(model, tokens, top, head)
+    assert bool((model.k_cache == 7.0).all())
