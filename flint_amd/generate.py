@@ -117,9 +117,13 @@ def _check_logprob_args(rows, vocab, tokens, top, dev):
         raise ValueError("tokens must be int32 or int64, on the logits' device")
     if tokens.numel() != rows:
         raise ValueError(f"tokens: {tokens.numel()} ids for {rows} rows")
-    if tokens.dtype == torch.int64:
-        tokens = tokens.clamp(-1, 2 ** 31 - 1)  # ids outside the vocabulary stay outside it
-    return tokens.reshape(-1).to(torch.int32).contiguous()
+    return _ids(tokens).contiguous()
+
+
+def _ids(tokens):
+    """tokens as int32 [n]; 64-bit ids outside the vocabulary stay outside it."""
+    tokens = tokens.reshape(-1)
+    return (tokens.clamp(-1, 2 ** 31 - 1) if tokens.dtype == torch.int64 else tokens).to(torch.int32)
 
 
 def logprobs(logits, tokens=None, top=0):
@@ -198,7 +202,7 @@ def score(model, tokens, top=0, head=None):
     quantize.DynamicInt8Linear (Transformer.int8_head): one pass over the prompt and its features through the
     8-bit head."""
     from . import _lib
-    x = tokens.reshape(-1).to(device=model.device, dtype=torch.int32)
+    x = _ids(tokens.to(model.device))
     n = x.numel() - 1
     if n < 1:
         raise ValueError("score needs two tokens or more")

@@ -80,3 +80,15 @@ def test_alternatives_that_are_refused_are_refused_first(given, head, top):
     with pytest.raises(ValueError):
         generate.score(model, torch.zeros(40, dtype=torch.int32), top, head)
     assert model.fed == [] and model.room == 0
+
+
+@pytest.mark.parametrize("head", [None, HEAD])
+def test_64_bit_ids_outside_the_vocabulary_stay_outside(given, head):
+    """As in logprobs: an id beyond 32 bits is not the one that its low bits make."""
+    model = Model(64)
+    generate.score(model, torch.tensor([1, 2 ** 32 + 5, -2 ** 40, 3, 2 ** 33 + 7]), 0, head)
+    fed = sum((t for _, t in model.fed), [])
+    assert len(given) == 4 and len(fed) == 4
+    outside = lambda t: not 0 <= t < 50  # noqa: E731
+    assert [outside(t) for t in given] == [True, True, False, True]
+    assert [outside(t) for t in fed] == [False, True, True, False]

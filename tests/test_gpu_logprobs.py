@@ -538,3 +538,17 @@ def test_score_refuses_before_it_runs(dev, model):
             with pytest.raises(ValueError):
                 generate.score(model, tokens, top, head)
     assert bool((model.k_cache == 7.0).all())
+
+
+def test_score_of_an_id_beyond_32_bits(dev):
+    """Asked for last, it is outside the vocabulary; fed, the state says so."""
+    model = Transformer.from_weights(ModelArgs.from_name("tiny"), synth_weights(ModelArgs.from_name("tiny"), seed=0), "cuda:0")
+    tokens = torch.tensor([3, 4, 5, 2 ** 32 + 6], device=dev)
+    for head in (None, model.int8_head()):
+        out = generate.score(model, tokens, 2, head)
+        model.check()
+        assert out.rank.tolist()[2] == -1 and out.logprob.isnan().tolist() == [False, False, True]
+    generate.score(model, tokens.flip(0), 2)
+    with pytest.raises(_lib.FlError):
+        model.check()
+    model.reset_state()
