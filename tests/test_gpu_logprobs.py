@@ -552,3 +552,40 @@ def test_score_of_an_id_beyond_32_bits(dev):
     with pytest.raises(_lib.FlError):
         model.check()
     model.reset_state()
+
+
+def seams(rows, vocab, step=4096, most=32, workgroups=1024):
+    """(values of a chunk, chunks) as the launcher cuts a row: chunks of as many whole steps as the largest needs, evenly
+    filled in multiples of eight."""
+    steps = -(-vocab // step)
+    n = max(1, min(most, steps, workgroups // rows))
+    n = -(-steps // -(-steps // n))
+    per = -(-(-(-vocab // n)) // 8) * 8
+    return per, -(-vocab // per)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,chunks,chunk_steps", [
+    (1, 131073, 17, 2), (1, 131072, 32, 1), (1, 400001, 25, 4), (40, 131073, 17, 2), (100, 49152, 6, 2), (128, 49152, 6, 2),
+    (200, 49155, 5, 3), (300, 49155, 3, 5), (512, 20001, 2, 3), (1000, 20001, 1, 5)])
+def test_tokens_and_ties_at_the_seams_of_chunks_of_several_steps(dev, rows, vocab, chunks, chunk_steps, dtype):
+    """Equal values on both sides of every seam of chunks and of steps within them, the largest ones among them, and the
+    tokens there."""
+    per, n = seams(rows, vocab)
+    assert n == chunks and -(-per // 4096) == chunk_steps
+    g = torch.Generator().manual_seed(vocab + rows)
+    logits = torch.randint(0, 5, (rows, vocab), generator=g).to(dtype)
+    logits[torch.rand(rows, vocab, generator=g) < 0.01] = -math.inf
+    starts = [c * per for c in range(1, n)]
+    inner = [c * per + s * 4096 for c in range(n) for s in range(1, chunk_steps) if c * per + s * 4096 < min(vocab, (c + 1) * per)]
+    ends = [min(vocab, (c + 1) * per) for c in range(n)]
+    at = [p + d for p in starts + inner for d in (-1, 0)] + [ends[-1] - 1, 0]
+    some = sorted({0, rows // 2, rows - 1})
+    for r in some[:2]:  # the alternatives lie at the seams, in the order of their indices; the last row has them by chance
+        logits[r, at] = 9.0
+    logits = logits.to(dev)
+    for t in sorted(set(at))[:: max(1, len(set(at)) // 14)] + [starts[0] if starts else 0, per - 1]:
+        tokens = torch.full((rows,), t, dtype=torch.int32)
+        out = host(generate.logprobs(logits, tokens.to(dev), 11))
+        check(generate.TokenLogprobs(*(f[some] for f in out)), logits[some].cpu(), tokens[some], 11)
+        assert out.top_ids[0].tolist() == sorted(set(at))[:11] or len(set(at)) < 11
