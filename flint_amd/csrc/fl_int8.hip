@@ -158,7 +158,9 @@ __host__ __device__ inline int qf_log_waves(int m) { return m > 4 ? 0 : m > 2 ? 
 // - up to 4 rows: 2 x 5003 x 2560 7.3 and 8.0, 4 x 8192 x 2560 8.4 and 9.3, 4 x 16384 x 4096 15.2 and 17.0; but
 //   4 x 49152 x 512 11.7 and 10.4, the rows again in every workgroup beside a short K;
 // - up to 8: 8 x 8192 x 1024 6.0 and 7.0, 8 x 5003 x 1600 6.5 and 6.5, 8 x 8192 x 2560 9.2 and 9.3, 8 x 49152 x 2560 26.8
-//   and 29.8; 8 x 4096 x 4096 9.4 and 8.7, 8 x 16384 x 1600 10.5 and 9.8;
+//   and 29.8; 8 x 4096 x 4096 9.4 and 8.7, 8 x 16384 x 1600 10.5 and 9.8; between the two lines 8 x 16384 x 2560 12.8 and
+//   12.6, 5 x 16384 x 2560 12.5 both, but 8 x 24576 x 2560 15.0 and 15.6, 8 x 32752 x 2560 17.0 and 18.8: the upper line could
+//   lie lower;
 // - up to 16: 12 x 8192 x 1024 6.5 and 7.2, 16 x 5003 x 1024 7.1 and 7.2 (10 x 5003 x 1600 7.5 and 6.5: then the calls
 //   decide); 16 x 12000 x 1024 8.5 and 8.0, 16 x 49152 x 2048 24.0 and 23.5.
 inline bool qf_pays(int m, int n, int k) {
