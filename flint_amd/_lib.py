@@ -34,6 +34,7 @@ EXPORTS = [
     "fl_prefill_workspace", "fl_prefill", "fl_prefill_feat",
     "fl_quantize_int8", "fl_gemm_int8_workspace", "fl_gemm_int8", "fl_linear_int8_workspace", "fl_linear_int8",
     "fl_logprobs_workspace", "fl_logprobs", "fl_head_logprobs_workspace", "fl_head_logprobs",
+    "fl_tree_attention_workspace", "fl_tree_attention", "fl_attention_weights", "fl_evict", "fl_accept",
 ]
 
 
@@ -41,6 +42,16 @@ class FlError(RuntimeError):
     def __init__(self, fn, code):
         super().__init__(f"{fn} failed: {ERRORS.get(code, code)}")
         self.code = code
+
+
+class AttnDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("b", "m", "heads", "groups", "dim", "slots", "fp16", "pos0")] \
+        + [("scale", ctypes.c_float)] \
+        + [(n, ctypes.c_int64) for n in ("q_b", "q_m", "q_h", "k_b", "k_g", "k_s", "v_b", "v_g", "v_s", "mask_b")]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("outer", "inner", "row")]
 
 
 class ModelDesc(ctypes.Structure):
@@ -114,6 +125,11 @@ def load(path=LIB_PATH):
         "fl_logprobs": ([vp, i32, i64, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp], i32),
         "fl_head_logprobs_workspace": ([i32, i32, i32, i32, pi64], i32),
         "fl_head_logprobs": ([vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp], i32),
+        "fl_tree_attention_workspace": ([ctypes.POINTER(AttnDesc), i32, pi64], i32),
+        "fl_tree_attention": ([ctypes.POINTER(AttnDesc)] + [vp] * 9, i32),
+        "fl_attention_weights": ([ctypes.POINTER(AttnDesc)] + [vp] * 6 + [i32, vp], i32),
+        "fl_evict": ([ctypes.POINTER(Rows)] * 2 + [vp] + [i32] * 8 + [vp] + [ctypes.POINTER(Rows)] * 2 + [vp, i32, vp], i32),
+        "fl_accept": ([vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp], i32),
         "fl_kv_move": ([vp, vp, vp, i32, vp], i32),
         "fl_sample": ([vp, i32, i32, f32, i32, ctypes.c_uint64, ctypes.c_uint64, vp, vp, vp, vp], i32),
         "fl_sample_noalloc": ([vp, i32, i32, f32, i32, ctypes.c_uint64, ctypes.c_uint64, vp, vp, vp, vp], i32),

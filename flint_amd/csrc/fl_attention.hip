@@ -1,0 +1,742 @@
+// Attention of the nodes of a drafted tree (or chain, or one token) over a K/V cache, and the weight that every
+// cached key gathers from them.
+//
+// The rows of a key head are its (node, query head) pairs, node-major: row t * rep + j. Scores are taken transposed,
+// S^T = K Q^T on 32x32x16 MFMAs, so that a lane holds one row (r = lane % 32) and registers hold its keys; the softmax
+// is online, per lane, in the log2 domain (p = exp2(s c - m), c = scale log2 e), in fp32; O^T += V^T P^T takes a step's
+// 16 keys in the order in which the score registers already hold them, so P never crosses lanes. V^T comes out of LDS
+// through the transposing read (a 16-lane group receives four rows of 16 values by column). P is split into two 16-bit
+// terms: one alone would round every weight by 2^-9 (bf16), which showed as 1.4 times the output's own rounding.
+#include <algorithm>
+#include "fl_gemm.h"
+
+namespace {
+
+typedef _Float16 fl_f16x8 __attribute__((ext_vector_type(8)));
+typedef short at_s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) at_s16x4 at_lds4;
+
+struct AttnArgs {
+  const uint16_t *q, *k, *v;
+  const int32_t* pos;   // per sequence, or null: pos0
+  const uint8_t* mask;  // [M][M] per sequence, or null: a chain
+  uint16_t* out;        // [B][M][heads][D]
+  float* lse;           // [B][M][heads] or null (read by k_attn_weights)
+  float* part;          // with key parts: o [parts][B][groups][R][D], then (m, l) [parts][B][groups][R][2]
+  int b, m, heads, groups, rep, slots, pos0, R;
+  int blocks, parts;    // row blocks per key head; key parts
+  float sc;             // scale * log2 e
+  int64_t q_b, q_m, q_h, k_b, k_g, k_s, v_b, v_g, v_s, mask_b;
+};
+
+template <bool H>
+__device__ __forceinline__ fl_f32x16 mma(uint4 a, uint4 b, fl_f32x16 c) {
+  if constexpr (H)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(fl_f16x8, a), __builtin_bit_cast(fl_f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(fl_bf16x8, a), __builtin_bit_cast(fl_bf16x8, b), c, 0, 0, 0);
+}
+template <bool H>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (H) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 v = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    return pack_bf16x2(a, b);
+  }
+}
+template <bool H>
+__device__ __forceinline__ float lo16(uint32_t w) {
+  if constexpr (H) return (float)__builtin_bit_cast(_Float16, (uint16_t)w);
+  else return bflo(w);
+}
+template <bool H>
+__device__ __forceinline__ float hi16(uint32_t w) {
+  if constexpr (H) return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16));
+  else return bfhi(w);
+}
+template <bool H>
+__device__ __forceinline__ bool finite16(uint32_t w) {  // both values of a pair
+  constexpr uint32_t e = H ? 0x7C00u : 0x7F80u;
+  return (w & e) != e && (w & (e << 16)) != (e << 16);
+}
+template <bool H>
+__device__ __forceinline__ bool finite16(uint4 w) {
+  return finite16<H>(w.x) && finite16<H>(w.y) && finite16<H>(w.z) && finite16<H>(w.w);
+}
+template <bool H>
+__device__ __forceinline__ uint32_t only_finite(uint32_t w) {  // a value that is none becomes 0
+  constexpr uint32_t e = H ? 0x7C00u : 0x7F80u;
+  if ((w & e) == e) w &= 0xFFFF0000u;
+  if ((w & (e << 16)) == (e << 16)) w &= 0xFFFFu;
+  return w;
+}
+template <bool H>
+__device__ __forceinline__ uint4 only_finite(uint4 w) {
+  return make_uint4(only_finite<H>(w.x), only_finite<H>(w.y), only_finite<H>(w.z), only_finite<H>(w.w));
+}
+
+// Keys [0, keys) of a sequence and this workgroup's part of them; keys < 0: a pos outside the cache.
+struct Span {
+  int pos, keys, kb0, kend;
+};
+// Parts are whole multiples of `unit` keys, as even as those allow, so that a short sequence of a ragged batch has
+// fewer and its row of them is as long as any.
+__device__ __forceinline__ int part_keys(int keys, int parts, int unit) {
+  return ((keys + parts - 1) / parts + unit - 1) / unit * unit;
+}
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int part, int unit) {
+  Span s;
+  s.pos = a.pos ? a.pos[b] : a.pos0;
+  if (s.pos < 0 || s.pos > a.slots - a.m) {
+    s.keys = -1, s.kb0 = s.kend = 0;
+    return s;
+  }
+  s.keys = s.pos + a.m;
+  const int kpp = part_keys(s.keys, a.parts, unit);
+  s.kb0 = min(s.keys, part * kpp);
+  s.kend = min(s.keys, s.kb0 + kpp);
+  return s;
+}
+
+// Scores of the keys of a tile that node t does not see, or that lie behind `kend`, become -inf. A chain's node sees up
+// to itself; a tree's bits come from the mask by range-checked byte loads, all in flight together (an offset outside
+// reads 0).
+template <int KT>
+__device__ __forceinline__ void hide(const AttnArgs& a, const uint8_t* mask, int pos, int kend, int kb, int t, fl_f32x16 (&s)[KT]) {
+  const int hf = (threadIdx.x & 63) >> 5;
+  if (!mask) {
+    const int lim = min(kend, pos + t + 1) - kb - 4 * hf;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kt][i] = 32 * kt + 8 * (i >> 2) + (i & 3) < lim ? s[kt][i] : -INFINITY;
+    return;
+  }
+  const auto mr = buf_rsrc(mask, (uint32_t)a.m * (uint32_t)a.m);
+  const uint32_t row = (uint32_t)t * (uint32_t)a.m;
+  const int j0 = kb + 4 * hf - pos, jend = kend - pos;  // node of register 0; nodes before the end (one at least)
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+    uint32_t bit[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int j = j0 + 32 * kt + 8 * (i >> 2) + (i & 3);
+      bit[i] = __builtin_amdgcn_raw_buffer_load_b8(mr, (uint32_t)j < (uint32_t)jend ? row + (uint32_t)j : 0xFFFFFFF0u, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int j = j0 + 32 * kt + 8 * (i >> 2) + (i & 3);
+      s[kt][i] = (bit[i] | (uint32_t)(j >> 31)) != 0 ? s[kt][i] : -INFINITY;  // a cached key: j < 0
+    }
+    asm volatile("" ::: "memory");  // 16 registers for the bits, not 32
+  }
+}
+
+// A tile of TK keys from slot kb on: the range check makes what lies behind the part's end zeros. The base moves with
+// the tile (scalar arithmetic), so lane offsets are constants and no offset passes 32 bits however long the cache is.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const uint16_t* base, int64_t stride, int kb, int kend, int tk, int d) {
+  const int rem = min(kend - kb, tk);
+  const uint32_t bytes = rem <= 0 ? 0u : (uint32_t)((rem - 1) * stride + d) * 2u;
+  return buf_rsrc(base + (int64_t)kb * stride, bytes);
+}
+
+// 16 bytes at a lane's offset and a scalar one
+__device__ __forceinline__ uint4 tile_ld(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t soff) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, soff, 0));
+}
+
+// V in LDS: rows of D values, its 64-byte blocks swapped by row so that a transposing read's four rows lie on
+// different banks.
+template <int D>
+__device__ __forceinline__ int v_swz(int row) {
+  return D == 64 ? (row >> 1) & 1 : row & 3;
+}
+template <int D>
+__device__ __forceinline__ int v_at(int row, int c) {  // byte of the 16-byte chunk c of a row
+  return row * (2 * D) + ((c >> 2) ^ v_swz<D>(row)) * 64 + (c & 3) * 16;
+}
+__device__ __forceinline__ uint2 tr4(const unsigned char* p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds4*)(p)));
+}
+
+// The state of 32 rows: this lane's row's running max (log2 domain), sum, and O^T (dims 32 d + 8 (i / 4) + 4 hf + i % 4)
+template <int DT>
+struct Rows {
+  fl_f32x16 o[DT];
+  float m, l;
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    m = -INFINITY, l = 0.0f;
+  }
+};
+
+// One tile of 32 KT keys' scores into the state. s: raw scores, s[kt][i] of key 32 kt + 8 (i / 4) + 4 hf + i % 4, -inf
+// where not seen; vt: the tile's V in LDS.
+template <bool H, int D, int KT>
+__device__ __forceinline__ void softmax_pv(fl_f32x16 (&s)[KT], Rows<D / 32>& st, float sc, const unsigned char* vt) {
+  constexpr int DT = D / 32;
+  const int lane = threadIdx.x & 63, i16 = lane & 15, hf = lane >> 5;
+  float mx = -INFINITY;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
+  mx = xor32_max(mx) * sc;
+  if (__any(mx > st.m)) {  // rows whose maximum rises; the others' factor is 1
+    const float mn = fmaxf(st.m, mx), corr = st.m == mn ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
+    st.m = mn;
+    st.l *= corr;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[d][i] *= corr;
+  }
+  const float mu = st.m == -INFINITY ? 0.0f : st.m;
+  float ps = 0.0f;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], sc, -mu));
+      ps += s[kt][i];
+    }
+  st.l += xor32_sum(ps);
+  const int row = 4 * hf + (i16 >> 2);
+  const unsigned char* vp = vt + row * (2 * D) + (i16 & 3) * 8 + ((lane >> 4) & 1) * 32;
+#pragma unroll
+  for (int st16 = 0; st16 < 2 * KT; ++st16) {  // 16 keys
+    uint32_t ph[4], pl[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float p0 = s[st16 >> 1][8 * (st16 & 1) + 2 * e], p1 = s[st16 >> 1][8 * (st16 & 1) + 2 * e + 1];
+      ph[e] = pack16<H>(p0, p1);
+      pl[e] = pack16<H>(p0 - lo16<H>(ph[e]), p1 - hi16<H>(ph[e]));
+    }
+    const uint4 bh = make_uint4(ph[0], ph[1], ph[2], ph[3]), bl = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const unsigned char* vd = vp + st16 * 16 * (2 * D) + (d ^ v_swz<D>(row)) * 64;
+      const uint2 v0 = tr4(vd), v1 = tr4(vd + 8 * (2 * D));
+      const uint4 va = make_uint4(v0.x, v0.y, v1.x, v1.y);
+      st.o[d] = mma<H>(va, bh, st.o[d]);
+      st.o[d] = mma<H>(va, bl, st.o[d]);
+    }
+  }
+}
+
+// Values of V that are not finite, in slots that some rows see and others do not: the tile's V has zeros in their
+// place, and here they are added to the rows that see them (an infinity or a NaN stays one under any weight).
+template <bool H, int D>
+__device__ __forceinline__ void add_not_finite(const AttnArgs& a, const uint8_t* mask, const uint16_t* v, int pos, int kb,
+                                               int kend, int tk, int t, Rows<D / 32>& st) {
+  const int hf = (threadIdx.x & 63) >> 5;
+  const auto vr = tile_rsrc(v, a.v_s, kb, kend, tk, D);
+#pragma unroll 1
+  for (int key = max(kb, pos); key < min(kend, kb + tk); ++key) {
+    const int j = key - pos;
+    const bool seen = mask ? mask[(uint32_t)t * (uint32_t)a.m + (uint32_t)j] != 0 : j <= t;
+    const uint32_t off = seen ? (uint32_t)((key - kb) * a.v_s + 4 * hf) * 2u : 0xFFFFFF00u;  // not seen: zeros
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint2 w = buf_ld64(vr, off + 64 * d + 16 * e);
+        const float x[4] = {lo16<H>(w.x), hi16<H>(w.x), lo16<H>(w.y), hi16<H>(w.y)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[d][4 * e + i] += __builtin_isfinite(x[i]) ? 0.0f : x[i];
+        asm volatile("" ::: "memory");
+      }
+  }
+}
+
+template <bool H, int D>
+__device__ __forceinline__ void store_rows(const AttnArgs& a, const Rows<D / 32>& st, int b, int g, int part, int row, bool bad) {
+  if (row >= a.R) return;
+  const int hf = (threadIdx.x & 63) >> 5, t = row / a.rep, head = g * a.rep + row % a.rep;
+  if (a.parts == 1) {
+    const int64_t at = ((int64_t)b * a.m + t) * a.heads + head;
+    const float inv = bad ? NAN : st.l == 0.0f ? 0.0f : 1.0f / st.l;
+    uint16_t* d0 = a.out + at * D + 4 * hf;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<uint2*>(d0 + 32 * d + 8 * e) =
+            make_uint2(pack16<H>(st.o[d][4 * e] * inv, st.o[d][4 * e + 1] * inv),
+                       pack16<H>(st.o[d][4 * e + 2] * inv, st.o[d][4 * e + 3] * inv));
+    if (a.lse && hf == 0)
+      a.lse[at] = bad ? NAN : st.l == 0.0f ? -INFINITY : (st.m + __builtin_amdgcn_logf(st.l)) * 0.6931471805599453f;
+  } else {
+    const int64_t n = (int64_t)a.b * a.groups * a.R;
+    const int64_t idx = (int64_t)part * n + ((int64_t)b * a.groups + g) * a.R + row;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<fl_f32x4*>(a.part + idx * D + 32 * d + 8 * e + 4 * hf) =
+            fl_f32x4{st.o[d][4 * e], st.o[d][4 * e + 1], st.o[d][4 * e + 2], st.o[d][4 * e + 3]};
+    if (hf == 0) {
+      float* ml = a.part + (int64_t)a.parts * n * D + idx * 2;
+      ml[0] = st.m;
+      ml[1] = st.l;
+    }
+  }
+}
+
+// ---- few rows: every wave takes its own keys ------------------------------------------------------------
+// 32 rows of a key head and one part of the keys per workgroup; its waves take tiles of TK keys in turn, K straight from
+// memory into the MFMA's operand layout, V through a piece of LDS that only this wave uses, the next tile's loads in
+// flight behind the products. No barrier until the waves' (m, l, o) meet in LDS at the end.
+template <bool H, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void k_attn_few(AttnArgs a) {
+  constexpr int TK = 4096 / D, KT = TK / 32, ST = D / 16, DT = D / 32, CH = D / 8;  // CH: 16-byte chunks of a row
+  constexpr int VB = TK * D * 2, MB = 18 * 64 * 4;
+  __shared__ __align__(16) unsigned char smem[NW * (VB > MB ? VB : MB)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hf = lane >> 5;
+  int rest = blockIdx.x;
+  const int g = rest % a.groups;
+  rest /= a.groups;
+  const int blk = rest % a.blocks;
+  rest /= a.blocks;
+  const int part = rest % a.parts, b = rest / a.parts;
+  const Span sp = span_of(a, b, part, NW * TK);
+  if (a.parts > 1 && sp.kb0 >= sp.kend) return;  // the merge knows
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
+  const uint16_t* kp = a.k + (int64_t)b * a.k_b + (int64_t)g * a.k_g;
+  const uint16_t* vp = a.v + (int64_t)b * a.v_b + (int64_t)g * a.v_g;
+  const int row = blk * 32 + r, rowc = min(row, a.R - 1), t = rowc / a.rep, head = g * a.rep + rowc % a.rep;
+  uint4 qf[ST];
+  const uint16_t* qp = a.q + (int64_t)b * a.q_b + (int64_t)t * a.q_m + (int64_t)head * a.q_h;
+#pragma unroll
+  for (int s = 0; s < ST; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + s * 16 + hf * 8);
+  Rows<DT> st;
+  st.clear();
+  unsigned char* vt = smem + wave * VB;
+  unsigned char* vw = vt + v_at<D>(lane / CH, lane % CH);  // a sweep of 64 lanes is 1 KB of rows, at the same swizzle
+  const uint32_t ko = (uint32_t)(r * a.k_s + hf * 8) * 2u, kstep = (uint32_t)(32 * a.k_s) * 2u;
+  const uint32_t vo = (uint32_t)((lane / CH) * a.v_s + (lane % CH) * 8) * 2u, vstep = (uint32_t)((64 / CH) * a.v_s) * 2u;
+  uint4 kf[KT][ST], vf[8];
+  auto load = [&](int kb) {
+    const auto kr = tile_rsrc(kp, a.k_s, kb, sp.kend, TK, D), vr = tile_rsrc(vp, a.v_s, kb, sp.kend, TK, D);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int s = 0; s < ST; ++s) kf[kt][s] = tile_ld(kr, ko + s * 32, kt * kstep);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vf[i] = tile_ld(vr, vo, i * vstep);
+  };
+  int kb = sp.kb0 + wave * TK;
+  if (kb < sp.kend) load(kb);
+  for (; kb < sp.kend; kb += NW * TK) {
+    const bool nodes = kb + TK > sp.pos;  // some keys of the tile are nodes (or lie behind the end)
+    bool odd = false;
+    if (nodes) {
+      bool fin = true;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) fin = fin && finite16<H>(vf[i]);
+      odd = __any(!fin);
+      if (odd) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = kb + lane / CH + i * (64 / CH);
+          if (key >= sp.pos) vf[i] = only_finite<H>(vf[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(vw + i * 1024) = vf[i];
+    fl_f32x16 s[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < ST; ++e) s[kt] = mma<H>(kf[kt][e], qf[e], s[kt]);
+    }
+    const int kn = kb + NW * TK;
+    load(kn < sp.kend ? kn : sp.kend);  // behind the end: zeros, nothing read
+    if (nodes) hide<KT>(a, mask, sp.pos, sp.kend, kb, t, s);
+    softmax_pv<H, D, KT>(s, st, a.sc, vt);
+    if (odd) add_not_finite<H, D>(a, mask, vp, sp.pos, kb, sp.kend, TK, t, st);
+  }
+  // the waves' states, one 32-dim tile at a time: each wave sums its share of the registers over the waves
+  static_assert(16 % NW == 0 && 16 / NW == 2, "two registers each");
+  const int i0 = 2 * wave;  // dims 32 d + 8 (i0 / 4) + 4 hf + i0 % 4 and the next
+  float mm = -INFINITY, ll = 0.0f;
+  const int64_t n = (int64_t)a.b * a.groups * a.R, idx = (int64_t)part * n + ((int64_t)b * a.groups + g) * a.R + row;
+  const int64_t at = ((int64_t)b * a.m + t) * a.heads + head;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+    __syncthreads();
+    float* mine = reinterpret_cast<float*>(smem) + wave * 18 * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mine[i * 64] = st.o[d][i];
+    mine[16 * 64] = st.m;
+    mine[17 * 64] = st.l;
+    __syncthreads();
+    const float* all = reinterpret_cast<const float*>(smem) + lane;
+    if (d == 0) {
+#pragma unroll
+      for (int w = 0; w < NW; ++w) mm = fmaxf(mm, all[(w * 18 + 16) * 64]);
+    }
+    const float mu = mm == -INFINITY ? 0.0f : mm;
+    float o0 = 0.0f, o1 = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float e = __builtin_amdgcn_exp2f(all[(w * 18 + 16) * 64] - mu);
+      l += e * all[(w * 18 + 17) * 64];
+      o0 += e * all[(w * 18 + i0) * 64];
+      o1 += e * all[(w * 18 + i0 + 1) * 64];
+    }
+    ll = l;
+    const int dim = 32 * d + 8 * (i0 >> 2) + 4 * hf + (i0 & 3);
+    if (row < a.R) {
+      if (a.parts == 1) {
+        const float inv = sp.keys < 0 ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+        *reinterpret_cast<uint32_t*>(a.out + at * D + dim) = pack16<H>(o0 * inv, o1 * inv);
+      } else {
+        *reinterpret_cast<float2*>(a.part + idx * D + dim) = make_float2(o0, o1);
+      }
+    }
+  }
+  if (wave == 0 && hf == 0 && row < a.R) {
+    if (a.parts == 1) {
+      if (a.lse) a.lse[at] = sp.keys < 0 ? NAN : ll == 0.0f ? -INFINITY : (mm + __builtin_amdgcn_logf(ll)) * 0.6931471805599453f;
+    } else {
+      float* ml = a.part + (int64_t)a.parts * n * D + idx * 2;
+      ml[0] = mm;
+      ml[1] = ll;
+    }
+  }
+}
+
+// ---- many rows: the workgroup's waves share the keys ------------------------------------------------------
+// 32 rows per wave, four waves, one part of the keys in rounds of 64, K and V staged in LDS, double-buffered.
+template <bool H, int D>
+__global__ __launch_bounds__(256, 2) void k_attn_many(AttnArgs a) {
+  constexpr int TK = 64, KT = 2, ST = D / 16, DT = D / 32, CH = D / 8, PT = TK * CH / 256;  // PT: chunks per thread
+  __shared__ __align__(16) unsigned char ks[2][TK * D * 2];
+  __shared__ __align__(16) unsigned char vs[2][TK * D * 2];
+  __shared__ int odd[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hf = lane >> 5;
+  int rest = blockIdx.x;
+  const int g = rest % a.groups;
+  rest /= a.groups;
+  const int part = rest % a.parts;
+  rest /= a.parts;
+  const int blk = a.blocks - 1 - rest % a.blocks, b = rest / a.blocks;  // the longest rows first
+  Span sp = span_of(a, b, part, TK);
+  if (a.parts > 1 && sp.kb0 >= sp.kend) return;
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
+  const uint16_t* kp = a.k + (int64_t)b * a.k_b + (int64_t)g * a.k_g;
+  const uint16_t* vp = a.v + (int64_t)b * a.v_b + (int64_t)g * a.v_g;
+  const int row = blk * 128 + wave * 32 + r, rowc = min(row, a.R - 1), t = rowc / a.rep;
+  // a chain's rows see nothing behind their own node: the workgroup's last key, and the wave's
+  int kend = sp.kend, wend = sp.kend;
+  if (!mask && sp.keys > 0) {
+    kend = min(kend, sp.pos + min(a.m - 1, (blk * 128 + 127) / a.rep) + 1);
+    wend = min(kend, sp.pos + min(a.m - 1, (blk * 128 + wave * 32 + 31) / a.rep) + 1);
+  }
+  const int wfull = sp.pos + (mask ? 0 : min(a.m - 1, (blk * 128 + wave * 32) / a.rep) + 1);  // keys that all its rows see
+  uint4 qf[ST];
+  const uint16_t* qp = a.q + (int64_t)b * a.q_b + (int64_t)t * a.q_m + (int64_t)(g * a.rep + rowc % a.rep) * a.q_h;
+#pragma unroll
+  for (int s = 0; s < ST; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + s * 16 + hf * 8);
+  Rows<DT> st;
+  st.clear();
+  const int c = tid % CH, k0 = tid / CH;
+  const uint32_t ko = (uint32_t)(k0 * a.k_s + c * 8) * 2u, kstep = (uint32_t)((256 / CH) * a.k_s) * 2u;
+  const uint32_t vo = (uint32_t)(k0 * a.v_s + c * 8) * 2u, vstep = (uint32_t)((256 / CH) * a.v_s) * 2u;
+  uint4 kv[PT], vv[PT];
+  auto load = [&](int kb) {
+    const auto kr = tile_rsrc(kp, a.k_s, kb, kend, TK, D), vr = tile_rsrc(vp, a.v_s, kb, kend, TK, D);
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      kv[i] = tile_ld(kr, ko, i * kstep);
+      vv[i] = tile_ld(vr, vo, i * vstep);
+    }
+  };
+  auto k_at = [&](int key, int ch) {  // 16 rows' chunk on 16 different places
+    return key * (2 * D) + (ch ^ (D == 64 ? (key >> 1) & 7 : key & 15)) * 16;
+  };
+  const int kw = k_at(k0, c), vw = v_at<D>(k0, c);  // a sweep of 256 threads is 4 KB of rows, at the same swizzle
+  auto store = [&](int buf, int kb) {
+    if (kb + TK > sp.pos) {
+#pragma unroll
+      for (int i = 0; i < PT; ++i)
+        if (kb + k0 + i * (256 / CH) >= sp.pos && !finite16<H>(vv[i])) {
+          vv[i] = only_finite<H>(vv[i]);
+          odd[buf] = kb + 1;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      *reinterpret_cast<uint4*>(ks[buf] + kw + i * 4096) = kv[i];
+      *reinterpret_cast<uint4*>(vs[buf] + vw + i * 4096) = vv[i];
+    }
+  };
+  if (tid < 2) odd[tid] = 0;
+  __syncthreads();
+  if (sp.kb0 < kend) {
+    load(sp.kb0);
+    store(0, sp.kb0);
+  }
+  int buf = 0;
+  for (int kb = sp.kb0; kb < kend; kb += TK, buf ^= 1) {
+    const bool more = kb + TK < kend;
+    __syncthreads();
+    if (more) load(kb + TK);
+    if (kb < wend) {
+      fl_f32x16 s[KT];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < ST; ++e)
+          s[kt] = mma<H>(*reinterpret_cast<const uint4*>(ks[buf] + k_at(kt * 32 + r, 2 * e + hf)), qf[e], s[kt]);
+      }
+      if (kb + TK > wfull) hide<KT>(a, mask, sp.pos, kend, kb, t, s);
+      softmax_pv<H, D, KT>(s, st, a.sc, vs[buf]);
+      if (odd[buf] == kb + 1) add_not_finite<H, D>(a, mask, vp, sp.pos, kb, kend, TK, t, st);
+    }
+    if (more) store(buf ^ 1, kb + TK);
+  }
+  store_rows<H, D>(a, st, b, g, part, row, sp.keys < 0);
+}
+
+// The key parts of a row merged in order: a wave per row, lanes over dims
+template <bool H, int D>
+__global__ __launch_bounds__(256) void k_attn_merge(AttnArgs a, int unit) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)a.b * a.groups * a.R, w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= n) return;
+  const int row = (int)(w % a.R), g = (int)(w / a.R % a.groups), b = (int)(w / a.R / a.groups);
+  const Span sp = span_of(a, b, 0, unit);
+  const int parts = sp.keys < 0 ? 0 : (sp.keys + part_keys(sp.keys, a.parts, unit) - 1) / part_keys(sp.keys, a.parts, unit);
+  const float* ml = a.part + (int64_t)a.parts * n * D;
+  float mm = -INFINITY;
+  for (int p = 0; p < parts; ++p) mm = fmaxf(mm, ml[(p * n + w) * 2]);
+  const float mu = mm == -INFINITY ? 0.0f : mm;
+  float L = 0.0f, O[D / 64] = {};
+  for (int p = 0; p < parts; ++p) {
+    const float e = __builtin_amdgcn_exp2f(ml[(p * n + w) * 2] - mu);
+    L += ml[(p * n + w) * 2 + 1] * e;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) O[i] += a.part[(p * n + w) * D + lane + 64 * i] * e;
+  }
+  const int64_t at = ((int64_t)b * a.m + row / a.rep) * a.heads + g * a.rep + row % a.rep;
+  const float inv = sp.keys < 0 ? NAN : L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) a.out[at * D + lane + 64 * i] = (uint16_t)pack16<H>(O[i] * inv, 0.0f);
+  if (a.lse && lane == 0)
+    a.lse[at] = sp.keys < 0 ? NAN : L == 0.0f ? -INFINITY : (mm + __builtin_amdgcn_logf(L)) * 0.6931471805599453f;
+}
+
+// ---- the weight that every key gathers ---------------------------------------------------------------------
+// w[key] (+)= sum over rows of exp2(s c - lse log2 e). A wave holds 64 keys of a key head in its MFMA operands and walks
+// over the rows, 32 at a time, sums in registers; lanes meet at the end. SPLIT: the four waves of a workgroup share 64
+// keys and take the row tiles in turn (many rows), else each has 64 keys of its own. One workgroup writes a key, in a
+// fixed order: no atomics, the same bits every time.
+template <bool H, int D, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void k_attn_weights(AttnArgs a, float* __restrict__ w, int add) {
+  constexpr int KT = 2, ST = D / 16;
+  __shared__ float red[4][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hf = lane >> 5;
+  const int g = blockIdx.x % a.groups, rest = blockIdx.x / a.groups;
+  const int tiles = (a.slots + 63) / 64, per = SPLIT ? tiles : (tiles + 3) / 4;
+  const int b = rest / per, kb = (SPLIT ? rest % per : rest % per * 4 + wave) * 64;
+  int pos = a.pos ? a.pos[b] : a.pos0;
+  const bool bad = pos < 0 || pos > a.slots - a.m;
+  const int keys = bad ? 0 : pos + a.m;
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
+  float acc[KT][16];
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[kt][i] = 0.0f;
+  if (kb < keys) {
+    const uint16_t* kp = a.k + (int64_t)b * a.k_b + (int64_t)g * a.k_g;
+    const auto kr = tile_rsrc(kp, a.k_s, kb, keys, 64, D);
+    uint4 kf[KT][ST];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int s = 0; s < ST; ++s) kf[kt][s] = buf_ld128(kr, (uint32_t)((kt * 32 + r) * a.k_s + hf * 8 + s * 16) * 2u);
+    // a chain's nodes before the tile's first key see none of it
+    const int first = mask ? 0 : max(0, kb - pos) * a.rep / 32;
+    const int step = SPLIT ? 4 : 1;
+    for (int rt = first + (SPLIT ? wave : 0); rt * 32 < a.R; rt += step) {
+      const int row = rt * 32 + r, rowc = min(row, a.R - 1), t = rowc / a.rep, head = g * a.rep + rowc % a.rep;
+      const uint16_t* qp = a.q + (int64_t)b * a.q_b + (int64_t)t * a.q_m + (int64_t)head * a.q_h;
+      const float lse = a.lse[((int64_t)b * a.m + t) * a.heads + head];
+      const bool none = row >= a.R || lse == -INFINITY;
+      const float ref = lse * 1.4426950408889634f;
+      fl_f32x16 s[KT];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < ST; ++e) {
+        const uint4 qf = *reinterpret_cast<const uint4*>(qp + e * 16 + hf * 8);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) s[kt] = mma<H>(kf[kt][e], qf, s[kt]);
+      }
+      if (kb + 64 > pos) {
+        hide<KT>(a, mask, pos, keys, kb, t, s);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], a.sc, -ref));
+            acc[kt][i] += none || s[kt][i] == -INFINITY ? 0.0f : p;
+          }
+      } else {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], a.sc, -ref));
+            acc[kt][i] += none ? 0.0f : p;
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float v = group_sum(acc[kt][i], 32);
+      if (r == 0) red[wave][32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3)] = v;
+    }
+  __syncthreads();
+  float* row = w + ((int64_t)b * a.groups + g) * a.slots;
+  if (SPLIT) {
+    if (tid < 64 && kb + tid < a.slots) {
+      const float v = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+      if (bad) row[kb + tid] = NAN;
+      else if (!add) row[kb + tid] = v;
+      else if (kb + tid < keys) row[kb + tid] += v;
+    }
+  } else if (kb + lane < a.slots) {
+    const float v = red[wave][lane];
+    if (bad) row[kb + lane] = NAN;
+    else if (!add) row[kb + lane] = v;
+    else if (kb + lane < keys) row[kb + lane] += v;
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------
+constexpr int AT_NW = 8;  // waves of k_attn_few
+
+bool desc_ok(const fl_attn_desc* d) {
+  if (!d || d->b < 1 || d->m < 1 || d->heads < 1 || d->groups < 1 || d->slots < 1) return false;
+  if (d->heads % d->groups || (d->dim != 64 && d->dim != 128) || d->m > d->slots) return false;
+  if (d->b > 65536 || d->m > 32768 || d->heads > 4096 || (int64_t)d->m * (d->heads / d->groups) > (1 << 24)) return false;
+  if (!(d->scale > 0.0f) || d->scale > 3.0e38f) return false;
+  const int64_t st[] = {d->q_b, d->q_m, d->q_h, d->k_b, d->k_g, d->k_s, d->v_b, d->v_g, d->v_s};
+  for (int64_t x : st)
+    if (x < 0 || x % 8 || x > (int64_t)1 << 40) return false;
+  // a tile of 64 slots within 32 bits
+  return d->k_s <= 1 << 23 && d->v_s <= 1 << 23 && d->mask_b >= 0;
+}
+bool on16(const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+struct AttnPlan {
+  bool few;
+  int blocks, parts, unit;
+  int64_t bytes;
+};
+// `keys`: of the longest sequence, as far as the host knows
+AttnPlan attn_plan(const fl_attn_desc& d, bool pos_known) {
+  const int R = d.m * (d.heads / d.groups), keys = pos_known ? d.pos0 + d.m : d.slots;
+  AttnPlan p{};
+  p.few = R <= 64;
+  p.blocks = p.few ? (R + 31) / 32 : (R + 127) / 128;
+  p.unit = p.few ? AT_NW * 4096 / d.dim : 64;
+  const int64_t base = (int64_t)d.b * d.groups * p.blocks;
+  const int least = p.few ? p.unit : 256;
+  p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({p.few ? 64 : 16, 512 / base, keys / least}));
+  const int64_t n = (int64_t)d.b * d.groups * R;
+  p.bytes = p.parts == 1 ? 0 : p.parts * n * (d.dim + 2) * 4;
+  return p;
+}
+AttnArgs attn_args(const fl_attn_desc& d, const uint16_t* q, const uint16_t* k, const uint16_t* v, const int32_t* pos,
+                   const uint8_t* mask) {
+  AttnArgs a{};
+  a.q = q, a.k = k, a.v = v, a.pos = pos, a.mask = mask;
+  a.b = d.b, a.m = d.m, a.heads = d.heads, a.groups = d.groups, a.rep = d.heads / d.groups, a.slots = d.slots;
+  a.pos0 = d.pos0, a.R = d.m * a.rep;
+  a.blocks = a.parts = 1;
+  a.sc = d.scale * 1.4426950408889634f;
+  a.q_b = d.q_b, a.q_m = d.q_m, a.q_h = d.q_h, a.k_b = d.k_b, a.k_g = d.k_g, a.k_s = d.k_s;
+  a.v_b = d.v_b, a.v_g = d.v_g, a.v_s = d.v_s, a.mask_b = d.mask_b;
+  return a;
+}
+
+template <bool H, int D>
+int attn_launch(AttnArgs a, const AttnPlan& p, hipStream_t s) {
+  const int64_t wgs = (int64_t)a.b * a.groups * p.blocks * p.parts;
+  if (wgs > INT32_MAX) return FL_E_ARG;
+  const dim3 grid((uint32_t)wgs);
+  if (!p.few) hipLaunchKernelGGL((k_attn_many<H, D>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_attn_few<H, D, AT_NW>), grid, dim3(64 * AT_NW), 0, s, a);
+  if (p.parts > 1) {
+    const int64_t n = (int64_t)a.b * a.groups * a.R;
+    hipLaunchKernelGGL((k_attn_merge<H, D>), dim3((uint32_t)((n + 3) / 4)), dim3(256), 0, s, a, p.unit);
+  }
+  return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
+}
+template <bool H, int D>
+int weights_launch(AttnArgs a, float* w, int add, hipStream_t s) {
+  const bool split = a.R > 32;
+  const int tiles = (a.slots + 63) / 64, per = split ? tiles : (tiles + 3) / 4;
+  const int64_t wgs = (int64_t)a.b * a.groups * per;
+  if (wgs > INT32_MAX) return FL_E_ARG;
+  if (split) hipLaunchKernelGGL((k_attn_weights<H, D, true>), dim3((uint32_t)wgs), dim3(256), 0, s, a, w, add);
+  else hipLaunchKernelGGL((k_attn_weights<H, D, false>), dim3((uint32_t)wgs), dim3(256), 0, s, a, w, add);
+  return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fl_tree_attention_workspace(const fl_attn_desc* d, int32_t pos_known, int64_t* bytes) {
+  if (!desc_ok(d) || !bytes) return FL_E_ARG;
+  if (pos_known && (d->pos0 < 0 || d->pos0 > d->slots - d->m)) return FL_E_POS;
+  *bytes = attn_plan(*d, pos_known != 0).bytes;
+  return FL_OK;
+}
+
+int fl_tree_attention(const fl_attn_desc* d, const uint16_t* q, const uint16_t* k, const uint16_t* v, const int32_t* pos,
+                      const uint8_t* mask, uint16_t* out, float* lse, void* work, void* stream) {
+  if (!desc_ok(d) || !on16(q) || !on16(k) || !on16(v) || !on16(out)) return FL_E_ARG;
+  if (!pos && (d->pos0 < 0 || d->pos0 > d->slots - d->m)) return FL_E_POS;
+  const AttnPlan p = attn_plan(*d, pos == nullptr);
+  if (p.bytes && !on16(work)) return FL_E_ARG;
+  AttnArgs a = attn_args(*d, q, k, v, pos, mask);
+  a.out = out, a.lse = lse, a.part = static_cast<float*>(work), a.blocks = p.blocks, a.parts = p.parts;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (d->dim == 64) return d->fp16 ? attn_launch<true, 64>(a, p, s) : attn_launch<false, 64>(a, p, s);
+  return d->fp16 ? attn_launch<true, 128>(a, p, s) : attn_launch<false, 128>(a, p, s);
+}
+
+int fl_attention_weights(const fl_attn_desc* d, const uint16_t* q, const uint16_t* k, const float* lse, const int32_t* pos,
+                         const uint8_t* mask, float* weights, int32_t add, void* stream) {
+  if (!desc_ok(d) || !on16(q) || !on16(k) || !lse || !weights) return FL_E_ARG;
+  if (!pos && (d->pos0 < 0 || d->pos0 > d->slots - d->m)) return FL_E_POS;
+  AttnArgs a = attn_args(*d, q, k, nullptr, pos, mask);
+  a.lse = const_cast<float*>(lse);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (d->dim == 64) return d->fp16 ? weights_launch<true, 64>(a, weights, add, s) : weights_launch<false, 64>(a, weights, add, s);
+  return d->fp16 ? weights_launch<true, 128>(a, weights, add, s) : weights_launch<false, 128>(a, weights, add, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,192 @@
+// Eviction from a K/V cache by the weight that its keys have gathered: which slots of each head stay (k_evict_select)
+// and the move of their rows (k_evict_gather into another cache, k_evict_move in place).
+#include <algorithm>
+#include "fl_common.h"
+
+namespace {
+
+struct EvictArgs {
+  unsigned char *k, *v;          // source (and destination in place)
+  float* w;
+  unsigned char *ko, *vo;        // destination of k_evict_gather
+  float* wo;
+  int32_t* kept;                 // [heads][keep]
+  int n0, n1;                    // heads = n0 * n1
+  int slots, slots_out, n, keep, recent, sink, rb;  // rb: bytes of a row
+  // bytes between heads (outer, inner) and rows; w and wo are [heads][slots]
+  int64_t k0, k1, ks, v0, v1, vs, ko0, ko1, kos, vo0, vo1, vos;
+};
+
+constexpr int ES_NT = 1024, ES_NW = ES_NT / FL_WAVE;
+
+// ordered key of a weight: larger weight <-> larger key, a NaN above all, -0 as 0
+__device__ __forceinline__ uint32_t w_key(float w) {
+  if (w != w) return 0xFFFFFFFFu;
+  const uint32_t b = __float_as_uint(w + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+// One workgroup per head. The `free` largest of the slots between sink and recent by a radix select over the 32-bit
+// keys (four counts of 256 bins), ties to the lower slot; then the kept slots in order: each wave walks a contiguous
+// piece of the slots twice, counting and then placing by ballots.
+__global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
+  __shared__ int hist[ES_NW][256];
+  __shared__ int sum[256], sel[2], above_w[ES_NW], equal_w[ES_NW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.x;
+  const float* w = a.w + (int64_t)head * a.slots;
+  int32_t* kept = a.kept + (int64_t)head * a.keep;
+  const int lo = a.sink, hi = a.n - a.recent, want = a.keep - a.sink - a.recent;  // 0 <= want <= hi - lo
+  uint32_t prefix = 0;
+  int need = want;  // of those with the prefix so far
+  if (want > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = tid; i < ES_NW * 256; i += ES_NT) (&hist[0][0])[i] = 0;
+      __syncthreads();
+      for (int i = lo + tid; i < hi; i += ES_NT) {
+        const uint32_t key = w_key(w[i]);
+        if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[wave][(key >> shift) & 255], 1);
+      }
+      __syncthreads();
+      if (tid < 256) {
+        int n = 0;
+        for (int i = 0; i < ES_NW; ++i) n += hist[i][tid];
+        sum[tid] = n;
+      }
+      __syncthreads();
+      int above = 0;
+      const int bin = select_bin(sum, need, &above, sel);
+      prefix = (prefix << 8) | (uint32_t)bin;
+      need -= above;
+      __syncthreads();
+    }
+  }
+  // want = 0: nothing between sink and recent stays
+  const int piece = ((a.n + ES_NW - 1) / ES_NW + 63) / 64 * 64, p0 = min(a.n, wave * piece), p1 = min(a.n, p0 + piece);
+  int above = 0, equal = 0;
+  for (int i = p0 + lane; i - lane < p1; i += 64) {
+    const bool in = i < p1, mid = in && i >= lo && i < hi && want > 0;
+    const uint32_t key = mid ? w_key(w[i]) : 0;
+    above += __popcll(__ballot(mid ? key > prefix : in && (i < lo || i >= hi)));
+    equal += __popcll(__ballot(mid && key == prefix));
+  }
+  if (lane == 0) above_w[wave] = above, equal_w[wave] = equal;
+  __syncthreads();
+  int eq = 0, at = 0;  // equal ones before this wave, and the kept ones
+  for (int i = 0; i < wave; ++i) {
+    at += above_w[i] + min(equal_w[i], max(0, need - eq));
+    eq += equal_w[i];
+  }
+  for (int i = p0 + lane; i - lane < p1; i += 64) {
+    const bool in = i < p1, mid = in && i >= lo && i < hi && want > 0;
+    const uint32_t key = mid ? w_key(w[i]) : 0;
+    const unsigned long long e = __ballot(mid && key == prefix), below = (1ull << lane) - 1;
+    const bool stays = mid ? key > prefix || (key == prefix && eq + __popcll(e & below) < need) : in && (i < lo || i >= hi);
+    const unsigned long long s = __ballot(stays);
+    if (stays) kept[at + __popcll(s & below)] = i;
+    at += __popcll(s);
+    eq += __popcll(e);
+  }
+}
+
+__device__ __forceinline__ int64_t head_at(int head, int n1, int64_t s0, int64_t s1) {
+  return (int64_t)(head / n1) * s0 + (int64_t)(head % n1) * s1;
+}
+
+// Rows into another cache: 16 bytes a thread, K and V of a row by the same thread.
+__global__ __launch_bounds__(256) void k_evict_gather(EvictArgs a) {
+  const int per = a.rb / 16, head = blockIdx.y;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)a.keep * per) return;
+  const int j = (int)(i / per), c = (int)(i % per) * 16;
+  const int64_t src = a.kept[(int64_t)head * a.keep + j];
+  const uint4 x = *reinterpret_cast<const uint4*>(a.k + head_at(head, a.n1, a.k0, a.k1) + src * a.ks + c);
+  const uint4 y = *reinterpret_cast<const uint4*>(a.v + head_at(head, a.n1, a.v0, a.v1) + src * a.vs + c);
+  *reinterpret_cast<uint4*>(a.ko + head_at(head, a.n1, a.ko0, a.ko1) + (int64_t)j * a.kos + c) = x;
+  *reinterpret_cast<uint4*>(a.vo + head_at(head, a.n1, a.vo0, a.vo1) + (int64_t)j * a.vos + c) = y;
+  if (c == 0 && a.wo) a.wo[(int64_t)head * a.slots_out + j] = a.w[(int64_t)head * a.slots + src];
+}
+
+// In place: a workgroup takes a head's K rows, its V rows or its weights, in order, a batch at a time. A kept row never
+// moves up (kept[j] >= j), so what a later batch reads lies above all that the earlier ones write: the only wait is
+// for a batch's own reads before its writes.
+__global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
+  constexpr int U = 8;
+  const int tid = threadIdx.x, head = blockIdx.x, kind = blockIdx.y;  // 0: K, 1: V, 2: weights
+  const int32_t* kept = a.kept + (int64_t)head * a.keep;
+  if (kind == 2) {
+    float* w = a.w + (int64_t)head * a.slots;
+    for (int j0 = 0; j0 < a.keep; j0 += 256 * U) {
+      float x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * 256 + tid;
+        x[u] = j < a.keep ? w[kept[j]] : 0.0f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * 256 + tid;
+        if (j < a.keep) w[j] = x[u];
+      }
+    }
+    __syncthreads();
+    for (int j = a.keep + tid; j < a.n; j += 256) w[j] = 0.0f;
+    return;
+  }
+  unsigned char* base = kind == 0 ? a.k + head_at(head, a.n1, a.k0, a.k1) : a.v + head_at(head, a.n1, a.v0, a.v1);
+  const int64_t stride = kind == 0 ? a.ks : a.vs;
+  const int per = a.rb / 16, rows = 256 / per;  // rows of a sweep of the workgroup
+  const int c = tid % per * 16, r = tid / per;
+  for (int j0 = 0; j0 < a.keep; j0 += rows * U) {
+    uint4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * rows + r;
+      if (r < rows && j < a.keep) x[u] = *reinterpret_cast<const uint4*>(base + (int64_t)kept[j] * stride + c);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * rows + r;
+      if (r < rows && j < a.keep) *reinterpret_cast<uint4*>(base + (int64_t)j * stride + c) = x[u];
+    }
+  }
+}
+
+bool strides_ok(const fl_rows* r, int32_t rb) {
+  if (!r || !r->data || (reinterpret_cast<uintptr_t>(r->data) & 15)) return false;
+  return r->outer >= 0 && r->inner >= 0 && r->row >= rb && !(r->outer % 16) && !(r->inner % 16) && !(r->row % 16);
+}
+
+}  // namespace
+
+extern "C" {
+
+int fl_evict(const fl_rows* k, const fl_rows* v, float* weights, int32_t n_outer, int32_t n_inner, int32_t slots,
+             int32_t row_bytes, int32_t n, int32_t keep, int32_t recent, int32_t sink, int32_t* kept, const fl_rows* k_out,
+             const fl_rows* v_out, float* weights_out, int32_t slots_out, void* stream) {
+  if (!weights || !kept || n_outer < 1 || n_inner < 1 || (int64_t)n_outer * n_inner > 65535) return FL_E_ARG;
+  if (row_bytes < 16 || row_bytes > 4096 || row_bytes % 16 || !strides_ok(k, row_bytes) || !strides_ok(v, row_bytes)) return FL_E_ARG;
+  if (n < 1 || slots < n || keep < 1 || keep > n || recent < 0 || sink < 0 || (int64_t)recent + sink > keep) return FL_E_ARG;
+  if (!k_out != !v_out || (weights_out && !k_out)) return FL_E_ARG;
+  if (k_out && (!strides_ok(k_out, row_bytes) || !strides_ok(v_out, row_bytes) || slots_out < keep)) return FL_E_ARG;
+  const int heads = n_outer * n_inner;
+  EvictArgs a{};
+  a.k = static_cast<unsigned char*>(k->data), a.v = static_cast<unsigned char*>(v->data), a.w = weights, a.kept = kept;
+  a.n0 = n_outer, a.n1 = n_inner, a.slots = slots, a.slots_out = slots_out, a.n = n, a.keep = keep, a.recent = recent, a.sink = sink;
+  a.rb = row_bytes;
+  a.k0 = k->outer, a.k1 = k->inner, a.ks = k->row, a.v0 = v->outer, a.v1 = v->inner, a.vs = v->row;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(k_evict_select, dim3(heads), dim3(ES_NT), 0, s, a);
+  if (k_out) {
+    a.ko = static_cast<unsigned char*>(k_out->data), a.vo = static_cast<unsigned char*>(v_out->data), a.wo = weights_out;
+    a.ko0 = k_out->outer, a.ko1 = k_out->inner, a.kos = k_out->row, a.vo0 = v_out->outer, a.vo1 = v_out->inner, a.vos = v_out->row;
+    const int64_t threads = (int64_t)keep * (row_bytes / 16);
+    hipLaunchKernelGGL(k_evict_gather, dim3((uint32_t)((threads + 255) / 256), heads), dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL(k_evict_move, dim3(heads, 3), dim3(256), 0, s, a);
+  }
+  return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
+}
+
+}  // extern "C"

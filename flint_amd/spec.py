@@ -21,12 +21,13 @@ EAGLE head consumes, reference spec_mega.py:112). LookupDraft (prompt-lookup n-g
 needs no weights.
 """
 import time
+from collections import namedtuple
 
 import numpy as np
 import torch
 
 from . import _lib
-from .generate import prefill
+from .generate import _ids, prefill
 
 
 def tree_depths(parents):
@@ -89,6 +90,60 @@ def accept_tree(cand, parents, targets):
             return path
         path.append(nxt)
         cur = nxt
+
+
+# What accept_sampled returns, for B trees of M nodes: path int32 [B, M], the accepted nodes, 0 first, then -1; count
+# int32 [B] of them; token int32 [B], the one behind the path.
+Accepted = namedtuple("Accepted", "path count token")
+
+
+def accept_sampled(probs, tokens, accept_u, sample_u, parents=None, draft_probs=None):
+    """Speculative sampling on the GPU (fl_accept): which path of each drafted tree the target's distribution accepts,
+    and the token behind it, drawn so that path and token are distributed as the target's own samples. From given
+    random numbers in [0, 1), so the same call gives the same tokens.
+
+    probs: fp32 or bf16 device [B, M, V] (or [M, V]), row i the target's distribution after node i (as
+    generate.logits_to_probs gives it). tokens: int [B, M], of the nodes (node 0 is the root, its own is not looked
+    at). accept_u: fp32 [B, M], sample_u: fp32 [B]. parents: int [B, M], -1 at the root, parents before children
+    (None: a chain); a node without an earlier node as its parent (-1: padding) is no part of the tree. draft_probs:
+    of probs' type, [B, M - 1, V], row i the distribution from which the children of node i were drawn, independently
+    of each other; None: they were proposed without one (top candidates, a lookup).
+
+    Children are tried in order: child t is accepted where accept_u q(t) Z < w(t), with w = probs' row and Z = 1 at
+    first; a rejection takes Z q off w (all of t without draft_probs), not below 0, and Z becomes the sum of w. The last
+    node's token is the first index at which the running sum of w passes sample_u times its sum (-1 where that is not
+    a positive number). Returns Accepted (without B: of one tree, count and token of one element)."""
+    one = probs.dim() == 2
+    if one:
+        probs = probs[None]
+        draft_probs = None if draft_probs is None else draft_probs[None]
+    if not probs.is_cuda or probs.dim() != 3 or probs.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("probs must be an fp32 or bf16 CUDA (HIP) tensor [B, M, V]")
+    b, m, v = probs.shape
+    dev = probs.device
+    if not 1 <= m <= 1024 or not 1 <= v <= 1 << 20 or b > 65536:
+        raise ValueError("1..1024 nodes, a vocabulary of 1..2^20 and at most 65536 trees")
+    if draft_probs is not None and (draft_probs.dtype != probs.dtype or draft_probs.device != dev
+                                    or draft_probs.shape != (b, m - 1, v)):
+        raise ValueError(f"draft_probs must be [{b}, {m - 1}, {v}] of probs' type and device")
+    for t, name in ((tokens, "tokens"), (parents, "parents")):
+        if t is not None and (t.device != dev or t.dtype not in (torch.int32, torch.int64) or t.numel() != b * m):
+            raise ValueError(f"{name} must be {b * m} int32 or int64 on probs' device")
+    for t, name, n in ((accept_u, "accept_u", b * m), (sample_u, "sample_u", b)):
+        if t.device != dev or t.dtype != torch.float32 or t.numel() != n:
+            raise ValueError(f"{name} must be {n} fp32 numbers on probs' device")
+    path = torch.empty(b, m, dtype=torch.int32, device=dev)
+    count, token = torch.empty(b, dtype=torch.int32, device=dev), torch.empty(b, dtype=torch.int32, device=dev)
+    if b:
+        # in names, so that no copy's memory is given to the next before the launch
+        probs, tokens, accept_u, sample_u = (x.detach().contiguous() for x in (probs, _ids(tokens), accept_u, sample_u))
+        parents = None if parents is None else _ids(parents).contiguous()
+        draft_probs = None if draft_probs is None else draft_probs.detach().contiguous()
+        with torch.cuda.device(dev):
+            _lib.call("fl_accept", _lib.ptr(probs), _lib.ptr(draft_probs), int(probs.dtype == torch.bfloat16),
+                      _lib.ptr(tokens), _lib.ptr(parents), _lib.ptr(accept_u), _lib.ptr(sample_u), _lib.ptr(path),
+                      _lib.ptr(count), _lib.ptr(token), b, m, v, _lib.stream_ptr())
+    return Accepted(path[0] if one else path, count, token)
 
 
 def compaction_moves(path, pos):

@@ -185,6 +185,78 @@ int fl_head_logprobs(const uint16_t* x, const int8_t* wq, const float* ws, const
                      float* logprob, float* entropy, int32_t* rank, int32_t* top_ids, float* top_logprobs, void* work,
                      int32_t m, int32_t n, int32_t k, void* stream);
 
+/* ---- attention over a cache, and keys that leave it --------------------------------------------- */
+
+/* b sequences of m nodes each (a drafted tree, a chain, a prompt, or one token), `heads` query heads over `groups` key
+ * heads of dim 64 or 128, caches of `slots` slots; bf16, or fp16 where fp16 != 0. Strides count values, between
+ * sequences, nodes / key heads and query heads / slots; the last dimension is contiguous. Strides are multiples of 8,
+ * pointers 16-byte aligned, k_s and v_s at most 2^23. mask_b: bytes between the sequences' masks (0: one for all).
+ * scale: positive. pos0: cached keys of every sequence, for calls without `pos`. */
+typedef struct fl_attn_desc {
+  int32_t b, m, heads, groups, dim, slots, fp16, pos0;
+  float scale;
+  int64_t q_b, q_m, q_h;
+  int64_t k_b, k_g, k_s;
+  int64_t v_b, v_g, v_s;
+  int64_t mask_b;
+} fl_attn_desc;
+
+/* Attention of the nodes over the cache: node i of a sequence sits in slot pos + i (K and V are there already) and
+ * attends to the slots [0, pos) and to pos + j where mask[i][j] != 0 (uint8 [M][M]; NULL: a chain, j <= i), as
+ * fl_verify's tokens do. pos: device int32 [B], or NULL for pos0. out [B][M][heads][dim], rounded once from fp32;
+ * lse (optional, fp32 [B][M][heads]): log sum exp of the scaled scores, natural. A node that sees nothing gives 0 and
+ * -inf; a sequence whose pos lies outside 0 .. slots - m gives NaN. What a node does not see never reaches it,
+ * infinities and NaN included; slots behind pos + m are not read. work: 16-byte aligned, of
+ * fl_tree_attention_workspace's bytes (0: may be NULL; pos_known != 0 for calls without pos), free for reuse once the
+ * call's work on the stream is done, not to be shared by calls that may run at the same time.
+ * Replaces the attention of reference kernels/verify_mega.cu:106-244 (spec_tree.py:46-51) as a call of its own. */
+int fl_tree_attention_workspace(const fl_attn_desc* d, int32_t pos_known, int64_t* bytes);
+int fl_tree_attention(const fl_attn_desc* d, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                      const int32_t* pos, const uint8_t* mask, uint16_t* out, float* lse, void* work, void* stream);
+
+/* The weight that each slot gathers from the nodes: weights [B][groups][slots] (fp32) = the sum over the nodes and the
+ * query heads of the group of exp(scale q.k - lse), lse as fl_tree_attention writes it (a row of -inf adds nothing);
+ * 0 in slots that no node sees. add != 0: added to what is there, slots from pos + m on left as they are. A sequence
+ * whose pos lies outside 0 .. slots - m: NaN. Sums in a fixed order. d's v strides are not used.
+ * No counterpart in the reference. */
+int fl_attention_weights(const fl_attn_desc* d, const uint16_t* q, const uint16_t* k, const float* lse,
+                         const int32_t* pos, const uint8_t* mask, float* weights, int32_t add, void* stream);
+
+/* Rows of n_outer x n_inner heads: data, and the bytes between heads (outer, inner) and rows (multiples of 16). */
+typedef struct fl_rows {
+  void* data;
+  int64_t outer, inner, row;
+} fl_rows;
+
+/* Of each head's slots [0, n) the first `sink`, the last `recent` and of the others those of the largest weight stay,
+ * `keep` in all (equal weights: the lower slot; a NaN counts as the largest). kept [heads][keep]: their numbers,
+ * rising. Their rows of K and V (row_bytes each, a multiple of 16, at most 4096) move in this order to the slots 0 ..
+ * keep - 1: in place (k_out, v_out NULL), with the weights (fp32 [heads][slots]), and the weights of keep .. n - 1
+ * become 0, the rows there stay what they were; or into k_out and v_out (which do not overlap the caches) and, where
+ * given, weights_out [heads][slots_out], with the caches left as they are. 1 <= keep <= n <= slots, sink + recent <=
+ * keep, at most 65535 heads.
+ * No counterpart in the reference, whose cache only grows (engine/model.py:82-98). */
+int fl_evict(const fl_rows* k, const fl_rows* v, float* weights, int32_t n_outer, int32_t n_inner, int32_t slots,
+             int32_t row_bytes, int32_t n, int32_t keep, int32_t recent, int32_t sink, int32_t* kept,
+             const fl_rows* k_out, const fl_rows* v_out, float* weights_out, int32_t slots_out, void* stream);
+
+/* ---- verification of drafted tokens --------------------------------------------------------------- */
+
+/* Speculative sampling: walks each of b trees of m nodes (at most 1024, parents first; node 0 the root, whose token
+ * is decided) from the root. probs [B][M][V] (fp32, or bf16 where bf16 != 0): row i the target's distribution after
+ * node i. draft [B][M - 1][V], or NULL: row i the distribution that the children of node i were drawn from, each on
+ * its own; NULL: they were proposed without one. Children are tried in order of their index; child i with token t is
+ * accepted where accept_u[i] q(t) Z < w(t), at first w = probs' row and Z = 1; a rejection makes w = max(w - Z q, 0)
+ * (q all at t where draft is NULL) and Z the sum of w. Where no child is left, the token is the first index where the
+ * running sum of w passes sample_u times its sum (of the row itself should w hold nothing). parents [B][M] (NULL: a
+ * chain), the root's is ignored; a node whose parent is not an earlier node is no part of the tree, one whose token is
+ * outside the vocabulary is passed over. path [B][M]: the accepted nodes, 0 first, then -1; count [B] of them; token
+ * [B], -1 where the last row has no finite positive sum. Sums in 64 bits, in a fixed order. V at most 2^20.
+ * Replaces reference spec_mega.py:106-110 / spec_tree.py:109-118 (accepting against the greedy token) for sampling. */
+int fl_accept(const void* probs, const void* draft, int32_t bf16, const int32_t* tokens, const int32_t* parents,
+              const float* accept_u, const float* sample_u, int32_t* path, int32_t* count, int32_t* token, int32_t b,
+              int32_t m, int32_t vocab, void* stream);
+
 /* ---- decode state --------------------------------------------------------------------- */
 
 /* Binds a caller-owned bf16 KV cache (k_cache, v_cache: [NL, NKV, max_seq, 64] each, device)

@@ -1,0 +1,265 @@
+"""Attention of drafted trees over a cache, and the weight that keys gather, against 64 bits.
+
+Tolerances. q, k, v are 16-bit, so products are exact in fp32 and a score's error is at most dim roundings of its
+partial sums: dim 2^-24 sum|q k| scale, plus the exponent's own (2^-22 of its argument). The weights P go through the
+matrix cores as two 16-bit terms: 2^-16 relative at most. fp32 sums over n keys: n 2^-24. All of it acts on the
+numerator and the denominator of a mean of values no larger than max|v|; the output is rounded once to its type.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import cache as oracle
+
+pytestmark = pytest.mark.gpu
+
+
+def tree_mask(g, b, m, empty=False):
+    """bool [b, m, m]: ancestors in random trees; with `empty`, some nodes see nothing, not even themselves."""
+    mask = torch.zeros(b, m, m, dtype=torch.bool)
+    for s in range(b):
+        mask[s, 0, 0] = True
+        for i in range(1, m):
+            p = int(torch.randint(max(0, i - 4), i, (1,), generator=g))
+            mask[s, i] = mask[s, p]
+            mask[s, i, i] = True
+        if empty:
+            mask[s, 1::3] = False
+    return mask
+
+
+def make(b, m, heads, groups, dim, slots, dtype, seed=0, sharp=1.0):
+    g = torch.Generator().manual_seed(seed)
+    q = (torch.randn(b, m, heads, dim, generator=g) * 1.5 * sharp).to(dtype)
+    k = torch.randn(b, groups, slots, dim, generator=g).to(dtype)
+    v = torch.randn(b, groups, slots, dim, generator=g).to(dtype)
+    return g, q, k, v
+
+
+def score_error(q, k, scale, dim):
+    """A bound on any score's error: dim 2^-24 max|q| . |k| scale."""
+    qm = q.double().abs().nan_to_num(0, 0, 0).flatten(0, -2).amax(0)
+    km = k.double().abs().nan_to_num(0, 0, 0).flatten(0, -2).amax(0)
+    most = float((qm * km).sum() * scale)
+    return dim * 2.0 ** -24 * most + 2.0 ** -22 * most
+
+
+def check_attention(q, k, v, pos, mask, scale, out, lse):
+    dim, dtype = q.shape[-1], q.dtype
+    b = q.shape[0]
+    plist = [pos] * b if isinstance(pos, int) else [int(x) for x in pos]
+    o, l = oracle.tree_attention(q, k, v, plist, mask, scale)
+    n = max(plist) + q.shape[1]
+    es = score_error(q, k, scale, dim)
+    delta = 2.0 ** -16 + 2 * es + n * 2.0 ** -24 + 2.0 ** -20
+    vmax = float(v.double().nan_to_num(0, 0, 0).abs().max())
+    tol = torch.finfo(dtype).eps / 2 * o.abs() + 2 * delta * vmax + torch.finfo(dtype).smallest_normal * 2.0 ** -7
+    got = out.double().cpu()
+    assert torch.equal(got.isnan(), o.isnan())
+    fin = ~o.isnan() & ~o.isinf()
+    assert torch.equal(got[o.isinf()], o[o.isinf()])
+    bad = ((got - o).abs() > tol) & fin
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {float(((got - o).abs() / tol)[fin].max()):.2f} x"
+    none = l == -math.inf
+    assert torch.equal(lse.cpu().double()[none], l[none])
+    fin = ~none & ~l.isnan() & ~l.isinf()
+    ltol = es + n * 2.0 ** -24 + 2.0 ** -21 * (l.abs() + 1)
+    assert not (((lse.cpu().double() - l).abs() > ltol) & fin).any()
+
+
+SHAPES = [  # b, m, heads, groups, dim, ctx: one token to some hundred rows, lengths at the seams of tiles and parts
+    (1, 1, 40, 8, 64, 0), (1, 1, 40, 8, 64, 1), (1, 1, 40, 8, 64, 511), (1, 1, 40, 8, 64, 512), (1, 1, 7, 1, 64, 63),
+    (1, 1, 12, 12, 128, 256), (1, 8, 40, 8, 64, 1024), (1, 8, 8, 2, 64, 0), (2, 13, 16, 2, 128, 300), (3, 5, 6, 3, 64, 64),
+    (1, 33, 8, 2, 64, 100), (1, 32, 20, 4, 64, 31), (2, 70, 10, 2, 64, 129), (1, 130, 4, 1, 128, 65), (1, 6, 40, 8, 64, 2050),
+    (1, 12, 5, 1, 64, 700), (1, 13, 5, 1, 128, 700),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_attention(dev, shape, tree, dtype):
+    from flint_amd.attention import tree_attention
+    b, m, heads, groups, dim, ctx = shape
+    g, q, k, v = make(b, m, heads, groups, dim, ctx + m + 5, dtype, seed=m + ctx)
+    # what lies behind the nodes is not read
+    k[:, :, ctx + m:], v[:, :, ctx + m:] = math.nan, math.inf
+    mask = tree_mask(g, b, m) if tree else None
+    scale = dim ** -0.5
+    out, lse = tree_attention(q.to(dev), k.to(dev), v.to(dev), ctx, None if mask is None else mask.to(dev), return_lse=True)
+    k[:, :, ctx + m:], v[:, :, ctx + m:] = 0, 0
+    check_attention(q, k, v, ctx, mask, scale, out, lse)
+
+
+@pytest.mark.parametrize("m,heads,groups,dim", [(1, 10, 2, 64), (5, 10, 2, 64), (9, 8, 1, 128), (40, 8, 2, 64)])
+def test_ragged_positions(dev, m, heads, groups, dim):
+    """A length per sequence, from none to all slots; one outside gives NaN and touches no other."""
+    from flint_amd.attention import tree_attention
+    slots = 1500
+    pos = [0, 1, 700, slots - m, 64, -1, slots - m + 1, 2 ** 31 - 1]
+    g, q, k, v = make(len(pos), m, heads, groups, dim, slots, torch.bfloat16, seed=m)
+    mask = tree_mask(g, len(pos), m)
+    for pt in (torch.tensor(pos, dtype=torch.int32), torch.tensor(pos[:-1] + [2 ** 40], dtype=torch.int64)):
+        out, lse = tree_attention(q.to(dev), k.to(dev), v.to(dev), pt.to(dev), mask.to(dev), 0.2, True)
+        assert out[5:].isnan().all() and lse[5:].isnan().all()
+        check_attention(q[:5], k[:5], v[:5], pos[:5], mask[:5], 0.2, out[:5], lse[:5])
+
+
+@pytest.mark.parametrize("m,dim", [(4, 64), (9, 64), (9, 128), (40, 64)])
+@pytest.mark.parametrize("pos", [0, 100])
+def test_rows_that_see_nothing(dev, m, dim, pos):
+    from flint_amd.attention import tree_attention
+    g, q, k, v = make(2, m, 8, 2, dim, pos + m, torch.bfloat16, seed=pos)
+    mask = tree_mask(g, 2, m, empty=True)
+    out, lse = tree_attention(q.to(dev), k.to(dev), v.to(dev), pos, mask.to(dev), return_lse=True)
+    if pos == 0:
+        assert (out[:, 1] == 0).all() and (lse[:, 1] == -math.inf).all()
+    check_attention(q, k, v, pos, mask, dim ** -0.5, out, lse)
+
+
+@pytest.mark.parametrize("m,heads,groups,dim", [(6, 4, 2, 64), (16, 8, 2, 64), (16, 8, 2, 128), (40, 8, 2, 64), (40, 8, 1, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_masked_nodes_poison_no_row(dev, m, heads, groups, dim, dtype):
+    """Infinities and NaN in the K and V of nodes reach the nodes that see them and no other."""
+    from flint_amd.attention import tree_attention
+    pos = 70
+    g, q, k, v = make(1, m, heads, groups, dim, pos + m, dtype, seed=3)
+    mask = torch.eye(m, dtype=torch.bool)
+    mask[:, 0] = True
+    k[:, :, pos + 2], v[:, :, pos + 2] = math.nan, math.nan
+    v[:, :, pos + 3, 5] = math.inf
+    v[:, :, pos + 4, 7:9] = math.nan
+    k[:, :, pos + 5] = -math.inf
+    out, lse = tree_attention(q.to(dev), k.to(dev), v.to(dev), pos, mask.to(dev), return_lse=True)
+    got = out.cpu()[0]
+    assert got[2].isnan().all() and lse[0, 2].isnan().all()
+    assert (got[3, :, 5] == math.inf).all() and got[4, :, 7:9].isnan().all() and got[4, :, 9:].isfinite().all()
+    clean = [i for i in range(m) if i not in (2, 3, 4, 5)]
+    assert got[clean].isfinite().all()
+    k, v = k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0)
+    o, _ = oracle.tree_attention(q, k, v, [pos], mask, dim ** -0.5)
+    for i in clean:
+        es = score_error(q, k, dim ** -0.5, dim)
+        tol = torch.finfo(dtype).eps / 2 * o[0, i].abs() + 2 * (2.0 ** -16 + 2 * es + (pos + m) * 2.0 ** -24 + 2.0 ** -20) * float(v.abs().max())
+        assert ((got[i].double() - o[0, i]).abs() <= tol).all()
+
+
+def test_extreme_scores(dev):
+    """Scores that pass the exponential's range either way: one key takes all."""
+    from flint_amd.attention import tree_attention
+    g, q, k, v = make(1, 3, 4, 2, 64, 600, torch.bfloat16, seed=1, sharp=60.0)
+    out, lse = tree_attention(q.to(dev), k.to(dev), v.to(dev), 597, None, 4.0, True)
+    # scores up to 10^4, whose fp32 error is up to 0.1: compare where one key leads by 20, so that no other counts, and
+    # the leading weight's two 16-bit terms leave its value of v where it rounds to
+    es = score_error(q, k, 4.0, 64)
+    qd, kd = q.double(), k.double()
+    for i in range(3):
+        for h in range(4):
+            s = (kd[0, h // 2, :598 + i] @ qd[0, i, h]) * 4.0
+            top = s.topk(2).values
+            if top[0] - top[1] > 20:
+                assert torch.equal(out[0, i, h].cpu(), v[0, h // 2, int(s.argmax())])
+            assert abs(float(lse[0, i, h]) - float(torch.logsumexp(s, 0))) <= es + 600 * 2.0 ** -24
+    assert out.isfinite().all()
+
+
+@pytest.mark.parametrize("m", [1, 7, 40])
+def test_strides(dev, m):
+    """Caches as [B, slots, key heads, dim] views, windows of larger caches, q of every order."""
+    from flint_amd.attention import attention_weights, tree_attention
+    g, q, k, v = make(2, m, 8, 2, 64, 400, torch.bfloat16, seed=9)
+    mask = tree_mask(g, 2, m)
+    want, wl = tree_attention(q.to(dev), k.to(dev), v.to(dev), 300, mask.to(dev), return_lse=True)
+    ww = attention_weights(q.to(dev), k.to(dev), wl, 300, mask.to(dev))
+    kt = k.transpose(1, 2).contiguous().to(dev).transpose(1, 2)
+    big = torch.full((2, 3, 500, 64), math.nan, dtype=v.dtype, device=dev)
+    big[:, 1:, 60:460] = v.to(dev)
+    qt = q.permute(1, 2, 0, 3).contiguous().to(dev).permute(2, 0, 1, 3)
+    odd = torch.empty(q.numel() + 1, dtype=q.dtype, device=dev)[1:].view(q.shape).copy_(q)
+    for qq in (qt, odd):
+        out, lse = tree_attention(qq, kt, big[:, 1:, 60:460], 300, mask.to(dev).to(torch.uint8), return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, wl)
+        assert torch.equal(attention_weights(qq, kt, wl, 300, mask.to(dev)), ww)
+    one, ol = tree_attention(q[1].to(dev), k[1].to(dev), v[1].to(dev), 300, mask[1].to(dev), return_lse=True)
+    assert torch.equal(one, want[1]) and torch.equal(ol, wl[1])
+    assert torch.equal(attention_weights(q[1].to(dev), k[1].to(dev), ol, 300, mask[1].to(dev)), ww[1])
+
+
+def test_row_does_not_depend_on_repeats(dev):
+    """Twenty calls, the same bits; on another stream too."""
+    from flint_amd.attention import attention_weights, tree_attention
+    g, q, k, v = make(1, 16, 40, 8, 64, 3000, torch.bfloat16, seed=5)
+    q, k, v = q.to(dev), k.to(dev), v.to(dev)
+    first, l0 = tree_attention(q, k, v, 2900, return_lse=True)
+    w0 = attention_weights(q, k, l0, 2900)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    for i in range(20):
+        with torch.cuda.stream(s if i % 2 else torch.cuda.current_stream()):
+            out, lse = tree_attention(q, k, v, 2900, return_lse=True)
+            w = attention_weights(q, k, lse, 2900)
+        s.synchronize()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first) and torch.equal(lse, l0) and torch.equal(w, w0)
+
+
+WSHAPES = [(1, 1, 40, 8, 64, 0), (2, 1, 40, 8, 64, 130), (1, 1, 12, 12, 128, 64), (1, 6, 10, 2, 64, 63), (2, 7, 8, 1, 128, 200),
+           (1, 33, 8, 2, 64, 100), (1, 100, 5, 1, 64, 0), (1, 64, 4, 2, 128, 190)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("shape", WSHAPES)
+def test_weights(dev, shape, tree, dtype):
+    from flint_amd.attention import attention_weights, tree_attention
+    b, m, heads, groups, dim, ctx = shape
+    slots = ctx + m + 70
+    g, q, k, v = make(b, m, heads, groups, dim, slots, dtype, seed=m + ctx)
+    k[:, :, ctx + m:] = math.nan
+    mask = tree_mask(g, b, m, empty=True) if tree else None
+    dm = None if mask is None else mask.to(dev)
+    _, lse = tree_attention(q.to(dev), k.to(dev), v.to(dev), ctx, dm, return_lse=True)
+    w = attention_weights(q.to(dev), k.to(dev), lse, ctx, dm)
+    k[:, :, ctx + m:] = 0
+    want = oracle.attention_weights(q, k, lse.cpu(), [ctx] * b, mask, dim ** -0.5)
+    # each term e^(s - lse): the score's error and the exponent's argument's, then the sums over the rows
+    rel = score_error(q, k, dim ** -0.5, dim) + 2.0 ** -21 * (float(lse[lse > -math.inf].abs().max()) + 1) + m * heads * 2.0 ** -24
+    assert ((w.double().cpu() - want).abs() <= rel * want + 1e-30).all()
+    assert (w[:, :, ctx + m:] == 0).all()
+    base = torch.rand(w.shape, generator=g).to(dev)
+    base[:, :, ctx + m:] = math.nan  # left as it is
+    added = attention_weights(q.to(dev), k.to(dev), lse, ctx, dm, out=(acc := base.clone()))
+    assert added is acc
+    assert torch.equal(acc[:, :, :ctx + m], base[:, :, :ctx + m] + w[:, :, :ctx + m]) and acc[:, :, ctx + m:].isnan().all()
+
+
+def test_weights_sum_to_the_rows(dev):
+    """Every row hands out 1: over the keys of a head the weights sum to its rows."""
+    from flint_amd.attention import attention_weights, tree_attention
+    pos = torch.tensor([0, 17, 900, -1], dtype=torch.int32)
+    g, q, k, v = make(4, 5, 16, 4, 64, 1000, torch.bfloat16, seed=2)
+    _, lse = tree_attention(q.to(dev), k.to(dev), v.to(dev), pos.to(dev), return_lse=True)
+    w = attention_weights(q.to(dev), k.to(dev), lse, pos.to(dev))
+    assert ((w[:3].double().sum(-1) - 20.0).abs() <= 20 * (score_error(q, k, 0.125, 64) * 2 + 2.0 ** -18 + 1000 * 2.0 ** -24)).all()
+    assert w[3].isnan().all()
+
+
+def test_refusals(dev):
+    from flint_amd.attention import attention_weights, tree_attention
+    _, q, k, v = make(2, 3, 4, 2, 64, 20, torch.bfloat16)
+    q, k, v = q.to(dev), k.to(dev), v.to(dev)
+    lse = torch.zeros(2, 3, 4, device=dev)
+    ok = dict(q=q, k_cache=k, v_cache=v, pos=5)
+    eye = torch.eye(3, device=dev)
+    for kw in (dict(q=q.float()), dict(q=q.cpu()), dict(k_cache=k.half()), dict(v_cache=v[:, :, :10]), dict(k_cache=k[:1]), dict(pos=-1),
+               dict(pos=18), dict(pos=torch.tensor([1], device=dev)), dict(pos=torch.zeros(2, device=dev)), dict(pos=torch.zeros(2, dtype=torch.int32)),
+               dict(mask=eye), dict(mask=eye.bool()[:2]), dict(mask=eye.bool().cpu()), dict(scale=0.0), dict(scale=-0.1), dict(scale=math.nan),
+               dict(scale=math.inf), dict(q=q[..., :3, :]), dict(q=q[..., :32]), dict(q=q[:0], k_cache=k[:0], v_cache=v[:0]),
+               dict(k_cache=k.transpose(2, 3).contiguous().transpose(2, 3)), dict(k_cache=torch.cat([k, k], -1)[..., 4:68])):
+        with pytest.raises(ValueError):
+            tree_attention(**{**ok, **kw})
+    for kw in (dict(lse=lse.half()), dict(lse=lse[:1]), dict(out=torch.zeros(2, 2, 19, device=dev)), dict(out=torch.zeros(2, 2, 20)),
+               dict(out=torch.zeros(2, 2, 40, device=dev)[..., ::2])):
+        with pytest.raises(ValueError):
+            attention_weights(**{**dict(q=q, k_cache=k, lse=lse, pos=5), **kw})
