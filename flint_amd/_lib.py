@@ -35,6 +35,7 @@ EXPORTS = [
     "fl_quantize_int8", "fl_gemm_int8_workspace", "fl_gemm_int8", "fl_linear_int8_workspace", "fl_linear_int8",
     "fl_logprobs_workspace", "fl_logprobs", "fl_head_logprobs_workspace", "fl_head_logprobs",
     "fl_tree_attention_workspace", "fl_tree_attention", "fl_attention_weights", "fl_evict", "fl_accept",
+    "fl_prefill_extra_workspace", "fl_prefill_weights", "fl_prefill_tree",
 ]
 
 
@@ -115,6 +116,9 @@ def load(path=LIB_PATH):
         "fl_verify": ([ctypes.POINTER(Weights), vp, vp, i32, vp, vp, i32, vp, vp, vp, vp], i32),
         "fl_prefill_workspace": ([vp, i32, ctypes.POINTER(ctypes.c_int64)], i32),
         "fl_prefill": ([ctypes.POINTER(Weights), vp, vp, i32, i32, vp, vp, vp], i32),
+        "fl_prefill_extra_workspace": ([vp, i32, ctypes.POINTER(ctypes.c_int64)], i32),
+        "fl_prefill_weights": ([ctypes.POINTER(Weights), vp, vp, i32, i32, vp, vp, vp, i32, vp, vp], i32),
+        "fl_prefill_tree": ([ctypes.POINTER(Weights), vp, vp, i32, vp, vp, i32, vp, vp, vp], i32),
         "fl_prefill_feat": ([ctypes.POINTER(Weights), vp, vp, i32, i32, vp, vp, vp, vp], i32),
         "fl_quantize_int8": ([vp, vp, vp, i32, i32, vp], i32),
         "fl_gemm_int8_workspace": ([i32, i32, i32, pi64], i32),

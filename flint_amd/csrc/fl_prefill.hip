@@ -27,17 +27,28 @@ constexpr int PF_LM_GRID = 512;   // LM-head workgroups
 // ---- GEMM epilogues -----------------------------------------------------------------------------
 // v[0..3]: packed rows n..n+3 of one token, i.e. two NEOX / gate-up pairs
 
-// RoPE at pos + m, q rows out, K / V rows into the cache (engine/model.py:257-269, :88-98)
+// RoPE at pos + m (TREE: at pos + depth[m]), q rows out, K / V rows into the cache (engine/model.py:257-269, :88-98)
+template <bool TREE>
 struct EpiQkv {
   uint16_t *q, *kc, *vc;  // q [T][NH * 64]; kc / vc of this layer [NKV][S][64]
   const uint32_t* rope;   // [rope_len][32] (cos, sin) pairs
   int m, nh, nkv, S, pos;
+  const int32_t* depth;   // TREE: [T]
+  int rope_len;
+  int32_t* err;
+  __device__ __forceinline__ int rope_at(int mm) const {
+    if constexpr (!TREE) return pos + mm;
+    const int r = pos + depth[mm];
+    if (r >= 0 && r < rope_len) return r;
+    __hip_atomic_store(err, (int32_t)FL_E_POS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return min(max(r, 0), rope_len - 1);
+  }
   __device__ __forceinline__ void operator()(int n, int mm, fl_f32x4 v, int) const {
     if (mm >= m || n >= (nh + 2 * nkv) * 64) return;
     const int hh = n >> 6, j = (n & 63) >> 1;  // pairs j, j + 1 (j even) of head hh
     float a0 = rbf(v[0]), b0 = rbf(v[1]), a1 = rbf(v[2]), b1 = rbf(v[3]);
     if (hh < nh + nkv) {
-      const uint2 cs = *reinterpret_cast<const uint2*>(rope + (size_t)(pos + mm) * 32 + j);
+      const uint2 cs = *reinterpret_cast<const uint2*>(rope + (size_t)rope_at(mm) * 32 + j);
       const float c0 = bflo(cs.x), s0 = bfhi(cs.x), c1 = bflo(cs.y), s1 = bfhi(cs.y);
       const float ta0 = a0 * c0 - b0 * s0, tb0 = b0 * c0 + a0 * s0;
       const float ta1 = a1 * c1 - b1 * s1, tb1 = b1 * c1 + a1 * s1;
@@ -425,9 +436,38 @@ struct PfWs {
   uint16_t *h, *xn, *q, *attn, *act;
   float* part;
   unsigned long long* best;
+  float* lse;     // with Extra: the rows' lse, and fl_tree_attention's workspace
+  uint8_t* attn_work;
   size_t bytes;
 };
-PfWs pf_layout(const fl_model_desc& d, int T, uint8_t* base) {
+// What the plain prompt pass does not do: a tree of tokens in place of a chain, and the weight that each slot gathers.
+struct Extra {
+  const int32_t* depth;  // [n] with mask: one pass
+  const uint8_t* mask;   // [n][n]
+  float* weights;        // [NL][NKV][max_seq], added to
+  int window;            // the last tokens of the prompt that count
+};
+fl_attn_desc pf_attn_desc(const fl_model_desc& d, int max_seq, int T, int pos) {
+  fl_attn_desc a{};
+  a.b = 1, a.m = T, a.heads = d.n_head, a.groups = d.n_kv_head, a.dim = FL_HEAD_DIM, a.slots = max_seq, a.pos0 = pos;
+  a.scale = d.attn_scale;
+  a.q_m = (int64_t)d.n_head * FL_HEAD_DIM, a.q_h = FL_HEAD_DIM;
+  a.k_g = a.v_g = (int64_t)max_seq * FL_HEAD_DIM;
+  a.k_s = a.v_s = FL_HEAD_DIM;
+  return a;
+}
+// bytes of fl_tree_attention's workspace for passes of up to T tokens of n: the full passes and the last one, behind as many keys as fit
+int64_t pf_attn_work(const fl_model_desc& d, int max_seq, int n, int T) {
+  int64_t most = 0;
+  for (int t : {T, n % T ? n % T : T}) {
+    const fl_attn_desc a = pf_attn_desc(d, max_seq, t, max_seq - t);
+    int64_t bytes = 0;
+    if (fl_tree_attention_workspace(&a, 1, &bytes) != FL_OK) return -1;
+    most = std::max(most, bytes);
+  }
+  return most;
+}
+PfWs pf_layout(const fl_model_desc& d, int T, uint8_t* base, int64_t attn_work = -1) {
   PfWs w{};
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -446,6 +486,10 @@ PfWs pf_layout(const fl_model_desc& d, int T, uint8_t* base) {
   const size_t rows = std::min((size_t)PF_KEY_PARTS * T * d.n_head, (size_t)PA_WGS * 64);
   w.part = (float*)take(std::max((size_t)PF_SPLITS * T * d.dim * 4, rows * 66 * 4));
   w.best = (unsigned long long*)take(PF_LM_GRID * 8);
+  if (attn_work >= 0) {
+    w.lse = (float*)take((size_t)T * d.n_head * 4);
+    w.attn_work = take((size_t)attn_work);
+  }
   w.bytes = at;
   return w;
 }
@@ -534,9 +578,23 @@ void pf_attention(const fl_state* st, const PfWs& w, int l, int T, int pos, hipS
     hipLaunchKernelGGL(k_pf_attn_merge, dim3((a.nkv * T * a.rep + 3) / 4), dim3(256), 0, s, a);
 }
 
-// last: where the final-normed rows go (ws.xn, or the caller's features)
-void pf_pass(const fl_weights* w, fl_state* st, const PfWs& ws, const int32_t* tokens, int T, int pos, uint16_t* last,
-             hipStream_t s) {
+// The attention of a pass with Extra: fl_tree_attention and, of the rows from `first` on, the weights
+int pf_attention_extra(const fl_state* st, const PfWs& w, const Extra& x, int l, int T, int pos, int first, hipStream_t s) {
+  const fl_model_desc& d = st->d;
+  const size_t layer = (size_t)l * d.n_kv_head * st->max_seq * 64;
+  fl_attn_desc a = pf_attn_desc(d, st->max_seq, T, pos);
+  int rc = fl_tree_attention(&a, w.q, st->kc + layer, st->vc + layer, nullptr, x.mask, w.attn, x.weights ? w.lse : nullptr,
+                             w.attn_work, s);
+  if (rc != FL_OK || !x.weights || first >= T) return rc;
+  a = pf_attn_desc(d, st->max_seq, T - first, pos + first);
+  return fl_attention_weights(&a, w.q + (size_t)first * d.n_head * FL_HEAD_DIM, st->kc + layer, w.lse + (size_t)first * d.n_head, nullptr,
+                              x.mask, x.weights + (size_t)l * d.n_kv_head * st->max_seq, 1, s);
+}
+
+// last: where the final-normed rows go (ws.xn, or the caller's features); x: null, or what else the pass does, `first`
+// the first of its tokens whose weights count
+int pf_pass(const fl_weights* w, fl_state* st, const PfWs& ws, const int32_t* tokens, int T, int pos, uint16_t* last,
+            hipStream_t s, const Extra* x = nullptr, int first = 0) {
   const fl_model_desc& d = st->d;
   const int D = d.dim, F = d.inter, NQKV = (d.n_head + 2 * d.n_kv_head) * FL_HEAD_DIM, L = d.n_layer;
   auto mat = [&](const uint32_t* p, int l, int n, int k, int per) { return p + (size_t)l * n * (k / per); };
@@ -544,10 +602,22 @@ void pf_pass(const fl_weights* w, fl_state* st, const PfWs& ws, const int32_t* t
                      w->attn_norm, d.norm_eps, ws.h, ws.xn, st->err);
   for (int l = 0; l < L; ++l) {
     const size_t layer = (size_t)l * d.n_kv_head * st->max_seq * 64;
-    pf_gemm<false>(mat(w->wqkv_t, l, NQKV, D, 8), mat(w->wqkv_sz, l, NQKV, D, 128), ws.xn, T, NQKV, D,
-                   EpiQkv{ws.q, st->kc + layer, st->vc + layer, reinterpret_cast<const uint32_t*>(w->rope), T, d.n_head,
-                          d.n_kv_head, st->max_seq, pos}, s);
-    pf_attention(st, ws, l, T, pos, s);
+    auto qkv = [&](auto epi) {
+      pf_gemm<false>(mat(w->wqkv_t, l, NQKV, D, 8), mat(w->wqkv_sz, l, NQKV, D, 128), ws.xn, T, NQKV, D, epi, s);
+    };
+    const uint32_t* rope = reinterpret_cast<const uint32_t*>(w->rope);
+    if (x && x->depth)
+      qkv(EpiQkv<true>{ws.q, st->kc + layer, st->vc + layer, rope, T, d.n_head, d.n_kv_head, st->max_seq, pos, x->depth,
+                       w->rope_len, st->err});
+    else
+      qkv(EpiQkv<false>{ws.q, st->kc + layer, st->vc + layer, rope, T, d.n_head, d.n_kv_head, st->max_seq, pos, nullptr, 0,
+                        nullptr});
+    if (x) {
+      const int rc = pf_attention_extra(st, ws, *x, l, T, pos, first, s);
+      if (rc != FL_OK) return rc;
+    } else {
+      pf_attention(st, ws, l, T, pos, s);
+    }
     int parts = pf_gemm<true>(mat(w->wo_t, l, D, D, 8), mat(w->wo_sz, l, D, D, 128), ws.attn, T, D, D,
                               EpiSum{ws.part, T, D}, s);
     hipLaunchKernelGGL(k_pf_norm, dim3(T), dim3(PF_NT), 0, s, ws.part, parts, T, D, tokens, w->embed, d.vocab,
@@ -560,24 +630,29 @@ void pf_pass(const fl_weights* w, fl_state* st, const PfWs& ws, const int32_t* t
     hipLaunchKernelGGL(k_pf_norm, dim3(T), dim3(PF_NT), 0, s, ws.part, parts, T, D, tokens, w->embed, d.vocab,
                        d.resid_mult, next, d.norm_eps, ws.h, l + 1 < L ? ws.xn : last, st->err);
   }
+  return FL_OK;
 }
 
 // feat / token_out: null where not asked for
 int pf_run(const fl_weights* w, fl_state* st, const int32_t* tokens, int32_t n, int32_t pos, int32_t* token_out,
-           uint16_t* feat, void* workspace, void* stream) {
+           uint16_t* feat, void* workspace, void* stream, const Extra* x = nullptr) {
   if (!st || !tokens || !workspace || n < 1 || !fl_weights_ok(w)) return FL_E_ARG;
   // what fl_verify needs too: the tiled weight copies, a model that its kernels take
   if (!w->wqkv_t || !w->wo_t || !w->wgu_t || !w->wd_t || !st->verify_ok) return FL_E_ARG;
-  if (pos < 0 || pos > st->max_seq - n || pos > w->rope_len - n) return FL_E_POS;
+  // a tree's RoPE positions are checked on the device
+  if (pos < 0 || pos > st->max_seq - n || (!(x && x->depth) && pos > w->rope_len - n)) return FL_E_POS;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int most = std::min(n, PF_TOKENS);
-  const PfWs ws = pf_layout(st->d, most, static_cast<uint8_t*>(workspace));
+  int64_t attn_work = -1;
+  if (x && (attn_work = pf_attn_work(st->d, st->max_seq, n, most)) < 0) return FL_E_ARG;
+  const PfWs ws = pf_layout(st->d, most, static_cast<uint8_t*>(workspace), attn_work);
   int T = 0;
   uint16_t* last = ws.xn;
   for (int at = 0; at < n; at += T) {
     T = std::min(most, n - at);
     if (feat) last = feat + (size_t)at * st->d.dim;
-    pf_pass(w, st, ws, tokens + at, T, pos + at, last, s);
+    const int rc = pf_pass(w, st, ws, tokens + at, T, pos + at, last, s, x, x ? std::max(0, n - x->window - at) : 0);
+    if (rc != FL_OK) return rc;
   }
   if (token_out) {
     hipLaunchKernelGGL(k_pf_lmhead, dim3(PF_LM_GRID), dim3(PF_NT), 0, s, last + (size_t)(T - 1) * st->d.dim, w->embed,
@@ -607,6 +682,30 @@ int fl_prefill_feat(const fl_weights* w, fl_state* st, const int32_t* tokens, in
                     int32_t* token_out, uint16_t* feat, void* workspace, void* stream) {
   if (!feat || (reinterpret_cast<uintptr_t>(feat) & 15)) return FL_E_ARG;
   return pf_run(w, st, tokens, n, pos, token_out, feat, workspace, stream);
+}
+
+int fl_prefill_extra_workspace(fl_state* st, int32_t n, int64_t* bytes) {
+  if (!st || n < 1 || !bytes || n > st->max_seq) return FL_E_ARG;
+  const int most = std::min(n, PF_TOKENS);
+  const int64_t work = pf_attn_work(st->d, st->max_seq, n, most);
+  if (work < 0) return FL_E_ARG;
+  *bytes = (int64_t)pf_layout(st->d, most, nullptr, work).bytes;
+  return FL_OK;
+}
+
+int fl_prefill_weights(const fl_weights* w, fl_state* st, const int32_t* tokens, int32_t n, int32_t pos, int32_t* token_out,
+                       uint16_t* feat, float* weights, int32_t window, void* workspace, void* stream) {
+  if (!weights || window < 1 || (reinterpret_cast<uintptr_t>(feat) & 15)) return FL_E_ARG;
+  const Extra x{nullptr, nullptr, weights, window};
+  return pf_run(w, st, tokens, n, pos, token_out, feat, workspace, stream, &x);
+}
+
+int fl_prefill_tree(const fl_weights* w, fl_state* st, const int32_t* tokens, int32_t m, const int32_t* depth,
+                    const uint8_t* amask, int32_t pos, uint16_t* feat, void* workspace, void* stream) {
+  if (!depth || !amask || !feat || (reinterpret_cast<uintptr_t>(feat) & 15)) return FL_E_ARG;
+  if (m < 1 || m > PF_TOKENS) return FL_E_M;
+  const Extra x{depth, amask, nullptr, 0};
+  return pf_run(w, st, tokens, m, pos, nullptr, feat, workspace, stream, &x);
 }
 
 }  // extern "C"

@@ -63,6 +63,35 @@ def prefill(model, x, input_pos, chunk=32):
     return out
 
 
+KEEP_PASS = 1024  # tokens of a pass between two cuts of the cache: the longest prompt pass
+
+
+def prefill_keep(model, x, more, keep, recent=64, sink=4):
+    """Feed a text's tokens x (int32 device [T]) from slot 0, cutting the cache to `keep` slots after each pass of up to
+    1024 of them by the weight that its slots have gathered so far (prefill_weights, Transformer.evict). Sets up caches of
+    room for `more` slots behind the kept ones. Returns the number of slots in use: the next token's."""
+    keep, recent, sink = int(keep), int(recent), int(sink)
+    if keep < 1 or recent < 0 or sink < 0:
+        raise ValueError("keep must be 1 or more, recent and sink not negative")
+    if recent + sink > keep:
+        raise ValueError("recent and sink together must not exceed keep")
+    x = x.reshape(-1).to(device=model.device, dtype=torch.int32)
+    T = x.numel()
+    if T + int(more) > model.packed.rope.shape[0]:
+        raise ValueError("the text exceeds block_size (rope table)")
+    model.setup_caches(1, min(T, keep + KEEP_PASS) + int(more))
+    weights = model.new_weights()
+    slots = 0
+    for at in range(0, T, KEEP_PASS):
+        n = min(KEEP_PASS, T - at)
+        model.prefill_weights(x[at:at + n], slots, weights)
+        slots += n
+        if slots > keep:
+            model.evict(weights, slots, keep, recent, sink)
+            slots = keep
+    return slots
+
+
 def sample(logits, temperature=1.0, top_k=None, seed=0, offset=0, noise=None, probs=False):
     """Sample one token per logit row on the GPU (reference engine/generate.py:36-55:
     logits_to_probs + multinomial_sample_one_no_sync). logits: fp32 device [V] or [rows, V]
@@ -256,22 +285,29 @@ def decode_n_tokens(model, cur_token, input_pos, num_new_tokens, out=None):
 
 
 @torch.no_grad()
-def generate(model, prompt, max_new_tokens, temperature=None, top_k=None, seed=0, logprobs=None):
+def generate(model, prompt, max_new_tokens, temperature=None, top_k=None, seed=0, logprobs=None, keep=None, recent=64, sink=4):
     """Generate: returns int32 device [T + max_new_tokens] = prompt + new tokens. Greedy (the
     argmax fused into the decode kernel) unless temperature or top_k is given; then each step
     samples in the decode launch itself (fl_decode_sample) with the step's position as the noise
     counter. Tokens stay on the device either way (no host synchronisation in the loop).
     logprobs = n (0..32): (tokens, TokenLogprobs of the new ones with n alternatives each) of the
-    model's own distribution, before temperature and top_k."""
+    model's own distribution, before temperature and top_k.
+    keep = n: a prompt of more tokens than that goes through the cache in passes of up to 1024, and after each pass every
+    key head's cache is cut to the `keep` slots that the prompt's attention has weighed most, the first `sink` and the
+    last `recent` among them (Transformer.evict): room for keep + 1024 + max_new_tokens slots, and decoding reads no more."""
     if logprobs is not None:
         _check_logprob_args(1, model.config.vocab_size, None, int(logprobs), model.device)
     prompt = prompt.reshape(-1).to(device=model.device, dtype=torch.int32)
     T = prompt.numel()
-    model.setup_caches(1, T + max_new_tokens)
     seq = torch.empty(T + max_new_tokens, dtype=torch.int32, device=model.device)
     seq[:T] = prompt
-    if T > 1:
-        prefill(model, prompt[:-1], 0)
+    slot = T - 1  # of the last prompt token
+    if keep is not None and slot > int(keep):
+        slot = prefill_keep(model, prompt[:-1], max_new_tokens + 1, keep, recent, sink)
+    else:
+        model.setup_caches(1, T + max_new_tokens)
+        if T > 1:
+            prefill(model, prompt[:-1], 0)
     sampled = temperature is not None or top_k is not None
     t = 1.0 if temperature is None else temperature
     said, logits = [], None
@@ -282,9 +318,9 @@ def generate(model, prompt, max_new_tokens, temperature=None, top_k=None, seed=0
         p = T - 1 + i
         out = seq[p + 1:p + 2]
         if sampled:
-            model.decode_sample(seq[p:p + 1], p, t, top_k, seed=seed, offset=p, token_out=out, logits=logits)
+            model.decode_sample(seq[p:p + 1], slot + i, t, top_k, seed=seed, offset=p, token_out=out, logits=logits)
         else:
-            model.decode_step(seq[p:p + 1], p, token_out=out, logits=logits)
+            model.decode_step(seq[p:p + 1], slot + i, token_out=out, logits=logits)
         if logits is not None:
             said.append(_logprobs(logits, out, logprobs))
     if logits is None:

@@ -8,7 +8,8 @@ bf16 tensor, and one decode step is ONE cooperative kernel launch (fl_decode_ste
 import torch
 
 from . import _lib
-from .quantize import DynamicInt8Linear, quantize_int4, tile_int4
+from .attention import evict
+from .quantize import DynamicInt8Linear, quantize_int4, tile_int4, workspace
 from .synth import ModelArgs, freqs_cis_table
 
 
@@ -124,6 +125,7 @@ class Transformer:
         self._state = None
         self._cw = packed.c_weights()
         self.k_cache = self.v_cache = None
+        self.shift = 0
 
     @classmethod
     def from_weights(cls, args, sd, device="cuda"):
@@ -133,6 +135,7 @@ class Transformer:
     def setup_caches(self, max_batch_size, max_seq_length):
         if max_batch_size != 1:
             raise ValueError("batch-1 decode engine: max_batch_size must be 1")
+        self._set_shift(0)
         if self.max_seq_length >= max_seq_length and self._state is not None:
             return
         self.close()
@@ -153,6 +156,14 @@ class Transformer:
         self.max_seq_length = max_seq_length
         self.max_batch_size = max_batch_size
         self._tok_out = torch.zeros(_lib.MAX_VERIFY, dtype=torch.int32, device=self.device)
+
+    def _set_shift(self, shift):
+        """Slot s holds position s + shift from now on: the kernels index the RoPE table by slot, so its start moves."""
+        if not 0 <= shift < self.packed.rope.shape[0]:
+            raise ValueError("position outside the RoPE table")
+        self.shift = shift
+        self._cw.rope = self.packed.rope[shift:].data_ptr()
+        self._cw.rope_len = self.packed.rope.shape[0] - shift
 
     def close(self):
         if self._state is not None:
@@ -310,6 +321,63 @@ class Transformer:
         _lib.call("fl_prefill_feat", _lib.ctypes.byref(self._cw), self._state, _lib.ptr(tokens), n, int(pos),
                   _lib.ptr(token_out), _lib.ptr(feat), _lib.ptr(ws), _lib.stream_ptr())
         return feat
+
+    def _extra_args(self, tokens):
+        if self._state is None:
+            raise RuntimeError("call setup_caches first")
+        if not tokens.is_cuda or tokens.dtype != torch.int32:
+            raise ValueError(f"tokens must be a {torch.int32} device tensor")
+        tokens = tokens.reshape(-1).contiguous()
+        ws = workspace("fl_prefill_extra_workspace", self._state, tokens.numel(), device=self.device)
+        return tokens, tokens.numel(), ws
+
+    def new_weights(self):
+        """The weights that prefill_weights adds to and evict goes by, all 0: fp32 [layers, key heads, slots]."""
+        return torch.zeros(self.k_cache.shape[:3], dtype=torch.float32, device=self.device)
+
+    def prefill_weights(self, tokens, pos, weights, window=None, token_out=None, feat=None):
+        """prefill that also adds up, in weights (new_weights), the attention weight that every slot gathers from the
+        prompt's last `window` tokens (None: from all) (fl_prefill_weights). The greedy next token is computed only
+        where token_out (int32 device [1]) is given, the features where feat (bf16 device [n, dim]) is."""
+        tokens, n, ws = self._extra_args(tokens)
+        window = n if window is None else int(window)
+        if window < 1:
+            raise ValueError("window must be 1 or more")
+        for t, dt, shape, nm in ((weights, torch.float32, self.k_cache.shape[:3], "weights"), (token_out, torch.int32, (1,), "token_out"),
+                                 (feat, torch.bfloat16, (n, self.config.dim), "feat")):
+            if t is not None and (not t.is_cuda or t.dtype != dt or t.shape != shape or not t.is_contiguous()):
+                raise ValueError(f"{nm} must be a contiguous {dt} device tensor of {tuple(shape)}")
+        _lib.call("fl_prefill_weights", _lib.ctypes.byref(self._cw), self._state, _lib.ptr(tokens), n, int(pos),
+                  _lib.ptr(token_out), _lib.ptr(feat), _lib.ptr(weights), min(window, n), _lib.ptr(ws), _lib.stream_ptr())
+        return token_out
+
+    def tree_features(self, tokens, pos, depth, amask):
+        """Features (bf16 [M, dim], after the final norm) of a tree of up to 1024 tokens at cache slots pos..pos+M-1,
+        in one prompt pass (fl_prefill_tree); depth and amask as verify's, for trees wider than verify takes. Their
+        logits come from a head over them (int8_head)."""
+        tokens, m, ws = self._extra_args(tokens)
+        if m > 1024:
+            raise ValueError("at most 1024 tokens")
+        if depth.numel() != m or amask.shape != (m, m):
+            raise ValueError("depth must be [M] and amask [M, M]")
+        depth, amask = (t.to(device=self.device, dtype=dt).contiguous() for t, dt in ((depth, torch.int32), (amask, torch.uint8)))
+        feat = torch.empty(m, self.config.dim, dtype=torch.bfloat16, device=self.device)
+        _lib.call("fl_prefill_tree", _lib.ctypes.byref(self._cw), self._state, _lib.ptr(tokens), m, _lib.ptr(depth),
+                  _lib.ptr(amask), int(pos), _lib.ptr(feat), _lib.ptr(ws), _lib.stream_ptr())
+        return feat
+
+    def evict(self, weights, n, keep, recent=0, sink=0):
+        """Cut the cache from n slots to the `keep` of each layer and key head that gathered the most weight, the first
+        `sink` and the last `recent` among them (attention.evict, in place; weights move along). Keys keep the
+        position they were rotated for, and what follows goes on from there: feed the next token at slot `keep`, it
+        takes position n + shift as before (shift: the slots evicted so far; setup_caches starts over at 0). Returns
+        the kept slots, int32 [layers, key heads, keep]."""
+        if self._state is None:
+            raise RuntimeError("call setup_caches first")
+        kept = evict(self.k_cache, self.v_cache, weights, n, keep, recent, sink)
+        if n > kept.shape[-1]:
+            self._set_shift(self.shift + int(n) - kept.shape[-1])
+        return kept
 
     def int8_head(self):
         """The tied LM head with 8-bit weights (quantize.DynamicInt8Linear, 126 MB for flint-3b), its scales

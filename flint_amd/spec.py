@@ -19,6 +19,15 @@ where context is every token so far (prompt, emitted tokens, and last the pendin
 is a bf16 [n, dim] device view of the final-norm features of the verified tokens (the input an
 EAGLE head consumes, reference spec_mega.py:112). LookupDraft (prompt-lookup n-gram matching)
 needs no weights.
+
+With a temperature or top_k the loop samples (accept_sampled): the emitted tokens are distributed as
+the sampler's own (generate.sample), whatever the draft proposes. A draft that drew its tokens from
+distributions of its own also has
+
+    probs() -> fp32 device [nodes - 1, vocab] or None   of the proposal just made: row i the
+                                                        distribution that the children of node i were
+                                                        drawn from, each on its own (node 0 = the root;
+                                                        a chain's node i + 1 is its i-th token)
 """
 import time
 from collections import namedtuple
@@ -27,7 +36,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from .generate import _ids, prefill
+from .generate import _ids, logits_to_probs, prefill
+from .quantize import linear_int8
 
 
 def tree_depths(parents):
@@ -244,58 +254,95 @@ class SpecStats:
 
 
 class SpecDecoder:
-    """Greedy speculative decoding of one sequence on a flint_amd Transformer.
+    """Speculative decoding of one sequence on a flint_amd Transformer, greedy or sampled.
 
     generate(prompt, max_new, mode="chain" | "tree") sets up the model's caches (like
     generate.generate), prefills the prompt, and returns (prompt + new tokens as a host int list,
     SpecStats). Generation stops after max_new tokens or at the first eos token (which is kept).
     """
 
-    def __init__(self, model, draft=None, k=4):
+    def __init__(self, model, draft=None, k=4, head=None):
+        """head: a quantize.DynamicInt8Linear (Transformer.int8_head) through which a pass of more than 32 nodes gets its
+        logits (Transformer.tree_features; up to 1024 nodes then); such a pass gives the tokens of the model with that head."""
         self.model = model
         self.draft = draft if draft is not None else LookupDraft()
         self.k = int(k)
-        if not 0 <= self.k < _lib.MAX_VERIFY:
-            raise ValueError(f"k must be in [0, {_lib.MAX_VERIFY - 1}]")
+        self.head = head
+        nv = self._nodes = _lib.MAX_VERIFY if head is None else 1024
+        if not 0 <= self.k < nv:
+            raise ValueError(f"k must be in [0, {nv - 1}]")
         dev = model.device
-        nv = _lib.MAX_VERIFY
-        # tokens | depth | amask staged in one pinned buffer, one copy per pass
-        self._host = torch.zeros(2 * nv + nv * nv // 4, dtype=torch.int32, pin_memory=dev.type == "cuda")
+        # tokens | depth | parents | amask staged in one pinned buffer, one copy per pass
+        self._host = torch.zeros(3 * nv + nv * nv // 4, dtype=torch.int32, pin_memory=dev.type == "cuda")
         self._dev = torch.zeros_like(self._host, device=dev)
         self._tout = torch.empty(nv, dtype=torch.int32, device=dev)
         self._feat = torch.empty(nv, model.config.dim, dtype=torch.bfloat16, device=dev)
 
-    def _verify(self, cand, parents, pos):
+    def _verify(self, cand, parents, pos, logits=False):
+        """Stage a pass's nodes on the device and run them; (greedy tokens as a device tensor, logits or None, feat)."""
         m = len(cand)
-        nv = _lib.MAX_VERIFY
+        nv = self._nodes
         vocab = self.model.config.vocab_size
         if any(not 0 <= t < vocab for t in cand):
             raise ValueError(f"draft token outside [0, {vocab})")
         h = self._host.numpy()
         h[:m] = cand
         h[nv:nv + m] = tree_depths(parents)
-        h[2 * nv:].view(np.uint8)[:m * m] = tree_mask(parents).reshape(-1)
-        self._dev.copy_(self._host, non_blocking=True)
+        h[2 * nv:2 * nv + m] = parents
+        h[3 * nv:].view(np.uint8)[:m * m] = tree_mask(parents).reshape(-1)
+        used = 3 * nv + (m * m + 3) // 4
+        self._dev[:used].copy_(self._host[:used], non_blocking=True)
+        lg = torch.empty(m, vocab, dtype=torch.float32, device=self.model.device) if logits and m <= _lib.MAX_VERIFY else False
         if m == 1:
             # a lone root is one decode step (same cache slot, RoPE position, argmax and final-norm
             # feature as a verify of M = 1), and the decode kernel is the faster of the two
-            self.model.decode_step(self._dev[:1], pos, token_out=self._tout[:1], feat=self._feat[0])
-            return self._tout[:1].tolist(), self._feat[:1]
-        amask = self._dev[2 * nv:].view(torch.uint8)[:m * m].view(m, m)
-        tout, _, feat = self.model.verify(self._dev[:m], pos, depth=self._dev[nv:nv + m], amask=amask,
-                                          logits=False, feat=self._feat[:m], tokens_out=self._tout[:m])
-        return tout[:m].tolist(), feat
+            self.model.decode_step(self._dev[:1], pos, token_out=self._tout[:1], feat=self._feat[0],
+                                   logits=lg[0] if logits else None)
+            return self._tout[:1], lg, self._feat[:1]
+        depth = self._dev[nv:nv + m]
+        amask = self._dev[3 * nv:].view(torch.uint8)[:m * m].view(m, m)
+        if m > _lib.MAX_VERIFY:
+            feat = self.model.tree_features(self._dev[:m], pos, depth, amask)
+            lg = linear_int8(feat, self.head.weight, self.head.scales, torch.float32)
+            return lg.argmax(dim=1).int(), lg, feat
+        tout, lg, feat = self.model.verify(self._dev[:m], pos, depth=depth, amask=amask, logits=lg, feat=self._feat[:m],
+                                           tokens_out=self._tout[:m])
+        return tout[:m], lg, feat
+
+    def _greedy(self, cand, parents, pos):
+        """One pass: (accepted path, next token, features of all nodes)."""
+        tout, _, feat = self._verify(cand, parents, pos)
+        tgt = tout.tolist()
+        path = accept_tree(cand, parents, tgt)
+        return path, tgt[path[-1]], feat
+
+    def _sampled(self, cand, parents, pos, temperature, top_k, gen, draft_probs):
+        """The same, sampled."""
+        m, nv, dev = len(cand), self._nodes, self.model.device
+        _, logits, feat = self._verify(cand, parents, pos, logits=True)
+        probs = logits_to_probs(logits, temperature, top_k)
+        u = torch.rand(m + 1, generator=gen, device=dev)
+        got = accept_sampled(probs, self._dev[:m], u[:m], u[m:], parents=self._dev[2 * nv:2 * nv + m], draft_probs=draft_probs)
+        out = torch.cat([got.count, got.token, got.path]).tolist()
+        if out[1] < 0:
+            raise RuntimeError("a row of logits without a distribution")
+        return out[2:2 + out[0]], out[1], feat
 
     @torch.no_grad()
-    def generate(self, prompt, max_new, mode="chain", eos=None):
+    def generate(self, prompt, max_new, mode="chain", eos=None, temperature=None, top_k=None, seed=0):
+        """Greedy, or sampled where temperature or top_k is given (as generate.sample, from torch's generator seeded with
+        `seed`: a run repeats itself, and differs from generate.generate's Philox noise)."""
         if mode not in ("chain", "tree"):
             raise ValueError("mode is 'chain' or 'tree'")
+        if top_k is not None and int(top_k) < 1:
+            raise ValueError("top_k must be >= 1")
+        sampled = temperature is not None or top_k is not None
         if hasattr(self.draft, "reset"):
             self.draft.reset()
         ids = [int(t) for t in (prompt.reshape(-1).tolist() if torch.is_tensor(prompt) else prompt)]
         if not ids:
             raise ValueError("empty prompt")
-        model, nv = self.model, _lib.MAX_VERIFY
+        model, nv = self.model, self._nodes
         T = len(ids)
         max_seq = T + int(max_new) + nv
         model.setup_caches(1, max_seq)
@@ -308,9 +355,17 @@ class SpecDecoder:
             prefill(model, torch.tensor(ids[:-1], dtype=torch.int32), 0)
         pos = T - 1
         # reference spec_mega.py:92-93: the last prompt token through the verify kernel
-        tgt, vfeat = self._verify([ids[-1]], [-1], pos)
+        gen = torch.Generator(device=model.device).manual_seed(int(seed)) if sampled else None
+        temp = 1.0 if temperature is None else float(temperature)
+
+        def step(cand, parents, pos, draft_probs=None):
+            if sampled:
+                return self._sampled(cand, parents, pos, temp, top_k, gen, draft_probs)
+            return self._greedy(cand, parents, pos)
+
+        _, nxt, vfeat = step([ids[-1]], [-1], pos)
         feats[0:1].copy_(vfeat[:1])
-        n_feat, pos, nxt = 1, pos + 1, tgt[0]
+        n_feat, pos = 1, pos + 1
         new = 0
         t0 = time.perf_counter()
         while True:
@@ -330,12 +385,15 @@ class SpecDecoder:
                 toks, pars = [int(t) for t in toks][:room - 1], [int(p) for p in pars][:room - 1]
                 cand = [nxt] + toks
                 parents = [-1] + [p + 1 for p in pars]          # draft parents -> verify node indices
-            tgt, vfeat = self._verify(cand, parents, pos)
-            path = accept_tree(cand, parents, tgt)
+            q = None
+            if sampled and len(cand) > 1 and hasattr(self.draft, "probs"):
+                q = self.draft.probs()
+                q = None if q is None else q[:len(cand) - 1]  # a proposal cut to the room that is left
+            path, after, vfeat = step(cand, parents, pos, q)
             if mode == "tree":
                 src, dst = compaction_moves(path, pos)
-                if src:
-                    model.kv_move(src, dst)
+                for i in range(0, len(src), _lib.MAX_VERIFY):  # rising: a later move's source is no earlier one's destination
+                    model.kv_move(src[i:i + _lib.MAX_VERIFY], dst[i:i + _lib.MAX_VERIFY])
             if path[-1] == len(path) - 1:                      # a prefix of the nodes
                 feats[n_feat:n_feat + len(path)].copy_(vfeat[:len(path)])
             else:
@@ -354,7 +412,7 @@ class SpecDecoder:
             if stop:
                 break
             pos += len(path)
-            nxt = tgt[path[-1]]
+            nxt = after
         if model.device.type == "cuda":
             torch.cuda.synchronize()
         stats.seconds = time.perf_counter() - t0

@@ -360,6 +360,21 @@ int fl_prefill(const fl_weights* w, fl_state* st, const int32_t* tokens, int32_t
 int fl_prefill_feat(const fl_weights* w, fl_state* st, const int32_t* tokens, int32_t n, int32_t pos,
                     int32_t* token_out, uint16_t* feat, void* workspace, void* stream);
 
+/* fl_prefill that also adds up the weight that every slot gathers from the prompt's last `window` tokens (>= 1; n or
+ * more: from all), as fl_attention_weights: weights (device, fp32 [NL, NKV, max_seq]) is added to. token_out and feat
+ * (16-byte aligned, as fl_prefill_feat's) may be NULL. Its attention is fl_tree_attention, so results differ from
+ * fl_prefill's by fp32 summation order. workspace: of fl_prefill_extra_workspace's bytes for n, as fl_prefill's.
+ * No counterpart in the reference. */
+int fl_prefill_extra_workspace(fl_state* st, int32_t n, int64_t* bytes);
+int fl_prefill_weights(const fl_weights* w, fl_state* st, const int32_t* tokens, int32_t n, int32_t pos,
+                       int32_t* token_out, uint16_t* feat, float* weights, int32_t window, void* workspace, void* stream);
+/* The features of a tree of up to 1024 tokens in one prompt pass: token, depth and amask as fl_verify's (a RoPE
+ * position outside the table is recorded in the state), feat (device, bf16 [M, D], 16-byte aligned) the rows after the
+ * final norm. For trees wider than fl_verify takes. workspace of fl_prefill_extra_workspace's bytes for m.
+ * Replaces reference kernels/verify_mega.cu:246-283 beyond 32 tokens. */
+int fl_prefill_tree(const fl_weights* w, fl_state* st, const int32_t* tokens, int32_t m, const int32_t* depth,
+                    const uint8_t* amask, int32_t pos, uint16_t* feat, void* workspace, void* stream);
+
 /* KV cache compaction after a tree verify: for i = 0..n-1 (n <= FL_MAX_VERIFY) the K and V rows
  * of cache slot src[i] move to slot dst[i], in every layer and KV group. All n rows are read
  * before any is written, which equals moving them one at a time in order i whenever no source is

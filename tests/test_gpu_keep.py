@@ -1,0 +1,348 @@
+"""The cache operators as the engine runs them: prompts that gather weights, eviction and decoding from what stays,
+trees wider than a verify launch, and sampled speculation over all of them."""
+import pytest
+import torch
+
+from oracle import cache as oracle_cache
+from tests.helpers import check_rows, fill_kv_random, log, make_pair, oracle_pair
+
+pytestmark = pytest.mark.gpu
+
+
+def tokens(args, n, seed):
+    return torch.randint(0, args.vocab_size, (n,), generator=torch.Generator().manual_seed(seed), dtype=torch.int32)
+
+
+@pytest.mark.parametrize("n,pos,window", [(17, 0, None), (40, 30, 7), (300, 100, None), (5, 3, 5), (1, 50, 1)])
+def test_weights_of_a_prompt(dev, n, pos, window):
+    """Layer 0's weights against 64 bits from the oracle's q and k: q and k are one linear of the same inputs, so single
+    bf16 roundings apart (an ulp of one in a few hundred values: below 2^-8 of the score, e^s follows); every layer's
+    rows hand out 1 each; a call adds to what is there, and the cache is a plain prompt's."""
+    args, sd, eng, orc = make_pair("small", seed=3)
+    eng.setup_caches(1, 512)
+    orc.setup_caches(eng.max_seq_length)
+    if pos:
+        fill_kv_random(eng, orc, pos, seed=n)
+    x = tokens(args, n, n + pos)
+    w = eng.new_weights()
+    nxt = torch.empty(1, dtype=torch.int32, device=dev)
+    feat = torch.empty(n, args.dim, dtype=torch.bfloat16, device=dev)
+    eng.prefill_weights(x.to(dev), pos, w, window, nxt, feat)
+    eng.check()
+    count = min(window or n, n)
+    rep = args.n_head // args.n_local_heads
+    assert ((w.double().sum(-1) - count * rep).abs() <= count * rep * 2.0 ** -12).all()
+    assert (w[:, :, pos + n:] == 0).all()
+    orc.trace = []
+    orc.forward(x, pos)
+    t = orc.trace[0]
+    orc.trace = None
+    q = t["q"].view(1, n, args.n_head, 64)[:, n - count:]
+    k = orc.k_cache[0][None].clone()
+    _, lse = oracle_cache.tree_attention(q, k, k, [pos + n - count], None, args.attn_scale)
+    want = oracle_cache.attention_weights(q, k, lse, [pos + n - count], None, args.attn_scale)[0]
+    e = float((w[0].double().cpu() - want).norm() / want.norm())
+    log(f"weights of {n} tokens at {pos}: rel {e:.2e}")
+    assert e <= 2.0 ** -7
+    # the same call again adds the same
+    before = w.clone()
+    eng.prefill_weights(x.to(dev), pos, w, window)
+    assert torch.equal(w, before + before)
+    # K rows and features as a plain prompt's, up to fp32 order: layer 0's rows are the same linear
+    k0 = eng.k_cache.clone()
+    if n > 1:
+        f2 = eng.prefill_features(x.to(dev), pos)
+        assert torch.equal(eng.k_cache[0], k0[0])
+        (alt, af), (ref, rf) = oracle_pair(orc, lambda: tuple(v.float() for v in orc.forward(x, pos)))
+        d, f = float((feat.float() - f2.float()).norm() / f2.float().norm()), float((af - rf).norm() / rf.norm())
+        log(f"features: two attentions {d:.2e} apart, the oracle's implementations {f:.2e}")
+        assert d <= max(2 * f, 2.0 ** -8)
+
+
+def test_window_is_the_rest(dev):
+    """All weights = those of the first tokens + those of the window behind them, in two passes or one."""
+    args, _, eng, _ = make_pair("small", seed=3)
+    eng.setup_caches(1, 1400)
+    x = tokens(args, 1300, 5).to(dev)  # two passes: 1024 and 276
+    a, b, c = eng.new_weights(), eng.new_weights(), eng.new_weights()
+    eng.prefill_weights(x, 0, a)
+    eng.prefill_weights(x, 0, b, window=900)  # begins inside the first pass
+    eng.prefill_weights(x[:400], 0, c)
+    # the same rows; their K and V went through products of other shapes (1024 tokens against 400), a few roundings apart
+    rel = float((a - b - c).norm() / a.norm())
+    log(f"window: rel {rel:.2e}")
+    assert rel <= 2.0 ** -8
+    d = eng.new_weights()
+    eng.prefill_weights(x, 0, d, window=10 ** 6)
+    assert torch.equal(a, d)
+
+
+@pytest.mark.parametrize("n,keep,recent,sink", [(60, 20, 8, 2), (200, 199, 0, 0), (333, 64, 64, 0)])
+def test_decode_after_eviction(dev, n, keep, recent, sink):
+    """What stays is what the definition keeps, and decode, verify, prompt and sampling go on from it at the old
+    positions: the oracle on the same cut cache, its RoPE positions shifted."""
+    args, sd, eng, orc = make_pair("small", seed=3)
+    eng.setup_caches(1, 512)
+    orc.setup_caches(eng.max_seq_length)
+    x = tokens(args, n + 40, n)
+    w = eng.new_weights()
+    eng.prefill_weights(x[:n].to(dev), 0, w)
+    k, v, wc = eng.k_cache.cpu(), eng.v_cache.cpu(), w.cpu()
+    kept = eng.evict(w, n, keep, recent, sink)
+    assert eng.shift == n - keep
+    for l in range(args.n_layer):
+        for g in range(args.n_local_heads):
+            want = oracle_cache.kept_slots(wc[l, g].tolist(), n, keep, recent, sink)
+            assert kept[l, g].tolist() == want
+            assert torch.equal(eng.k_cache[l, g, :keep].cpu(), k[l, g, want]) and torch.equal(eng.v_cache[l, g, :keep].cpu(), v[l, g, want])
+            assert torch.equal(w[l, g, :keep].cpu(), wc[l, g, want]) and (w[l, g, keep:] == 0).all()
+    orc.k_cache.copy_(eng.k_cache.cpu())
+    orc.v_cache.copy_(eng.v_cache.cpu())
+
+    def orc_run(idx, slot):
+        m = idx.numel()
+        return oracle_pair(orc, lambda: (orc.forward(idx, slot, depth=torch.arange(m) + eng.shift)[0].float(),))
+    # decode, then a verify of 3, a prompt of 30, at slots keep ..
+    lg = torch.empty(args.vocab_size, dtype=torch.float32, device=dev)
+    eng.decode_step(x[n:n + 1].to(dev), keep, logits=lg)
+    (alt,), (ref,) = orc_run(x[n:n + 1], keep)
+    check_rows(lg.cpu().view(1, -1), ref, alt, "small", f"decode after eviction {n} -> {keep}")
+    _, vl, _ = eng.verify(x[n + 1:n + 4].to(dev), keep + 1)
+    (alt,), (ref,) = orc_run(x[n + 1:n + 4], keep + 1)
+    check_rows(vl.cpu(), ref, alt, "small", "verify after eviction")
+    from flint_amd.generate import prefill
+    prefill(eng, x[n + 4:n + 34], keep + 4)
+    eng.decode_step(x[n + 34:n + 35].to(dev), keep + 34, logits=lg)
+    (alt,), (ref,) = orc_run(x[n + 4:n + 35], keep + 4)
+    check_rows(lg.cpu().view(1, -1), ref[-1:], alt[-1:], "small", "prompt after eviction")
+    eng.check()
+    # a second cut, then a fresh start
+    eng.evict(w, keep + 35, 10, 0, 0)
+    assert eng.shift == n - keep + keep + 35 - 10
+    eng.setup_caches(1, 512)
+    assert eng.shift == 0
+    orc.setup_caches(eng.max_seq_length)
+    eng.decode_step(x[:1].to(dev), 0, logits=lg)
+    check_rows(lg.cpu().view(1, -1), orc.forward(x[:1], 0)[0].float(), orc.forward(x[:1], 0)[0].float(), "small", "fresh start")
+
+
+def test_nothing_evicted_changes_nothing(dev):
+    args, _, eng, _ = make_pair("small", seed=3)
+    eng.setup_caches(1, 256)
+    x = tokens(args, 50, 1).to(dev)
+    w = eng.new_weights()
+    eng.prefill_weights(x, 0, w)
+    k, w0 = eng.k_cache.clone(), w.clone()
+    eng.evict(w, 50, 50)
+    eng.evict(w, 50, 80, 10, 10)
+    assert eng.shift == 0 and torch.equal(eng.k_cache, k) and torch.equal(w, w0)
+
+
+def test_positions_end_at_the_table(dev):
+    from flint_amd import _lib
+    args, _, eng, _ = make_pair("tiny", seed=3)  # 1024 positions
+    eng.setup_caches(1, 1024)
+    x = tokens(args, 1020, 1).to(dev)
+    w = eng.new_weights()
+    eng.prefill_weights(x, 0, w)
+    eng.evict(w, 1020, 100, 10)
+    for i in range(4):  # positions 1020 .. 1023 at slots 100 .. 103
+        eng.decode_step(x[:1], 100 + i)
+    with pytest.raises(_lib.FlError):
+        eng.decode_step(x[:1], 104)
+    with pytest.raises(_lib.FlError):
+        eng.prefill_weights(x[:5], 100, w)
+    eng.check()
+
+
+def test_generate_keep(dev):
+    """generate(keep=...) is prefill_weights and evict pass by pass, then decoding; keep of the prompt or more is none."""
+    from flint_amd.generate import generate
+    args, _, eng, _ = make_pair("small", seed=3)
+    x = tokens(args, 1500, 9).to(dev)
+    full = generate(eng, x[:200], 20)
+    assert torch.equal(generate(eng, x[:200], 20, keep=199), full) and torch.equal(generate(eng, x[:200], 20, keep=1000), full)
+    for kw in (dict(), dict(temperature=0.8, top_k=50, seed=3), dict(logprobs=2)):
+        got = generate(eng, x, 12, keep=150, recent=40, sink=2, **kw)
+        seq, said = got if "logprobs" in kw else (got, None)
+        assert eng.shift == 1499 - 150
+        eng.setup_caches(1, 150 + 1024 + 13)
+        w = eng.new_weights()
+        eng.prefill_weights(x[:1024], 0, w)
+        eng.evict(w, 1024, 150, 40, 2)
+        eng.prefill_weights(x[1024:1499], 150, w)
+        eng.evict(w, 625, 150, 40, 2)
+        tok = torch.empty(13, dtype=torch.int32, device=dev)
+        tok[:1] = x[1499:]
+        for i in range(12):
+            if "temperature" in kw:
+                eng.decode_sample(tok[i:i + 1], 150 + i, 0.8, 50, seed=3, offset=1499 + i, token_out=tok[i + 1:i + 2])
+            else:
+                eng.decode_step(tok[i:i + 1], 150 + i, token_out=tok[i + 1:i + 2])
+        assert torch.equal(seq[:1500], x) and torch.equal(seq[1500:], tok[1:])
+        assert said is None or said.logprob.shape == (12,)
+    eng.check()
+    for kw in (dict(keep=0), dict(keep=50, recent=50), dict(keep=100, recent=-1)):
+        with pytest.raises(ValueError):
+            generate(eng, x, 4, **kw)
+    with pytest.raises(ValueError):
+        generate(eng, tokens(args, 2048, 1), 4, keep=100)
+
+
+def tree(m, seed):
+    from flint_amd.spec import tree_depths, tree_mask
+    g = torch.Generator().manual_seed(seed)
+    parents = [-1] + [int(torch.randint(max(0, i - 6), i, (1,), generator=g)) for i in range(1, m)]
+    return parents, torch.tensor(tree_depths(parents), dtype=torch.int32), torch.from_numpy(tree_mask(parents))
+
+
+@pytest.mark.parametrize("m,pos", [(1, 20), (20, 0), (33, 100), (130, 37), (300, 10)])
+def test_tree_features(dev, m, pos):
+    """A tree in a prompt pass: the oracle's logits of its nodes, from the features."""
+    args, sd, eng, orc = make_pair("small", seed=3)
+    eng.setup_caches(1, 512)
+    orc.setup_caches(eng.max_seq_length)
+    if pos:
+        fill_kv_random(eng, orc, pos, seed=m)
+    x = tokens(args, m, m)
+    _, depth, mask = tree(m, m)
+    feat = eng.tree_features(x.to(dev), pos, depth.to(dev), mask.to(dev))
+    eng.check()
+    (alt, af), (ref, rf) = oracle_pair(orc, lambda: tuple(v.float() for v in orc.forward(x, pos, depth, mask)))
+    lg = (torch.nn.functional.linear(feat.cpu(), orc.embed) / args.logits_scaling).float()
+    check_rows(lg, ref, alt, "small", f"tree of {m} at {pos}")
+
+
+def test_tree_refusals(dev):
+    from flint_amd import _lib
+    args, _, eng, _ = make_pair("tiny", seed=3)
+    with pytest.raises(RuntimeError):
+        eng.tree_features(torch.zeros(2, dtype=torch.int32, device=dev), 0, torch.zeros(2), torch.ones(2, 2))
+    eng.setup_caches(1, 64)
+    x = tokens(args, 40, 1).to(dev)
+    _, depth, mask = tree(40, 1)
+    for bad in (dict(depth=depth[:5]), dict(amask=mask[:5]), dict(tokens=x.long()), dict(tokens=x.cpu())):
+        with pytest.raises(ValueError):
+            eng.tree_features(**{**dict(tokens=x, pos=0, depth=depth, amask=mask), **bad})
+    with pytest.raises(_lib.FlError):
+        eng.tree_features(x, 30, depth, mask)
+    w = eng.new_weights()
+    for bad in (dict(weights=w[:1]), dict(weights=w.double()), dict(window=0), dict(token_out=torch.zeros(2, dtype=torch.int32, device=dev)),
+                dict(feat=torch.zeros(40, args.dim, device=dev))):
+        with pytest.raises(ValueError):
+            eng.prefill_weights(**{**dict(tokens=x, pos=0, weights=w), **bad})
+    with pytest.raises(ValueError):
+        eng.evict(w, 100, 10)
+    # a depth outside the RoPE table is recorded, as verify's
+    depth = depth.clone()
+    depth[3] = 5000
+    eng.tree_features(x, 0, depth.to(dev), mask.to(dev))
+    with pytest.raises(_lib.FlError):
+        eng.check()
+    eng.reset_state()
+
+
+class Proposes:
+    """A draft that draws every child from a distribution of its own, `branch` children per node, two levels."""
+
+    def __init__(self, vocab, device, branch, seed=0, tell=True):
+        g = torch.Generator(device=device).manual_seed(seed)
+        self.q = torch.softmax(torch.randn(vocab, generator=g, device=device) * 2, 0)
+        self.g, self.branch, self.tell, self.n = g, branch, tell, 0
+
+    def chain(self, context, feats, k):
+        self.n = min(k, 3)
+        return torch.multinomial(self.q, self.n, replacement=True, generator=self.g).tolist() if self.n else []
+
+    def tree(self, context, feats):
+        b = self.branch
+        parents = [-1] * b + [i // b for i in range(b * b)]
+        self.n = len(parents)
+        return torch.multinomial(self.q, self.n, replacement=True, generator=self.g).tolist(), parents
+
+    def probs(self):
+        return self.q.expand(self.n, -1) if self.tell else None
+
+
+@pytest.mark.parametrize("mode,tell", [("chain", True), ("tree", True), ("chain", False)])
+def test_sampled_speculation_is_the_samplers_distribution(dev, mode, tell):
+    """The first two tokens of 600 runs against the sampler's own probabilities (top-k 3: nine pairs). A draft
+    that tells its distribution draws tokens anew each run; one that does not proposes the same ones always. Five standard
+    deviations of a count."""
+    from flint_amd.generate import logits_to_probs, prefill
+    from flint_amd.spec import SpecDecoder
+    args, _, eng, _ = make_pair("tiny", seed=3)
+    p0 = tokens(args, 6, 3).tolist()
+    eng.setup_caches(1, 64)
+    prefill(eng, torch.tensor(p0[:-1], dtype=torch.int32), 0)
+    lg = torch.empty(args.vocab_size, dtype=torch.float32, device=dev)
+    eng.decode_step(torch.tensor(p0[-1:], dtype=torch.int32, device=dev), len(p0) - 1, logits=lg)
+    first = logits_to_probs(lg, 1.5, 3).cpu()
+    want = {}
+    for a in first.nonzero()[:, 0].tolist():
+        eng.decode_step(torch.tensor([a], dtype=torch.int32, device=dev), len(p0), logits=lg)
+        second = logits_to_probs(lg, 1.5, 3).cpu()
+        for b in second.nonzero()[:, 0].tolist():
+            want[a, b] = float(first[a] * second[b])
+    draft = Proposes(args.vocab_size, dev, 2, tell=tell)
+    draft.q = torch.zeros_like(draft.q)
+    draft.q[[a for a, _ in want] + [b for _, b in want]] = 1.0  # so that some are accepted
+    draft.q /= draft.q.sum()
+    if not tell:
+        fixed = [b for _, b in want][:3]
+        draft.chain = lambda context, feats, k: fixed[:k]
+    dec = SpecDecoder(eng, draft=draft, k=3)
+    n, count, accepted = 600, dict.fromkeys(want, 0), 0
+    for seed in range(n):
+        out, stats = dec.generate(p0, 3, mode=mode, temperature=1.5, top_k=3, seed=seed)
+        count[tuple(out[6:8])] += 1
+        accepted += stats.tokens - stats.passes
+    total = sum(want.values())  # bf16 probabilities: not quite 1
+    for pair, p in want.items():
+        p /= total
+        # probabilities are bf16 and the verify kernel's logits a rounding off the decode kernel's: 2 % of p
+        assert abs(count[pair] - n * p) <= 5 * (n * p * (1 - p)) ** 0.5 + 0.02 * n * p + 1, (pair, count, want)
+    log(f"{mode}: {accepted} of {n} runs' tokens were accepted drafts")
+    assert accepted > 0
+
+
+def test_top_k_1_is_greedy(dev):
+    """One candidate: the sampled loop emits the greedy loop's tokens (equal largest logits stay candidates: none here)."""
+    from flint_amd.spec import LookupDraft, SpecDecoder
+    args, _, eng, _ = make_pair("small", seed=3)
+    p0 = (tokens(args, 12, 4).tolist() * 3)[:30]
+    for mode in ("chain", "tree"):
+        greedy, _ = SpecDecoder(eng, k=4).generate(p0, 24, mode=mode)
+        sampled, _ = SpecDecoder(eng, k=4).generate(p0, 24, mode=mode, top_k=1, seed=7)
+        again, _ = SpecDecoder(eng, k=4).generate(p0, 24, mode=mode, top_k=1, temperature=0.3, seed=8)
+        same = next((i for i in range(len(greedy)) if greedy[i] != sampled[i]), len(greedy))
+        log(f"{mode}: sampled and greedy agree for {same} of {len(greedy)}")
+        assert sampled == again or same >= 30
+        assert same >= 34
+    assert LookupDraft().max_nodes == 32
+    with pytest.raises(ValueError):
+        SpecDecoder(eng).generate(p0, 4, top_k=0)
+
+
+def test_wide_trees(dev):
+    """Trees of more than 32 nodes through the prompt pass and the 8-bit head: repeatable, and as many tokens as asked for."""
+    from flint_amd.spec import LookupDraft, SpecDecoder
+    args, _, eng, _ = make_pair("small", seed=3)
+    eng.setup_caches(1, 8)
+    head = eng.int8_head()
+
+    class Wide:
+        def tree(self, context, feats):
+            t = [(context[-1] * 7 + i * 13) % args.vocab_size for i in range(70)]
+            return t, [-1] * 5 + [i // 5 for i in range(65)]
+    for draft in (Wide(), LookupDraft(width=8, depth=10)):
+        dec = SpecDecoder(eng, draft=draft, head=head)
+        p0 = (tokens(args, 9, 4).tolist() * 4)[:33]
+        for kw in (dict(), dict(temperature=0.9, seed=5)):
+            a, sa = dec.generate(p0, 15, mode="tree", **kw)
+            b, sb = dec.generate(p0, 15, mode="tree", **kw)
+            assert a == b and len(a) >= 33 + 15 and a[:33] == p0
+    eng.check()
+    with pytest.raises(ValueError):
+        SpecDecoder(eng, k=32)
+    assert SpecDecoder(eng, k=100, head=head).k == 100
