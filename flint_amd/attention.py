@@ -6,11 +6,22 @@ sequence sits in cache slot pos + m and attends to [0, pos) and to pos + j where
 [..., key heads, slots, dim], as Transformer's k_cache and v_cache; other orders come as transposed views.
 """
 import math
+import os
 
 import torch
 
 from . import _lib
 from .quantize import workspace
+
+# each operator in one call of the torch extension, for the arguments it takes as they are, as quantize's linears
+_tree_attention_fast = _attention_weights_fast = _evict_fast = None
+if "FLINT_AMD_LIB" not in os.environ:
+    try:
+        from ._torch_ops import attention_weights_fast as _attention_weights_fast
+        from ._torch_ops import evict_fast as _evict_fast
+        from ._torch_ops import tree_attention_fast as _tree_attention_fast
+    except ImportError:
+        pass
 
 
 def _check(cond, text):
@@ -82,6 +93,13 @@ def tree_attention(q, k_cache, v_cache, pos, mask=None, scale=None, return_lse=F
     slots - M gives NaN). mask bool or uint8 [M, M] or [B, M, M]: node i sees node j (None: a chain, j <= i).
     scale: of the scores, positive (None: dim ** -0.5). Returns the output in q's shape and type and, with return_lse, the log sum
     exp of the scaled scores (fp32 [B, M, heads]). A node that sees nothing gives 0 and -inf. No gradient."""
+    if _tree_attention_fast is not None and q.is_cuda:
+        at, p0 = (None, pos) if type(pos) is int else (pos, 0)
+        if at is None or type(at) is torch.Tensor:
+            r = _tree_attention_fast(q, k_cache, v_cache, at, p0, mask, q.shape[-1] ** -0.5 if scale is None else scale,
+                                     return_lse, torch._C._cuda_getCurrentRawStream(q.get_device()))
+            if r is not None:
+                return r if return_lse else r[0]
     one = q.dim() == 3
     if one:
         q, k_cache, v_cache = q[None], k_cache[None], v_cache[None]
@@ -104,6 +122,13 @@ def attention_weights(q, k_cache, lse, pos, mask=None, scale=None, out=None):
     the nodes and the query heads of a key head of softmax's probability; 0 in slots that no node sees. Arguments as
     tree_attention's, lse as it returns it. out: a contiguous tensor of that shape to add to (slots from pos + M on are
     left as they are); it is returned. Sums have a fixed order."""
+    if _attention_weights_fast is not None and out is None and q.is_cuda:
+        at, p0 = (None, pos) if type(pos) is int else (pos, 0)
+        if at is None or type(at) is torch.Tensor:
+            r = _attention_weights_fast(q, k_cache, lse, at, p0, mask, q.shape[-1] ** -0.5 if scale is None else scale,
+                                        torch._C._cuda_getCurrentRawStream(q.get_device()))
+            if r is not None:
+                return r
     one = q.dim() == 3
     if one:
         q, k_cache, lse = q[None], k_cache[None], lse[None]
@@ -151,6 +176,12 @@ def evict(k_cache, v_cache, weights, n, keep, recent=0, sink=0, out=None):
     with the rows, those of keep .. n - 1 become 0, and the rows there stay what they were. out = (k, v) or (k, v, weights) of
     [..., keep or more, ...] takes them instead and leaves the caches alone; it must not overlap them. Returns the
     kept slots, int32 [..., keep], rising. keep >= n keeps all."""
+    if _evict_fast is not None and k_cache.is_cuda and (out is None or len(out) in (2, 3)):
+        ko, vo, wo = (None, None, None) if out is None else out if len(out) == 3 else (*out, None)
+        kept = _evict_fast(k_cache, v_cache, weights, n, keep, recent, sink, ko, vo, wo,
+                           torch._C._cuda_getCurrentRawStream(k_cache.get_device()))
+        if kept is not None:
+            return kept
     lead = k_cache.shape[:-2]
     _check(k_cache.dim() >= 2 and v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype
            and v_cache.device == k_cache.device, "k_cache and v_cache must be of one shape, type and device")

@@ -7,12 +7,11 @@
 // C. Without draft probabilities (q all at the token) w is p without the rejected tokens. Child t is accepted where u
 // q(t) Z < w(t). All of it in 64 bits: sums of 49152 values in another order than the caller's own must not move a
 // token across a border.
-#include <algorithm>
 #include "fl_common.h"
 
 namespace {
 
-constexpr int AC_NT = 1024, AC_NW = AC_NT / FL_WAVE, AC_M = 1024;
+constexpr int AC_NT = 1024, AC_NW = AC_NT / FL_WAVE, AC_M = 1024, AC_U = 16;
 
 struct AcceptArgs {
   const void *p, *q;              // [B][M][V] and [B][M - 1][V] (or null), fp32 or bf16
@@ -27,85 +26,157 @@ __device__ __forceinline__ float at(const void* p, int64_t i) {
   if constexpr (BF) return bf2f(static_cast<const uint16_t*>(p)[i]);
   else return static_cast<const float*>(p)[i];
 }
-
-__device__ __forceinline__ double wave_dsum(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-
-// One workgroup per sequence.
+// a row behind a range check: 0 past its end
 template <bool BF>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* p, int64_t row, int v) {
+  return buf_rsrc(static_cast<const char*>(p) + row * v * (BF ? 2 : 4), (uint32_t)v * (BF ? 2u : 4u));
+}
+template <bool BF>
+__device__ __forceinline__ float row_ld(__amdgpu_buffer_rsrc_t r, uint32_t i) {
+  if constexpr (BF) return bf2f(__builtin_amdgcn_raw_buffer_load_b16(r, 2u * i, 0, 0));
+  else return __uint_as_float(buf_ld32(r, 4u * i));
+}
+// the sum over a wave's lanes, in every lane, by VALU exchanges of both halves
+template <typename F>
+__device__ __forceinline__ double dsum_step(double v, F lane) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = __float_as_uint(lane(__uint_as_float((uint32_t)u))), hi = __float_as_uint(lane(__uint_as_float((uint32_t)(u >> 32))));
+  return v + __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_dsum(double v) {
+  v = dsum_step(v, lane_xor1);
+  v = dsum_step(v, lane_xor2);
+  v = dsum_step(v, lane_half_mirror);
+  v = dsum_step(v, lane_mirror);
+  v = dsum_step(v, lane_xor16);
+  return dsum_step(v, lane_xor32);
+}
+__device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
+
+// One workgroup per tree; its waves sum pieces of a row, AC_U loads of a lane in flight, for the rejections that need Z
+// and for the last token. One CU reads a row of 49152 fp32 values and its draft row in 2.6 us at its 64 bytes a cycle,
+// about what one exchange between workgroups costs, so a row stays with one. (Held in registers between two sums, the
+// row's 96 values a lane and their conversions spilled.)
+template <bool BF, bool DRAFT>
 __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
-  __shared__ int par[AC_M], tok[AC_M], gone[AC_M];
-  __shared__ float pt[AC_M], qt[AC_M];
-  __shared__ double red[AC_NW], red2[AC_NW];
-  __shared__ int found[AC_NW];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x, V = a.v;
+  __shared__ double red[2][AC_NW];
+  __shared__ int gone[AC_M];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), b = blockIdx.x, V = a.v;
   const int64_t prow = (int64_t)b * a.m, qrow = (int64_t)b * (a.m - 1);
-  const bool draft = a.q != nullptr;
-  for (int i = tid; i < a.m; i += AC_NT) {
-    int p = i == 0 ? -1 : a.parents ? a.parents[prow + i] : i - 1, t = i == 0 ? -1 : a.tokens[prow + i];
-    if (p < 0 || p >= i) p = -1;  // no node of the tree: nothing leads to it
-    if (t < 0 || t >= V) t = -1;
-    par[i] = p, tok[i] = t;
-    const bool real = p >= 0 && t >= 0;
-    pt[i] = real ? at<BF>(a.p, (prow + p) * V + t) : 0.0f;
-    qt[i] = !draft ? 1.0f : real ? at<BF>(a.q, (qrow + p) * V + t) : 0.0f;
-  }
-  __syncthreads();
-  // w of an index of node `cur`'s row
-  int cur = 0, n = 1, ngone = 0;
-  double C = 0.0, Z = 1.0;
-  bool zok = true;  // Z is that of C (with no draft: of the tokens gone)
-  auto weight = [&](int i) -> double {
-    const float p = at<BF>(a.p, (prow + cur) * V + i);
-    double w = p;
-    if (draft) {
-      if (cur < a.m - 1 && C > 0.0) w -= C * (double)at<BF>(a.q, (qrow + cur) * V + i);
-    } else {
-      for (int k = 0; k < ngone; ++k)
-        if (gone[k] == i) w = 0.0;
-    }
+  const int seg = ((V + AC_NW - 1) / AC_NW + 63) / 64 * 64;  // a wave's piece of a row
+  int cur = 0, n = 1, ngone = 0, turn = 0;  // node; nodes of the path; tokens rejected at the node
+  bool fresh = true;                        // Z is the sum of w (or 1)
+  double C = 0.0, Z = 1.0, S = -1.0;        // S: without draft probabilities, the sum of the node's row (once known)
+  __amdgpu_buffer_rsrc_t pr, qr;
+  auto open = [&] {
+    pr = row_rsrc<BF>(a.p, prow + cur, V);
+    // the last node has no children and no draft row: C stays 0 there
+    qr = DRAFT && cur < a.m - 1 ? row_rsrc<BF>(a.q, qrow + cur, V) : buf_rsrc(a.p, 0);
+  };
+  auto cut = [&](float p, float q) -> double {
+    const double w = DRAFT ? __builtin_fma(-C, (double)q, (double)p) : (double)p;
     return w > 0.0 ? w : 0.0;
   };
-  const int seg = (V + AC_NW - 1) / AC_NW, s0 = min(V, wave * seg), s1 = min(V, s0 + seg);
-  auto total = [&]() -> double {  // red: the waves' sums over their segments
+  // this wave's sum of w over [s0, s1)
+  auto piece = [&](int s0, int s1) -> double {
+    double s[4] = {};
+    for (int i0 = s0; i0 < s1; i0 += 64 * AC_U) {
+      float p[AC_U], q[DRAFT ? AC_U : 1];
+#pragma unroll
+      for (int j = 0; j < AC_U; ++j) {
+        const int i = i0 + 64 * j + lane;
+        p[j] = row_ld<BF>(pr, i < s1 ? (uint32_t)i : 0x3FFFFFFFu);
+        if (DRAFT) q[j] = row_ld<BF>(qr, i < s1 ? (uint32_t)i : 0x3FFFFFFFu);
+      }
+      if (!DRAFT)
+        for (int k = 0; k < ngone; ++k) {
+          const int d = gone[k] - i0 - lane;
+#pragma unroll
+          for (int j = 0; j < AC_U; ++j) p[j] = d == 64 * j ? 0.0f : p[j];
+        }
+#pragma unroll
+      for (int j = 0; j < AC_U; ++j) s[j & 3] += cut(p[j], DRAFT ? q[j] : 0.0f);
+    }
+    return wave_dsum((s[0] + s[1]) + (s[2] + s[3]));
+  };
+  // all waves' sums of their pieces of [g0, g1) to red[turn]
+  auto pieces = [&](int g0, int g1, int len) {
+    turn ^= 1;
+    const int s0 = min(g1, g0 + wave * len);
+    const double s = piece(s0, min(g1, s0 + len));
+    if (lane == 0) red[turn][wave] = s;
+    __syncthreads();
+  };
+  auto total = [&]() -> double {
+    open();
+    pieces(0, V, seg);
     double s = 0.0;
-    for (int i = s0 + lane; i < s1; i += 64) s += weight(i);
-    s = wave_dsum(s);
-    __syncthreads();
-    if (lane == 0) red[wave] = s;
-    __syncthreads();
-    s = 0.0;
-    for (int i = 0; i < AC_NW; ++i) s += red[i];
+#pragma unroll
+    for (int i = 0; i < AC_NW; ++i) s += red[turn][i];
     return s;
   };
   if (tid == 0) a.path[prow] = 0;
-  for (int i = 1; i < a.m; ++i) {
-    if (par[i] != cur || tok[i] < 0) continue;
-    if (!zok) {
-      Z = total();
-      zok = true;
+  for (int n0 = 0; n0 < a.m; n0 += 64) {  // nodes in order, 64 at a time, one per lane
+    const int i = n0 + lane;
+    int par = -1, tok = -1;
+    float pt = 0.0f, qt = 1.0f, u = 0.0f;
+    if (i > 0 && i < a.m) {
+      par = a.parents ? a.parents[prow + i] : i - 1;
+      tok = a.tokens[prow + i];
+      u = a.ua[prow + i];
+      if (par >= 0 && par < i && tok >= 0 && tok < V) {
+        pt = at<BF>(a.p, (prow + par) * V + tok);
+        if (DRAFT) qt = at<BF>(a.q, (qrow + par) * V + tok);
+      } else {
+        par = -1;  // no node of the tree, or no token: passed over
+      }
     }
-    double w = pt[i];
-    if (draft) w -= C * (double)qt[i];
-    else
-      for (int k = 0; k < ngone; ++k)
-        if (gone[k] == tok[i]) w = 0.0;
-    if ((double)a.ua[prow + i] * (double)qt[i] * Z < w) {
-      cur = i, C = 0.0, Z = 1.0, zok = true, ngone = 0;
-      if (tid == 0) a.path[prow + n] = i;
-      ++n;
-      __syncthreads();
-    } else {
-      C += Z;
-      zok = false;
-      if (!draft) {
-        __syncthreads();
-        if (tid == 0) gone[ngone] = tok[i];
-        ++ngone;
-        __syncthreads();
+    unsigned long long ahead = ~0ull;  // of these 64 not yet passed
+    for (;;) {
+      const unsigned long long kids = __ballot(par == cur) & ahead;
+      if (!kids) break;
+      const int l = __ffsll(kids) - 1;
+      ahead = l == 63 ? 0 : ~0ull << (l + 1);
+      const int t = __builtin_amdgcn_readlane(tok, l);
+      const float p1 = lane_of(pt, l), q1 = lane_of(qt, l), u1 = lane_of(u, l);
+      if (!fresh) {
+        if (DRAFT) {
+          Z = total();
+        } else {  // the row's sum without the tokens gone
+          if (S < 0.0) {
+            const int keep = ngone;
+            ngone = 0;
+            S = total();
+            ngone = keep;
+          }
+          Z = S;
+          for (int k = 0; k < ngone; ++k) {
+            bool twice = false;  // a token that was proposed again
+            for (int j = 0; j < k; ++j) twice = twice || gone[j] == gone[k];
+            const float g = row_ld<BF>(pr, (uint32_t)gone[k]);
+            Z -= twice || !(g > 0.0f) ? 0.0 : (double)g;
+          }
+          Z = Z > 0.0 ? Z : 0.0;
+        }
+        fresh = true;
+      }
+      double w = cut(p1, q1);
+      if (!DRAFT)
+        for (int k = 0; k < ngone; ++k)
+          if (gone[k] == t) w = 0.0;
+      if ((double)u1 * (double)q1 * Z < w) {
+        cur = n0 + l, C = 0.0, Z = 1.0, S = -1.0, ngone = 0, fresh = true;
+        if (tid == 0) a.path[prow + n] = cur;
+        ++n;
+        if (!DRAFT) __syncthreads();  // gone is free again
+      } else {
+        C += Z;
+        fresh = false;
+        if (!DRAFT) {
+          if (tid == 0) gone[ngone] = t;
+          ++ngone;
+          __syncthreads();
+        }
       }
     }
   }
@@ -115,44 +186,56 @@ __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
     C = 0.0, ngone = 0;
     sum = total();
   }
-  // the first index where the running sum passes `want`: the segment, then the piece of it, then the lane
-  const double want = (double)a.us[b] * sum;
-  double run = 0.0;
-  int sg = -1;
-  double before = 0.0;
-  int last = -1;  // the last segment with any weight
-  double before_last = 0.0;
-  for (int i = 0; i < AC_NW; ++i) {
-    if (sg < 0 && run + red[i] > want) sg = i, before = run;
-    if (red[i] > 0.0) last = i, before_last = run;
-    run += red[i];
-  }
-  if (sg < 0) sg = last, before = before_last;
   int result = -1;
-  if (sg >= 0 && sum > 0.0 && sum < INFINITY) {
-    const int g0 = min(V, sg * seg), g1 = min(V, g0 + seg);
-    // wave 0 walks the segment, 64 values at a time
-    if (wave == 0) {
-      int best = -1, tail = -1;
-      for (int i0 = g0; i0 < g1 && best < 0; i0 += 64) {
-        const int i = i0 + lane;
-        const double w = i < g1 ? weight(i) : 0.0;
-        double inc = w;
+  if (sum > 0.0 && sum < INFINITY) {
+    // the first index at which the running sum passes `want`: the wave's piece, then pieces of that until a few are left
+    const double want = (double)a.us[b] * sum;
+    double before = 0.0;
+    int g0 = 0, g1 = V, len = seg;
+    for (;;) {
+      int pick = -1, tail = 0;
+      double run = before, at_pick = before, at_tail = before;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const double u = __shfl_up(inc, o, 64);
-          if (lane >= o) inc += u;
-        }
-        const unsigned long long hit = __ballot(w > 0.0 && before + inc > want), any = __ballot(w > 0.0);
-        if (hit) best = i0 + __ffsll((unsigned long long)hit) - 1;
-        if (any) tail = i0 + 63 - __clzll((long long)any);
-        before += __shfl(inc, 63, 64);
+      for (int i = 0; i < AC_NW; ++i) {
+        const double r = red[turn][i];
+        if (pick < 0 && run + r > want) pick = i, at_pick = run;
+        if (r > 0.0) tail = i, at_tail = run;
+        run += r;
       }
-      result = best >= 0 ? best : tail;
+      if (pick < 0) pick = tail, at_pick = at_tail;  // the sums of pieces differ in their last bits
+      before = at_pick;
+      g0 = min(g1, g0 + pick * len);
+      g1 = min(g1, g0 + len);
+      if (g1 - g0 <= 256) break;
+      len = ((g1 - g0 + AC_NW - 1) / AC_NW + 63) / 64 * 64;
+      pieces(g0, g1, len);
     }
+    int tail = -1;
+    for (int i0 = g0; i0 < g1 && result < 0; i0 += 64) {
+      const int i = i0 + lane;
+      double w = i < g1 ? cut(row_ld<BF>(pr, i), DRAFT ? row_ld<BF>(qr, i) : 0.0f) : 0.0;
+      if (!DRAFT)
+        for (int k = 0; k < ngone; ++k)
+          if (gone[k] == i) w = 0.0;
+      double inc = w;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double x = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += x;
+      }
+      const unsigned long long hit = __ballot(w > 0.0 && before + inc > want), any = __ballot(w > 0.0);
+      if (hit) result = i0 + __ffsll(hit) - 1;
+      if (any) tail = i0 + 63 - __clzll((long long)any);
+      before += __shfl(inc, 63, 64);
+    }
+    if (result < 0) result = tail;
   }
   if (tid == 0) a.token[b] = result, a.count[b] = n;
-  (void)red2, (void)found;
+}
+
+template <bool BF, bool DRAFT>
+void accept_launch(const AcceptArgs& a, int b, hipStream_t s) {
+  hipLaunchKernelGGL((k_accept<BF, DRAFT>), dim3(b), dim3(AC_NT), 0, s, a);
 }
 
 }  // namespace
@@ -166,8 +249,8 @@ int fl_accept(const void* probs, const void* draft, int32_t bf16, const int32_t*
   if (b < 1 || b > 65536 || m < 1 || m > AC_M || vocab < 1 || vocab > 1 << 20) return FL_E_ARG;
   const AcceptArgs a{probs, m > 1 ? draft : nullptr, tokens, parents, accept_u, sample_u, path, count, token, m, vocab};
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (bf16) hipLaunchKernelGGL(k_accept<true>, dim3(b), dim3(AC_NT), 0, s, a);
-  else hipLaunchKernelGGL(k_accept<false>, dim3(b), dim3(AC_NT), 0, s, a);
+  if (a.q) bf16 ? accept_launch<true, true>(a, b, s) : accept_launch<false, true>(a, b, s);
+  else bf16 ? accept_launch<true, false>(a, b, s) : accept_launch<false, false>(a, b, s);
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
 }
 

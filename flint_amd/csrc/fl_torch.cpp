@@ -388,6 +388,182 @@ pybind11::object head_logprobs_fast(const torch::Tensor& x, const torch::Tensor&
   return rc == FL_OK ? o.cast() : pybind11::object(pybind11::none());
 }
 
+// ---- attention over a cache, eviction, verification: as int8_fast -----------------------------------------------
+
+// strides that the kernels' 16-byte loads take; those of dimensions of one element do not count
+bool strides8(const torch::Tensor& t, int64_t* out, int n) {
+  if (t.stride(-1) != 1 || !on16(t)) return false;
+  for (int i = 0; i < n; ++i) {
+    out[i] = t.size(i) > 1 ? t.stride(i) : 0;
+    if (out[i] % 8 || out[i] < 0) return false;
+  }
+  return true;
+}
+// fl_attn_desc of four-dimensional tensors (v undefined: none); false for what the general path decides
+bool describe(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const std::optional<torch::Tensor>& pos,
+              int64_t pos0, const std::optional<torch::Tensor>& mask, double scale, fl_attn_desc* d) {
+  const auto dt = q.scalar_type();
+  if (!q.is_cuda() || (dt != torch::kBFloat16 && dt != torch::kFloat16) || q.dim() != 4 || k.dim() != 4 || k.scalar_type() != dt ||
+      q.layout() != torch::kStrided || k.layout() != torch::kStrided)
+    return false;
+  if (v.defined() && (v.scalar_type() != dt || v.layout() != torch::kStrided || v.sizes() != k.sizes())) return false;
+  for (int i = 0; i < 4; ++i)
+    if (q.size(i) < 1 || q.size(i) > INT32_MAX || k.size(i) < 1 || k.size(i) > INT32_MAX) return false;
+  *d = fl_attn_desc{};
+  d->b = (int32_t)q.size(0), d->m = (int32_t)q.size(1), d->heads = (int32_t)q.size(2), d->dim = (int32_t)q.size(3);
+  d->groups = (int32_t)k.size(1), d->slots = (int32_t)k.size(2), d->fp16 = dt == torch::kFloat16;
+  if (k.size(0) != d->b || k.size(3) != d->dim) return false;
+  int64_t st[3];
+  if (!strides8(q, st, 3)) return false;
+  d->q_b = st[0], d->q_m = st[1], d->q_h = st[2];
+  if (!strides8(k, st, 3)) return false;
+  d->k_b = st[0], d->k_g = st[1], d->k_s = st[2];
+  if (v.defined()) {
+    if (!strides8(v, st, 3)) return false;
+    d->v_b = st[0], d->v_g = st[1], d->v_s = st[2];
+  }
+  if (pos) {
+    if (pos->scalar_type() != torch::kInt32 || pos->numel() != d->b || !pos->is_contiguous()) return false;
+  } else {
+    if (pos0 < 0 || pos0 > INT32_MAX) return false;
+    d->pos0 = (int32_t)pos0;
+  }
+  if (mask) {
+    const auto mt = mask->scalar_type();
+    if ((mt != torch::kBool && mt != torch::kUInt8) || !mask->is_contiguous() || mask->dim() < 2 || mask->dim() > 3 ||
+        mask->size(-1) != d->m || mask->size(-2) != d->m || (mask->dim() == 3 && mask->size(0) != d->b))
+      return false;
+    d->mask_b = mask->dim() == 3 && d->b > 1 ? (int64_t)d->m * d->m : 0;
+  }
+  d->scale = (float)scale;
+  return here(q, {&k, &v, pos ? &*pos : &q, mask ? &*mask : &q});
+}
+const int32_t* ints_of(const std::optional<torch::Tensor>& t) { return t ? static_cast<const int32_t*>(t->data_ptr()) : nullptr; }
+const uint16_t* halves_of(const torch::Tensor& t) { return static_cast<const uint16_t*>(t.data_ptr()); }
+const uint8_t* mask_of(const std::optional<torch::Tensor>& t) { return t ? static_cast<const uint8_t*>(t->data_ptr()) : nullptr; }
+
+// attention.tree_attention: (out, lse or None)
+pybind11::object tree_attention_fast(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                                     const std::optional<torch::Tensor>& pos, int64_t pos0,
+                                     const std::optional<torch::Tensor>& mask, double scale, bool want_lse, int64_t stream) {
+  fl_attn_desc d;
+  int64_t need = 0;
+  if (!v.defined() || !describe(q, k, v, pos, pos0, mask, scale, &d) || fl_tree_attention_workspace(&d, !pos, &need) != FL_OK)
+    return pybind11::none();
+  torch::Tensor out, lse;
+  int rc = FL_E_HIP;
+  try {
+    pybind11::gil_scoped_release nogil;
+    const auto opt = q.options().requires_grad(false);
+    out = torch::empty(q.sizes(), opt);
+    if (want_lse) lse = torch::empty({d.b, d.m, d.heads}, opt.dtype(torch::kFloat32));
+    const torch::Tensor work = bytes_of(need, q);
+    rc = fl_tree_attention(&d, halves_of(q), halves_of(k), halves_of(v), ints_of(pos), mask_of(mask),
+                           static_cast<uint16_t*>(out.data_ptr()), static_cast<float*>(data_of(lse)), data_of(work),
+                           stream_of(stream));
+  } catch (const c10::OutOfMemoryError&) {
+  }
+  if (rc != FL_OK) return pybind11::none();
+  return pybind11::make_tuple(out, want_lse ? pybind11::cast(lse) : pybind11::object(pybind11::none()));
+}
+
+// attention.attention_weights without `out`
+pybind11::object attention_weights_fast(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& lse,
+                                        const std::optional<torch::Tensor>& pos, int64_t pos0,
+                                        const std::optional<torch::Tensor>& mask, double scale, int64_t stream) {
+  fl_attn_desc d;
+  if (!describe(q, k, torch::Tensor(), pos, pos0, mask, scale, &d) || !plain(lse, torch::kFloat32, 3) || lse.size(0) != d.b ||
+      lse.size(1) != d.m || lse.size(2) != d.heads || !here(q, {&lse}))
+    return pybind11::none();
+  torch::Tensor w;
+  int rc = FL_E_HIP;
+  try {
+    pybind11::gil_scoped_release nogil;
+    w = torch::empty({d.b, d.groups, d.slots}, q.options().dtype(torch::kFloat32).requires_grad(false));
+    rc = fl_attention_weights(&d, halves_of(q), halves_of(k), static_cast<const float*>(lse.data_ptr()), ints_of(pos), mask_of(mask),
+                              static_cast<float*>(w.data_ptr()), 0, stream_of(stream));
+  } catch (const c10::OutOfMemoryError&) {
+  }
+  return rc == FL_OK ? pybind11::cast(w) : pybind11::object(pybind11::none());
+}
+
+bool overlap(const torch::Tensor& a, const torch::Tensor& b) {  // of contiguous tensors
+  const char *a0 = static_cast<const char*>(a.data_ptr()), *b0 = static_cast<const char*>(b.data_ptr());
+  return a0 < b0 + b.nbytes() && b0 < a0 + a.nbytes();
+}
+
+// attention.evict of contiguous tensors, from which something leaves
+pybind11::object evict_fast(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& w, int64_t n, int64_t keep,
+                            int64_t recent, int64_t sink, const std::optional<torch::Tensor>& ko,
+                            const std::optional<torch::Tensor>& vo, const std::optional<torch::Tensor>& wo, int64_t stream) {
+  const int64_t dims = k.dim();
+  if (dims < 2 || !plain(k, k.scalar_type(), dims) || !plain(v, k.scalar_type(), dims) || !plain(w, torch::kFloat32, dims - 1) ||
+      v.sizes() != k.sizes() || w.sizes() != k.sizes().slice(0, dims - 1) || k.numel() == 0 || !on16(k) || !on16(v))
+    return pybind11::none();
+  const int64_t slots = k.size(-2), rb = k.size(-1) * (int64_t)k.element_size(), heads = k.numel() / (slots * k.size(-1));
+  if (heads > 65535 || slots > INT32_MAX || rb > 4096 || n < 1 || n > slots || keep < 1 || keep >= n || recent < 0 || sink < 0 ||
+      recent + sink > keep || !here(k, {&v, &w}) || ko.has_value() != vo.has_value() || (wo && !ko))
+    return pybind11::none();
+  const fl_rows kr{k.data_ptr(), 0, slots * rb, rb}, vr{v.data_ptr(), 0, slots * rb, rb};
+  fl_rows kor{}, vor{};
+  int64_t so = 0;
+  if (ko) {
+    if (!plain(*ko, k.scalar_type(), dims) || !plain(*vo, k.scalar_type(), dims) || ko->sizes() != vo->sizes() || !on16(*ko) ||
+        !on16(*vo) || ko->size(-1) != k.size(-1) || ko->sizes().slice(0, dims - 2) != k.sizes().slice(0, dims - 2) ||
+        !here(k, {&*ko, &*vo, wo ? &*wo : &k}))
+      return pybind11::none();
+    so = ko->size(-2);
+    if (so < keep || so > INT32_MAX) return pybind11::none();
+    if (wo && (!plain(*wo, torch::kFloat32, dims - 1) || wo->sizes() != ko->sizes().slice(0, dims - 1))) return pybind11::none();
+    for (const torch::Tensor* t : {&*ko, &*vo, wo ? &*wo : &*ko})
+      for (const torch::Tensor* from : {&k, &v, &w})
+        if (overlap(*t, *from)) return pybind11::none();
+    kor = fl_rows{ko->data_ptr(), 0, so * rb, rb}, vor = fl_rows{vo->data_ptr(), 0, so * rb, rb};
+  }
+  torch::Tensor kept;
+  int rc = FL_E_HIP;
+  try {
+    pybind11::gil_scoped_release nogil;
+    auto sizes = w.sizes().vec();
+    sizes.back() = keep;
+    kept = torch::empty(sizes, w.options().dtype(torch::kInt32).requires_grad(false));
+    rc = fl_evict(&kr, &vr, static_cast<float*>(w.data_ptr()), 1, (int32_t)heads, (int32_t)slots, (int32_t)rb, (int32_t)n,
+                  (int32_t)keep, (int32_t)recent, (int32_t)sink, static_cast<int32_t*>(kept.data_ptr()), ko ? &kor : nullptr,
+                  vo ? &vor : nullptr, wo ? static_cast<float*>(wo->data_ptr()) : nullptr, (int32_t)so, stream_of(stream));
+  } catch (const c10::OutOfMemoryError&) {
+  }
+  return rc == FL_OK ? pybind11::cast(kept) : pybind11::object(pybind11::none());
+}
+
+// spec.accept_sampled: (path, count, token)
+pybind11::object accept_fast(const torch::Tensor& p, const torch::Tensor& tokens, const torch::Tensor& ua, const torch::Tensor& us,
+                             const std::optional<torch::Tensor>& parents, const std::optional<torch::Tensor>& q, int64_t stream) {
+  const auto dt = p.scalar_type();
+  if ((dt != torch::kFloat32 && dt != torch::kBFloat16) || !plain(p, dt, 3) || p.numel() == 0) return pybind11::none();
+  const int64_t b = p.size(0), m = p.size(1), v = p.size(2);
+  auto fits = [](const torch::Tensor& t, torch::ScalarType want, int64_t n) { return plain(t, want, t.dim()) && t.numel() == n; };
+  if (!fits(tokens, torch::kInt32, b * m) || !fits(ua, torch::kFloat32, b * m) || !fits(us, torch::kFloat32, b) ||
+      (parents && !fits(*parents, torch::kInt32, b * m)) ||
+      (q && (!plain(*q, dt, 3) || q->size(0) != b || q->size(1) != m - 1 || q->size(2) != v)) ||
+      !here(p, {&tokens, &ua, &us, parents ? &*parents : &p, q ? &*q : &p}) || b > INT32_MAX || m > INT32_MAX || v > INT32_MAX)
+    return pybind11::none();
+  torch::Tensor path, count, token;
+  int rc = FL_E_HIP;
+  try {
+    pybind11::gil_scoped_release nogil;
+    const torch::Tensor all = bytes_of(4 * (b * m + 2 * b), p);  // the three in one allocation, all int32
+    path = piece(all, 0, {b, m}, torch::kInt32);
+    count = piece(all, 4 * b * m, {b}, torch::kInt32);
+    token = piece(all, 4 * (b * m + b), {b}, torch::kInt32);
+    rc = fl_accept(p.data_ptr(), q ? q->data_ptr() : nullptr, dt == torch::kBFloat16, static_cast<const int32_t*>(tokens.data_ptr()),
+                   ints_of(parents), static_cast<const float*>(ua.data_ptr()), static_cast<const float*>(us.data_ptr()),
+                   static_cast<int32_t*>(path.data_ptr()), static_cast<int32_t*>(count.data_ptr()),
+                   static_cast<int32_t*>(token.data_ptr()), (int32_t)b, (int32_t)m, (int32_t)v, stream_of(stream));
+  } catch (const c10::OutOfMemoryError&) {
+  }
+  return rc == FL_OK ? pybind11::object(pybind11::make_tuple(path, count, token)) : pybind11::object(pybind11::none());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -405,5 +581,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("int8_fast", &int8_fast);
   m.def("logprobs_fast", &logprobs_fast);
   m.def("head_logprobs_fast", &head_logprobs_fast);
+  m.def("tree_attention_fast", &tree_attention_fast);
+  m.def("attention_weights_fast", &attention_weights_fast);
+  m.def("evict_fast", &evict_fast);
+  m.def("accept_fast", &accept_fast);
   m.def("version", []() { return fl_version(); });
 }

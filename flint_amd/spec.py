@@ -29,6 +29,7 @@ distributions of its own also has
                                                         drawn from, each on its own (node 0 = the root;
                                                         a chain's node i + 1 is its i-th token)
 """
+import os
 import time
 from collections import namedtuple
 
@@ -38,6 +39,14 @@ import torch
 from . import _lib
 from .generate import _ids, logits_to_probs, prefill
 from .quantize import linear_int8
+
+# accept_sampled as one call of the torch extension, as quantize's linears
+_accept_fast = None
+if "FLINT_AMD_LIB" not in os.environ:
+    try:
+        from ._torch_ops import accept_fast as _accept_fast
+    except ImportError:
+        pass
 
 
 def tree_depths(parents):
@@ -123,6 +132,11 @@ def accept_sampled(probs, tokens, accept_u, sample_u, parents=None, draft_probs=
     first; a rejection takes Z q off w (all of t without draft_probs), not below 0, and Z becomes the sum of w. The last
     node's token is the first index at which the running sum of w passes sample_u times its sum (-1 where that is not
     a positive number). Returns Accepted (without B: of one tree, count and token of one element)."""
+    if _accept_fast is not None and probs.is_cuda:
+        r = _accept_fast(probs, tokens, accept_u, sample_u, parents, draft_probs,
+                         torch._C._cuda_getCurrentRawStream(probs.get_device()))
+        if r is not None:
+            return Accepted(*r)
     one = probs.dim() == 2
     if one:
         probs = probs[None]
