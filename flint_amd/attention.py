@@ -61,6 +61,7 @@ def _describe(q, k, v, pos, mask, scale):
     d = _lib.AttnDesc(b=b, m=m, heads=heads, groups=groups, dim=dim, slots=slots, fp16=int(q.dtype == torch.float16),
                       scale=scale)
     d.q_b, d.q_m, d.q_h = _strides16(q, "q")
+    _check((m - 1) * d.q_m + (heads - 1) * d.q_h + dim <= 1 << 30, "q: a sequence's queries within 2^30 values")
     d.k_b, d.k_g, d.k_s = _strides16(k, "k_cache")
     _check(d.k_s <= 1 << 23, "k_cache: slots at most 2^23 values apart")
     if v is not None:

@@ -24,7 +24,7 @@ struct AttnArgs {
   float* lse;           // [B][M][heads] or null (read by k_attn_weights)
   float* part;          // with key parts: o [parts][B][groups][R][D], then (m, l) [parts][B][groups][R][2]
   int b, m, heads, groups, rep, slots, pos0, R;
-  int blocks, parts;    // row blocks per key head; key parts
+  int blocks, parts, kpp;  // row blocks per key head; key parts, keys of a part
   float sc;             // scale * log2 e
   int64_t q_b, q_m, q_h, k_b, k_g, k_s, v_b, v_g, v_s, mask_b;
 };
@@ -81,22 +81,18 @@ __device__ __forceinline__ uint4 only_finite(uint4 w) {
 struct Span {
   int pos, keys, kb0, kend;
 };
-// Parts are whole multiples of `unit` keys, as even as those allow, so that a short sequence of a ragged batch has
-// fewer and its row of them is as long as any.
-__device__ __forceinline__ int part_keys(int keys, int parts, int unit) {
-  return ((keys + parts - 1) / parts + unit - 1) / unit * unit;
-}
-__device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int part, int unit) {
+// Every part has kpp keys, so that the workgroups of a ragged batch take as long as each other; a short sequence has
+// fewer parts.
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int part) {
   Span s;
-  s.pos = a.pos ? a.pos[b] : a.pos0;
+  s.pos = a.pos ? __builtin_amdgcn_readfirstlane(a.pos[b]) : a.pos0;  // the wave's, in a scalar register
   if (s.pos < 0 || s.pos > a.slots - a.m) {
     s.keys = -1, s.kb0 = s.kend = 0;
     return s;
   }
   s.keys = s.pos + a.m;
-  const int kpp = part_keys(s.keys, a.parts, unit);
-  s.kb0 = min(s.keys, part * kpp);
-  s.kend = min(s.keys, s.kb0 + kpp);
+  s.kb0 = (int)min((int64_t)s.keys, (int64_t)part * a.kpp);
+  s.kend = min(s.keys - s.kb0, a.kpp) + s.kb0;
   return s;
 }
 
@@ -185,9 +181,11 @@ __device__ __forceinline__ void softmax_pv(fl_f32x16 (&s)[KT], Rows<D / 32>& st,
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
+    for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(s[kt][i], s[kt][i + 1]), mx);  // one three-way maximum each
   mx = xor32_max(mx) * sc;
-  if (__any(mx > st.m)) {  // rows whose maximum rises; the others' factor is 1
+  // m is any reference near the maximum: it follows only where a row's passed it by 2^8 (p and l stay far inside their
+  // range), which after a row's first tile hardly happens; some row of 32 has a new maximum in half of all tiles
+  if (__any(mx > st.m + 8.0f)) {
     const float mn = fmaxf(st.m, mx), corr = st.m == mn ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
     st.m = mn;
     st.l *= corr;
@@ -197,36 +195,38 @@ __device__ __forceinline__ void softmax_pv(fl_f32x16 (&s)[KT], Rows<D / 32>& st,
       for (int i = 0; i < 16; ++i) st.o[d][i] *= corr;
   }
   const float mu = st.m == -INFINITY ? 0.0f : st.m;
-  float ps = 0.0f;
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], sc, -mu));
-      ps += s[kt][i];
-    }
-  st.l += xor32_sum(ps);
   const int row = 4 * hf + (i16 >> 2);
   const unsigned char* vp = vt + row * (2 * D) + (i16 & 3) * 8 + ((lane >> 4) & 1) * 32;
+  float ps[4] = {};
+  // 16 keys at a time: their exponentials and terms of P while the matrix cores run the 16 before
 #pragma unroll
-  for (int st16 = 0; st16 < 2 * KT; ++st16) {  // 16 keys
-    uint32_t ph[4], pl[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float p0 = s[st16 >> 1][8 * (st16 & 1) + 2 * e], p1 = s[st16 >> 1][8 * (st16 & 1) + 2 * e + 1];
-      ph[e] = pack16<H>(p0, p1);
-      pl[e] = pack16<H>(p0 - lo16<H>(ph[e]), p1 - hi16<H>(ph[e]));
-    }
-    const uint4 bh = make_uint4(ph[0], ph[1], ph[2], ph[3]), bl = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+  for (int st16 = 0; st16 < 2 * KT; ++st16) {
+    uint2 v0[DT], v1[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const unsigned char* vd = vp + st16 * 16 * (2 * D) + (d ^ v_swz<D>(row)) * 64;
-      const uint2 v0 = tr4(vd), v1 = tr4(vd + 8 * (2 * D));
-      const uint4 va = make_uint4(v0.x, v0.y, v1.x, v1.y);
-      st.o[d] = mma<H>(va, bh, st.o[d]);
-      st.o[d] = mma<H>(va, bl, st.o[d]);
+      v0[d] = tr4(vd), v1[d] = tr4(vd + 8 * (2 * D));
     }
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st16 >> 1][8 * (st16 & 1) + i], sc, -mu));
+      ps[i & 3] += p[i];
+    }
+    uint32_t ph[4], pl[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      ph[e] = pack16<H>(p[2 * e], p[2 * e + 1]);
+      asm("" : "+v"(ph[e]));  // read back from the pair, not converted again
+      pl[e] = pack16<H>(p[2 * e] - lo16<H>(ph[e]), p[2 * e + 1] - hi16<H>(ph[e]));
+    }
+    const uint4 bh = make_uint4(ph[0], ph[1], ph[2], ph[3]), bl = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) st.o[d] = mma<H>(make_uint4(v0[d].x, v0[d].y, v1[d].x, v1[d].y), bh, st.o[d]);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) st.o[d] = mma<H>(make_uint4(v0[d].x, v0[d].y, v1[d].x, v1[d].y), bl, st.o[d]);
   }
+  st.l += xor32_sum((ps[0] + ps[1]) + (ps[2] + ps[3]));
 }
 
 // Values of V that are not finite, in slots that some rows see and others do not: the tile's V has zeros in their
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_few(AttnArgs a) {
   const int blk = rest % a.blocks;
   rest /= a.blocks;
   const int part = rest % a.parts, b = rest / a.parts;
-  const Span sp = span_of(a, b, part, NW * TK);
+  const Span sp = span_of(a, b, part);
   if (a.parts > 1 && sp.kb0 >= sp.kend) return;  // the merge knows
   const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
   const uint16_t* kp = a.k + (int64_t)b * a.k_b + (int64_t)g * a.k_g;
@@ -416,13 +416,15 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_few(AttnArgs a) {
 }
 
 // ---- many rows: the workgroup's waves share the keys ------------------------------------------------------
-// 32 rows per wave, four waves, one part of the keys in rounds of 64, K and V staged in LDS, double-buffered.
+// 32 rows per wave, four waves, one part of the keys in rounds of TK. K and V go straight from memory into a ring of
+// three LDS stages, two rounds ahead (a round takes less than a microsecond, about what a load does; through registers,
+// one round ahead, the waves waited for it every time), swizzled by what each lane loads; one barrier a round.
 template <bool H, int D>
-__global__ __launch_bounds__(256, 2) void k_attn_many(AttnArgs a) {
-  constexpr int TK = 64, KT = 2, ST = D / 16, DT = D / 32, CH = D / 8, PT = TK * CH / 256;  // PT: chunks per thread
-  __shared__ __align__(16) unsigned char ks[2][TK * D * 2];
-  __shared__ __align__(16) unsigned char vs[2][TK * D * 2];
-  __shared__ int odd[2];
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_many(AttnArgs a) {
+  constexpr int TK = 4096 / D, KT = TK / 32, ST = D / 16, DT = D / 32, CH = D / 8, NS = 3;
+  constexpr int TILE = TK * D * 2, PW = TILE / 4096;  // bytes of K or V of a round (8 KB); 1 KB loads of a wave of each
+  __shared__ __align__(16) unsigned char ring[NS][2][TILE];
+  __shared__ int odd[NS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hf = lane >> 5;
   int rest = blockIdx.x;
   const int g = rest % a.groups;
@@ -430,7 +432,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_many(AttnArgs a) {
   const int part = rest % a.parts;
   rest /= a.parts;
   const int blk = a.blocks - 1 - rest % a.blocks, b = rest / a.blocks;  // the longest rows first
-  Span sp = span_of(a, b, part, TK);
+  const Span sp = span_of(a, b, part);
   if (a.parts > 1 && sp.kb0 >= sp.kend) return;
   const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
   const uint16_t* kp = a.k + (int64_t)b * a.k_b + (int64_t)g * a.k_g;
@@ -442,6 +444,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_many(AttnArgs a) {
     kend = min(kend, sp.pos + min(a.m - 1, (blk * 128 + 127) / a.rep) + 1);
     wend = min(kend, sp.pos + min(a.m - 1, (blk * 128 + wave * 32 + 31) / a.rep) + 1);
   }
+  kend = __builtin_amdgcn_readfirstlane(kend);
   const int wfull = sp.pos + (mask ? 0 : min(a.m - 1, (blk * 128 + wave * 32) / a.rep) + 1);  // keys that all its rows see
   uint4 qf[ST];
   const uint16_t* qp = a.q + (int64_t)b * a.q_b + (int64_t)t * a.q_m + (int64_t)(g * a.rep + rowc % a.rep) * a.q_h;
@@ -449,48 +452,45 @@ __global__ __launch_bounds__(256, 2) void k_attn_many(AttnArgs a) {
   for (int s = 0; s < ST; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + s * 16 + hf * 8);
   Rows<DT> st;
   st.clear();
-  const int c = tid % CH, k0 = tid / CH;
-  const uint32_t ko = (uint32_t)(k0 * a.k_s + c * 8) * 2u, kstep = (uint32_t)((256 / CH) * a.k_s) * 2u;
-  const uint32_t vo = (uint32_t)(k0 * a.v_s + c * 8) * 2u, vstep = (uint32_t)((256 / CH) * a.v_s) * 2u;
-  uint4 kv[PT], vv[PT];
-  auto load = [&](int kb) {
-    const auto kr = tile_rsrc(kp, a.k_s, kb, kend, TK, D), vr = tile_rsrc(vp, a.v_s, kb, kend, TK, D);
-#pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      kv[i] = tile_ld(kr, ko, i * kstep);
-      vv[i] = tile_ld(vr, vo, i * vstep);
-    }
-  };
+  // 16-byte chunk i * 256 + tid of a tile's LDS: a row of it, and there the chunk that the swizzle puts in its place
   auto k_at = [&](int key, int ch) {  // 16 rows' chunk on 16 different places
     return key * (2 * D) + (ch ^ (D == 64 ? (key >> 1) & 7 : key & 15)) * 16;
   };
-  const int kw = k_at(k0, c), vw = v_at<D>(k0, c);  // a sweep of 256 threads is 4 KB of rows, at the same swizzle
-  auto store = [&](int buf, int kb) {
-    if (kb + TK > sp.pos) {
+  const int k0 = tid / CH, slot = tid % CH;  // a sweep of 256 threads is 256 / CH rows, at the same swizzle
+  const uint32_t ko = (uint32_t)(k0 * a.k_s) * 2u + (uint32_t)(slot ^ (D == 64 ? (k0 >> 1) & 7 : k0 & 15)) * 16u;
+  const uint32_t vo = (uint32_t)(k0 * a.v_s) * 2u + (uint32_t)(((slot >> 2) ^ v_swz<D>(k0)) * 4 + (slot & 3)) * 16u;
+  const uint32_t kstep = (uint32_t)(256 / CH * a.k_s) * 2u, vstep = (uint32_t)(256 / CH * a.v_s) * 2u;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)&ring[0][0][0] + (uint32_t)wave * 1024u;
+  auto load = [&](int kb, int stage) {  // behind the end: zeros, nothing read
+    const int rem = min(max(kend - kb, 0), TK);
+    const fl_u32x4 kw = buffer_words(kp + (int64_t)kb * a.k_s, rem ? (uint32_t)((rem - 1) * a.k_s + D) * 2u : 0u);
+    const fl_u32x4 vw = buffer_words(vp + (int64_t)kb * a.v_s, rem ? (uint32_t)((rem - 1) * a.v_s + D) * 2u : 0u);
+    const uint32_t at = lds0 + (uint32_t)stage * (2 * TILE);
 #pragma unroll
-      for (int i = 0; i < PT; ++i)
-        if (kb + k0 + i * (256 / CH) >= sp.pos && !finite16<H>(vv[i])) {
-          vv[i] = only_finite<H>(vv[i]);
-          odd[buf] = kb + 1;
-        }
-    }
+    for (int i = 0; i < PW; ++i) dma_1k(kw, at + i * 4096, ko, i * kstep);
 #pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      *reinterpret_cast<uint4*>(ks[buf] + kw + i * 4096) = kv[i];
-      *reinterpret_cast<uint4*>(vs[buf] + vw + i * 4096) = vv[i];
-    }
+    for (int i = 0; i < PW; ++i) dma_1k(vw, at + TILE + i * 4096, vo, i * vstep);
   };
-  if (tid < 2) odd[tid] = 0;
+  if (tid < NS) odd[tid] = 0;
   __syncthreads();
-  if (sp.kb0 < kend) {
-    load(sp.kb0);
-    store(0, sp.kb0);
-  }
-  int buf = 0;
-  for (int kb = sp.kb0; kb < kend; kb += TK, buf ^= 1) {
-    const bool more = kb + TK < kend;
-    __syncthreads();
-    if (more) load(kb + TK);
+  load(sp.kb0, 0);
+  load(sp.kb0 + TK, 1);
+  int stage = 0;
+  for (int kb = sp.kb0; kb < kend; kb += TK) {
+    unsigned char *ks = ring[stage][0], *vs = ring[stage][1];
+    wait_loads<2 * PW>();  // this round's have landed, the next one's may be in flight
+    if (kb + TK > sp.pos) {  // nodes: values of V that are not finite become zeros, each lane's own chunks
+#pragma unroll
+      for (int i = 0; i < PW; ++i) {
+        uint4* x = reinterpret_cast<uint4*>(vs + i * 4096 + tid * 16);
+        if (kb + k0 + i * (256 / CH) >= sp.pos && !finite16<H>(*x)) {
+          *x = only_finite<H>(*x);
+          odd[stage] = kb + 1;
+        }
+      }
+    }
+    lds_barrier();  // every wave's loads have landed, and the stage before this one has been read
+    load(kb + 2 * TK, stage == 0 ? 2 : stage - 1);
     if (kb < wend) {
       fl_f32x16 s[KT];
 #pragma unroll
@@ -499,67 +499,86 @@ __global__ __launch_bounds__(256, 2) void k_attn_many(AttnArgs a) {
         for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
 #pragma unroll
         for (int e = 0; e < ST; ++e)
-          s[kt] = mma<H>(*reinterpret_cast<const uint4*>(ks[buf] + k_at(kt * 32 + r, 2 * e + hf)), qf[e], s[kt]);
+          s[kt] = mma<H>(*reinterpret_cast<const uint4*>(ks + k_at(kt * 32 + r, 2 * e + hf)), qf[e], s[kt]);
       }
       if (kb + TK > wfull) hide<KT>(a, mask, sp.pos, kend, kb, t, s);
-      softmax_pv<H, D, KT>(s, st, a.sc, vs[buf]);
-      if (odd[buf] == kb + 1) add_not_finite<H, D>(a, mask, vp, sp.pos, kb, kend, TK, t, st);
+      softmax_pv<H, D, KT>(s, st, a.sc, vs);
+      if (odd[stage] == kb + 1) add_not_finite<H, D>(a, mask, vp, sp.pos, kb, kend, TK, t, st);
     }
-    if (more) store(buf ^ 1, kb + TK);
+    stage = stage == NS - 1 ? 0 : stage + 1;
   }
+  wait_loads<0>();  // what was loaded ahead has landed before the LDS is given away
   store_rows<H, D>(a, st, b, g, part, row, sp.keys < 0);
 }
 
-// The key parts of a row merged in order: a wave per row, lanes over dims
+// The key parts of a row (up to 64) merged: a wave per row, 16 bytes of a part's o a lane, 256 / D parts at a time
+// and four of those loads in flight; the lanes of a dim meet at the end in a fixed order.
 template <bool H, int D>
-__global__ __launch_bounds__(256) void k_attn_merge(AttnArgs a, int unit) {
+__global__ __launch_bounds__(256) void k_attn_merge(AttnArgs a) {
+  constexpr int LP = D / 4, PP = 64 / LP;  // lanes of a part, parts side by side
   const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)a.b * a.groups * a.R, w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= n) return;
-  const int row = (int)(w % a.R), g = (int)(w / a.R % a.groups), b = (int)(w / a.R / a.groups);
-  const Span sp = span_of(a, b, 0, unit);
-  const int parts = sp.keys < 0 ? 0 : (sp.keys + part_keys(sp.keys, a.parts, unit) - 1) / part_keys(sp.keys, a.parts, unit);
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), b = blockIdx.y / a.groups, g = blockIdx.y % a.groups;
+  if (row >= a.R) return;
+  const int64_t n = (int64_t)a.b * a.groups * a.R, w = (int64_t)blockIdx.y * a.R + row;
+  const Span sp = span_of(a, b, 0);
+  const int parts = sp.keys < 0 ? 0 : (sp.keys - 1) / a.kpp + 1;
   const float* ml = a.part + (int64_t)a.parts * n * D;
-  float mm = -INFINITY;
-  for (int p = 0; p < parts; ++p) mm = fmaxf(mm, ml[(p * n + w) * 2]);
-  const float mu = mm == -INFINITY ? 0.0f : mm;
-  float L = 0.0f, O[D / 64] = {};
-  for (int p = 0; p < parts; ++p) {
-    const float e = __builtin_amdgcn_exp2f(ml[(p * n + w) * 2] - mu);
-    L += ml[(p * n + w) * 2 + 1] * e;
+  float2 own = make_float2(-INFINITY, 0.0f);  // lane p: part p
+  if (lane < parts) own = *reinterpret_cast<const float2*>(ml + (lane * n + w) * 2);
+  const float mm = wave_max(own.x), mu = mm == -INFINITY ? 0.0f : mm;
+  const float e = __builtin_amdgcn_exp2f(own.x - mu);  // 0 behind the last part
+  const float L = wave_sum(e * own.y);
+  const int p0 = lane / LP, d0 = lane % LP * 4;
+  fl_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int p = p0; p - p0 < parts; p += 4 * PP) {
+    fl_f32x4 x[4];
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) O[i] += a.part[(p * n + w) * D + lane + 64 * i] * e;
+    for (int i = 0; i < 4; ++i)
+      x[i] = *reinterpret_cast<const fl_f32x4*>(a.part + (min(p + i * PP, parts - 1) * n + w) * D + d0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = __shfl(e, (p + i * PP) & 63, 64);
+      o += x[i] * (p + i * PP < parts ? f : 0.0f);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (LP == 16) o[i] = xor16_sum(o[i]);
+    o[i] = xor32_sum(o[i]);
   }
   const int64_t at = ((int64_t)b * a.m + row / a.rep) * a.heads + g * a.rep + row % a.rep;
   const float inv = sp.keys < 0 ? NAN : L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) a.out[at * D + lane + 64 * i] = (uint16_t)pack16<H>(O[i] * inv, 0.0f);
+  if (p0 == 0)
+    *reinterpret_cast<uint2*>(a.out + at * D + d0) = make_uint2(pack16<H>(o[0] * inv, o[1] * inv), pack16<H>(o[2] * inv, o[3] * inv));
   if (a.lse && lane == 0)
     a.lse[at] = sp.keys < 0 ? NAN : L == 0.0f ? -INFINITY : (mm + __builtin_amdgcn_logf(L)) * 0.6931471805599453f;
 }
 
 // ---- the weight that every key gathers ---------------------------------------------------------------------
-// w[key] (+)= sum over rows of exp2(s c - lse log2 e). A wave holds 64 keys of a key head in its MFMA operands and walks
-// over the rows, 32 at a time, sums in registers; lanes meet at the end. SPLIT: the four waves of a workgroup share 64
-// keys and take the row tiles in turn (many rows), else each has 64 keys of its own. One workgroup writes a key, in a
+// w[key] (+)= sum over rows of exp2(s c - lse log2 e). Here the scores are taken as S = Q K^T, so that a lane is a key
+// and registers are rows: the sum over rows stays in the lane. A wave holds 64 keys of a key head in its MFMA operands
+// and walks over the rows, 32 at a time, which come in whole cache lines, the next 32 in flight, and turn into the
+// operand layout in a piece of LDS that only this wave uses (loaded in that layout, 16 rows to an instruction's quarter,
+// they took 64 cycles an instruction: 512 tokens over 8704 keys 79 us). SPLIT: the four waves of a workgroup share
+// 64 keys and take the row tiles in turn (many rows), else each has 64 keys of its own. One workgroup writes a key, in a
 // fixed order: no atomics, the same bits every time.
 template <bool H, int D, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void k_attn_weights(AttnArgs a, float* __restrict__ w, int add) {
-  constexpr int KT = 2, ST = D / 16;
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_weights(AttnArgs a, float* __restrict__ w, int add) {
+  constexpr int KT = 2, ST = D / 16, CH = D / 8, RS = 64 / CH;  // RS: rows of a load of the wave
+  __shared__ __align__(16) unsigned char qs[4][32 * D * 2];
+  __shared__ __align__(16) float refs[4][32];
+  __shared__ __align__(16) int nodes[4][32];
   __shared__ float red[4][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hf = lane >> 5;
   const int g = blockIdx.x % a.groups, rest = blockIdx.x / a.groups;
   const int tiles = (a.slots + 63) / 64, per = SPLIT ? tiles : (tiles + 3) / 4;
-  const int b = rest / per, kb = (SPLIT ? rest % per : rest % per * 4 + wave) * 64;
-  int pos = a.pos ? a.pos[b] : a.pos0;
+  // the last slots first: the nodes' own tiles take longest
+  const int b = rest / per, kb = (SPLIT ? per - 1 - rest % per : (per - 1 - rest % per) * 4 + wave) * 64;
+  const int pos = a.pos ? __builtin_amdgcn_readfirstlane(a.pos[b]) : a.pos0;
   const bool bad = pos < 0 || pos > a.slots - a.m;
   const int keys = bad ? 0 : pos + a.m;
   const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.mask_b : nullptr;
-  float acc[KT][16];
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[kt][i] = 0.0f;
+  float acc[KT] = {0.0f, 0.0f};
   if (kb < keys) {
     const uint16_t* kp = a.k + (int64_t)b * a.k_b + (int64_t)g * a.k_g;
     const auto kr = tile_rsrc(kp, a.k_s, kb, keys, 64, D);
@@ -568,15 +587,51 @@ __global__ __launch_bounds__(256, 2) void k_attn_weights(AttnArgs a, float* __re
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int s = 0; s < ST; ++s) kf[kt][s] = buf_ld128(kr, (uint32_t)((kt * 32 + r) * a.k_s + hf * 8 + s * 16) * 2u);
+    const int step = SPLIT ? 4 : 1, tiles_r = (a.R + 31) / 32;
     // a chain's nodes before the tile's first key see none of it
-    const int first = mask ? 0 : max(0, kb - pos) * a.rep / 32;
-    const int step = SPLIT ? 4 : 1;
-    for (int rt = first + (SPLIT ? wave : 0); rt * 32 < a.R; rt += step) {
-      const int row = rt * 32 + r, rowc = min(row, a.R - 1), t = rowc / a.rep, head = g * a.rep + rowc % a.rep;
-      const uint16_t* qp = a.q + (int64_t)b * a.q_b + (int64_t)t * a.q_m + (int64_t)head * a.q_h;
-      const float lse = a.lse[((int64_t)b * a.m + t) * a.heads + head];
-      const bool none = row >= a.R || lse == -INFINITY;
-      const float ref = lse * 1.4426950408889634f;
+    int rt = (mask ? 0 : max(0, kb - pos) * a.rep / 32) + (SPLIT ? wave : 0);
+    // queries and lse of the group's first head; of the rows that this lane loads, (node, head of the group) and the
+    // offset, which move on by 32 step rows
+    const uint16_t* qg = a.q + (int64_t)b * a.q_b + (int64_t)(g * a.rep) * a.q_h;
+    const float* lg = a.lse + (int64_t)b * a.m * a.heads + g * a.rep;
+    const auto qr = buf_rsrc(qg, (uint32_t)((a.m - 1) * a.q_m + (a.rep - 1) * a.q_h + D) * 2u);
+    const int dn = 32 * step / a.rep, dj = 32 * step % a.rep;
+    const uint32_t qm = (uint32_t)a.q_m * 2u, qh = (uint32_t)a.q_h * 2u;
+    int rj[ST];
+    uint32_t ro[ST];
+#pragma unroll
+    for (int i = 0; i < ST; ++i) {
+      const int row = rt * 32 + lane / CH + i * RS;
+      rj[i] = row % a.rep;
+      ro[i] = (uint32_t)(row / a.rep) * qm + (uint32_t)rj[i] * qh + (uint32_t)(lane % CH) * 16u;
+    }
+    int ln = (rt * 32 + r) / a.rep, lj = (rt * 32 + r) % a.rep;  // of row r, whose lse this lane loads
+    uint4 qv[ST];
+    float lse;
+    int node;
+    auto load = [&] {
+#pragma unroll
+      for (int i = 0; i < ST; ++i) {
+        qv[i] = buf_ld128(qr, ro[i]);  // rows behind the last: zeros, or another head's, which add nothing
+        rj[i] += dj;
+        ro[i] += (uint32_t)dn * qm + (uint32_t)dj * qh;
+        if (rj[i] >= a.rep) rj[i] -= a.rep, ro[i] += qm - (uint32_t)a.rep * qh;
+      }
+      node = ln;
+      lse = ln < a.m ? lg[(int64_t)ln * a.heads + lj] : -INFINITY;
+      ln += dn, lj += dj;
+      if (lj >= a.rep) lj -= a.rep, ++ln;
+    };
+    unsigned char* mine = qs[wave];
+    auto q_at = [&](int row, int c) { return row * (2 * D) + (c ^ (D == 64 ? (row >> 1) & 7 : row & 15)) * 16; };
+    if (rt < tiles_r) load();
+    for (; rt < tiles_r; rt += step) {
+#pragma unroll
+      for (int i = 0; i < ST; ++i) *reinterpret_cast<uint4*>(mine + q_at(lane / CH + i * RS, lane % CH)) = qv[i];
+      // rows behind the last, and rows that see nothing, add nothing: e^-inf
+      if (hf == 0) refs[wave][r] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+      if (hf == 1) nodes[wave][r] = node;
+      if (rt + step < tiles_r) load();
       fl_f32x16 s[KT];
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
@@ -584,52 +639,62 @@ __global__ __launch_bounds__(256, 2) void k_attn_weights(AttnArgs a, float* __re
         for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
 #pragma unroll
       for (int e = 0; e < ST; ++e) {
-        const uint4 qf = *reinterpret_cast<const uint4*>(qp + e * 16 + hf * 8);
+        const uint4 qf = *reinterpret_cast<const uint4*>(mine + q_at(r, 2 * e + hf));
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) s[kt] = mma<H>(kf[kt][e], qf, s[kt]);
+        for (int kt = 0; kt < KT; ++kt) s[kt] = mma<H>(qf, kf[kt][e], s[kt]);
       }
-      if (kb + 64 > pos) {
-        hide<KT>(a, mask, pos, keys, kb, t, s);
+      // s[kt][i]: row 8 (i / 4) + 4 hf + i % 4 of the tile, key 32 kt + r
+      // all of the tile's keys are cached, or (a chain) no later than the rows' first node
+      if (kb + 64 <= pos || (!mask && kb + 63 - pos <= rt * 32 / a.rep)) {
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const fl_f32x4 ref = *reinterpret_cast<const fl_f32x4*>(&refs[wave][8 * q4 + 4 * hf]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], a.sc, -ref));
-            acc[kt][i] += none || s[kt][i] == -INFINITY ? 0.0f : p;
+          for (int kt = 0; kt < KT; ++kt) {
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][4 * q4 + i], a.sc, -ref[i]));
+            acc[kt] += (p[0] + p[1]) + (p[2] + p[3]);
           }
+        }
       } else {
+        const auto mr = buf_rsrc(mask, mask ? (uint32_t)a.m * (uint32_t)a.m : 0u);
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const fl_f32x4 ref = *reinterpret_cast<const fl_f32x4*>(&refs[wave][8 * q4 + 4 * hf]);
+          const int4 at = *reinterpret_cast<const int4*>(&nodes[wave][8 * q4 + 4 * hf]);
+          const int t[4] = {at.x, at.y, at.z, at.w};
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], a.sc, -ref));
-            acc[kt][i] += none ? 0.0f : p;
+          for (int kt = 0; kt < KT; ++kt) {
+            const int j = kb + 32 * kt + r - pos;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][4 * q4 + i], a.sc, -ref[i]));
+              const uint32_t off = j >= 0 && j < a.m && t[i] < a.m ? (uint32_t)t[i] * (uint32_t)a.m + (uint32_t)j : 0xFFFFFFF0u;
+              const bool sees = mask ? __builtin_amdgcn_raw_buffer_load_b8(mr, off, 0, 0) != 0 : j <= t[i];
+              // a key behind the end is a zero: no score of its own, and j <= t holds for no node
+              acc[kt] += j < 0 || (sees && j < a.m) ? p : 0.0f;
+            }
           }
+        }
       }
     }
   }
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float v = group_sum(acc[kt][i], 32);
-      if (r == 0) red[wave][32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3)] = v;
-    }
+  for (int kt = 0; kt < KT; ++kt) {
+    const float v = xor32_sum(acc[kt]);
+    if (hf == 0) red[wave][32 * kt + r] = v;
+  }
   __syncthreads();
   float* row = w + ((int64_t)b * a.groups + g) * a.slots;
-  if (SPLIT) {
-    if (tid < 64 && kb + tid < a.slots) {
-      const float v = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
-      if (bad) row[kb + tid] = NAN;
-      else if (!add) row[kb + tid] = v;
-      else if (kb + tid < keys) row[kb + tid] += v;
-    }
-  } else if (kb + lane < a.slots) {
-    const float v = red[wave][lane];
-    if (bad) row[kb + lane] = NAN;
-    else if (!add) row[kb + lane] = v;
-    else if (kb + lane < keys) row[kb + lane] += v;
-  }
+  auto put = [&](int slot, float v) {
+    if (slot >= a.slots) return;
+    if (bad) row[slot] = NAN;
+    else if (!add) row[slot] = v;
+    else if (slot < keys) row[slot] += v;
+  };
+  if (!SPLIT) put(kb + lane, red[wave][lane]);
+  else if (tid < 64) put(kb + tid, (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]));
 }
 
 // ---- host -------------------------------------------------------------------------------------------------
@@ -643,26 +708,33 @@ bool desc_ok(const fl_attn_desc* d) {
   const int64_t st[] = {d->q_b, d->q_m, d->q_h, d->k_b, d->k_g, d->k_s, d->v_b, d->v_g, d->v_s};
   for (int64_t x : st)
     if (x < 0 || x % 8 || x > (int64_t)1 << 40) return false;
-  // a tile of 64 slots within 32 bits
-  return d->k_s <= 1 << 23 && d->v_s <= 1 << 23 && d->mask_b >= 0;
+  // a tile of 64 slots, and a sequence's queries, within 32 bits
+  return d->k_s <= 1 << 23 && d->v_s <= 1 << 23 && d->mask_b >= 0 &&
+         (d->m - 1) * d->q_m + (d->heads - 1) * d->q_h + d->dim <= 1 << 30;
 }
 bool on16(const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 struct AttnPlan {
   bool few;
-  int blocks, parts, unit;
+  int blocks, parts, kpp;
   int64_t bytes;
 };
-// `keys`: of the longest sequence, as far as the host knows
+// `pos_known`: the host knows how many keys there are; else up to d.slots, and sequences of any length
 AttnPlan attn_plan(const fl_attn_desc& d, bool pos_known) {
   const int R = d.m * (d.heads / d.groups), keys = pos_known ? d.pos0 + d.m : d.slots;
   AttnPlan p{};
   p.few = R <= 64;
   p.blocks = p.few ? (R + 31) / 32 : (R + 127) / 128;
-  p.unit = p.few ? AT_NW * 4096 / d.dim : 64;
+  const int unit = p.few ? AT_NW * 4096 / d.dim : 64, least = p.few ? unit : 256;
   const int64_t base = (int64_t)d.b * d.groups * p.blocks;
-  const int least = p.few ? p.unit : 256;
-  p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({p.few ? 64 : 16, 512 / base, keys / least}));
+  // Workgroups that cutting the keys may reach. Few rows: one per CU, whose eight waves have 128 KB in flight (131072 keys
+  // 53 us, with two rounds of workgroups 60). Many rows: of the three (dim 64) or two that a CU holds, one and a third
+  // times as many as there are places (1024 tokens behind 4096: 640 116 us, 1024 104, 1600 112; 16 trees of 13 and
+  // 128 dims: 640 56, 1024 67).
+  const int64_t fill = p.few ? 256 : d.dim == 64 ? 1024 : 640;
+  const int most = (int)std::max<int64_t>(1, std::min<int64_t>({p.few ? 64 : 16, (fill + base - 1) / base, keys / least}));
+  p.kpp = (int)(((int64_t)(keys + most - 1) / most + unit - 1) / unit * unit);
+  p.parts = (keys - 1) / p.kpp + 1;
   const int64_t n = (int64_t)d.b * d.groups * R;
   p.bytes = p.parts == 1 ? 0 : p.parts * n * (d.dim + 2) * 4;
   return p;
@@ -673,7 +745,7 @@ AttnArgs attn_args(const fl_attn_desc& d, const uint16_t* q, const uint16_t* k, 
   a.q = q, a.k = k, a.v = v, a.pos = pos, a.mask = mask;
   a.b = d.b, a.m = d.m, a.heads = d.heads, a.groups = d.groups, a.rep = d.heads / d.groups, a.slots = d.slots;
   a.pos0 = d.pos0, a.R = d.m * a.rep;
-  a.blocks = a.parts = 1;
+  a.blocks = a.parts = 1, a.kpp = INT32_MAX;
   a.sc = d.scale * 1.4426950408889634f;
   a.q_b = d.q_b, a.q_m = d.q_m, a.q_h = d.q_h, a.k_b = d.k_b, a.k_g = d.k_g, a.k_s = d.k_s;
   a.v_b = d.v_b, a.v_g = d.v_g, a.v_s = d.v_s, a.mask_b = d.mask_b;
@@ -688,8 +760,7 @@ int attn_launch(AttnArgs a, const AttnPlan& p, hipStream_t s) {
   if (!p.few) hipLaunchKernelGGL((k_attn_many<H, D>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((k_attn_few<H, D, AT_NW>), grid, dim3(64 * AT_NW), 0, s, a);
   if (p.parts > 1) {
-    const int64_t n = (int64_t)a.b * a.groups * a.R;
-    hipLaunchKernelGGL((k_attn_merge<H, D>), dim3((uint32_t)((n + 3) / 4)), dim3(256), 0, s, a, p.unit);
+    hipLaunchKernelGGL((k_attn_merge<H, D>), dim3((a.R + 3) / 4, a.b * a.groups), dim3(256), 0, s, a);
   }
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;
 }
@@ -722,7 +793,7 @@ int fl_tree_attention(const fl_attn_desc* d, const uint16_t* q, const uint16_t* 
   const AttnPlan p = attn_plan(*d, pos == nullptr);
   if (p.bytes && !on16(work)) return FL_E_ARG;
   AttnArgs a = attn_args(*d, q, k, v, pos, mask);
-  a.out = out, a.lse = lse, a.part = static_cast<float*>(work), a.blocks = p.blocks, a.parts = p.parts;
+  a.out = out, a.lse = lse, a.part = static_cast<float*>(work), a.blocks = p.blocks, a.parts = p.parts, a.kpp = p.kpp;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (d->dim == 64) return d->fp16 ? attn_launch<true, 64>(a, p, s) : attn_launch<false, 64>(a, p, s);
   return d->fp16 ? attn_launch<true, 128>(a, p, s) : attn_launch<false, 128>(a, p, s);

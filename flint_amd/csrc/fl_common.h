@@ -369,6 +369,26 @@ __device__ __forceinline__ uint2 buf_ld64_coh(__amdgpu_buffer_rsrc_t r, uint32_t
   return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 16));
 }
 
+// ---- memory straight into LDS -------------------------------------------------------------------
+typedef uint32_t fl_u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+// buf_rsrc's four words
+__device__ __forceinline__ fl_u32x4 buffer_words(const void* base, uint32_t bytes) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(base);
+  return fl_u32x4{(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, bytes, 0x00020000u};
+}
+// 64 lanes x 16 bytes from the buffer at voff + soff into LDS from `at` on, in lane order (past the range: zeros). In
+// asm: the builtin's LDS write would make the compiler wait for every load in flight before it reads any LDS. No
+// register waits for it.
+__device__ __forceinline__ void dma_1k(fl_u32x4 rsrc, uint32_t at, uint32_t voff, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :: "s"(at), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // until at most N of this wave's loads are in flight
+  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+
 // Workgroup barrier that orders LDS accesses only. __syncthreads also waits for every global
 // load and store the wave has in flight (prefetched weights, published activations); this one
 // does not, so a barrier between LDS producers and consumers never stalls on HBM traffic.

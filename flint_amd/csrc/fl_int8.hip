@@ -16,7 +16,6 @@
 namespace {
 
 typedef int i8_x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t i8_u32x4 __attribute__((ext_vector_type(4)));
 
 // ---- quantisation -------------------------------------------------------------------------------
 
@@ -110,24 +109,6 @@ __global__ __launch_bounds__(Q8_NT) void k_quantize_i8(const uint16_t* __restric
 }
 
 // ---- the product ----------------------------------------------------------------------------------
-
-typedef __attribute__((address_space(3))) unsigned char lds_byte;
-
-// buf_rsrc's four words
-__device__ __forceinline__ i8_u32x4 buffer_words(const void* base, uint32_t bytes) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(base);
-  return i8_u32x4{(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, bytes, 0x00020000u};
-}
-// 64 lanes x 16 bytes from the buffer at voff + soff into LDS from `at` on, in lane order. In asm: the builtin's LDS
-// write would make the compiler wait for every load in flight before it reads any LDS. No register waits for it.
-__device__ __forceinline__ void dma_1k(i8_u32x4 rsrc, uint32_t at, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :: "s"(at), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void wait_loads() {  // until at most N of this wave's loads are in flight
-  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
-}
 
 template <bool F32>
 __device__ __forceinline__ void i8_store(void* y, int64_t at, int acc, float s) {
@@ -231,7 +212,7 @@ __global__ __launch_bounds__(64 * FEW_KW, 4) void k_i8_few(I8Few a) {
   };
   if constexpr (XKB > 0 && !QUANT) {  // a row per wave; beyond k of the last step: what LDS holds, times zeros
     const uint32_t at = (uint32_t)(uintptr_t)(lds_byte*)xl;
-    const i8_u32x4 xv = buffer_words(a.x, (uint32_t)m * (uint32_t)k);
+    const fl_u32x4 xv = buffer_words(a.x, (uint32_t)m * (uint32_t)k);
     for (int i = wave; i < m; i += KW)
       for (int p = 0; p < k; p += 1024)
         if (p + lane * 16 < k) dma_1k(xv, at + (uint32_t)(i * pitch + p), (uint32_t)(lane * 16), (uint32_t)(i * k + p));
@@ -406,8 +387,8 @@ __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k
   const int p0 = split * a.sps, p1 = min(steps, p0 + a.sps), per = (p1 - p0 + KW - 1) / KW;
   const int s0 = p0 + way * per, s1 = min(p1, s0 + per);
   const int rows_n = min(T, a.n - n0), rows_m = min(T, a.m - m0);
-  const i8_u32x4 wv = buffer_words(a.wq + (int64_t)n0 * a.k, (uint32_t)rows_n * (uint32_t)a.k);
-  const i8_u32x4 xv = buffer_words(a.xq + (int64_t)m0 * a.k, (uint32_t)rows_m * (uint32_t)a.k);
+  const fl_u32x4 wv = buffer_words(a.wq + (int64_t)n0 * a.k, (uint32_t)rows_n * (uint32_t)a.k);
+  const fl_u32x4 xv = buffer_words(a.xq + (int64_t)m0 * a.k, (uint32_t)rows_m * (uint32_t)a.k);
   // this lane's piece of the wave's loads of a unit; the buffers' range check makes rows past the end zeros
   auto piece = [&](int i) { return (lane & 7) ^ (((wave * PER + i) & 1) * 4 + (lane >> 4)); };
   uint32_t off[PER];
@@ -422,7 +403,7 @@ __global__ __launch_bounds__(64 * KW * WM * WN, KW * WM * WN > 4 ? 2 : 1) void k
     const int s = s0 + (u >> 1);
     if (s >= s1) return;
     const bool cut = s == steps - 1 && tail != 0;  // pieces past the end of a row are zeros too
-    const i8_u32x4 v = u & 1 ? xv : wv;
+    const fl_u32x4 v = u & 1 ? xv : wv;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       dma_1k(v, base + (uint32_t)(slot * UNIT + i * 1024), cut && piece(i) * 16 >= tail ? 0x80000000u : off[i],
