@@ -7,11 +7,12 @@
 // C. Without draft probabilities (q all at the token) w is p without the rejected tokens. Child t is accepted where u
 // q(t) Z < w(t). All of it in 64 bits: sums of 49152 values in another order than the caller's own must not move a
 // token across a border.
+#include <type_traits>
 #include "fl_common.h"
 
 namespace {
 
-constexpr int AC_NT = 1024, AC_NW = AC_NT / FL_WAVE, AC_M = 1024, AC_U = 16;
+constexpr int AC_NT = 1024, AC_NW = AC_NT / FL_WAVE, AC_M = 1024;
 
 struct AcceptArgs {
   const void *p, *q;              // [B][M][V] and [B][M - 1][V] (or null), fp32 or bf16
@@ -53,7 +54,7 @@ __device__ __forceinline__ double wave_dsum(double v) {
 }
 __device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
 
-// One workgroup per tree; its waves sum pieces of a row, AC_U loads of a lane in flight, for the rejections that need Z
+// One workgroup per tree; its waves sum pieces of a row for the rejections that need Z
 // and for the last token. One CU reads a row of 49152 fp32 values and its draft row in 2.6 us at its 64 bytes a cycle,
 // about what one exchange between workgroups costs, so a row stays with one. (Held in registers between two sums, the
 // row's 96 values a lane and their conversions spilled.)
@@ -77,39 +78,41 @@ __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
     const double w = DRAFT ? __builtin_fma(-C, (double)q, (double)p) : (double)p;
     return w > 0.0 ? w : 0.0;
   };
-  // this wave's sum of w over [s0, s1)
-  auto piece = [&](int s0, int s1) -> double {
+  // This wave's sum of w over [s0, s1), U loads of a lane and row in flight. Loads past the end cost as much as others, so
+  // U is what a piece needs; the next U in flight behind the sums cost more than they gave (48 trees 23 us a call, 21).
+  auto piece = [&](auto unroll, int s0, int s1) -> double {
+    constexpr int U = decltype(unroll)::value;
     double s[4] = {};
-    for (int i0 = s0; i0 < s1; i0 += 64 * AC_U) {
-      float p[AC_U], q[DRAFT ? AC_U : 1];
+    for (int i0 = s0; i0 < s1; i0 += 64 * U) {
+      float p[U], q[U];
 #pragma unroll
-      for (int j = 0; j < AC_U; ++j) {
+      for (int j = 0; j < U; ++j) {
         const int i = i0 + 64 * j + lane;
         p[j] = row_ld<BF>(pr, i < s1 ? (uint32_t)i : 0x3FFFFFFFu);
-        if (DRAFT) q[j] = row_ld<BF>(qr, i < s1 ? (uint32_t)i : 0x3FFFFFFFu);
+        q[j] = DRAFT ? row_ld<BF>(qr, i < s1 ? (uint32_t)i : 0x3FFFFFFFu) : 0.0f;
       }
       if (!DRAFT)
         for (int k = 0; k < ngone; ++k) {
           const int d = gone[k] - i0 - lane;
 #pragma unroll
-          for (int j = 0; j < AC_U; ++j) p[j] = d == 64 * j ? 0.0f : p[j];
+          for (int j = 0; j < U; ++j) p[j] = d == 64 * j ? 0.0f : p[j];
         }
 #pragma unroll
-      for (int j = 0; j < AC_U; ++j) s[j & 3] += cut(p[j], DRAFT ? q[j] : 0.0f);
+      for (int j = 0; j < U; ++j) s[j & 3] += cut(p[j], q[j]);
     }
     return wave_dsum((s[0] + s[1]) + (s[2] + s[3]));
   };
   // all waves' sums of their pieces of [g0, g1) to red[turn]
-  auto pieces = [&](int g0, int g1, int len) {
+  auto pieces = [&](auto unroll, int g0, int g1, int len) {
     turn ^= 1;
     const int s0 = min(g1, g0 + wave * len);
-    const double s = piece(s0, min(g1, s0 + len));
+    const double s = piece(unroll, s0, min(g1, s0 + len));
     if (lane == 0) red[turn][wave] = s;
     __syncthreads();
   };
   auto total = [&]() -> double {
     open();
-    pieces(0, V, seg);
+    pieces(std::integral_constant<int, 16>{}, 0, V, seg);
     double s = 0.0;
 #pragma unroll
     for (int i = 0; i < AC_NW; ++i) s += red[turn][i];
@@ -188,7 +191,8 @@ __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
   }
   int result = -1;
   if (sum > 0.0 && sum < INFINITY) {
-    // the first index at which the running sum passes `want`: the wave's piece, then pieces of that until a few are left
+    // the first index at which the running sum passes `want`: the wave's piece, pieces of that until 256 values are left,
+    // then four in a row a lane
     const double want = (double)a.us[b] * sum;
     double before = 0.0;
     int g0 = 0, g1 = V, len = seg;
@@ -208,27 +212,37 @@ __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
       g1 = min(g1, g0 + len);
       if (g1 - g0 <= 256) break;
       len = ((g1 - g0 + AC_NW - 1) / AC_NW + 63) / 64 * 64;
-      pieces(g0, g1, len);
+      pieces(std::integral_constant<int, 4>{}, g0, g1, len);
     }
-    int tail = -1;
-    for (int i0 = g0; i0 < g1 && result < 0; i0 += 64) {
-      const int i = i0 + lane;
-      double w = i < g1 ? cut(row_ld<BF>(pr, i), DRAFT ? row_ld<BF>(qr, i) : 0.0f) : 0.0;
+    double w[4], own = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = g0 + 4 * lane + j;
+      w[j] = i < g1 ? cut(row_ld<BF>(pr, i), DRAFT ? row_ld<BF>(qr, i) : 0.0f) : 0.0;
       if (!DRAFT)
         for (int k = 0; k < ngone; ++k)
-          if (gone[k] == i) w = 0.0;
-      double inc = w;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double x = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += x;
-      }
-      const unsigned long long hit = __ballot(w > 0.0 && before + inc > want), any = __ballot(w > 0.0);
-      if (hit) result = i0 + __ffsll(hit) - 1;
-      if (any) tail = i0 + 63 - __clzll((long long)any);
-      before += __shfl(inc, 63, 64);
+          if (gone[k] == i) w[j] = 0.0;
+      own += w[j];
     }
-    if (result < 0) result = tail;
+    double inc = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double x = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += x;
+    }
+    const unsigned long long hit = __ballot(own > 0.0 && before + inc > want), any = __ballot(own > 0.0);
+    if (any) {  // none: a piece whose sum was its last bits
+      const int l = hit ? __ffsll(hit) - 1 : 63 - __clzll((long long)any);
+      double run = before + (inc - own);
+      int mine = -1;
+      bool done = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        run += w[j];
+        if (!done && w[j] > 0.0) mine = g0 + 4 * lane + j, done = run > want;
+      }
+      result = __builtin_amdgcn_readlane(mine, l);
+    }
   }
   if (tid == 0) a.token[b] = result, a.count[b] = n;
 }

@@ -19,17 +19,19 @@ struct EvictArgs {
 
 constexpr int ES_NT = 1024, ES_NW = ES_NT / FL_WAVE;
 
-// ordered key of a weight: larger weight <-> larger key, a NaN above all, -0 as 0
+// ordered key of a weight: larger weight <-> larger key, a NaN above all, -0 as 0. Keys 0 (no slot) and 2^32 - 1 (a
+// slot that always stays) are free.
 __device__ __forceinline__ uint32_t w_key(float w) {
-  if (w != w) return 0xFFFFFFFFu;
+  if (w != w) return 0xFFFFFFFEu;
   const uint32_t b = __float_as_uint(w + 0.0f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// One workgroup per head. The `want` largest of the slots between sink and recent by a radix select over the 32-bit
-// keys (four counts of 256 bins), ties to the lower slot; then the kept slots in order: each wave has a contiguous
-// piece of the slots, counts and then places by ballots. A lane holds its E keys in registers (8192 slots of 320 heads:
-// 24 us with six reads of the weights instead); E = 0: more slots, read again for every count, eight loads in flight.
+// One workgroup per head. The `keep` largest keys by a radix select over 32 bits (four counts of 256 bins), ties to the
+// lower slot, the first `sink` and the last `recent` slots above all others; then the kept slots in order: each wave has
+// a contiguous piece of the slots, counts and then places by ballots. A lane holds its E keys in registers. Bound by
+// the instructions of a key, some 50 over the six walks (8192 slots of 320 heads on 256 CUs: 24 us with the slots'
+// cases told apart in every walk); E = 0: more slots, read again for every walk, eight loads in flight.
 template <int E>
 __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
   __shared__ int hist[ES_NW][256];
@@ -37,68 +39,62 @@ __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.x;
   const float* w = a.w + (int64_t)head * a.slots;
   int32_t* kept = a.kept + (int64_t)head * a.keep;
-  const int lo = a.sink, hi = a.n - a.recent, want = a.keep - a.sink - a.recent;  // 0 <= want <= hi - lo
   const int piece = ((a.n + ES_NW - 1) / ES_NW + 63) / 64 * 64, p0 = min(a.n, wave * piece), p1 = min(a.n, p0 + piece);
+  auto key_of = [&](int i, float x) -> uint32_t {
+    return i >= p1 ? 0u : i < a.sink || i >= a.n - a.recent ? 0xFFFFFFFFu : w_key(x);
+  };
   uint32_t held[E ? E : 1];
   if constexpr (E > 0) {
+    float x[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = p0 + e * 64 + lane;
-      held[e] = i < p1 ? w_key(w[i]) : 0u;
-    }
+    for (int e = 0; e < E; ++e) x[e] = p0 + e * 64 + lane < p1 ? w[p0 + e * 64 + lane] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) held[e] = key_of(p0 + e * 64 + lane, x[e]);
   }
-  // f(slot, key, within): every lane of the wave, for every slot of its piece, in order
+  // f(slot, key): every lane of the wave, for every slot of its piece, in order
   auto walk = [&](auto f) {
     if constexpr (E > 0) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int i = p0 + e * 64 + lane;
-        f(i, held[e], i < p1);
-      }
+      for (int e = 0; e < E; ++e) f(p0 + e * 64 + lane, held[e]);
     } else {
       for (int i0 = p0; i0 < p1; i0 += 512) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int i = i0 + e * 64 + lane;
-          x[e] = i < p1 ? w[i] : 0.0f;
-        }
+        for (int e = 0; e < 8; ++e) x[e] = i0 + e * 64 + lane < p1 ? w[i0 + e * 64 + lane] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f(i0 + e * 64 + lane, w_key(x[e]), i0 + e * 64 + lane < p1);
+        for (int e = 0; e < 8; ++e) f(i0 + e * 64 + lane, key_of(i0 + e * 64 + lane, x[e]));
       }
     }
   };
   uint32_t prefix = 0;
-  int need = want;  // of those with the prefix so far
-  if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
+  int need = a.keep;  // of those with the prefix so far (no slot's key 0 lies below all: never reached)
+  for (int shift = 24; shift >= 0; shift -= 8) {
 #pragma unroll
-      for (int i = 0; i < ES_NW * 256 / ES_NT; ++i) (&hist[0][0])[i * ES_NT + tid] = 0;
-      __syncthreads();
-      walk([&](int i, uint32_t key, bool in) {
-        if (in && i >= lo && i < hi && (shift == 24 || (key >> (shift + 8)) == prefix))
-          atomicAdd(&hist[wave][(key >> shift) & 255], 1);
+    for (int i = 0; i < ES_NW * 256 / ES_NT; ++i) (&hist[0][0])[i * ES_NT + tid] = 0;
+    __syncthreads();
+    if (shift == 24)
+      walk([&](int, uint32_t key) { atomicAdd(&hist[wave][key >> 24], 1); });
+    else
+      walk([&](int, uint32_t key) {
+        if ((key >> (shift + 8)) == prefix) atomicAdd(&hist[wave][(key >> shift) & 255], 1);
       });
-      __syncthreads();
-      if (tid < 256) {
-        int n = 0;
+    __syncthreads();
+    if (tid < 256) {
+      int n = 0;
 #pragma unroll
-        for (int i = 0; i < ES_NW; ++i) n += hist[i][tid];
-        sum[tid] = n;
-      }
-      __syncthreads();
-      int above = 0;
-      const int bin = select_bin(sum, need, &above, sel);
-      prefix = (prefix << 8) | (uint32_t)bin;
-      need -= above;
+      for (int i = 0; i < ES_NW; ++i) n += hist[i][tid];
+      sum[tid] = n;
     }
+    __syncthreads();
+    int above = 0;
+    const int bin = select_bin(sum, need, &above, sel);
+    prefix = (prefix << 8) | (uint32_t)bin;
+    need -= above;
   }
-  // want = 0: nothing between sink and recent stays
   int above = 0, equal = 0;
-  walk([&](int i, uint32_t key, bool in) {
-    const bool mid = in && i >= lo && i < hi && want > 0;
-    above += __popcll(__ballot(mid ? key > prefix : in && (i < lo || i >= hi)));
-    equal += __popcll(__ballot(mid && key == prefix));
+  walk([&](int, uint32_t key) {
+    above += __popcll(__ballot(key > prefix));
+    equal += __popcll(__ballot(key == prefix));
   });
   if (lane == 0) above_w[wave] = above, equal_w[wave] = equal;
   __syncthreads();
@@ -108,12 +104,10 @@ __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
     eq += equal_w[i];
   }
   const unsigned long long below = (1ull << lane) - 1;
-  walk([&](int i, uint32_t key, bool in) {
-    const bool mid = in && i >= lo && i < hi && want > 0;
-    const unsigned long long e = __ballot(mid && key == prefix);
-    const bool stays = mid ? key > prefix || (key == prefix && eq + __popcll(e & below) < need) : in && (i < lo || i >= hi);
-    const unsigned long long s = __ballot(stays);
-    if (stays) kept[at + __popcll(s & below)] = i;
+  walk([&](int i, uint32_t key) {
+    const unsigned long long e = __ballot(key == prefix);
+    const unsigned long long s = __ballot(key > prefix || (key == prefix && eq + __popcll(e & below) < need));
+    if ((s >> lane) & 1) kept[at + __popcll(s & below)] = i;
     at += __popcll(s);
     eq += __popcll(e);
   });
@@ -211,6 +205,7 @@ int fl_evict(const fl_rows* k, const fl_rows* v, float* weights, int32_t n_outer
   const int per = ((n + ES_NW - 1) / ES_NW + 63) / 64;  // slots of a lane
   if (per <= 2) hipLaunchKernelGGL(k_evict_select<2>, dim3(heads), dim3(ES_NT), 0, s, a);
   else if (per <= 8) hipLaunchKernelGGL(k_evict_select<8>, dim3(heads), dim3(ES_NT), 0, s, a);
+  else if (per <= 16) hipLaunchKernelGGL(k_evict_select<16>, dim3(heads), dim3(ES_NT), 0, s, a);
   else if (per <= 32) hipLaunchKernelGGL(k_evict_select<32>, dim3(heads), dim3(ES_NT), 0, s, a);
   else hipLaunchKernelGGL(k_evict_select<0>, dim3(heads), dim3(ES_NT), 0, s, a);
   if (k_out) {
