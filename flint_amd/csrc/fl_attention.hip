@@ -523,23 +523,30 @@ __global__ __launch_bounds__(256) void k_attn_merge(AttnArgs a) {
   const Span sp = span_of(a, b, 0);
   const int parts = sp.keys < 0 ? 0 : (sp.keys - 1) / a.kpp + 1;
   const float* ml = a.part + (int64_t)a.parts * n * D;
+  const int p0 = lane / LP, d0 = lane % LP * 4;
+  // four groups of PP parts at a time; a group with no part in it is not loaded (uniform), a lane with none reads the last
+  fl_f32x4 x[4];
+  auto load = [&](int g0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (g0 + i * PP < parts)
+        x[i] = *reinterpret_cast<const fl_f32x4*>(a.part + (min(g0 + i * PP + p0, parts - 1) * n + w) * D + d0);
+  };
+  load(0);
   float2 own = make_float2(-INFINITY, 0.0f);  // lane p: part p
   if (lane < parts) own = *reinterpret_cast<const float2*>(ml + (lane * n + w) * 2);
   const float mm = wave_max(own.x), mu = mm == -INFINITY ? 0.0f : mm;
   const float e = __builtin_amdgcn_exp2f(own.x - mu);  // 0 behind the last part
   const float L = wave_sum(e * own.y);
-  const int p0 = lane / LP, d0 = lane % LP * 4;
   fl_f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int p = p0; p - p0 < parts; p += 4 * PP) {
-    fl_f32x4 x[4];
+  for (int g0 = 0; g0 < parts; g0 += 4 * PP) {
+    if (g0) load(g0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      x[i] = *reinterpret_cast<const fl_f32x4*>(a.part + (min(p + i * PP, parts - 1) * n + w) * D + d0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float f = __shfl(e, (p + i * PP) & 63, 64);
-      o += x[i] * (p + i * PP < parts ? f : 0.0f);
-    }
+      if (g0 + i * PP < parts) {
+        const float f = __shfl(e, (g0 + i * PP + p0) & 63, 64);
+        o += x[i] * (g0 + i * PP + p0 < parts ? f : 0.0f);
+      }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -723,16 +730,25 @@ struct AttnPlan {
 AttnPlan attn_plan(const fl_attn_desc& d, bool pos_known) {
   const int R = d.m * (d.heads / d.groups), keys = pos_known ? d.pos0 + d.m : d.slots;
   AttnPlan p{};
-  p.few = R <= 64;
+  // Few rows: a wave's own keys need no barrier but meet in LDS at the end, which pays where one launch does (up to three
+  // tiles a wave) and where memory is the bound; in between the shared ring's kernel starts and ends sooner. us, one
+  // token, few / many: 1000 keys 10.9 / 11.6, 2000 13.5 / 10.7, 8000 13.5 / 11.8, 131072 44 / 67; 24 sequences of 3000
+  // 34 / 40, 8 trees of 8 behind 2000 16.7 / 17.5; 40 rows behind 4000 14.9 / 11.6, behind 30000 20.7 / 24.8.
+  const int few_unit = AT_NW * 4096 / d.dim;
+  p.few = R <= 64 && (keys <= 3 * few_unit || (int64_t)d.b * d.groups * keys * d.dim >= 6 << 20);
   p.blocks = p.few ? (R + 31) / 32 : (R + 127) / 128;
-  const int unit = p.few ? AT_NW * 4096 / d.dim : 64, least = p.few ? unit : 256;
+  const int unit = p.few ? few_unit : 64, least = p.few ? unit : 256;
   const int64_t base = (int64_t)d.b * d.groups * p.blocks;
   // Workgroups that cutting the keys may reach. Few rows: one per CU, whose eight waves have 128 KB in flight (131072 keys
   // 53 us, with two rounds of workgroups 60). Many rows: of the three (dim 64) or two that a CU holds, one and a third
   // times as many as there are places (1024 tokens behind 4096: 640 116 us, 1024 104, 1600 112; 16 trees of 13 and
   // 128 dims: 640 56, 1024 67).
   const int64_t fill = p.few ? 256 : d.dim == 64 ? 1024 : 640;
-  const int most = (int)std::max<int64_t>(1, std::min<int64_t>({p.few ? 64 : 16, (fill + base - 1) / base, keys / least}));
+  // a wave of few rows takes three tiles in less than the launch that joins parts costs (1032 keys: 11.6 uncut, 13.5 in
+  // two parts; 2000: 16.0 and 13.5)
+  const int most = p.few && keys <= 3 * unit
+                       ? 1
+                       : (int)std::max<int64_t>(1, std::min<int64_t>({64, (fill + base - 1) / base, keys / least}));
   p.kpp = (int)(((int64_t)(keys + most - 1) / most + unit - 1) / unit * unit);
   p.parts = (keys - 1) / p.kpp + 1;
   const int64_t n = (int64_t)d.b * d.groups * R;
