@@ -50,7 +50,7 @@ def _describe(q, k, v, pos, mask, scale):
     _check(dim in (64, 128), "heads of 64 or 128 dimensions")
     _check(b >= 1 and m >= 1 and groups >= 1 and heads >= 1 and heads % groups == 0,
            "one sequence, node and head at least, and as many query heads for each key head")
-    _check(m <= slots, "more nodes than slots")
+    _check(m <= slots <= 1 << 30, "at least as many slots as nodes, at most 2^30")
     _check(b <= 65536 and m <= 32768 and heads <= 4096 and m * (heads // groups) <= 1 << 24,
            "at most 65536 sequences, 32768 nodes, 4096 heads and 2^24 rows of a key head")
     scale = dim ** -0.5 if scale is None else float(scale)
@@ -97,7 +97,7 @@ def tree_attention(q, k_cache, v_cache, pos, mask=None, scale=None, return_lse=F
     if _tree_attention_fast is not None and q.is_cuda:
         at, p0 = (None, pos) if type(pos) is int else (pos, 0)
         if at is None or type(at) is torch.Tensor:
-            r = _tree_attention_fast(q, k_cache, v_cache, at, p0, mask, q.shape[-1] ** -0.5 if scale is None else scale,
+            r = _tree_attention_fast(q, k_cache, v_cache, at, p0, mask, q.shape[-1] ** -0.5 if scale is None else float(scale),
                                      return_lse, torch._C._cuda_getCurrentRawStream(q.get_device()))
             if r is not None:
                 return r if return_lse else r[0]
@@ -126,7 +126,7 @@ def attention_weights(q, k_cache, lse, pos, mask=None, scale=None, out=None):
     if _attention_weights_fast is not None and out is None and q.is_cuda:
         at, p0 = (None, pos) if type(pos) is int else (pos, 0)
         if at is None or type(at) is torch.Tensor:
-            r = _attention_weights_fast(q, k_cache, lse, at, p0, mask, q.shape[-1] ** -0.5 if scale is None else scale,
+            r = _attention_weights_fast(q, k_cache, lse, at, p0, mask, q.shape[-1] ** -0.5 if scale is None else float(scale),
                                         torch._C._cuda_getCurrentRawStream(q.get_device()))
             if r is not None:
                 return r

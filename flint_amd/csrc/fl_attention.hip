@@ -708,7 +708,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_weights(AttnArgs 
 constexpr int AT_NW = 8;  // waves of k_attn_few
 
 bool desc_ok(const fl_attn_desc* d) {
-  if (!d || d->b < 1 || d->m < 1 || d->heads < 1 || d->groups < 1 || d->slots < 1) return false;
+  if (!d || d->b < 1 || d->m < 1 || d->heads < 1 || d->groups < 1 || d->slots < 1 || d->slots > 1 << 30) return false;
   if (d->heads % d->groups || (d->dim != 64 && d->dim != 128) || d->m > d->slots) return false;
   if (d->b > 65536 || d->m > 32768 || d->heads > 4096 || (int64_t)d->m * (d->heads / d->groups) > (1 << 24)) return false;
   if (!(d->scale > 0.0f) || d->scale > 3.0e38f) return false;

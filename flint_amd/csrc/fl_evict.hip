@@ -167,7 +167,7 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + u * rows + r;
-      if (r < rows && j < a.keep) x[u] = *reinterpret_cast<const uint4*>(base + (int64_t)kept[j] * stride + c);
+      x[u] = r < rows && j < a.keep ? *reinterpret_cast<const uint4*>(base + (int64_t)kept[j] * stride + c) : make_uint4(0u, 0u, 0u, 0u);
     }
     __syncthreads();
 #pragma unroll

@@ -359,6 +359,8 @@ class SpecDecoder:
         model, nv = self.model, self._nodes
         T = len(ids)
         max_seq = T + int(max_new) + nv
+        if self.head is not None:  # room for the widest tree, as far as there are positions
+            max_seq = max(T + int(max_new) + _lib.MAX_VERIFY, min(max_seq, model.packed.rope.shape[0] // 8 * 8))
         model.setup_caches(1, max_seq)
         feats = torch.empty(max_seq, model.config.dim, dtype=torch.bfloat16, device=model.device)
         stats = SpecStats()

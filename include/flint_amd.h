@@ -190,7 +190,7 @@ int fl_head_logprobs(const uint16_t* x, const int8_t* wq, const float* ws, const
 /* b sequences of m nodes each (a drafted tree, a chain, a prompt, or one token), `heads` query heads over `groups` key
  * heads of dim 64 or 128, caches of `slots` slots; bf16, or fp16 where fp16 != 0. Strides count values, between
  * sequences, nodes / key heads and query heads / slots; the last dimension is contiguous. Strides are multiples of 8,
- * pointers 16-byte aligned, k_s and v_s at most 2^23, a sequence's queries within 2^30 values, m at most 32768. mask_b: bytes between the sequences' masks (0: one for all).
+ * pointers 16-byte aligned, k_s and v_s at most 2^23, a sequence's queries within 2^30 values, m at most 32768, slots at most 2^30. mask_b: bytes between the sequences' masks (0: one for all).
  * scale: positive. pos0: cached keys of every sequence, for calls without `pos`. */
 typedef struct fl_attn_desc {
   int32_t b, m, heads, groups, dim, slots, fp16, pos0;

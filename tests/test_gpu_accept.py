@@ -142,3 +142,40 @@ def test_refusals(dev):
                dict(draft_probs=q.bfloat16()), dict(draft_probs=p), dict(probs=torch.zeros(1, 1025, 4, device=dev)), dict(probs=p[..., :0])):
         with pytest.raises(ValueError):
             accept_sampled(**{**ok, **kw})
+
+
+def test_captured_and_replayed(dev):
+    from flint_amd.spec import accept_sampled
+    ins = [[x.to(dev) for x in make(5, 9, 700, seed)] for seed in range(3)]
+    held = [x.clone() for x in ins[0]]
+
+    def call(x):
+        return accept_sampled(x[0], x[2], x[4], x[5], x[3], x[1])
+    want = [[y.clone() for y in call(x)] for x in ins]
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        got = call(held)
+    for i in (0, 1, 2, 0, 2):
+        for h, x in zip(held, ins[i]):
+            h.copy_(x)
+        gr.replay()
+        call(ins[(i + 1) % 3])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+
+
+@pytest.mark.parametrize("v", [15, 16, 17, 1023, 1024, 1025, 16384, 16385, 262145])
+@pytest.mark.parametrize("where", ["first", "last", "seam"])
+def test_weight_in_one_place(dev, v, where):
+    """All of a row's weight in one or two indices, at the seams of the waves' pieces: the last token is one of them."""
+    from flint_amd.spec import accept_sampled
+    seg = -(-(-(-v // 16)) // 64) * 64
+    at = {"first": 0, "last": v - 1, "seam": min(v - 1, seg)}[where]
+    other = max(0, at - 1)
+    p = torch.zeros(3, 1, v, device=dev)
+    p[:, 0, at] = 0.5
+    p[1, 0, other] += 0.25
+    us = torch.tensor([0.999, 0.0, 0.999], device=dev)
+    got = accept_sampled(p, torch.zeros(3, 1, dtype=torch.int32, device=dev), torch.zeros(3, 1, device=dev), us)
+    assert got.token.tolist() == [at, other, at] and got.count.tolist() == [1, 1, 1]

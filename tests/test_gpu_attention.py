@@ -263,3 +263,79 @@ def test_refusals(dev):
                dict(out=torch.zeros(2, 2, 40, device=dev)[..., ::2])):
         with pytest.raises(ValueError):
             attention_weights(**{**dict(q=q, k_cache=k, lse=lse, pos=5), **kw})
+
+
+@pytest.mark.parametrize("b,m,ctx,dim", [(1, 1, 300, 64), (1, 8, 3000, 64), (3, 40, 700, 128), (2, 1, 9000, 64)])
+def test_captured_and_replayed(dev, b, m, ctx, dim):
+    """A captured call replays to the eager one's bits, on new inputs, with eager work in between; two graphs that were
+    captured one after the other share nothing."""
+    from flint_amd.attention import attention_weights, tree_attention
+    slots = ctx + m
+    ins = []
+    for seed in range(3):
+        g, q, k, v = make(b, m, 8, 2, dim, slots, torch.bfloat16, seed=seed)
+        pos = torch.tensor([ctx - 5 * i * seed for i in range(b)], dtype=torch.int32)
+        ins.append([x.to(dev) for x in (q, k, v, pos, tree_mask(g, b, m))])
+    held = [x.clone() for x in ins[0]]
+
+    def call(x):
+        out, lse = tree_attention(x[0], x[1], x[2], x[3], x[4], return_lse=True)
+        return out, lse, attention_weights(x[0], x[1], lse, x[3], x[4])
+    want = [[y.clone() for y in call(x)] for x in ins]
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            got = call(held)
+        graphs.append((gr, got))
+    for i in (0, 1, 2, 1, 0, 2):
+        for h, x in zip(held, ins[i]):
+            h.copy_(x)
+        for gr, got in graphs:
+            gr.replay()
+        call(ins[(i + 1) % 3])
+        torch.cuda.synchronize()
+        for gr, got in graphs:
+            assert all(torch.equal(a, w) for a, w in zip(got, want[i]))
+
+
+def test_two_streams_at_once(dev):
+    """Calls that run at the same time have a workspace each."""
+    from flint_amd.attention import tree_attention
+    _, q, k, v = make(1, 9, 40, 8, 64, 20000, torch.bfloat16, seed=1)
+    q, k, v = q.to(dev), k.to(dev), v.to(dev)
+    want = [tree_attention(q, k, v, p) for p in (19000, 12345)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(15):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(tree_attention(q, k, v, (19000, 12345)[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
+@pytest.mark.parametrize("slots,b,groups", [(20000, 1, 1), (3000, 40, 8), (1 << 17, 1, 2)])
+def test_single_tokens_of_many_lengths(dev, slots, b, groups):
+    """One token a sequence behind every kind of length, parts of them empty for the shorter ones, against a float64
+    product on the device."""
+    from flint_amd.attention import tree_attention
+    g = torch.Generator(device=dev).manual_seed(slots)
+    heads = groups * 5
+    q = torch.randn(b, 1, heads, 64, generator=g, device=dev).bfloat16()
+    k, v = (torch.randn(b, groups, slots, 64, generator=g, device=dev).bfloat16() for _ in range(2))
+    for lens in ([slots - 1] * b, [(slots - 1) * i // b for i in range(b)], [i % 3 for i in range(b)]):
+        pos = torch.tensor(lens, dtype=torch.int32, device=dev)
+        out, lse = tree_attention(q, k, v, pos, return_lse=True)
+        n = max(lens) + 1
+        seen = torch.arange(n, device=dev) <= pos[:, None]
+        for j in range(groups):
+            s = torch.matmul(q[:, 0, 5 * j:5 * j + 5].double(), k[:, j, :n].double().transpose(1, 2).contiguous()) * 0.125
+            s = s.masked_fill(~seen[:, None], -math.inf)
+            o = torch.matmul(torch.softmax(s, -1), v[:, j, :n].double())
+            es = 64 * 2.0 ** -24 * 64 * 16 * 0.125 + 2.0 ** -20 * 16  # |q|, |k| below 5 in these draws: sum|q k| < 64 * 16
+            tol = 2.0 ** -8 * o.abs() + 2 * (2.0 ** -16 + es + n * 2.0 ** -24) * 5.5
+            assert ((out[:, 0, 5 * j:5 * j + 5].double() - o).abs() <= tol).all()
+            assert ((lse[:, 0, 5 * j:5 * j + 5].double() - torch.logsumexp(s, -1)).abs() <= es + n * 2.0 ** -24 + 2.0 ** -18).all()

@@ -130,3 +130,43 @@ def test_refusals(dev):
                dict(out=(new, new.clone(), w[..., :20])), dict(k_cache=k[..., :4], v_cache=v[..., :4])):
         with pytest.raises(ValueError):
             evict(**{**dict(k_cache=k, v_cache=v, weights=w, n=40, keep=10), **kw})
+
+
+def test_captured_and_replayed(dev):
+    from flint_amd.attention import evict
+    ins = [[x.to(dev) for x in make((3, 2), 2000, 64, seed=s, kind="ties")] for s in range(3)]
+    held = [x.clone() for x in ins[0]]
+    out = (torch.zeros(3, 2, 600, 64, dtype=torch.bfloat16, device=dev), torch.zeros(3, 2, 600, 64, dtype=torch.bfloat16, device=dev),
+           torch.zeros(3, 2, 600, device=dev))
+    want = [(evict(*x, 1900, 600, 50, 4, out).clone(), *[t.clone() for t in out]) for x in ins]
+    torch.cuda.synchronize()
+    gr, gp = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        kept = evict(*held, 1900, 600, 50, 4, out)
+    with torch.cuda.graph(gp):
+        in_place = evict(*held, 1900, 600, 50, 4)
+    for i in (0, 2, 1, 0):
+        for h, x in zip(held, ins[i]):
+            h.copy_(x)
+        for t in out:
+            t.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(kept, want[i][0]) and all(torch.equal(a, b) for a, b in zip(out, want[i][1:]))
+        gp.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(in_place, want[i][0]) and torch.equal(held[0][..., :600, :], want[i][1])
+        assert torch.equal(held[1][..., :600, :], want[i][2]) and (held[2][..., 600:1900] == 0).all()
+
+
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 2048, 2049, 8192, 8193, 32768, 32769, 70001])
+def test_lengths_at_the_seams(dev, n):
+    """A lane's keys in registers, two to thirty-two of them, and read again beyond: against a stable sort."""
+    from flint_amd.attention import evict
+    k, v, w = make((2,), n, 8, seed=n, kind="ties")
+    keep = n // 3 + 1
+    kept = evict(k.to(dev), v.to(dev), w.to(dev), n, keep, recent=5, sink=3)
+    score = w.clone()
+    score[:, :3], score[:, n - 5:] = math.inf, math.inf
+    want = score.sort(dim=1, descending=True, stable=True).indices[:, :keep].sort(dim=1).values
+    assert torch.equal(kept.cpu().long(), want)
