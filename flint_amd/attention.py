@@ -217,6 +217,9 @@ def evict(k_cache, v_cache, weights, n, keep, recent=0, sink=0, out=None):
         for t in [x for x in out if x is not None]:
             for src in (k_cache, v_cache, weights):
                 _check(not _overlap(t, src), "out must not overlap the caches or the weights")
+    for t, other, name in ((k_cache, v_cache, "caches"),) if out is None else ((out[0], out[1], "out"),):
+        _check(t.numel() == 0 or t.data_ptr() != other.data_ptr(), f"{name}: K and V must not be the same memory")
+        _check(all(s for x in (t, other) for s, c in zip(x.stride()[:-1], x.shape) if c > 1), f"{name}: expanded dimensions cannot be written")
     kept = torch.empty(*lead, keep, dtype=torch.int32, device=dev)
     if heads == 0 or n == 0:
         return kept

@@ -71,8 +71,8 @@ __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
   __amdgpu_buffer_rsrc_t pr, qr;
   auto open = [&] {
     pr = row_rsrc<BF>(a.p, prow + cur, V);
-    // the last node has no children and no draft row: C stays 0 there
-    qr = DRAFT && cur < a.m - 1 ? row_rsrc<BF>(a.q, qrow + cur, V) : buf_rsrc(a.p, 0);
+    // before a rejection q does not count, and a leaf's row may hold anything (the last node has none): not read
+    qr = DRAFT && C > 0.0 ? row_rsrc<BF>(a.q, qrow + cur, V) : buf_rsrc(a.p, 0);
   };
   auto cut = [&](float p, float q) -> double {
     const double w = DRAFT ? __builtin_fma(-C, (double)q, (double)p) : (double)p;

@@ -6,9 +6,12 @@
 // is online, per lane, in the log2 domain (p = exp2(s c - m), c = scale log2 e), in fp32; O^T += V^T P^T takes a step's
 // 16 keys in the order in which the score registers already hold them, so P never crosses lanes. V^T comes out of LDS
 // through the transposing read (a 16-lane group receives four rows of 16 values by column). P is split into two 16-bit
-// terms: one alone would round every weight by 2^-9 (bf16), which showed as 1.4 times the output's own rounding.
+// terms, 2^-17 of a weight together in bf16: with one alone 1024 tokens behind 4096 take 82 us in place of 102, but their
+// outputs lie 1.3 times as far from 64 bits (0.0021 in place of 0.0016 of their norm), and the model's attention is fp32
+// times V.
 #include <algorithm>
 #include "fl_gemm.h"
+#include "fl_state.h"
 
 namespace {
 
@@ -87,7 +90,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int part) {
   Span s;
   s.pos = a.pos ? __builtin_amdgcn_readfirstlane(a.pos[b]) : a.pos0;  // the wave's, in a scalar register
   if (s.pos < 0 || s.pos > a.slots - a.m) {
-    s.keys = -1, s.kb0 = s.kend = 0;
+    s.pos = 0, s.keys = -1, s.kb0 = s.kend = 0;
     return s;
   }
   s.keys = s.pos + a.m;
@@ -705,7 +708,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_weights(AttnArgs 
 }
 
 // ---- host -------------------------------------------------------------------------------------------------
-constexpr int AT_NW = 8;  // waves of k_attn_few
+constexpr int AT_NW = 8;      // waves of k_attn_few
+constexpr int AT_FEW = 64;    // rows that it takes at most
+constexpr int AT_PARTS = 64;  // key parts at most: a lane of the merge each
 
 bool desc_ok(const fl_attn_desc* d) {
   if (!d || d->b < 1 || d->m < 1 || d->heads < 1 || d->groups < 1 || d->slots < 1 || d->slots > 1 << 30) return false;
@@ -726,34 +731,39 @@ struct AttnPlan {
   int blocks, parts, kpp;
   int64_t bytes;
 };
-// `pos_known`: the host knows how many keys there are; else up to d.slots, and sequences of any length
-AttnPlan attn_plan(const fl_attn_desc& d, bool pos_known) {
-  const int R = d.m * (d.heads / d.groups), keys = pos_known ? d.pos0 + d.m : d.slots;
+// The plan for sequences of up to `keys` keys. Within a kind its parts grow with the keys, so the workspace for all that
+// a cache can hold is the larger of the two kinds' (attn_work_bound).
+AttnPlan attn_plan_of(const fl_attn_desc& d, int keys, bool few) {
+  const int R = d.m * (d.heads / d.groups);
   AttnPlan p{};
-  // Few rows: a wave's own keys need no barrier but meet in LDS at the end, which pays where one launch does (up to three
-  // tiles a wave) and where memory is the bound; in between the shared ring's kernel starts and ends sooner. us, one
-  // token, few / many: 1000 keys 10.9 / 11.6, 2000 13.5 / 10.7, 8000 13.5 / 11.8, 131072 44 / 67; 24 sequences of 3000
-  // 34 / 40, 8 trees of 8 behind 2000 16.7 / 17.5; 40 rows behind 4000 14.9 / 11.6, behind 30000 20.7 / 24.8.
-  const int few_unit = AT_NW * 4096 / d.dim;
-  p.few = R <= 64 && (keys <= 3 * few_unit || (int64_t)d.b * d.groups * keys * d.dim >= 6 << 20);
-  p.blocks = p.few ? (R + 31) / 32 : (R + 127) / 128;
-  const int unit = p.few ? few_unit : 64, least = p.few ? unit : 256;
+  p.few = few;
+  p.blocks = few ? (R + 31) / 32 : (R + 127) / 128;
+  const int unit = few ? AT_NW * 4096 / d.dim : 64, least = few ? unit : 256;
   const int64_t base = (int64_t)d.b * d.groups * p.blocks;
   // Workgroups that cutting the keys may reach. Few rows: one per CU, whose eight waves have 128 KB in flight (131072 keys
   // 53 us, with two rounds of workgroups 60). Many rows: of the three (dim 64) or two that a CU holds, one and a third
   // times as many as there are places (1024 tokens behind 4096: 640 116 us, 1024 104, 1600 112; 16 trees of 13 and
   // 128 dims: 640 56, 1024 67).
-  const int64_t fill = p.few ? 256 : d.dim == 64 ? 1024 : 640;
+  const int64_t fill = few ? 256 : d.dim == 64 ? 1024 : 640;
   // a wave of few rows takes three tiles in less than the launch that joins parts costs (1032 keys: 11.6 uncut, 13.5 in
   // two parts; 2000: 16.0 and 13.5)
-  const int most = p.few && keys <= 3 * unit
+  const int most = few && keys <= 3 * unit
                        ? 1
-                       : (int)std::max<int64_t>(1, std::min<int64_t>({64, (fill + base - 1) / base, keys / least}));
+                       : (int)std::max<int64_t>(1, std::min<int64_t>({AT_PARTS, (fill + base - 1) / base, keys / least}));
   p.kpp = (int)(((int64_t)(keys + most - 1) / most + unit - 1) / unit * unit);
   p.parts = (keys - 1) / p.kpp + 1;
-  const int64_t n = (int64_t)d.b * d.groups * R;
-  p.bytes = p.parts == 1 ? 0 : p.parts * n * (d.dim + 2) * 4;
+  p.bytes = most == 1 ? 0 : most * ((int64_t)d.b * d.groups * R) * (d.dim + 2) * 4;
   return p;
+}
+// `pos_known`: the host knows how many keys there are; else up to d.slots, and sequences of any length
+AttnPlan attn_plan(const fl_attn_desc& d, bool pos_known) {
+  const int R = d.m * (d.heads / d.groups), keys = pos_known ? d.pos0 + d.m : d.slots;
+  // Few rows: a wave's own keys need no barrier but meet in LDS at the end, which pays where one launch does (up to three
+  // tiles a wave) and where memory is the bound; in between the shared ring's kernel starts and ends sooner. us, one
+  // token, few / many: 1000 keys 10.9 / 11.6, 2000 13.5 / 10.7, 8000 13.5 / 11.8, 131072 44 / 67; 24 sequences of 3000
+  // 34 / 40, 8 trees of 8 behind 2000 16.7 / 17.5; 40 rows behind 4000 14.9 / 11.6, behind 30000 20.7 / 24.8.
+  const bool few = R <= AT_FEW && (keys <= 3 * AT_NW * 4096 / d.dim || (int64_t)d.b * d.groups * keys * d.dim >= 6 << 20);
+  return attn_plan_of(d, keys, few);
 }
 AttnArgs attn_args(const fl_attn_desc& d, const uint16_t* q, const uint16_t* k, const uint16_t* v, const int32_t* pos,
                    const uint8_t* mask) {
@@ -792,6 +802,12 @@ int weights_launch(AttnArgs a, float* w, int add, hipStream_t s) {
 }
 
 }  // namespace
+
+int64_t fl_attn_work_bound(const fl_attn_desc& d) {
+  if (!desc_ok(&d)) return -1;
+  const int64_t few = d.m * (d.heads / d.groups) <= AT_FEW ? attn_plan_of(d, d.slots, true).bytes : 0;
+  return std::max(few, attn_plan_of(d, d.slots, false).bytes);
+}
 
 extern "C" {
 

@@ -194,6 +194,10 @@ int fl_evict(const fl_rows* k, const fl_rows* v, float* weights, int32_t n_outer
   if (row_bytes < 16 || row_bytes > 4096 || row_bytes % 16 || !strides_ok(k, row_bytes) || !strides_ok(v, row_bytes)) return FL_E_ARG;
   if (n < 1 || slots < n || keep < 1 || keep > n || recent < 0 || sink < 0 || (int64_t)recent + sink > keep) return FL_E_ARG;
   if (!k_out != !v_out || (weights_out && !k_out)) return FL_E_ARG;
+  // heads that share their rows can be read, not written
+  auto apart = [&](const fl_rows* r) { return (n_outer == 1 || r->outer != 0) && (n_inner == 1 || r->inner != 0); };
+  const fl_rows *kd = k_out ? k_out : k, *vd = v_out ? v_out : v;
+  if (!apart(kd) || !apart(vd) || kd->data == vd->data) return FL_E_ARG;
   if (k_out && (!strides_ok(k_out, row_bytes) || !strides_ok(v_out, row_bytes) || slots_out < keep)) return FL_E_ARG;
   const int heads = n_outer * n_inner;
   EvictArgs a{};

@@ -456,13 +456,13 @@ fl_attn_desc pf_attn_desc(const fl_model_desc& d, int max_seq, int T, int pos) {
   a.k_s = a.v_s = FL_HEAD_DIM;
   return a;
 }
-// bytes of fl_tree_attention's workspace for passes of up to T tokens of n: the full passes and the last one, behind as many keys as fit
+// bytes of fl_tree_attention's workspace for passes of up to T tokens of n, the full ones and the last, behind any number of
+// keys
 int64_t pf_attn_work(const fl_model_desc& d, int max_seq, int n, int T) {
   int64_t most = 0;
   for (int t : {T, n % T ? n % T : T}) {
-    const fl_attn_desc a = pf_attn_desc(d, max_seq, t, max_seq - t);
-    int64_t bytes = 0;
-    if (fl_tree_attention_workspace(&a, 1, &bytes) != FL_OK) return -1;
+    const int64_t bytes = fl_attn_work_bound(pf_attn_desc(d, max_seq, t, 0));
+    if (bytes < 0) return -1;
     most = std::max(most, bytes);
   }
   return most;

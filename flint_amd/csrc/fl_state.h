@@ -48,3 +48,7 @@ struct fl_state {
 
 // every pointer that all entry points need is set (fl_decode.hip)
 bool fl_weights_ok(const fl_weights* w);
+
+// bytes of fl_tree_attention's workspace that suffice for any number of cached keys; -1 for a description that it refuses
+// (fl_attention.hip)
+int64_t fl_attn_work_bound(const fl_attn_desc& d);

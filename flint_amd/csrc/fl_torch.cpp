@@ -504,6 +504,7 @@ pybind11::object evict_fast(const torch::Tensor& k, const torch::Tensor& v, cons
   if (heads > 65535 || slots > INT32_MAX || rb > 4096 || n < 1 || n > slots || keep < 1 || keep >= n || recent < 0 || sink < 0 ||
       recent + sink > keep || !here(k, {&v, &w}) || ko.has_value() != vo.has_value() || (wo && !ko))
     return pybind11::none();
+  if (ko ? ko->data_ptr() == vo->data_ptr() : k.data_ptr() == v.data_ptr()) return pybind11::none();
   const fl_rows kr{k.data_ptr(), 0, slots * rb, rb}, vr{v.data_ptr(), 0, slots * rb, rb};
   fl_rows kor{}, vor{};
   int64_t so = 0;

@@ -233,8 +233,8 @@ typedef struct fl_rows {
  * rising. Their rows of K and V (row_bytes each, a multiple of 16, at most 4096) move in this order to the slots 0 ..
  * keep - 1: in place (k_out, v_out NULL), with the weights (fp32 [heads][slots]), and the weights of keep .. n - 1
  * become 0, the rows there stay what they were; or into k_out and v_out (which do not overlap the caches) and, where
- * given, weights_out [heads][slots_out], with the caches left as they are. 1 <= keep <= n <= slots, sink + recent <=
- * keep, at most 65535 heads.
+ * given, weights_out [heads][slots_out], with the caches left as they are. K and V, and the heads, that are written must
+ * not share rows. 1 <= keep <= n <= slots, sink + recent <= keep, at most 65535 heads.
  * No counterpart in the reference, whose cache only grows (engine/model.py:82-98). */
 int fl_evict(const fl_rows* k, const fl_rows* v, float* weights, int32_t n_outer, int32_t n_inner, int32_t slots,
              int32_t row_bytes, int32_t n, int32_t keep, int32_t recent, int32_t sink, int32_t* kept,

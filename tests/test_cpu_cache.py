@@ -86,11 +86,13 @@ def test_c_entries_refuse():
     def rows(data=P, outer=2048, inner=1024, row=128):
         return ctypes.byref(_lib.Rows(data, outer, inner, row))
 
-    def evict(k=rows(), v=rows(), w=P, n0=1, n1=2, slots=16, rb=128, n=10, keep=5, recent=1, sink=1, kept=P, ko=None, vo=None, wo=None, so=0):
+    def evict(k=rows(), v=rows(data=2 * P), w=P, n0=1, n1=2, slots=16, rb=128, n=10, keep=5, recent=1, sink=1, kept=P, ko=None, vo=None, wo=None, so=0):
         return l.fl_evict(k, v, w, n0, n1, slots, rb, n, keep, recent, sink, kept, ko, vo, wo, so, None)
+    ko, vo = rows(data=3 * P), rows(data=4 * P)
     for kw in (dict(w=None), dict(kept=None), dict(n0=0), dict(n0=70000), dict(rb=24), dict(rb=8192), dict(n=17), dict(keep=0), dict(keep=11),
-               dict(recent=5), dict(recent=-1), dict(sink=-1), dict(k=rows(data=0)), dict(k=rows(data=P + 8)), dict(v=rows(row=64)),
-               dict(v=rows(inner=8)), dict(ko=rows()), dict(wo=P), dict(ko=rows(), vo=rows(), so=4), dict(ko=rows(), vo=rows(row=8), so=8)):
+               dict(recent=5), dict(recent=-1), dict(sink=-1), dict(k=rows(data=0)), dict(k=rows(data=P + 8)), dict(v=rows(data=2 * P, row=64)),
+               dict(v=rows(data=2 * P, inner=8)), dict(v=rows()), dict(k=rows(inner=0)), dict(ko=ko), dict(wo=P), dict(ko=ko, vo=vo, so=4),
+               dict(ko=ko, vo=rows(data=4 * P, row=8), so=8), dict(ko=ko, vo=ko, so=8), dict(ko=ko, vo=rows(data=4 * P, inner=0), so=8)):
         assert evict(**kw) == -1, kw
 
     def accept(p=P, t=P, ua=P, us=P, path=P, b=1, m=2, v=10):

@@ -179,3 +179,16 @@ def test_weight_in_one_place(dev, v, where):
     us = torch.tensor([0.999, 0.0, 0.999], device=dev)
     got = accept_sampled(p, torch.zeros(3, 1, dtype=torch.int32, device=dev), torch.zeros(3, 1, device=dev), us)
     assert got.token.tolist() == [at, other, at] and got.count.tolist() == [1, 1, 1]
+
+
+def test_rows_of_leaves_are_not_looked_at(dev):
+    """A draft row that no child was drawn from may hold anything; so may one whose first child is accepted."""
+    from flint_amd.spec import accept_sampled
+    p, q, tokens, parents, ua, us = make(6, 8, 3000, 21)
+    inner = torch.zeros(6, 7, dtype=torch.bool)
+    for s in range(6):
+        inner[s, parents[s, 1:].long()] = True
+    want = accept_sampled(*(x.to(dev) for x in (p, tokens, ua, us, parents, q)))
+    for junk in (float("nan"), float("inf"), -1.0):
+        got = accept_sampled(*(x.to(dev) for x in (p, tokens, ua, us, parents, torch.where(inner[..., None], q, junk))))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

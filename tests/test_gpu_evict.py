@@ -170,3 +170,21 @@ def test_lengths_at_the_seams(dev, n):
     score[:, :3], score[:, n - 5:] = math.inf, math.inf
     want = score.sort(dim=1, descending=True, stable=True).indices[:, :keep].sort(dim=1).values
     assert torch.equal(kept.cpu().long(), want)
+
+
+def test_shared_rows_are_not_written(dev):
+    from flint_amd.attention import evict
+    k, v, w = (x.to(dev) for x in make((2, 2), 50, 64))
+    new = torch.zeros(2, 2, 20, 64, dtype=k.dtype, device=dev)
+    with pytest.raises(ValueError):
+        evict(k, k, w, 40, 10)
+    with pytest.raises(ValueError):
+        evict(k, v, w, 40, 10, out=(new, new))
+    wide = k[:1].expand(2, 2, 50, 64)
+    with pytest.raises(ValueError):
+        evict(wide, v, w, 40, 10)
+    with pytest.raises(ValueError):
+        evict(k, v, w, 40, 10, out=(new[:1].expand(2, 2, 20, 64), new.clone()))
+    # to be read they may be shared
+    kept = evict(wide, v, w, 40, 10, out=(new, new.clone()))
+    assert torch.equal(new[:, :, :10].cpu(), moved(wide.cpu(), kept.cpu().long()))

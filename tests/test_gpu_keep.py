@@ -346,3 +346,47 @@ def test_wide_trees(dev):
     with pytest.raises(ValueError):
         SpecDecoder(eng, k=32)
     assert SpecDecoder(eng, k=100, head=head).k == 100
+
+
+def test_workspace_covers_every_position(dev):
+    """A prompt pass that gathers weights asks for a workspace before it knows how many keys are cached: enough for all."""
+    from flint_amd import _lib
+    args, _, eng, _ = make_pair("small", seed=3, block_size=16384)
+    for slots in (64, 2048, 16384):
+        eng.close()
+        eng.max_seq_length = -1
+        eng.setup_caches(1, slots)
+        for m in (1, 2, 5, 12, 13, 40, 64, 200, 1024, 1025, 1100):
+            if m > slots:
+                continue
+            plain, extra, need = (_lib.ctypes.c_int64() for _ in range(3))
+            _lib.call("fl_prefill_workspace", eng._state, m, _lib.ctypes.byref(plain))
+            _lib.call("fl_prefill_extra_workspace", eng._state, m, _lib.ctypes.byref(extra))
+            room = extra.value - plain.value - min(m, 1024) * args.n_head * 4
+            for t in {min(m, 1024), m % 1024 or min(m, 1024)}:
+                d = _lib.AttnDesc(b=1, m=t, heads=args.n_head, groups=args.n_local_heads, dim=64, slots=slots, scale=0.125,
+                                  q_m=args.n_head * 64, q_h=64, k_g=slots * 64, k_s=64, v_g=slots * 64, v_s=64)
+                for pos in {0, 1, 500, 700, 1000, 1500, 2000, 4000, 8000, 11000, 12000, 12300, 14000, slots - t}:
+                    if pos <= slots - t:
+                        d.pos0 = pos
+                        _lib.call("fl_tree_attention_workspace", _lib.ctypes.byref(d), 1, _lib.ctypes.byref(need))
+                        assert need.value <= room, (slots, m, t, pos)
+
+
+@pytest.mark.parametrize("pos", [3000, 11000, 15000])
+def test_short_prompt_far_into_the_cache(dev, pos):
+    """A few tokens behind many: the weights sum to the rows and the features are a plain prompt's."""
+    args, _, eng, _ = make_pair("small", seed=3, block_size=16384)
+    eng.setup_caches(1, 16384)
+    g = torch.Generator(device=dev).manual_seed(pos)
+    for c in (eng.k_cache, eng.v_cache):
+        c[:, :, :pos].copy_(torch.randn(c[:, :, :pos].shape, generator=g, device=dev) * 0.5)
+    x = tokens(args, 12, 3).to(dev)
+    w = eng.new_weights()
+    feat = torch.empty(12, args.dim, dtype=torch.bfloat16, device=dev)
+    eng.prefill_weights(x, pos, w, feat=feat)
+    rep = args.n_head // args.n_local_heads
+    assert ((w.double().sum(-1) - 12 * rep).abs() <= 12 * rep * 2.0 ** -10).all()
+    plain = eng.prefill_features(x, pos)
+    assert float((feat.float() - plain.float()).norm() / plain.float().norm()) <= 2.0 ** -6
+    eng.check()
