@@ -67,7 +67,8 @@ __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
   const int seg = ((V + AC_NW - 1) / AC_NW + 63) / 64 * 64;  // a wave's piece of a row
   int cur = 0, n = 1, ngone = 0, turn = 0;  // node; nodes of the path; tokens rejected at the node
   bool fresh = true;                        // Z is the sum of w (or 1)
-  double C = 0.0, Z = 1.0, S = -1.0;        // S: without draft probabilities, the sum of the node's row (once known)
+  double C = 0.0, Z = 1.0;
+  double rest = -1.0, last = 0.0;  // without draft probabilities: the row's sum (once known) without the tokens gone but the last; its p
   __amdgpu_buffer_rsrc_t pr, qr;
   auto open = [&] {
     pr = row_rsrc<BF>(a.p, prow + cur, V);
@@ -146,29 +147,25 @@ __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
         if (DRAFT) {
           Z = total();
         } else {  // the row's sum without the tokens gone
-          if (S < 0.0) {
-            const int keep = ngone;
+          if (rest < 0.0) {  // one token is gone: taken off here, as the later ones are one by one
             ngone = 0;
-            S = total();
-            ngone = keep;
+            rest = total();
+            ngone = 1;
           }
-          Z = S;
-          for (int k = 0; k < ngone; ++k) {
-            bool twice = false;  // a token that was proposed again
-            for (int j = 0; j < k; ++j) twice = twice || gone[j] == gone[k];
-            const float g = row_ld<BF>(pr, (uint32_t)gone[k]);
-            Z -= twice || !(g > 0.0f) ? 0.0 : (double)g;
-          }
-          Z = Z > 0.0 ? Z : 0.0;
+          rest -= last;
+          rest = rest > 0.0 ? rest : 0.0;
+          Z = rest;
         }
         fresh = true;
       }
       double w = cut(p1, q1);
-      if (!DRAFT)
-        for (int k = 0; k < ngone; ++k)
-          if (gone[k] == t) w = 0.0;
+      if (!DRAFT) {
+        bool again = false;  // proposed and rejected before
+        for (int k = lane; k < ngone; k += 64) again = again || gone[k] == t;
+        if (__any(again)) w = 0.0;
+      }
       if ((double)u1 * (double)q1 * Z < w) {
-        cur = n0 + l, C = 0.0, Z = 1.0, S = -1.0, ngone = 0, fresh = true;
+        cur = n0 + l, C = 0.0, Z = 1.0, rest = -1.0, ngone = 0, fresh = true;
         if (tid == 0) a.path[prow + n] = cur;
         ++n;
         if (!DRAFT) __syncthreads();  // gone is free again
@@ -176,6 +173,7 @@ __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
         C += Z;
         fresh = false;
         if (!DRAFT) {
+          last = w;
           if (tid == 0) gone[ngone] = t;
           ++ngone;
           __syncthreads();

@@ -192,3 +192,18 @@ def test_rows_of_leaves_are_not_looked_at(dev):
     for junk in (float("nan"), float("inf"), -1.0):
         got = accept_sampled(*(x.to(dev) for x in (p, tokens, ua, us, parents, torch.where(inner[..., None], q, junk))))
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("draft", [True, False])
+def test_many_children_of_one_node(dev, draft):
+    """A root with 1023 children, unlikely ones and many of them twice, nearly all rejected."""
+    m, v = 1024, 1500
+    p, q, _, _, ua, us = make(3, m, v, 31, draft=draft)
+    g = torch.Generator().manual_seed(32)
+    low = p[:, 0].argsort(dim=1)[:, :1000].int()
+    tokens = low.gather(1, torch.randint(0, 1000, (3, m), generator=g))
+    parents = torch.zeros(3, m, dtype=torch.int32)
+    parents[:, 0] = -1
+    ua = 1.0 - 0.01 * ua
+    ua[1, 1000] = ua[2, 70] = 0.0
+    check((p, q, tokens, parents, ua, us), dev)
