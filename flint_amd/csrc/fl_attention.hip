@@ -616,17 +616,20 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_weights(AttnArgs 
       ro[i] = (uint32_t)(row / a.rep) * qm + (uint32_t)rj[i] * qh + (uint32_t)(lane % CH) * 16u;
     }
     int ln = (rt * 32 + r) / a.rep, lj = (rt * 32 + r) % a.rep;  // of row r, whose lse this lane loads
+    int left = a.R - rt * 32 - lane / CH;                        // rows from this lane's first one on
     uint4 qv[ST];
     float lse;
     int node;
     auto load = [&] {
 #pragma unroll
       for (int i = 0; i < ST; ++i) {
-        qv[i] = buf_ld128(qr, ro[i]);  // rows behind the last: zeros, or another head's, which add nothing
+        // rows behind the last are zeros, not what lies there: another head's NaN would reach keys that it does not see
+        qv[i] = buf_ld128(qr, i * RS < left ? ro[i] : 0xFFFFFF00u);
         rj[i] += dj;
         ro[i] += (uint32_t)dn * qm + (uint32_t)dj * qh;
         if (rj[i] >= a.rep) rj[i] -= a.rep, ro[i] += qm - (uint32_t)a.rep * qh;
       }
+      left -= 32 * step;
       node = ln;
       lse = ln < a.m ? lg[(int64_t)ln * a.heads + lj] : -INFINITY;
       ln += dn, lj += dj;

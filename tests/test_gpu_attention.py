@@ -339,3 +339,18 @@ def test_single_tokens_of_many_lengths(dev, slots, b, groups):
             tol = 2.0 ** -8 * o.abs() + 2 * (2.0 ** -16 + es + n * 2.0 ** -24) * 5.5
             assert ((out[:, 0, 5 * j:5 * j + 5].double() - o).abs() <= tol).all()
             assert ((lse[:, 0, 5 * j:5 * j + 5].double() - torch.logsumexp(s, -1)).abs() <= es + n * 2.0 ** -24 + 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("m,rep,dim", [(40, 2, 64), (11, 3, 128), (21, 5, 64)])
+def test_a_query_that_is_no_number_reaches_what_its_node_sees(dev, m, rep, dim):
+    """Queries ordered by head: behind a head's last node lies the next head's first, which is NaN here."""
+    from flint_amd.attention import attention_weights
+    g, q, k, v = make(1, m, rep, 1, dim, 300, torch.bfloat16, seed=5)
+    q[0, 0, 1] = math.nan
+    pos = 55
+    _, l = oracle.tree_attention(q, k, v, [pos], None, dim ** -0.5)
+    want = oracle.attention_weights(q, k, l, [pos], None, dim ** -0.5)
+    assert want.isnan().sum() == pos + 1
+    qd = q.to(dev).transpose(1, 2).contiguous().transpose(1, 2)
+    got = attention_weights(qd, k.to(dev), l.float().to(dev), pos).cpu()
+    assert torch.equal(got.isnan(), want.isnan())
