@@ -187,6 +187,7 @@ def evict(k_cache, v_cache, weights, n, keep, recent=0, sink=0, out=None):
     _check(k_cache.dim() >= 2 and v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype
            and v_cache.device == k_cache.device, "k_cache and v_cache must be of one shape, type and device")
     dev, slots = k_cache.device, k_cache.shape[-2]
+    _check(slots <= 1 << 30, "at most 2^30 slots")
     _check(weights.is_cuda and weights.device == dev and weights.dtype == torch.float32
            and weights.shape == k_cache.shape[:-1] and weights.is_contiguous(),
            "weights must be contiguous fp32 [..., slots] on the caches' device")

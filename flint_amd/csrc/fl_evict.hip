@@ -192,7 +192,7 @@ int fl_evict(const fl_rows* k, const fl_rows* v, float* weights, int32_t n_outer
              const fl_rows* v_out, float* weights_out, int32_t slots_out, void* stream) {
   if (!weights || !kept || n_outer < 1 || n_inner < 1 || (int64_t)n_outer * n_inner > 65535) return FL_E_ARG;
   if (row_bytes < 16 || row_bytes > 4096 || row_bytes % 16 || !strides_ok(k, row_bytes) || !strides_ok(v, row_bytes)) return FL_E_ARG;
-  if (n < 1 || slots < n || keep < 1 || keep > n || recent < 0 || sink < 0 || (int64_t)recent + sink > keep) return FL_E_ARG;
+  if (n < 1 || slots < n || slots > 1 << 30 || keep < 1 || keep > n || recent < 0 || sink < 0 || (int64_t)recent + sink > keep) return FL_E_ARG;
   if (!k_out != !v_out || (weights_out && !k_out)) return FL_E_ARG;
   // heads that share their rows can be read, not written
   auto apart = [&](const fl_rows* r) { return (n_outer == 1 || r->outer != 0) && (n_inner == 1 || r->inner != 0); };

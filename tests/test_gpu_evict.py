@@ -188,3 +188,10 @@ def test_shared_rows_are_not_written(dev):
     # to be read they may be shared
     kept = evict(wide, v, w, 40, 10, out=(new, new.clone()))
     assert torch.equal(new[:, :, :10].cpu(), moved(wide.cpu(), kept.cpu().long()))
+
+
+def test_more_slots_than_indices_reach(dev):
+    from flint_amd.attention import evict
+    k, v = (torch.zeros(1, 16, dtype=torch.uint8, device=dev).expand(2 ** 30 + 1, 16) for _ in range(2))
+    with pytest.raises(ValueError, match="slots"):
+        evict(k, v, torch.zeros(1, device=dev).expand(2 ** 30 + 1), 100, 10)
