@@ -29,12 +29,14 @@ __device__ __forceinline__ uint32_t w_key(float w) {
 
 // One workgroup per head. The `keep` largest keys by a radix select over 32 bits (four counts of 256 bins), ties to the
 // lower slot, the first `sink` and the last `recent` slots above all others; then the kept slots in order: each wave has
-// a contiguous piece of the slots, counts and then places by ballots. A lane holds its E keys in registers. Bound by
-// the instructions of a key, some 50 over the six walks (8192 slots of 320 heads on 256 CUs: 24 us with the slots'
-// cases told apart in every walk); E = 0: more slots, read again for every walk, eight loads in flight.
+// a contiguous piece of the slots, whose counts above the border it has from its own histograms, and places by ballots.
+// The counts end where a bin's keys all stay. A lane holds its E keys in registers; E = 0: more slots, read again for
+// every walk, eight loads in flight. Bound by the walks, two to four counts and the places, at some 24 clocks of the CU
+// for 64 keys (with four counts and a walk for the sums above: 8192 slots of 8 heads 11.9 us with the move of 1024
+// rows, now 10.8; 131072 of 2 heads 145, now 103).
 template <int E>
 __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
-  __shared__ int hist[ES_NW][256];
+  __shared__ __align__(16) int hist[ES_NW][256];
   __shared__ int sum[256], sel[2], above_w[ES_NW], equal_w[ES_NW];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.x;
   const float* w = a.w + (int64_t)head * a.slots;
@@ -68,10 +70,14 @@ __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
   };
   uint32_t prefix = 0;
   int need = a.keep;  // of those with the prefix so far (no slot's key 0 lies below all: never reached)
-  for (int shift = 24; shift >= 0; shift -= 8) {
-#pragma unroll
-    for (int i = 0; i < ES_NW * 256 / ES_NT; ++i) (&hist[0][0])[i * ES_NT + tid] = 0;
-    __syncthreads();
+  int above = 0;      // this lane's part of the wave's keys above the prefix, from the wave's own counts
+  int shift = 32;
+  bool all = false;  // the rest of the bits do not matter: every key with the prefix stays
+  while (shift > 0 && !all) {
+    shift -= 8;
+    // a wave's counts are its own until they are summed: no barrier between these and those
+    *reinterpret_cast<int4*>(&hist[wave][4 * lane]) = make_int4(0, 0, 0, 0);
+    __builtin_amdgcn_wave_barrier();
     if (shift == 24)
       walk([&](int, uint32_t key) { atomicAdd(&hist[wave][key >> 24], 1); });
     else
@@ -86,17 +92,22 @@ __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
       sum[tid] = n;
     }
     __syncthreads();
-    int above = 0;
-    const int bin = select_bin(sum, need, &above, sel);
+    int higher = 0;
+    const int bin = select_bin(sum, need, &higher, sel);
     prefix = (prefix << 8) | (uint32_t)bin;
-    need -= above;
+    need -= higher;
+    all = sum[bin] == need;
+    const int4 c = *reinterpret_cast<const int4*>(&hist[wave][4 * lane]);
+    above += (4 * lane > bin ? c.x : 0) + (4 * lane + 1 > bin ? c.y : 0) + (4 * lane + 2 > bin ? c.z : 0) + (4 * lane + 3 > bin ? c.w : 0);
+    if (lane == 0) equal_w[wave] = hist[wave][bin];  // of the last turn
   }
-  int above = 0, equal = 0;
-  walk([&](int, uint32_t key) {
-    above += __popcll(__ballot(key > prefix));
-    equal += __popcll(__ballot(key == prefix));
-  });
-  if (lane == 0) above_w[wave] = above, equal_w[wave] = equal;
+  if constexpr (E > 0) {
+    above = (int)wave_sum((float)above);  // at most 64 E
+  } else {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) above += __shfl_xor(above, o, 64);
+  }
+  if (lane == 0) above_w[wave] = above;
   __syncthreads();
   int eq = 0, at = 0;  // equal ones before this wave, and the kept ones
   for (int i = 0; i < wave; ++i) {
@@ -105,8 +116,9 @@ __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
   }
   const unsigned long long below = (1ull << lane) - 1;
   walk([&](int i, uint32_t key) {
-    const unsigned long long e = __ballot(key == prefix);
-    const unsigned long long s = __ballot(key > prefix || (key == prefix && eq + __popcll(e & below) < need));
+    const uint32_t top = key >> shift;
+    const unsigned long long e = __ballot(top == prefix);
+    const unsigned long long s = all ? __ballot(top >= prefix) : __ballot(top > prefix || (top == prefix && eq + __popcll(e & below) < need));
     if ((s >> lane) & 1) kept[at + __popcll(s & below)] = i;
     at += __popcll(s);
     eq += __popcll(e);
