@@ -79,7 +79,9 @@ __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
     *reinterpret_cast<int4*>(&hist[wave][4 * lane]) = make_int4(0, 0, 0, 0);
     __builtin_amdgcn_wave_barrier();
     if (shift == 24)
-      walk([&](int, uint32_t key) { atomicAdd(&hist[wave][key >> 24], 1); });
+      walk([&](int, uint32_t key) {
+        if (key) atomicAdd(&hist[wave][key >> 24], 1);  // no slot: 64 lanes at one address take 64 turns
+      });
     else
       walk([&](int, uint32_t key) {
         if ((key >> (shift + 8)) == prefix) atomicAdd(&hist[wave][(key >> shift) & 255], 1);
