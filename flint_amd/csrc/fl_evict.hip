@@ -98,7 +98,7 @@ __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
     const int bin = select_bin(sum, need, &higher, sel);
     prefix = (prefix << 8) | (uint32_t)bin;
     need -= higher;
-    all = sum[bin] == need;
+    all = sum[bin] == need && prefix != 0;  // a prefix of 0 is also that of no slot
     const int4 c = *reinterpret_cast<const int4*>(&hist[wave][4 * lane]);
     above += (4 * lane > bin ? c.x : 0) + (4 * lane + 1 > bin ? c.y : 0) + (4 * lane + 2 > bin ? c.z : 0) + (4 * lane + 3 > bin ? c.w : 0);
     if (lane == 0) equal_w[wave] = hist[wave][bin];  // of the last turn

@@ -195,3 +195,16 @@ def test_more_slots_than_indices_reach(dev):
     k, v = (torch.zeros(1, 16, dtype=torch.uint8, device=dev).expand(2 ** 30 + 1, 16) for _ in range(2))
     with pytest.raises(ValueError, match="slots"):
         evict(k, v, torch.zeros(1, device=dev).expand(2 ** 30 + 1), 100, 10)
+
+
+@pytest.mark.parametrize("low", [-math.inf, -3e38])
+@pytest.mark.parametrize("n,keep", [(100, 100), (100, 99), (1100, 1100), (3000, 3000), (3000, 2990), (33000, 33000), (70001, 70001)])
+def test_lowest_weights(dev, n, keep, low):
+    """Weights whose ordered keys begin with zeros, as empty places' do: the slots kept, and nothing behind them."""
+    from flint_amd.attention import evict
+    k, v = (torch.randn(2, n, 8, device=dev) for _ in range(2))
+    w = torch.full((2, n), low, device=dev)
+    w[1, ::7] = 1.0
+    kept = evict(k, v, w, n, keep, out=(torch.zeros(2, keep, 8, device=dev), torch.zeros(2, keep, 8, device=dev)))
+    for h in range(2):
+        assert kept[h].tolist() == oracle.kept_slots(w[h].tolist(), n, keep, 0, 0)
