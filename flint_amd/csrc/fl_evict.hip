@@ -37,6 +37,7 @@ __device__ __forceinline__ uint32_t w_key(float w) {
 template <int E>
 __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
   __shared__ __align__(16) int hist[ES_NW][256];
+  constexpr int U = 8;
   __shared__ int sum[256], sel[2], above_w[ES_NW], equal_w[ES_NW];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.x;
   const float* w = a.w + (int64_t)head * a.slots;
@@ -59,12 +60,12 @@ __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) f(p0 + e * 64 + lane, held[e]);
     } else {
-      for (int i0 = p0; i0 < p1; i0 += 512) {
-        float x[8];
+      for (int i0 = p0; i0 < p1; i0 += 64 * U) {
+        float x[U];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = i0 + e * 64 + lane < p1 ? w[i0 + e * 64 + lane] : 0.0f;
+        for (int e = 0; e < U; ++e) x[e] = i0 + e * 64 + lane < p1 ? w[i0 + e * 64 + lane] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f(i0 + e * 64 + lane, key_of(i0 + e * 64 + lane, x[e]));
+        for (int e = 0; e < U; ++e) f(i0 + e * 64 + lane, key_of(i0 + e * 64 + lane, x[e]));
       }
     }
   };
@@ -116,14 +117,21 @@ __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
     at += above_w[i] + min(equal_w[i], max(0, need - eq));
     eq += equal_w[i];
   }
-  const unsigned long long below = (1ull << lane) - 1;
+  // slots that always stay are no more than `keep`: a border among them is all of them, and no key is above it
+  const uint32_t least = prefix + (all ? 0u : 1u);
+  auto before = [](unsigned long long m) { return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u)); };
   walk([&](int i, uint32_t key) {
     const uint32_t top = key >> shift;
-    const unsigned long long e = __ballot(top == prefix);
-    const unsigned long long s = all ? __ballot(top >= prefix) : __ballot(top > prefix || (top == prefix && eq + __popcll(e & below) < need));
-    if ((s >> lane) & 1) kept[at + __popcll(s & below)] = i;
+    unsigned long long s = __ballot(top >= least);
+    if (!all) {
+      const unsigned long long e = __ballot(top == prefix);
+      if (e) {
+        s |= e & __ballot(eq + before(e) < need);
+        eq += __popcll(e);
+      }
+    }
+    if ((s >> lane) & 1) kept[at + before(s)] = i;
     at += __popcll(s);
-    eq += __popcll(e);
   });
 }
 
@@ -225,6 +233,9 @@ int fl_evict(const fl_rows* k, const fl_rows* v, float* weights, int32_t n_outer
   else if (per <= 8) hipLaunchKernelGGL(k_evict_select<8>, dim3(heads), dim3(ES_NT), 0, s, a);
   else if (per <= 16) hipLaunchKernelGGL(k_evict_select<16>, dim3(heads), dim3(ES_NT), 0, s, a);
   else if (per <= 32) hipLaunchKernelGGL(k_evict_select<32>, dim3(heads), dim3(ES_NT), 0, s, a);
+  // held, a lane's 64 keys leave room for one workgroup a CU: 65536 slots of 2 heads 48 us, read again 56; 40000 of 320
+  // heads 204 and 189
+  else if (per <= 64 && heads <= 256) hipLaunchKernelGGL(k_evict_select<64>, dim3(heads), dim3(ES_NT), 0, s, a);
   else hipLaunchKernelGGL(k_evict_select<0>, dim3(heads), dim3(ES_NT), 0, s, a);
   if (k_out) {
     a.ko = static_cast<unsigned char*>(k_out->data), a.vo = static_cast<unsigned char*>(v_out->data), a.wo = weights_out;
