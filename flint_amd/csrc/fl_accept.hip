@@ -54,8 +54,8 @@ __device__ __forceinline__ double wave_dsum(double v) {
 }
 __device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
 
-// One workgroup per tree; its waves sum pieces of a row for the rejections that need Z
-// and for the last token. One CU reads a row of 49152 fp32 values and its draft row in 2.6 us at its 64 bytes a cycle,
+// One workgroup per tree; its waves sum pieces of a row for the rejections that need Z and for the last token (without draft
+// probabilities a node's row is summed once, and a rejected token taken off). One CU reads a row of 49152 fp32 values and its draft row in 2.6 us at its 64 bytes a cycle,
 // about what one exchange between workgroups costs, so a row stays with one. (Held in registers between two sums, the
 // row's 96 values a lane and their conversions spilled.)
 template <bool BF, bool DRAFT>
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
     return w > 0.0 ? w : 0.0;
   };
   // This wave's sum of w over [s0, s1), U loads of a lane and row in flight. Loads past the end cost as much as others, so
-  // U is what a piece needs; the next U in flight behind the sums cost more than they gave (48 trees 23 us a call, 21).
+  // U is what a piece needs; the next U in flight behind the sums cost more than they gave (48 trees 23 us a call, 21 without).
   auto piece = [&](auto unroll, int s0, int s1) -> double {
     constexpr int U = decltype(unroll)::value;
     double s[4] = {};

@@ -33,11 +33,11 @@ __device__ __forceinline__ uint32_t w_key(float w) {
 // The counts end where a bin's keys all stay. A lane holds its E keys in registers; E = 0: more slots, read again for
 // every walk, eight loads in flight. Bound by the walks, two to four counts and the places, at some 24 clocks of the CU
 // for 64 keys (with four counts and a walk for the sums above: 8192 slots of 8 heads 11.9 us with the move of 1024
-// rows, now 10.8; 131072 of 2 heads 145, now 103).
+// rows, now 10.8; 131072 of 2 heads 145, now 99).
 template <int E>
 __global__ __launch_bounds__(ES_NT) void k_evict_select(EvictArgs a) {
-  __shared__ __align__(16) int hist[ES_NW][256];
   constexpr int U = 8;
+  __shared__ __align__(16) int hist[ES_NW][256];
   __shared__ int sum[256], sel[2], above_w[ES_NW], equal_w[ES_NW];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.x;
   const float* w = a.w + (int64_t)head * a.slots;
@@ -233,8 +233,8 @@ int fl_evict(const fl_rows* k, const fl_rows* v, float* weights, int32_t n_outer
   else if (per <= 8) hipLaunchKernelGGL(k_evict_select<8>, dim3(heads), dim3(ES_NT), 0, s, a);
   else if (per <= 16) hipLaunchKernelGGL(k_evict_select<16>, dim3(heads), dim3(ES_NT), 0, s, a);
   else if (per <= 32) hipLaunchKernelGGL(k_evict_select<32>, dim3(heads), dim3(ES_NT), 0, s, a);
-  // held, a lane's 64 keys leave room for one workgroup a CU: 65536 slots of 2 heads 48 us, read again 56; 40000 of 320
-  // heads 204 and 189
+  // held, a lane's 64 keys leave room for one workgroup a CU: 65536 slots of 2 heads 47 us, read again 56; 40000 of 320
+  // heads 204 and 187
   else if (per <= 64 && heads <= 256) hipLaunchKernelGGL(k_evict_select<64>, dim3(heads), dim3(ES_NT), 0, s, a);
   else hipLaunchKernelGGL(k_evict_select<0>, dim3(heads), dim3(ES_NT), 0, s, a);
   if (k_out) {
