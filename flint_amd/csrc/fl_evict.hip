@@ -233,9 +233,9 @@ int fl_evict(const fl_rows* k, const fl_rows* v, float* weights, int32_t n_outer
   else if (per <= 8) hipLaunchKernelGGL(k_evict_select<8>, dim3(heads), dim3(ES_NT), 0, s, a);
   else if (per <= 16) hipLaunchKernelGGL(k_evict_select<16>, dim3(heads), dim3(ES_NT), 0, s, a);
   else if (per <= 32) hipLaunchKernelGGL(k_evict_select<32>, dim3(heads), dim3(ES_NT), 0, s, a);
-  // held, a lane's 64 keys leave room for one workgroup a CU: 65536 slots of 2 heads 47 us, read again 56; 40000 of 320
-  // heads 204 and 187
-  else if (per <= 64 && heads <= 256) hipLaunchKernelGGL(k_evict_select<64>, dim3(heads), dim3(ES_NT), 0, s, a);
+  // held, a lane's 48 keys leave room for one workgroup a CU: 40000 slots of 2 heads 27 us, read again 37; of 320 heads 191
+  // and 187 (64 keys spill)
+  else if (per <= 48 && heads <= 256) hipLaunchKernelGGL(k_evict_select<48>, dim3(heads), dim3(ES_NT), 0, s, a);
   else hipLaunchKernelGGL(k_evict_select<0>, dim3(heads), dim3(ES_NT), 0, s, a);
   if (k_out) {
     a.ko = static_cast<unsigned char*>(k_out->data), a.vo = static_cast<unsigned char*>(v_out->data), a.wo = weights_out;
