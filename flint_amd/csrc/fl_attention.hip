@@ -569,7 +569,7 @@ __global__ __launch_bounds__(256) void k_attn_merge(AttnArgs a) {
 // and registers are rows: the sum over rows stays in the lane. A wave holds 64 keys of a key head in its MFMA operands
 // and walks over the rows, 32 at a time, which come in whole cache lines, the next 32 in flight, and turn into the
 // operand layout in a piece of LDS that only this wave uses (loaded in that layout, 16 rows to an instruction's quarter,
-// they took 64 cycles an instruction: 512 tokens over 8704 keys 79 us). SPLIT: the four waves of a workgroup share
+// they took 64 cycles an instruction: 512 tokens over 8704 keys 76 us). SPLIT: the four waves of a workgroup share
 // 64 keys and take the row tiles in turn (many rows), else each has 64 keys of its own. One workgroup writes a key, in a
 // fixed order: no atomics, the same bits every time.
 template <bool H, int D, bool SPLIT>
