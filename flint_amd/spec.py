@@ -1,4 +1,4 @@
-"""Speculative greedy decoding over fl_verify: the chain loop (reference spec_mega.py:89-117) and
+"""Speculative decoding, greedy or sampled, over fl_verify: the chain loop (reference spec_mega.py:89-117) and
 the tree loop with KV compaction (reference spec_tree.py:85-133).
 
 Each pass feeds the pending token (the root, not yet in the cache) plus a draft to one verify
