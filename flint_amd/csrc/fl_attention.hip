@@ -6,9 +6,10 @@
 // is online, per lane, in the log2 domain (p = exp2(s c - m), c = scale log2 e), in fp32; O^T += V^T P^T takes a step's
 // 16 keys in the order in which the score registers already hold them, so P never crosses lanes. V^T comes out of LDS
 // through the transposing read (a 16-lane group receives four rows of 16 values by column). P is split into two 16-bit
-// terms, 2^-17 of a weight together in bf16: with one alone 1024 tokens behind 4096 take 82 us in place of 102, but their
+// terms. In bf16 they leave 2^-17 of a weight: with one alone 1024 tokens behind 4096 take 82 us in place of 102, but their
 // outputs lie 1.3 times as far from 64 bits (0.0021 in place of 0.0016 of their norm), and the model's attention is fp32
-// times V.
+// times V. In fp16 they share steps of 2^-24, so P is held near the top of fp16's range, tile by tile (softmax_pv): they
+// leave 2^-28 of the largest weight of a tile's row, and 2^-36 of the row's largest.
 #include <algorithm>
 #include "fl_gemm.h"
 #include "fl_state.h"
@@ -160,24 +161,38 @@ __device__ __forceinline__ uint2 tr4(const unsigned char* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds4*)(p)));
 }
 
-// The state of 32 rows: this lane's row's running max (log2 domain), sum, and O^T (dims 32 d + 8 (i / 4) + 4 hf + i % 4)
-template <int DT>
+// The state of 32 rows: this lane's row's reference (log2 domain), sum, and O^T (dims 32 d + 8 (i / 4) + 4 hf + i % 4),
+// the last two in units of 2^m; fp16 also has an integer near the row's largest score, to which its reference returns at
+// the end
+template <bool H, int DT>
 struct Rows {
   fl_f32x16 o[DT];
-  float m, l;
+  float m, l, top;
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-    m = -INFINITY, l = 0.0f;
+    m = top = -INFINITY, l = 0.0f;
+  }
+  __device__ __forceinline__ void refer_to(float mn) {
+    const float corr = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= corr;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] *= corr;
+  }
+  __device__ __forceinline__ void finish() {
+    if constexpr (H) refer_to(top);
   }
 };
 
 // One tile of 32 KT keys' scores into the state. s: raw scores, s[kt][i] of key 32 kt + 8 (i / 4) + 4 hf + i % 4, -inf
 // where not seen; vt: the tile's V in LDS.
 template <bool H, int D, int KT>
-__device__ __forceinline__ void softmax_pv(fl_f32x16 (&s)[KT], Rows<D / 32>& st, float sc, const unsigned char* vt) {
+__device__ __forceinline__ void softmax_pv(fl_f32x16 (&s)[KT], Rows<H, D / 32>& st, float sc, const unsigned char* vt) {
   constexpr int DT = D / 32;
   const int lane = threadIdx.x & 63, i16 = lane & 15, hf = lane >> 5;
   float mx = -INFINITY;
@@ -186,16 +201,24 @@ __device__ __forceinline__ void softmax_pv(fl_f32x16 (&s)[KT], Rows<D / 32>& st,
 #pragma unroll
     for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(s[kt][i], s[kt][i + 1]), mx);  // one three-way maximum each
   mx = xor32_max(mx) * sc;
-  // m is any reference near the maximum: it follows only where a row's passed it by 2^8 (p and l stay far inside their
-  // range), which after a row's first tile hardly happens; some row of 32 has a new maximum in half of all tiles
-  if (__any(mx > st.m + 8.0f)) {
-    const float mn = fmaxf(st.m, mx), corr = st.m == mn ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
-    st.m = mn;
-    st.l *= corr;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) st.o[d][i] *= corr;
+  if constexpr (H) {
+    // m is an integer, 11 below the scores of some tile: p lies below 2^15 (fp16 ends at 2^16) and a tile's largest at
+    // 2^3 or more, so that what lies far below a row's maximum keeps its bits. It follows a tile's maximum both ways
+    // (o and l then grow by that power of two), down to 40 below the row's: 2^-76 of its largest weight may be dropped,
+    // and o stays below 2^(56 + 16) times the number of keys. 16 trees of 13 behind 8011 keys 59 us; with the reference
+    // of bf16, which lost those, 57.
+    if (__any(fabsf(mx - (st.m + 9.0f)) > 6.0f)) {
+      const float mn = floorf(fmaxf(mx, st.top - 40.0f)) - 11.0f;
+      const bool move = mx > st.m + 15.0f || (mx > -INFINITY && mn < st.m - 8.0f);
+      if (__any(move)) {
+        st.refer_to(move ? mn : st.m);
+        st.top = fmaxf(st.top, st.m + 11.0f);
+      }
+    }
+  } else {
+    // m is any reference near the maximum: it follows only where a row's passed it by 2^8 (p and l stay far inside their
+    // range), which after a row's first tile hardly happens; some row of 32 has a new maximum in half of all tiles
+    if (__any(mx > st.m + 8.0f)) st.refer_to(fmaxf(st.m, mx));
   }
   const float mu = st.m == -INFINITY ? 0.0f : st.m;
   const int row = 4 * hf + (i16 >> 2);
@@ -236,7 +259,7 @@ __device__ __forceinline__ void softmax_pv(fl_f32x16 (&s)[KT], Rows<D / 32>& st,
 // place, and here they are added to the rows that see them (an infinity or a NaN stays one under any weight).
 template <bool H, int D>
 __device__ __forceinline__ void add_not_finite(const AttnArgs& a, const uint8_t* mask, const uint16_t* v, int pos, int kb,
-                                               int kend, int tk, int t, Rows<D / 32>& st) {
+                                               int kend, int tk, int t, Rows<H, D / 32>& st) {
   const int hf = (threadIdx.x & 63) >> 5;
   const auto vr = tile_rsrc(v, a.v_s, kb, kend, tk, D);
 #pragma unroll 1
@@ -258,7 +281,7 @@ __device__ __forceinline__ void add_not_finite(const AttnArgs& a, const uint8_t*
 }
 
 template <bool H, int D>
-__device__ __forceinline__ void store_rows(const AttnArgs& a, const Rows<D / 32>& st, int b, int g, int part, int row, bool bad) {
+__device__ __forceinline__ void store_rows(const AttnArgs& a, const Rows<H, D / 32>& st, int b, int g, int part, int row, bool bad) {
   if (row >= a.R) return;
   const int hf = (threadIdx.x & 63) >> 5, t = row / a.rep, head = g * a.rep + row % a.rep;
   if (a.parts == 1) {
@@ -317,7 +340,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_few(AttnArgs a) {
   const uint16_t* qp = a.q + (int64_t)b * a.q_b + (int64_t)t * a.q_m + (int64_t)head * a.q_h;
 #pragma unroll
   for (int s = 0; s < ST; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + s * 16 + hf * 8);
-  Rows<DT> st;
+  Rows<H, DT> st;
   st.clear();
   unsigned char* vt = smem + wave * VB;
   unsigned char* vw = vt + v_at<D>(lane / CH, lane % CH);  // a sweep of 64 lanes is 1 KB of rows, at the same swizzle
@@ -367,6 +390,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_few(AttnArgs a) {
     softmax_pv<H, D, KT>(s, st, a.sc, vt);
     if (odd) add_not_finite<H, D>(a, mask, vp, sp.pos, kb, sp.kend, TK, t, st);
   }
+  st.finish();
   // the waves' states, one 32-dim tile at a time: each wave sums its share of the registers over the waves
   static_assert(16 % NW == 0 && 16 / NW == 2, "two registers each");
   const int i0 = 2 * wave;  // dims 32 d + 8 (i0 / 4) + 4 hf + i0 % 4 and the next
@@ -453,7 +477,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_many(AttnArgs a) 
   const uint16_t* qp = a.q + (int64_t)b * a.q_b + (int64_t)t * a.q_m + (int64_t)(g * a.rep + rowc % a.rep) * a.q_h;
 #pragma unroll
   for (int s = 0; s < ST; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + s * 16 + hf * 8);
-  Rows<DT> st;
+  Rows<H, DT> st;
   st.clear();
   // 16-byte chunk i * 256 + tid of a tile's LDS: a row of it, and there the chunk that the swizzle puts in its place
   auto k_at = [&](int key, int ch) {  // 16 rows' chunk on 16 different places
@@ -511,6 +535,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_many(AttnArgs a) 
     stage = stage == NS - 1 ? 0 : stage + 1;
   }
   wait_loads<0>();  // what was loaded ahead has landed before the LDS is given away
+  st.finish();
   store_rows<H, D>(a, st, b, g, part, row, sp.keys < 0);
 }
 

@@ -354,3 +354,94 @@ def test_a_query_that_is_no_number_reaches_what_its_node_sees(dev, m, rep, dim):
     qd = q.to(dev).transpose(1, 2).contiguous().transpose(1, 2)
     got = attention_weights(qd, k.to(dev), l.float().to(dev), pos).cpu()
     assert torch.equal(got.isnan(), want.isnan())
+
+
+FAR = [  # b, m, heads, groups, dim, ctx: either kernel, one part of the keys and many
+    (1, 1, 8, 2, 64, 64), (1, 1, 8, 2, 64, 1100), (1, 1, 8, 2, 64, 20000), (1, 1, 8, 2, 128, 30000), (1, 6, 8, 2, 64, 60000),
+    (1, 40, 8, 2, 64, 5000), (1, 16, 8, 1, 128, 9000), (8, 300, 48, 48, 64, 1500),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gap", [10.0, 15.0, 17.375, 20.0, 24.0])
+@pytest.mark.parametrize("shape", FAR)
+def test_weights_far_below_a_leading_key(dev, shape, gap, dtype):
+    """Three leading keys whose values are 0, all others `gap` (or, of odd heads, half of that) below them: what these
+    add up to, to the output's own precision.
+
+    Scores are exact here (powers of two and multiples of 1/64). A weight's exponent and the factors that join parts have
+    arguments below 64 in log2: 2^-19 each, three of them and the exponential's own error below 2^-16 of the weight. Its
+    two terms leave 2^-17 of it in bf16; in fp16 2^-28 of the largest weight of its tile of up to 64 keys, which in the three
+    tiles of a leading key is 2^-36 of that key's, elsewhere far below 2^-17 of the sum. fp32 sums in sequence: n / 8
+    additions, at 2^-24 each, of the numerator and of the denominator."""
+    from flint_amd.attention import tree_attention
+    b, m, heads, groups, dim, ctx = shape
+    rep, n = heads // groups, ctx + m
+    g = torch.Generator(device=dev).manual_seed(ctx)
+    q = torch.zeros(b, m, heads, dim, device=dev)
+    q[..., 0] = 8.0
+    if rep > 1:
+        q[:, :, 1::2, 0] = 4.0
+    k = torch.zeros(b, groups, n, dim, device=dev)
+    k[..., 0] = torch.randint(-32, 33, (b, groups, n), generator=g, device=dev) / 64
+    v = 32 * (0.5 + torch.rand(b, groups, n, dim, generator=g, device=dev))
+    lead = [0, ctx // 2, ctx - 1]
+    k[:, :, lead, 0] = gap
+    v[:, :, lead] = 0
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    assert (k[:, :, lead, 0] == gap).all()
+    out, lse = tree_attention(q, k, v, ctx, None, 0.125, True)
+    hidden = torch.arange(n, device=dev) > ctx + torch.arange(m, device=dev)[:, None]
+    vmax = 48.0
+    for s in range(b):
+        for j in range(groups):
+            sc = torch.matmul(q[s, :, j * rep:(j + 1) * rep].transpose(0, 1).double(), k[s, j].double().t().contiguous()) * 0.125
+            sc = sc.masked_fill(hidden, -math.inf)
+            o = torch.matmul(torch.softmax(sc, -1), v[s, j].double()).transpose(0, 1)
+            rel = 2 * (2.0 ** -16 + 2.0 ** -17 + n / 8 * 2.0 ** -24)
+            tol = torch.finfo(dtype).eps / 2 * o * (1 + rel) + rel * o + (3 * 64 * 2.0 ** -36 * vmax + 2.0 ** -25 if dtype == torch.float16 else 0.0)
+            err = (out[s, :, j * rep:(j + 1) * rep].double() - o).abs()
+            assert (err <= tol).all(), f"{float((err / tol).max()):.2f} x, {float((err / o).max()):.2e} of the value"
+            l = torch.logsumexp(sc, -1).t()
+            assert ((lse[s, :, j * rep:(j + 1) * rep].double() - l).abs() <= 2.0 ** -16 + n / 8 * 2.0 ** -24 + 2.0 ** -21 * l.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("order", ["rising", "falling", "back and forth"])
+@pytest.mark.parametrize("m,heads,groups,dim,ctx", [(1, 4, 2, 64, 1400), (1, 4, 4, 64, 9000), (40, 4, 2, 64, 5000), (16, 8, 1, 128, 1000)])
+def test_scores_that_rise_and_fall(dev, m, heads, groups, dim, ctx, order, dtype):
+    """Levels of scores over 60, a hundred slots each, the keys of the highest level with values of 0: rel as
+    above, and what the highest level's own tiles (two of 64 keys at 100 slots) leave, 2^-36 of its weight each."""
+    from flint_amd.attention import tree_attention
+    n = ctx + m
+    g = torch.Generator(device=dev).manual_seed(ctx)
+    level = torch.arange(n, device=dev) // 100
+    steps = int(level[-1]) + 1
+    height = torch.linspace(0, 1, steps, device=dev)
+    if order == "falling":
+        height = height.flip(0)
+    elif order == "back and forth":
+        height = torch.where(torch.arange(steps, device=dev) % 2 == 0, height, 1 - height)
+    top = int(height.argmax())
+    # from 0 to 44 below the highest level, that one 16 above the next
+    score = ((height * 28).round() + 16 * (torch.arange(steps, device=dev) == top))[level]
+    q = torch.zeros(1, m, heads, dim, device=dev)
+    q[..., 0] = 8.0
+    k = torch.zeros(1, groups, n, dim, device=dev)
+    k[..., 0] = score
+    v = 32 * (0.5 + torch.rand(1, groups, n, dim, generator=g, device=dev))
+    v[:, :, level == top] = 0
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    out, lse = tree_attention(q, k, v, ctx, None, 0.125, True)
+    rep = heads // groups
+    hidden = torch.arange(n, device=dev) > ctx + torch.arange(m, device=dev)[:, None]
+    for j in range(groups):
+        sc = torch.matmul(q[0, :, j * rep:(j + 1) * rep].transpose(0, 1).double(), k[0, j].double().t().contiguous()) * 0.125
+        sc = sc.masked_fill(hidden, -math.inf)
+        o = torch.matmul(torch.softmax(sc, -1), v[0, j].double()).transpose(0, 1)
+        rel = 2 * (2.0 ** -16 + 2.0 ** -17 + n / 8 * 2.0 ** -24)
+        # a row's sum is its highest weight or more, so what is left out of a weight is 2^-36 of the sum at most
+        tol = torch.finfo(dtype).eps / 2 * o * (1 + rel) + rel * o + (3 * 64 * 2.0 ** -36 * 48 + 2.0 ** -25 if dtype == torch.float16 else 0.0)
+        err = (out[0, :, j * rep:(j + 1) * rep].double() - o).abs()
+        assert (err <= tol).all(), f"{float((err / tol).max()):.2f} x"
+        assert ((lse[0, :, j * rep:(j + 1) * rep].double() - torch.logsumexp(sc, -1).t()).abs() <= 2.0 ** -14 + n / 8 * 2.0 ** -24).all()
