@@ -93,7 +93,9 @@ def tree_attention(q, k_cache, v_cache, pos, mask=None, scale=None, return_lse=F
     contiguous last dimension and the rest on 16 bytes. pos: cached keys before node 0, an int or a device int per sequence (one outside 0 ..
     slots - M gives NaN). mask bool or uint8 [M, M] or [B, M, M]: node i sees node j (None: a chain, j <= i).
     scale: of the scores, positive (None: dim ** -0.5). Returns the output in q's shape and type and, with return_lse, the log sum
-    exp of the scaled scores (fp32 [B, M, heads]). A node that sees nothing gives 0 and -inf. No gradient."""
+    exp of the scaled scores (fp32 [B, M, heads]). A node that sees nothing gives 0 and -inf; an infinity or a NaN in the
+    value of a slot that it sees makes that dimension the same, however small its weight (infinities of both signs: NaN). No
+    gradient."""
     if _tree_attention_fast is not None and q.is_cuda:
         at, p0 = (None, pos) if type(pos) is int else (pos, 0)
         if at is None or type(at) is torch.Tensor:

@@ -255,30 +255,49 @@ __device__ __forceinline__ void softmax_pv(fl_f32x16 (&s)[KT], Rows<H, D / 32>& 
   st.l += xor32_sum((ps[0] + ps[1]) + (ps[2] + ps[3]));
 }
 
-// Values of V that are not finite, in slots that some rows see and others do not: the tile's V has zeros in their
-// place, and here they are added to the rows that see them (an infinity or a NaN stays one under any weight).
-template <bool H, int D>
-__device__ __forceinline__ void add_not_finite(const AttnArgs& a, const uint8_t* mask, const uint16_t* v, int pos, int kb,
-                                               int kend, int tk, int t, Rows<H, D / 32>& st) {
+// Values of V that are not finite, once a wave's keys (tiles of TK from kb0 on, `step` apart) are through: a row that sees
+// one has it in that dimension under any weight, where the sums may hold 0 times infinity, or what a second term of the
+// other sign or a factor of 0 left of it. Any that met a matrix instruction shows in o; of those that were made zeros
+// `odd` tells. Rows whose sum l is no number are none anyway.
+template <bool H, int D, int TK>
+__device__ __forceinline__ void settle_not_finite(const AttnArgs& a, const uint8_t* mask, const uint16_t* v, int pos, int kb0, int kend,
+                                                  int step, int t, bool odd, Rows<H, D / 32>& st) {
   const int hf = (threadIdx.x & 63) >> 5;
-  const auto vr = tile_rsrc(v, a.v_s, kb, kend, tk, D);
+  float z[4] = {};
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i & 3] = __builtin_fmaf(st.o[d][i], 0.0f, z[i & 3]);
+  const bool none = __builtin_isfinite((z[0] + z[1]) + (z[2] + z[3])) || !__builtin_isfinite(st.l);
+  if (__builtin_expect(!__any(odd || !none), 1)) return;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) {
+    float sum[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] = 0.0f;
 #pragma unroll 1
-  for (int key = max(kb, pos); key < min(kend, kb + tk); ++key) {
-    const int j = key - pos;
-    const bool seen = mask ? mask[(uint32_t)t * (uint32_t)a.m + (uint32_t)j] != 0 : j <= t;
-    const uint32_t off = seen ? (uint32_t)((key - kb) * a.v_s + 4 * hf) * 2u : 0xFFFFFF00u;  // not seen: zeros
+    for (int kb = kb0; kb < kend; kb += step) {
+      const auto vr = tile_rsrc(v, a.v_s, kb, kend, TK, D);
+#pragma unroll 1
+      for (int key = kb; key < min(kend, kb + TK); ++key) {
+        const int j = key - pos;
+        const bool seen = j < 0 || (mask ? mask[(uint32_t)t * (uint32_t)a.m + (uint32_t)j] != 0 : j <= t);
+        const uint32_t off = seen ? (uint32_t)((key - kb) * a.v_s + 4 * hf) * 2u : 0xFFFFFF00u;  // not seen: zeros
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+        for (int e = 0; e < 4; ++e) {
+          const uint2 w = buf_ld64(vr, off + 64 * d + 16 * e);
+          const float x[4] = {lo16<H>(w.x), hi16<H>(w.x), lo16<H>(w.y), hi16<H>(w.y)};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint2 w = buf_ld64(vr, off + 64 * d + 16 * e);
-        const float x[4] = {lo16<H>(w.x), hi16<H>(w.x), lo16<H>(w.y), hi16<H>(w.y)};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st.o[d][4 * e + i] += __builtin_isfinite(x[i]) ? 0.0f : x[i];
-        asm volatile("" ::: "memory");
+          for (int i = 0; i < 4; ++i) sum[4 * e + i] += __builtin_isfinite(x[i]) ? 0.0f : x[i];
+        }
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) st.o[d][i] = sum[i] == 0.0f ? st.o[d][i] : sum[i];
   }
 }
+// a part's share of a sum: what is not finite stays that under any factor
+__device__ __forceinline__ float share(float f, float x) { return __builtin_isfinite(x) ? f * x : x; }
 
 template <bool H, int D>
 __device__ __forceinline__ void store_rows(const AttnArgs& a, const Rows<H, D / 32>& st, int b, int g, int part, int row, bool bad) {
@@ -356,17 +375,17 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_few(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) vf[i] = tile_ld(vr, vo, i * vstep);
   };
+  bool odd = false;  // some node's V is not finite
   int kb = sp.kb0 + wave * TK;
   if (kb < sp.kend) load(kb);
   for (; kb < sp.kend; kb += NW * TK) {
     const bool nodes = kb + TK > sp.pos;  // some keys of the tile are nodes (or lie behind the end)
-    bool odd = false;
     if (nodes) {
       bool fin = true;
 #pragma unroll
       for (int i = 0; i < 8; ++i) fin = fin && finite16<H>(vf[i]);
-      odd = __any(!fin);
-      if (odd) {
+      if (__any(!fin)) {
+        odd = true;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int key = kb + lane / CH + i * (64 / CH);
@@ -388,9 +407,9 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_few(AttnArgs a) {
     load(kn < sp.kend ? kn : sp.kend);  // behind the end: zeros, nothing read
     if (nodes) hide<KT>(a, mask, sp.pos, sp.kend, kb, t, s);
     softmax_pv<H, D, KT>(s, st, a.sc, vt);
-    if (odd) add_not_finite<H, D>(a, mask, vp, sp.pos, kb, sp.kend, TK, t, st);
   }
   st.finish();
+  settle_not_finite<H, D, TK>(a, mask, vp, sp.pos, sp.kb0 + wave * TK, sp.kend, NW * TK, t, odd, st);
   // the waves' states, one 32-dim tile at a time: each wave sums its share of the registers over the waves
   static_assert(16 % NW == 0 && 16 / NW == 2, "two registers each");
   const int i0 = 2 * wave;  // dims 32 d + 8 (i0 / 4) + 4 hf + i0 % 4 and the next
@@ -421,6 +440,15 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_few(AttnArgs a) {
       o1 += e * all[(w * 18 + i0 + 1) * 64];
     }
     ll = l;
+    if (__builtin_expect(__any(!__builtin_isfinite(o0 + o1)), 0)) {
+      o0 = o1 = 0.0f;
+#pragma unroll 1
+      for (int w = 0; w < NW; ++w) {
+        const float e = __builtin_amdgcn_exp2f(all[(w * 18 + 16) * 64] - mu);
+        o0 += share(e, all[(w * 18 + i0) * 64]);
+        o1 += share(e, all[(w * 18 + i0 + 1) * 64]);
+      }
+    }
     const int dim = 32 * d + 8 * (i0 >> 2) + 4 * hf + (i0 & 3);
     if (row < a.R) {
       if (a.parts == 1) {
@@ -451,7 +479,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_many(AttnArgs a) 
   constexpr int TK = 4096 / D, KT = TK / 32, ST = D / 16, DT = D / 32, CH = D / 8, NS = 3;
   constexpr int TILE = TK * D * 2, PW = TILE / 4096;  // bytes of K or V of a round (8 KB); 1 KB loads of a wave of each
   __shared__ __align__(16) unsigned char ring[NS][2][TILE];
-  __shared__ int odd[NS];
+  __shared__ int odd;  // some node's V is not finite
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hf = lane >> 5;
   int rest = blockIdx.x;
   const int g = rest % a.groups;
@@ -498,7 +526,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_many(AttnArgs a) 
 #pragma unroll
     for (int i = 0; i < PW; ++i) dma_1k(vw, at + TILE + i * 4096, vo, i * vstep);
   };
-  if (tid < NS) odd[tid] = 0;
+  if (tid == 0) odd = 0;
   __syncthreads();
   load(sp.kb0, 0);
   load(sp.kb0 + TK, 1);
@@ -512,7 +540,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_many(AttnArgs a) 
         uint4* x = reinterpret_cast<uint4*>(vs + i * 4096 + tid * 16);
         if (kb + k0 + i * (256 / CH) >= sp.pos && !finite16<H>(*x)) {
           *x = only_finite<H>(*x);
-          odd[stage] = kb + 1;
+          odd = 1;  // read behind the last round's barrier
         }
       }
     }
@@ -530,12 +558,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_many(AttnArgs a) 
       }
       if (kb + TK > wfull) hide<KT>(a, mask, sp.pos, kend, kb, t, s);
       softmax_pv<H, D, KT>(s, st, a.sc, vs);
-      if (odd[stage] == kb + 1) add_not_finite<H, D>(a, mask, vp, sp.pos, kb, kend, TK, t, st);
     }
     stage = stage == NS - 1 ? 0 : stage + 1;
   }
   wait_loads<0>();  // what was loaded ahead has landed before the LDS is given away
   st.finish();
+  settle_not_finite<H, D, TK>(a, mask, vp, sp.pos, sp.kb0, wend, TK, t, odd != 0, st);
   store_rows<H, D>(a, st, b, g, part, row, sp.keys < 0);
 }
 
@@ -573,8 +601,21 @@ __global__ __launch_bounds__(256) void k_attn_merge(AttnArgs a) {
     for (int i = 0; i < 4; ++i)
       if (g0 + i * PP < parts) {
         const float f = __shfl(e, (g0 + i * PP + p0) & 63, 64);
-        o += x[i] * (g0 + i * PP + p0 < parts ? f : 0.0f);
+        o += g0 + i * PP + p0 < parts ? x[i] * f : fl_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
+  }
+  if (__builtin_expect(__any(!__builtin_isfinite((o[0] + o[1]) + (o[2] + o[3]))), 0)) {
+    o = fl_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int g0 = 0; g0 < parts; g0 += 4 * PP) {
+      load(g0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = __shfl(e, (g0 + i * PP + p0) & 63, 64);
+        if (g0 + i * PP + p0 < parts)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[c] += share(f, x[i][c]);
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {

@@ -445,3 +445,38 @@ def test_scores_that_rise_and_fall(dev, m, heads, groups, dim, ctx, order, dtype
         err = (out[0, :, j * rep:(j + 1) * rep].double() - o).abs()
         assert (err <= tol).all(), f"{float((err / tol).max()):.2f} x"
         assert ((lse[0, :, j * rep:(j + 1) * rep].double() - torch.logsumexp(sc, -1).t()).abs() <= 2.0 ** -14 + n / 8 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,heads,groups,dim", [(1, 10, 2, 64), (6, 8, 2, 128), (40, 8, 2, 64), (150, 4, 1, 128)])
+@pytest.mark.parametrize("ctx", [70, 1500, 2300, 3100, 5200, 50000])
+def test_values_that_are_no_numbers(dev, ctx, m, heads, groups, dim, dtype):
+    """An infinity or a NaN in the value of a slot that a node sees makes that dimension of it the same, however small its
+    weight and however the keys are cut; infinities of both signs give NaN; the other dimensions keep their bits."""
+    from flint_amd.attention import tree_attention
+    n = ctx + m
+    g, q, k, v = make(1, m, heads, groups, dim, n, dtype, seed=ctx + m)
+    q, k, v = q.to(dev), k.to(dev), v.to(dev)
+    q[..., 0] = 2.0
+    k[:, :, 20, 0] = -60.0   # a weight of e^-15 and less
+    k[:, :, 21, 0] = -2000.0  # e^-500: no fp32 number
+    k[:, :, ctx // 2, 0] = 400.0  # takes all
+    clean, lse = tree_attention(q, k, v, ctx, None, 0.125, True)
+    bad = v.clone()
+    bad[:, :, 0, 1] = math.inf
+    bad[:, :, 20, 2] = -math.inf
+    bad[:, :, 21, 3] = math.inf
+    bad[:, :, ctx - 1, 4] = -math.inf
+    bad[:, :, ctx // 2, 5] = math.inf
+    bad[:, :, 5, 6], bad[:, :, ctx - 2, 6] = math.inf, -math.inf
+    bad[:, :, 33, 7] = math.nan
+    bad[:, :, ctx, 40] = -math.inf        # node 0
+    bad[:, :, 9, 41], bad[:, :, ctx, 41] = -math.inf, math.inf
+    bad[:, :, n - 1, 63] = math.inf       # the last node: seen by itself alone
+    out, l2 = tree_attention(q, k, bad, ctx, None, 0.125, True)
+    want = clean.clone()
+    for d, x in ((1, math.inf), (2, -math.inf), (3, math.inf), (4, -math.inf), (5, math.inf), (6, math.nan), (7, math.nan), (40, -math.inf), (41, math.nan)):
+        want[..., d] = x
+    want[:, -1, :, 63] = math.inf
+    assert torch.equal(l2, lse) and torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out.nan_to_num(0.0, 7e4, -7e4), want.nan_to_num(0.0, 7e4, -7e4))
