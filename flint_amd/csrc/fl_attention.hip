@@ -11,6 +11,7 @@
 // times V. In fp16 they share steps of 2^-24, so P is held near the top of fp16's range, tile by tile (softmax_pv): they
 // leave 2^-28 of the largest weight of a tile's row, and 2^-36 of the row's largest.
 #include <algorithm>
+#include <type_traits>
 #include "fl_gemm.h"
 #include "fl_state.h"
 
@@ -707,8 +708,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_weights(AttnArgs 
     for (; rt < tiles_r; rt += step) {
 #pragma unroll
       for (int i = 0; i < ST; ++i) *reinterpret_cast<uint4*>(mine + q_at(lane / CH + i * RS, lane % CH)) = qv[i];
-      // rows behind the last, and rows that see nothing, add nothing: e^-inf
-      if (hf == 0) refs[wave][r] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+      // rows behind the last, and rows that see nothing, add nothing, not even to a key whose score is no number
+      const bool gaps = __any(lse == -INFINITY);
+      if (hf == 0) refs[wave][r] = lse * 1.4426950408889634f;
       if (hf == 1) nodes[wave][r] = node;
       if (rt + step < tiles_r) load();
       fl_f32x16 s[KT];
@@ -724,7 +726,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_weights(AttnArgs 
       }
       // s[kt][i]: row 8 (i / 4) + 4 hf + i % 4 of the tile, key 32 kt + r
       // all of the tile's keys are cached, or (a chain) no later than the rows' first node
-      if (kb + 64 <= pos || (!mask && kb + 63 - pos <= rt * 32 / a.rep)) {
+      auto add_all = [&](auto with_gaps) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
           const fl_f32x4 ref = *reinterpret_cast<const fl_f32x4*>(&refs[wave][8 * q4 + 4 * hf]);
@@ -732,10 +734,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_weights(AttnArgs 
           for (int kt = 0; kt < KT; ++kt) {
             float p[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][4 * q4 + i], a.sc, -ref[i]));
+            for (int i = 0; i < 4; ++i) {
+              p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][4 * q4 + i], a.sc, -ref[i]));
+              if (decltype(with_gaps)::value) p[i] = ref[i] == -INFINITY ? 0.0f : p[i];
+            }
             acc[kt] += (p[0] + p[1]) + (p[2] + p[3]);
           }
         }
+      };
+      if (kb + 64 <= pos || (!mask && kb + 63 - pos <= rt * 32 / a.rep)) {
+        gaps ? add_all(std::true_type{}) : add_all(std::false_type{});
       } else {
         const auto mr = buf_rsrc(mask, mask ? (uint32_t)a.m * (uint32_t)a.m : 0u);
 #pragma unroll
@@ -752,7 +760,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_attn_weights(AttnArgs 
               const uint32_t off = j >= 0 && j < a.m && t[i] < a.m ? (uint32_t)t[i] * (uint32_t)a.m + (uint32_t)j : 0xFFFFFFF0u;
               const bool sees = mask ? __builtin_amdgcn_raw_buffer_load_b8(mr, off, 0, 0) != 0 : j <= t[i];
               // a key behind the end is a zero: no score of its own, and j <= t holds for no node
-              acc[kt] += j < 0 || (sees && j < a.m) ? p : 0.0f;
+              acc[kt] += ref[i] != -INFINITY && (j < 0 || (sees && j < a.m)) ? p : 0.0f;
             }
           }
         }

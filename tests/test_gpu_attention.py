@@ -480,3 +480,25 @@ def test_values_that_are_no_numbers(dev, ctx, m, heads, groups, dim, dtype):
     want[:, -1, :, 63] = math.inf
     assert torch.equal(l2, lse) and torch.equal(out.isnan(), want.isnan())
     assert torch.equal(out.nan_to_num(0.0, 7e4, -7e4), want.nan_to_num(0.0, 7e4, -7e4))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,heads,groups,dim", [(1, 5, 1, 64), (1, 10, 2, 128), (7, 6, 2, 64), (40, 4, 2, 64), (33, 3, 3, 128)])
+def test_a_key_that_no_row_can_weigh(dev, m, heads, groups, dim, dtype):
+    """A key whose scores are all -inf gathers 0, whatever stands behind the last row; a row whose lse is -inf adds nothing,
+    not even to a key whose score is no number."""
+    from flint_amd.attention import attention_weights, tree_attention
+    pos = 100
+    g, q, k, v = make(1, m, heads, groups, dim, pos + m + 3, dtype, seed=m)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    k[:, :, 17, 3] = -math.inf
+    k[:, :, pos, 3] = -math.inf
+    _, lse = tree_attention(q.to(dev), k.to(dev), v.to(dev), pos, return_lse=True)
+    got = attention_weights(q.to(dev), k.to(dev), lse, pos).cpu()
+    want = oracle.attention_weights(q, k, lse.cpu(), [pos], None, dim ** -0.5)
+    assert (want[:, :, [17, pos]] == 0).all() and (got[:, :, [17, pos]] == 0).all()
+    rel = score_error(q, k.nan_to_num(0, 0, 0), dim ** -0.5, dim) + 2.0 ** -21 * (float(lse.abs().max()) + 1) + m * heads * 2.0 ** -24
+    assert ((got.double() - want).abs() <= rel * want + 1e-30).all()
+    k[:, :, 17, 3], k[:, :, 18, 3], k[:, :, 19, 5] = math.inf, math.nan, math.inf
+    none = torch.full((1, m, heads), -math.inf, device=dev)
+    assert (attention_weights(q.to(dev), k.to(dev), none, pos) == 0).all()
