@@ -68,7 +68,9 @@ __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
   int cur = 0, n = 1, ngone = 0, turn = 0;  // node; nodes of the path; tokens rejected at the node
   bool fresh = true;                        // Z is the sum of w (or 1)
   double C = 0.0, Z = 1.0;
-  double rest = -1.0, last = 0.0;  // without draft probabilities: the row's sum (once known) without the tokens gone but the last; its p
+  // without draft probabilities: the row's sum (once known) without the tokens gone but the last, whose p is `last`; what it
+  // was when it was last summed
+  double rest = -1.0, last = 0.0, whole = 0.0;
   __amdgpu_buffer_rsrc_t pr, qr;
   auto open = [&] {
     pr = row_rsrc<BF>(a.p, prow + cur, V);
@@ -149,11 +151,12 @@ __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
         } else {  // the row's sum without the tokens gone
           if (rest < 0.0) {  // one token is gone: taken off here, as the later ones are one by one
             ngone = 0;
-            rest = total();
+            whole = rest = total();
             ngone = 1;
           }
           rest -= last;
-          rest = rest > 0.0 ? rest : 0.0;
+          // where little is left, the difference is what rounding left of it: summed anew (else it is good to 2^-40)
+          if (!(rest >= whole * 0x1p-10)) whole = rest = total();
           Z = rest;
         }
         fresh = true;

@@ -207,3 +207,26 @@ def test_many_children_of_one_node(dev, draft):
     ua = 1.0 - 0.01 * ua
     ua[1, 1000] = ua[2, 70] = 0.0
     check((p, q, tokens, parents, ua, us), dev)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [70, 3000, 49152])
+def test_what_little_is_left(dev, v, dtype):
+    """Rejected tokens that hold nearly all of a row: Z is the sum of what is left, not a difference of large numbers."""
+    m = 8
+    g = torch.Generator().manual_seed(v)
+    p = (torch.rand(6, 1, v, generator=g) + 0.5).repeat(1, m, 1) * 2.0 ** -70
+    p[:, :, 5] = 0.5
+    p[1:, :, 9] = 2.0 ** -30
+    p[2, :, 7] = 2.0 ** -50
+    p[3, :, 5] = 3.0e38
+    p[4, :, 5] = math.inf
+    p = p.to(dtype)
+    tokens = torch.tensor([[0, 5, 9, 7, 5, 11, 12, 13]] * 6, dtype=torch.int32)
+    parents = torch.tensor([[-1] + [0] * 7] * 6, dtype=torch.int32)
+    ua = torch.full((6, m), 1.0 - 2.0 ** -24)
+    ua[:, 5:] = torch.rand(6, 3, generator=g)
+    ua[5, 5:] = 1e-5
+    us = torch.rand(6, generator=g)
+    got = check((p, None, tokens, parents, ua, us), dev)
+    assert int(got.count[0]) == 1 and int(got.token[0]) not in (5, 9, 7)
