@@ -254,8 +254,8 @@ def score(model, tokens, top=0, head=None):
 
 
 def decode_one_token(model, x, input_pos, logits=None, temperature=None, top_k=None, seed=0):
-    """(next_token int32 device [1], logits) for one token at input_pos: greedy, or sampled when
-    temperature or top_k is given (reference generate.py:62-66, sample at :52-55), with the
+    """(next_token int32 device [1], logits) for one token at slot input_pos: greedy, or sampled when
+    temperature or top_k is given (reference generate.py:62-66, sample at :52-55), with its
     position as the noise counter."""
     pos = int(input_pos.reshape(-1)[0]) if torch.is_tensor(input_pos) else int(input_pos)
     if logits is None:
@@ -264,7 +264,7 @@ def decode_one_token(model, x, input_pos, logits=None, temperature=None, top_k=N
     tok = x.reshape(-1)[:1].to(torch.int32)
     if temperature is not None or top_k is not None:  # sampled in the decode launch itself
         t = 1.0 if temperature is None else temperature
-        model.decode_sample(tok, pos, t, top_k, seed=seed, offset=pos, token_out=out, logits=logits)
+        model.decode_sample(tok, pos, t, top_k, seed=seed, token_out=out, logits=logits)
     else:
         model.decode_step(tok, pos, token_out=out, logits=logits)
     return out, logits

@@ -230,8 +230,8 @@ class Transformer:
     def decode_sample(self, token, pos, temperature=1.0, top_k=None, seed=0, offset=None,
                       token_out=None, logits=None, feat=None):
         """One decode step whose token is sampled in the same launch (temperature / top-k, reference
-        engine/generate.py:38-55): Philox noise keyed by seed at counter offset (default: pos).
-        Returns token_out (int32 device [1])."""
+        engine/generate.py:38-55): Philox noise keyed by seed at counter offset (default: the token's position, which is
+        the slot pos + shift). Returns token_out (int32 device [1])."""
         if self._state is None:
             raise RuntimeError("call setup_caches first")
         if token_out is None:
@@ -242,7 +242,7 @@ class Transformer:
                 raise ValueError(f"{nm} must be a {dt} device tensor")
         if top_k is not None and int(top_k) < 1:
             raise ValueError("top_k must be >= 1")
-        off = int(pos) if offset is None else int(offset)
+        off = int(pos) + self.shift if offset is None else int(offset)
         _lib.call("fl_decode_sample", _lib.ctypes.byref(self._cw), self._state, _lib.ptr(token), int(pos),
                   float(temperature), int(top_k or 0), int(seed) & (2 ** 64 - 1), off & (2 ** 64 - 1),
                   _lib.ptr(token_out), _lib.ptr(logits), _lib.ptr(feat), _lib.stream_ptr())

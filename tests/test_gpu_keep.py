@@ -390,3 +390,33 @@ def test_short_prompt_far_into_the_cache(dev, pos):
     plain = eng.prefill_features(x, pos)
     assert float((feat.float() - plain.float()).norm() / plain.float().norm()) <= 2.0 ** -6
     eng.check()
+
+
+def test_noise_counts_positions(dev):
+    """decode_sample's default counter is the token's position, also where eviction has made slots and positions differ:
+    the same slot again, at another position, has other noise."""
+    args, _, eng, _ = make_pair("small", seed=3)
+    eng.setup_caches(1, 256)
+    x = tokens(args, 100, 1).to(dev)
+    w = eng.new_weights()
+    eng.prefill_weights(x, 0, w)
+    out = torch.empty(2, dtype=torch.int32, device=dev)
+    lg = torch.empty(args.vocab_size, dtype=torch.float32, device=dev)
+
+    def both(slot, position, seed):
+        eng.decode_sample(x[:1], slot, 50.0, None, seed=seed, token_out=out[:1], logits=lg)  # nearly flat: noise decides
+        eng.decode_sample(x[:1], slot, 50.0, None, seed=seed, offset=position, token_out=out[1:])
+        return out.tolist()
+    for seed in range(8):
+        a, b = both(100, 100, seed)
+        assert a == b
+    eng.evict(w, 100, 30, 4, 2)
+    slots = 0
+    from flint_amd.generate import decode_one_token
+    for seed in range(8):
+        a, b = both(30, 100, seed)
+        assert a == b == int(decode_one_token(eng, x[:1], 30, temperature=50.0, seed=seed)[0])
+        eng.decode_sample(x[:1], 30, 50.0, None, seed=seed, offset=30, token_out=out[:1])
+        slots += int(out[0]) == a
+    assert slots < 8
+    eng.check()
