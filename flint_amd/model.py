@@ -374,6 +374,8 @@ class Transformer:
         the kept slots, int32 [layers, key heads, keep]."""
         if self._state is None:
             raise RuntimeError("call setup_caches first")
+        if int(keep) < int(n) and int(n) + self.shift > self.packed.rope.shape[0]:
+            raise ValueError("more slots than there are positions")
         kept = evict(self.k_cache, self.v_cache, weights, n, keep, recent, sink)
         if n > kept.shape[-1]:
             self._set_shift(self.shift + int(n) - kept.shape[-1])

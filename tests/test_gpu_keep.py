@@ -420,3 +420,21 @@ def test_noise_counts_positions(dev):
         slots += int(out[0]) == a
     assert slots < 8
     eng.check()
+
+
+def test_more_slots_than_positions_are_refused_whole(dev):
+    """An eviction whose slots would lie behind the RoPE table is refused before a row moves."""
+    args, _, eng, _ = make_pair("tiny", seed=3)  # 1024 positions
+    eng.setup_caches(1, 1024)
+    x = tokens(args, 1020, 1).to(dev)
+    w = eng.new_weights()
+    eng.prefill_weights(x, 0, w)
+    eng.evict(w, 1020, 100, 10)
+    assert eng.shift == 920
+    k, v, w0 = eng.k_cache.clone(), eng.v_cache.clone(), w.clone()
+    for n in (105, 1024):
+        with pytest.raises(ValueError):
+            eng.evict(w, n, 50, 10)
+        assert eng.shift == 920 and torch.equal(eng.k_cache, k) and torch.equal(eng.v_cache, v) and torch.equal(w, w0)
+    eng.evict(w, 104, 50, 10)
+    assert eng.shift == 974
