@@ -208,3 +208,20 @@ def test_lowest_weights(dev, n, keep, low):
     kept = evict(k, v, w, n, keep, out=(torch.zeros(2, keep, 8, device=dev), torch.zeros(2, keep, 8, device=dev)))
     for h in range(2):
         assert kept[h].tolist() == oracle.kept_slots(w[h].tolist(), n, keep, 0, 0)
+
+
+@pytest.mark.parametrize("heads,n", [(2, 49152), (2, 49153), (257, 32769), (257, 40001), (257, 49152), (256, 49152)])
+def test_lengths_at_the_last_seams(dev, heads, n):
+    """Up to forty-eight keys of a lane in registers, for up to 256 heads: against a stable sort."""
+    from flint_amd.attention import evict
+    k, v = (torch.zeros(heads, n, 8, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    g = torch.Generator(device=dev).manual_seed(n)
+    w = (torch.rand(heads, n, generator=g, device=dev) * 50).floor()
+    k[..., 0] = w
+    keep = n // 3 + 1
+    score = w.clone()
+    score[:, :3], score[:, n - 5:] = math.inf, math.inf
+    want = score.sort(dim=1, descending=True, stable=True).indices[:, :keep].sort(dim=1).values
+    kept = evict(k, v, w, n, keep, recent=5, sink=3)
+    assert torch.equal(kept.long(), want)
+    assert torch.equal(k[:, :keep, 0], w[:, :keep].bfloat16()) and (w[:, keep:] == 0).all()

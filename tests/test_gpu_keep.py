@@ -438,3 +438,90 @@ def test_more_slots_than_positions_are_refused_whole(dev):
         assert eng.shift == 920 and torch.equal(eng.k_cache, k) and torch.equal(eng.v_cache, v) and torch.equal(w, w0)
     eng.evict(w, 104, 50, 10)
     assert eng.shift == 974
+
+
+def leads(eng, text, tok):
+    """How far the largest logit behind `text` lies before that of `tok` (0: it is a largest one)."""
+    from flint_amd.generate import prefill
+    lg = torch.empty(eng.config.vocab_size, dtype=torch.float32, device=eng.device)
+    prefill(eng, torch.tensor(text[:-1], dtype=torch.int32), 0)
+    eng.decode_step(torch.tensor(text[-1:], dtype=torch.int32, device=eng.device), len(text) - 1, logits=lg)
+    return float(lg.max() - lg[tok])
+
+
+@pytest.mark.parametrize("mode", ["chain", "tree"])
+def test_top_k_1_at_any_temperature(dev, mode):
+    """One candidate: whatever the temperature and the seed, each run is the greedy loop's up to a place where two logits
+    are equal, or an ulp of bf16 apart (the decode kernel's logits against the verify kernel's)."""
+    from flint_amd.spec import SpecDecoder
+    args, _, eng, _ = make_pair("small", seed=3)
+    p0 = (tokens(args, 12, 4).tolist() * 3)[:30]
+    greedy, _ = SpecDecoder(eng, k=4).generate(p0, 24, mode=mode)
+    runs = [greedy] + [SpecDecoder(eng, k=4).generate(p0, 24, mode=mode, top_k=1, temperature=t, seed=s)[0] for t, s in ((1.0, 7), (0.3, 8), (2.0, 9))]
+    assert len(greedy) >= 54
+    for run in runs[1:]:
+        at = next((i for i in range(54) if greedy[i] != run[i]), None)
+        log(f"{mode}: agree for {'all' if at is None else at}")
+        if at is not None:
+            gap = [leads(eng, greedy[:at], t) for t in (greedy[at], run[at])]
+            assert max(gap) <= 2.0 ** -7 * 8, gap  # logits below 8 here: two roundings to bf16
+
+
+class Interleaved:
+    """Proposes the text's own continuation, every node of it behind one that is no part of the text."""
+
+    def __init__(self, text, vocab, depth):
+        self.text, self.vocab, self.depth, self.at = text, vocab, depth, []
+
+    def tree(self, context, feats):
+        n = len(context)
+        self.at.append(n)
+        if list(context) != self.text[:n]:
+            return [], []
+        toks, pars, last = [], [], -1
+        for t in self.text[n:n + self.depth]:
+            toks += [(t + 1) % self.vocab, t]
+            pars += [last, last]
+            last = len(toks) - 1
+        return toks, pars
+
+
+class Junk:
+    def __init__(self, vocab):
+        self.vocab = vocab
+
+    def tree(self, context, feats):
+        return [(context[-1] + 1 + i) % self.vocab for i in range(40)], [-1] * 40
+
+
+def test_wide_trees_of_the_right_tokens(dev):
+    """A path of some forty nodes that are no prefix of the tree: the tokens are those that the 8-bit head puts first
+    behind the emitted text, and the cache rows those of that text."""
+    from flint_amd.quantize import linear_int8
+    from flint_amd.spec import SpecDecoder
+    args, _, eng, _ = make_pair("small", seed=3)
+    eng.setup_caches(1, 8)
+    head = eng.int8_head()
+    p0 = tokens(args, 20, 6).tolist()
+    text, slow = SpecDecoder(eng, draft=Junk(args.vocab_size), head=head).generate(p0, 60, mode="tree")
+    text = text[:80]
+    draft = Interleaved(text, args.vocab_size, 45)
+    out, fast = SpecDecoder(eng, draft=draft, head=head).generate(p0, 60, mode="tree")
+    got = out[:80]
+    log(f"{slow.passes} and {fast.passes} passes; agree for {next((i for i in range(80) if got[i] != text[i]), 80)} of 80")
+    assert max(b - a for a, b in zip(draft.at, draft.at[1:])) > 33  # a path that is moved in two pieces
+    n = 79
+    k = eng.k_cache[:, :, :n].clone()
+    feat = eng.prefill_features(torch.tensor(got[:n], dtype=torch.int32, device=dev), 0)
+    lg = linear_int8(feat, head.weight, head.scales, torch.float32)
+    top = lg.max(dim=1).values
+    said = lg[torch.arange(19, n), torch.tensor(got[20:], device=dev)]
+    # the same rows through products of other shapes: features some bf16 roundings apart
+    size = float(lg.abs().max())
+    assert (top[19:] - said <= 2.0 ** -5 * size).all(), (top[19:] - said).max()
+    assert (lg[19:].argmax(1).tolist() == got[20:]) or int((top[19:] - said > 0).sum()) <= 6
+    ref = eng.k_cache[:, :, :n].float()
+    rel = ((k.float() - ref).square().sum((0, 1, 3)) / ref.square().sum((0, 1, 3))).sqrt()  # of each slot
+    log(f"rows of the cache: worst slot {float(rel.max()):.2e} off")
+    assert (rel[20:n] <= 2.0 ** -4).all()
+    eng.check()
