@@ -177,8 +177,9 @@ def evict(k_cache, v_cache, weights, n, keep, recent=0, sink=0, out=None):
     k_cache, v_cache: device [..., slots, dim] of any type (rows of whole 16 bytes, at most 4096), strided in the
     leading dimensions and between slots; weights: contiguous fp32 [..., slots]. In place (out None) the weights move
     with the rows, those of keep .. n - 1 become 0, and the rows there stay what they were. out = (k, v) or (k, v, weights) of
-    [..., keep or more, ...] takes them instead and leaves the caches alone; it must not overlap them. Returns the
-    kept slots, int32 [..., keep], rising. keep >= n keeps all."""
+    [..., keep or more, ...] takes them instead and leaves the caches alone; it must not overlap them. What is written
+    must not overlap itself or each other either; K and V may lie between each other's rows. Returns the kept slots, int32
+    [..., keep], rising. keep >= n keeps all."""
     if _evict_fast is not None and k_cache.is_cuda and (out is None or len(out) in (2, 3)):
         ko, vo, wo = (None, None, None) if out is None else out if len(out) == 3 else (*out, None)
         kept = _evict_fast(k_cache, v_cache, weights, n, keep, recent, sink, ko, vo, wo,
@@ -220,9 +221,12 @@ def evict(k_cache, v_cache, weights, n, keep, recent=0, sink=0, out=None):
         for t in [x for x in out if x is not None]:
             for src in (k_cache, v_cache, weights):
                 _check(not _overlap(t, src), "out must not overlap the caches or the weights")
-    for t, other, name in ((k_cache, v_cache, "caches"),) if out is None else ((out[0], out[1], "out"),):
-        _check(t.numel() == 0 or t.data_ptr() != other.data_ptr(), f"{name}: K and V must not be the same memory")
-        _check(all(s for x in (t, other) for s, c in zip(x.stride()[:-1], x.shape) if c > 1), f"{name}: expanded dimensions cannot be written")
+    # what is written: no row twice, and none by two workgroups that do not wait for each other
+    written, name = ((k_cache, v_cache, weights), "caches") if out is None else ((*out, None)[:3], "out")
+    for t in written[:2]:
+        _check(t.numel() == 0 or _apart(t), f"{name}: rows that heads or slots share cannot be written")
+        _check(written[2] is None or not _overlap(t, written[2]), f"{name}: K and V must not overlap the weights")
+    _check(not _rows_meet(*written[:2]), f"{name}: K and V must not be the same memory")
     kept = torch.empty(*lead, keep, dtype=torch.int32, device=dev)
     if heads == 0 or n == 0:
         return kept
@@ -250,6 +254,34 @@ def evict(k_cache, v_cache, weights, n, keep, recent=0, sink=0, out=None):
                   sink, _lib.ptr(kept), ref[2], ref[3], _lib.ptr(w_out), 0 if out is None else out[0].shape[-2],
                   _lib.stream_ptr())
     return kept
+
+
+def _apart(t):
+    """Whether t's elements are all at addresses of their own, dimension within dimension (so that no row is another's)."""
+    extent = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s < extent:
+            return False
+        extent += (n - 1) * s
+    return True
+
+
+def _rows_meet(a, b):
+    """Whether K and V share memory; both _apart. Two views of other strides whose spans meet count as sharing; views of the
+    same strides may lie between each other, as K and V of a slot next to each other do."""
+    if not _overlap(a, b):
+        return False
+    dims = sorted(((s, n) for s, n in zip(a.stride(), a.shape) if n > 1), reverse=True)
+    if dims != sorted(((s, n) for s, n in zip(b.stride(), b.shape) if n > 1), reverse=True):
+        return True
+    d, odd = divmod(b.data_ptr() - a.data_ptr(), a.element_size())
+
+    def meet(d, i):  # two elements d apart in a's dimensions from i on: of the outer one, the multiple below d or above it
+        if i == len(dims):
+            return d == 0
+        s, n = dims[i]
+        return any(abs(k) < n and meet(d - k * s, i + 1) for k in (d // s, d // s + 1))
+    return odd != 0 or meet(d, 0)
 
 
 def _overlap(a, b):

@@ -504,7 +504,7 @@ pybind11::object evict_fast(const torch::Tensor& k, const torch::Tensor& v, cons
   if (heads > 65535 || slots > INT32_MAX || rb > 4096 || n < 1 || n > slots || keep < 1 || keep >= n || recent < 0 || sink < 0 ||
       recent + sink > keep || !here(k, {&v, &w}) || ko.has_value() != vo.has_value() || (wo && !ko))
     return pybind11::none();
-  if (ko ? ko->data_ptr() == vo->data_ptr() : k.data_ptr() == v.data_ptr()) return pybind11::none();
+  if (!ko && (overlap(k, v) || overlap(k, w) || overlap(v, w))) return pybind11::none();
   const fl_rows kr{k.data_ptr(), 0, slots * rb, rb}, vr{v.data_ptr(), 0, slots * rb, rb};
   fl_rows kor{}, vor{};
   int64_t so = 0;
@@ -513,6 +513,7 @@ pybind11::object evict_fast(const torch::Tensor& k, const torch::Tensor& v, cons
         !on16(*vo) || ko->size(-1) != k.size(-1) || ko->sizes().slice(0, dims - 2) != k.sizes().slice(0, dims - 2) ||
         !here(k, {&*ko, &*vo, wo ? &*wo : &k}))
       return pybind11::none();
+    if (overlap(*ko, *vo) || (wo && (overlap(*ko, *wo) || overlap(*vo, *wo)))) return pybind11::none();
     so = ko->size(-2);
     if (so < keep || so > INT32_MAX) return pybind11::none();
     if (wo && (!plain(*wo, torch::kFloat32, dims - 1) || wo->sizes() != ko->sizes().slice(0, dims - 1))) return pybind11::none();

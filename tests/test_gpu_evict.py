@@ -225,3 +225,44 @@ def test_lengths_at_the_last_seams(dev, heads, n):
     kept = evict(k, v, w, n, keep, recent=5, sink=3)
     assert torch.equal(kept.long(), want)
     assert torch.equal(k[:, :keep, 0], w[:, :keep].bfloat16()) and (w[:, keep:] == 0).all()
+
+
+def test_rows_that_meet_are_not_written(dev):
+    """K and V, heads or weights that share a part of their memory; views that only lie between each other go through."""
+    from flint_amd.attention import evict
+    _, _, w = (x.to(dev) for x in make((2, 2), 50, 64))
+    flat = torch.randn(2 * 2 * 50 * 64 + 4096, device=dev).bfloat16()
+
+    def view(start, *strides, slots=50):
+        return flat.as_strided((2, 2, slots, 64), (*strides, 1), start)
+    k = view(0, 6400, 3200, 64)
+    for v in (view(64, 6400, 3200, 64), view(3200, 6400, 3200, 64), view(32, 6400, 3200, 64), view(8, 6400, 3200, 64), view(0, 64, 128, 256)):
+        with pytest.raises(ValueError, match="same memory"):
+            evict(k, v, w, 40, 10)
+    far = torch.randn(2, 2, 50, 64, device=dev).bfloat16()
+    for bad in (view(0, 3200, 1600, 64), view(0, 64, 3200, 64), view(0, 8, 3200, 64)):
+        with pytest.raises(ValueError, match="share"):
+            evict(bad, far, w, 40, 10)
+        with pytest.raises(ValueError, match="share"):
+            evict(far, far.clone(), w, 40, 10, out=(bad, far.clone()))
+    new = torch.zeros(2 * 2 * 20 * 64 + 640, dtype=torch.bfloat16, device=dev)
+    a, b = new[:5120].view(2, 2, 20, 64), new[64:5184].view(2, 2, 20, 64)
+    with pytest.raises(ValueError, match="same memory"):
+        evict(far, far.clone(), w, 40, 10, out=(a, b))
+    with pytest.raises(ValueError, match="overlap"):
+        evict(far, far.clone(), w, 40, 10, out=(a, torch.zeros_like(a), new[16:176].view(torch.float32).view(2, 2, 20)))
+    with pytest.raises(ValueError, match="overlap"):
+        evict(far, far.clone(), far.view(-1)[:400].view(torch.float32).view(2, 2, 50), 40, 10)
+    # K and V of a slot next to each other, of a head next to each other, of a sequence next to each other
+    for shape, dim in (((2, 2, 50, 2, 64), 3), ((2, 2, 2, 50, 64), 2), ((2, 2, 2, 50, 64), 1)):
+        both = torch.randn(shape, device=dev).bfloat16()
+        kk, vv = both.unbind(dim)
+        k0, v0, w0 = kk.clone(), vv.clone(), w.clone()
+        want = evict(k0, v0, w0, 40, 10, 2, 1)
+        wi = w.clone()
+        assert torch.equal(evict(kk, vv, wi, 40, 10, 2, 1), want)
+        assert torch.equal(kk, k0) and torch.equal(vv, v0) and torch.equal(wi, w0)
+    # slots before heads
+    t = [torch.randn(2, 50, 2, 64, device=dev).bfloat16().transpose(1, 2) for _ in range(2)]
+    c = [x.clone() for x in t]
+    assert torch.equal(evict(*t, w.clone(), 40, 10), evict(*c, w.clone(), 40, 10)) and all(torch.equal(x, y) for x, y in zip(t, c))
