@@ -90,12 +90,13 @@ def tree_attention(q, k_cache, v_cache, pos, mask=None, scale=None, return_lse=F
 
     q bf16 or fp16 device [B, M, heads, dim], k_cache and v_cache [B, key heads, slots, dim] (without B: one sequence),
     dim 64 or 128; the nodes' own K and V are in the caches already. Strided caches are read as they lie, given a
-    contiguous last dimension and the rest on 16 bytes. pos: cached keys before node 0, an int or a device int per sequence (one outside 0 ..
-    slots - M gives NaN). mask bool or uint8 [M, M] or [B, M, M]: node i sees node j (None: a chain, j <= i).
-    scale: of the scores, positive (None: dim ** -0.5). Returns the output in q's shape and type and, with return_lse, the log sum
-    exp of the scaled scores (fp32 [B, M, heads]). A node that sees nothing gives 0 and -inf; an infinity or a NaN in the
-    value of a slot that it sees makes that dimension the same, however small its weight (infinities of both signs: NaN). No
-    gradient."""
+    contiguous last dimension and the rest on 16 bytes. pos: cached keys before node 0, an int or a device int per
+    sequence (one outside 0 .. slots - M gives NaN). mask bool or uint8 [M, M] or [B, M, M]: node i sees node j (None: a
+    chain, j <= i). scale: of the scores, positive (None: dim ** -0.5). Returns the output in q's shape and type and, with
+    return_lse, the log sum exp of the scaled scores (fp32 [B, M, heads]). A node that sees nothing gives 0 and -inf; an
+    infinity or a NaN in the value of a slot that it sees makes that dimension the same, however small its weight
+    (infinities of both signs: NaN). Calls of 2^32 threads or more (one token each of 65536 sequences of 128 key heads)
+    raise FlError. No gradient."""
     if _tree_attention_fast is not None and q.is_cuda:
         at, p0 = (None, pos) if type(pos) is int else (pos, 0)
         if at is None or type(at) is torch.Tensor:

@@ -855,10 +855,13 @@ AttnArgs attn_args(const fl_attn_desc& d, const uint16_t* q, const uint16_t* k, 
   return a;
 }
 
+// one launch holds fewer than 2^32 threads
+bool launchable(int64_t wgs, int threads) { return wgs * threads <= (int64_t)UINT32_MAX; }
+
 template <bool H, int D>
 int attn_launch(AttnArgs a, const AttnPlan& p, hipStream_t s) {
   const int64_t wgs = (int64_t)a.b * a.groups * p.blocks * p.parts;
-  if (wgs > INT32_MAX) return FL_E_ARG;
+  if (!launchable(wgs, p.few ? 64 * AT_NW : 256)) return FL_E_ARG;
   const dim3 grid((uint32_t)wgs);
   if (!p.few) hipLaunchKernelGGL((k_attn_many<H, D>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((k_attn_few<H, D, AT_NW>), grid, dim3(64 * AT_NW), 0, s, a);
@@ -872,7 +875,7 @@ int weights_launch(AttnArgs a, float* w, int add, hipStream_t s) {
   const bool split = a.R > 32;
   const int tiles = (a.slots + 63) / 64, per = split ? tiles : (tiles + 3) / 4;
   const int64_t wgs = (int64_t)a.b * a.groups * per;
-  if (wgs > INT32_MAX) return FL_E_ARG;
+  if (!launchable(wgs, 256)) return FL_E_ARG;
   if (split) hipLaunchKernelGGL((k_attn_weights<H, D, true>), dim3((uint32_t)wgs), dim3(256), 0, s, a, w, add);
   else hipLaunchKernelGGL((k_attn_weights<H, D, false>), dim3((uint32_t)wgs), dim3(256), 0, s, a, w, add);
   return hipGetLastError() == hipSuccess ? FL_OK : FL_E_LAUNCH;

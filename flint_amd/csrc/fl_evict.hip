@@ -221,6 +221,7 @@ int fl_evict(const fl_rows* k, const fl_rows* v, float* weights, int32_t n_outer
   const fl_rows *kd = k_out ? k_out : k, *vd = v_out ? v_out : v;
   if (!apart(kd) || !apart(vd) || kd->data == vd->data) return FL_E_ARG;
   if (k_out && (!strides_ok(k_out, row_bytes) || !strides_ok(v_out, row_bytes) || slots_out < keep)) return FL_E_ARG;
+  if (k_out && (int64_t)keep * (row_bytes / 16) > (int64_t)UINT32_MAX - 255) return FL_E_ARG;  // threads of a launch
   const int heads = n_outer * n_inner;
   EvictArgs a{};
   a.k = static_cast<unsigned char*>(k->data), a.v = static_cast<unsigned char*>(v->data), a.w = weights, a.kept = kept;

@@ -190,7 +190,10 @@ int fl_head_logprobs(const uint16_t* x, const int8_t* wq, const float* ws, const
 /* b sequences of m nodes each (a drafted tree, a chain, a prompt, or one token), `heads` query heads over `groups` key
  * heads of dim 64 or 128, caches of `slots` slots; bf16, or fp16 where fp16 != 0. Strides count values, between
  * sequences, nodes / key heads and query heads / slots; the last dimension is contiguous. Strides are multiples of 8,
- * pointers 16-byte aligned, k_s and v_s at most 2^23, a sequence's queries within 2^30 values, m at most 32768, slots at most 2^30. mask_b: bytes between the sequences' masks (0: one for all).
+ * pointers 16-byte aligned, k_s and v_s at most 2^23, a sequence's queries within 2^30 values, m at most 32768, slots at
+ * most 2^30. A call whose launch would have 2^32 threads or more (one token each of 65536 sequences of 128 key heads,
+ * say, or weights of more than 2^24 tiles of 64 slots) is refused. mask_b: bytes between the sequences' masks (0: one
+ * for all).
  * scale: positive. pos0: cached keys of every sequence, for calls without `pos`. */
 typedef struct fl_attn_desc {
   int32_t b, m, heads, groups, dim, slots, fp16, pos0;
@@ -237,7 +240,8 @@ typedef struct fl_rows {
  * keep - 1: in place (k_out, v_out NULL), with the weights (fp32 [heads][slots]), and the weights of keep .. n - 1
  * become 0, the rows there stay what they were; or into k_out and v_out (which do not overlap the caches) and, where
  * given, weights_out [heads][slots_out], with the caches left as they are. K and V, and the heads, that are written must
- * not share rows. 1 <= keep <= n <= slots, sink + recent <= keep, at most 65535 heads.
+ * not share rows. 1 <= keep <= n <= slots, sink + recent <= keep, at most 65535 heads, and into another cache fewer than
+ * 2^32 - 255 pieces of 16 bytes of a head's K.
  * No counterpart in the reference, whose cache only grows (engine/model.py:82-98). */
 int fl_evict(const fl_rows* k, const fl_rows* v, float* weights, int32_t n_outer, int32_t n_inner, int32_t slots,
              int32_t row_bytes, int32_t n, int32_t keep, int32_t recent, int32_t sink, int32_t* kept,

@@ -118,3 +118,17 @@ def test_python_entries_refuse():
         evict(k, k[..., :8, :], torch.zeros(1, 2, 16), 10, 5)
     with pytest.raises(ValueError, match="CUDA"):
         accept_sampled(torch.zeros(1, 2, 9), torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, 2), torch.zeros(1))
+
+
+def test_more_than_a_launch_holds():
+    """2^32 threads and more are refused before a launch."""
+    _lib, l = lib()
+    P = 4096
+    d = _lib.AttnDesc(b=65536, m=1, heads=256, groups=256, dim=64, slots=1, fp16=0, pos0=0, scale=0.125, q_h=64, k_g=64, v_g=64)
+    assert l.fl_tree_attention(ctypes.byref(d), P, P, P, None, None, P, None, P, None) == -1
+    assert l.fl_attention_weights(ctypes.byref(d), P, P, P, None, None, P, 0, None) == -1
+    d = _lib.AttnDesc(b=16, m=40, heads=16, groups=16, dim=64, slots=1 << 30, fp16=0, pos0=0, scale=0.125, q_m=1024, q_h=64, k_s=64, v_s=64)
+    assert l.fl_attention_weights(ctypes.byref(d), P, P, P, None, None, P, 0, None) == -1
+    r = [ctypes.byref(_lib.Rows(i * P, 0, 0, 4096)) for i in range(1, 5)]
+    n = 1 << 25
+    assert l.fl_evict(r[0], r[1], P, 1, 1, n, 4096, n, n, 0, 0, P, r[2], r[3], None, n, None) == -1
