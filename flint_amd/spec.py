@@ -49,6 +49,9 @@ if "FLINT_AMD_LIB" not in os.environ:
         pass
 
 
+WIDE_NODES = 1024  # of a tree in a prompt pass (Transformer.tree_features)
+
+
 def tree_depths(parents):
     """Depth of each node of a tree in verify order (node 0 = root, parents[0] = -1, every other
     parent an earlier node); raises ValueError on any other parent array. Reference
@@ -186,14 +189,15 @@ class LookupDraft:
     """Prompt-lookup draft: find earlier occurrences of the context's last n tokens (n from
     max_ngram down to min_ngram, the most recent occurrence first) and propose what followed
     them. tree() merges up to `width` distinct continuations into a trie of at most
-    max_nodes - 1 nodes below the root."""
+    max_nodes - 1 nodes below the root: up to 1024 nodes in all, of which a SpecDecoder without a
+    head takes 32."""
 
     def __init__(self, max_ngram=3, min_ngram=1, width=2, depth=4, max_nodes=_lib.MAX_VERIFY):
         if not 1 <= min_ngram <= max_ngram:
             raise ValueError("need 1 <= min_ngram <= max_ngram")
         self.max_ngram, self.min_ngram = int(max_ngram), int(min_ngram)
         self.width, self.depth = int(width), int(depth)
-        self.max_nodes = min(int(max_nodes), _lib.MAX_VERIFY)
+        self.max_nodes = min(int(max_nodes), WIDE_NODES)
 
     def reset(self):
         """Forget the indexed context (SpecDecoder.generate calls this at the start of a run)."""
@@ -282,7 +286,7 @@ class SpecDecoder:
         self.draft = draft if draft is not None else LookupDraft()
         self.k = int(k)
         self.head = head
-        nv = self._nodes = _lib.MAX_VERIFY if head is None else 1024
+        nv = self._nodes = _lib.MAX_VERIFY if head is None else WIDE_NODES
         if not 0 <= self.k < nv:
             raise ValueError(f"k must be in [0, {nv - 1}]")
         dev = model.device

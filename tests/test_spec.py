@@ -400,3 +400,16 @@ def test_lookup_draft_reused_on_a_different_context():
     assert reused.chain(ext, None, 4) == LookupDraft(max_ngram=3, width=3, depth=4).chain(ext, None, 4)
     reused.reset()
     assert reused.tree(a, None) == LookupDraft(max_ngram=3, width=3, depth=4).tree(a, None)
+
+
+def test_lookup_draft_proposes_as_many_nodes_as_asked_for():
+    """More than a verify launch takes, for a decoder with a head; without one the loop cuts the proposal."""
+    from flint_amd.spec import LookupDraft
+    ctx = []
+    for i in range(40):  # after every 7 another continuation
+        ctx += [7] + [100 * i + j for j in range(10, 22)]
+    ctx += [7]
+    for most, want in ((32, 31), (200, 199), (10 ** 6, 480)):
+        toks, pars = LookupDraft(max_ngram=1, width=40, depth=12, max_nodes=most).tree(ctx, None)
+        assert len(toks) == len(pars) == want
+    assert LookupDraft(max_nodes=10 ** 6).max_nodes == 1024 and LookupDraft().max_nodes == 32
