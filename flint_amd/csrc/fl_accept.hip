@@ -55,9 +55,10 @@ __device__ __forceinline__ double wave_dsum(double v) {
 __device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
 
 // One workgroup per tree; its waves sum pieces of a row for the rejections that need Z and for the last token (without draft
-// probabilities a node's row is summed once, and a rejected token taken off). One CU reads a row of 49152 fp32 values and its draft row in 2.6 us at its 64 bytes a cycle,
-// about what one exchange between workgroups costs, so a row stays with one. (Held in registers between two sums, the
-// row's 96 values a lane and their conversions spilled.)
+// probabilities a node's row is summed once and rejected tokens are taken off, and again where little is left). One CU
+// reads a row of 49152 fp32 values and its draft row in 2.6 us at its 64 bytes a cycle, about what one exchange between
+// workgroups costs, so a row stays with one. (Held in registers between two sums, the row's 96 values a lane and their
+// conversions spilled.)
 template <bool BF, bool DRAFT>
 __global__ __launch_bounds__(AC_NT) void k_accept(AcceptArgs a) {
   __shared__ double red[2][AC_NW];

@@ -818,9 +818,9 @@ AttnPlan attn_plan_of(const fl_attn_desc& d, int keys, bool few) {
   const int unit = few ? AT_NW * 4096 / d.dim : 64, least = few ? unit : 256;
   const int64_t base = (int64_t)d.b * d.groups * p.blocks;
   // Workgroups that cutting the keys may reach. Few rows: one per CU, whose eight waves have 128 KB in flight (131072 keys
-  // 53 us, with two rounds of workgroups 60). Many rows: of the three (dim 64) or two that a CU holds, one and a third
-  // times as many as there are places (1024 tokens behind 4096: 640 116 us, 1024 104, 1600 112; 16 trees of 13 and
-  // 128 dims: 640 56, 1024 67).
+  // 55 us, with two rounds of workgroups 62). Many rows: of the three (dim 64) or two that a CU holds, one and a third
+  // times as many as there are places (1024 tokens behind 4096: 640 113 us, 1024 103, 1600 109; 16 trees of 13 and
+  // 128 dims: 640 59, 1024 70).
   const int64_t fill = few ? 256 : d.dim == 64 ? 1024 : 640;
   // a wave of few rows takes three tiles in less than the launch that joins parts costs (1032 keys: 11.6 uncut, 13.5 in
   // two parts; 2000: 16.0 and 13.5)
@@ -837,8 +837,8 @@ AttnPlan attn_plan(const fl_attn_desc& d, bool pos_known) {
   const int R = d.m * (d.heads / d.groups), keys = pos_known ? d.pos0 + d.m : d.slots;
   // Few rows: a wave's own keys need no barrier but meet in LDS at the end, which pays where one launch does (up to three
   // tiles a wave) and where memory is the bound; in between the shared ring's kernel starts and ends sooner. us, one
-  // token, few / many: 1000 keys 10.9 / 11.6, 2000 13.5 / 10.7, 8000 13.5 / 11.8, 131072 44 / 67; 24 sequences of 3000
-  // 34 / 40, 8 trees of 8 behind 2000 16.7 / 17.5; 40 rows behind 4000 14.9 / 11.6, behind 30000 20.7 / 24.8.
+  // token, few / many: 1000 keys 11.2 / 11.5, 2000 13.6 / 10.7, 8000 13.5 / 11.8, 131072 46 / 68; 24 sequences of 3000
+  // 34 / 40, 8 trees of 8 behind 2000 17.0 / 18.6; 40 rows behind 4000 14.7 / 11.5, behind 30000 21.1 / 25.8.
   const bool few = R <= AT_FEW && (keys <= 3 * AT_NW * 4096 / d.dim || (int64_t)d.b * d.groups * keys * d.dim >= 6 << 20);
   return attn_plan_of(d, keys, few);
 }
