@@ -207,9 +207,9 @@ typedef struct fl_attn_desc {
 /* Attention of the nodes over the cache: node i of a sequence sits in slot pos + i (K and V are there already) and
  * attends to the slots [0, pos) and to pos + j where mask[i][j] != 0 (uint8 [M][M]; NULL: a chain, j <= i), as
  * fl_verify's tokens do. pos: device int32 [B], or NULL for pos0. out [B][M][heads][dim], rounded once from sums in fp32
- * of the weights times V, each weight as two 16-bit terms: off by up to 2^-17 of itself (bf16), 2^-28 of the largest of
- * the up to 64 keys next to it (fp16; 2^-76 of the row's largest at least). lse (optional, fp32 [B][M][heads]): log sum
- * exp of the scaled scores, natural. A node that sees nothing gives 0 and -inf; a sequence whose pos lies outside 0 ..
+ * of the weights times V, each weight as two 16-bit terms: off by up to 2^-17 of itself (bf16) or 2^-28 of the largest of
+ * its tile of up to 64 keys (fp16, where weights below 2^-76 of a row's largest may be lost). lse (optional, fp32
+ * [B][M][heads]): log sum exp of the scaled scores, natural. A node that sees nothing gives 0 and -inf; a sequence whose pos lies outside 0 ..
  * slots - m gives NaN. What a node does not see never reaches it, infinities and NaN included; an infinity or a NaN in
  * the value of a slot that it sees makes that dimension the same, however small its weight (infinities of both signs:
  * NaN). Slots behind pos + m are not read. work: 16-byte aligned, of
