@@ -202,15 +202,27 @@ __device__ __forceinline__ void softmax_pv(fl_f32x16 (&s)[KT], Rows<H, D / 32>& 
 #pragma unroll
     for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(s[kt][i], s[kt][i + 1]), mx);  // one three-way maximum each
   mx = xor32_max(mx) * sc;
+  // Arguments are s c - m rounded once, m a rounded s c. From 2^22 on that one's own rounding would show in all of a row's
+  // weights alike (from 2^31 on beyond what fp32 holds, from 2^24 on fp16): there s c is rounded first, as m is.
+  if (__builtin_expect(__any(fabsf(mx) >= 0x1p22f && mx > -INFINITY), 0)) {
+    const bool big = fabsf(mx) >= 0x1p22f && mx > -INFINITY;
+    const float f = big ? sc : 1.0f;
+    sc = big ? 1.0f : sc;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kt][i] *= f;
+  }
   if constexpr (H) {
     // m is an integer, 11 below the scores of some tile: p lies below 2^15 (fp16 ends at 2^16) and a tile's largest at
     // 2^3 or more, so that what lies far below a row's maximum keeps its bits. It follows a tile's maximum both ways
     // (o and l then grow by that power of two), down to 40 below the row's: 2^-76 of its largest weight may be dropped,
     // and o stays below 2^(56 + 16) times the number of keys. 16 trees of 13 behind 8011 keys 59 us; with the reference
     // of bf16, which lost those, 57.
-    if (__any(fabsf(mx - (st.m + 9.0f)) > 6.0f)) {
-      const float mn = floorf(fmaxf(mx, st.top - 40.0f)) - 11.0f;
-      const bool move = mx > st.m + 15.0f || (mx > -INFINITY && mn < st.m - 8.0f);
+    if (__any(fabsf((mx - st.m) - 9.0f) > 6.0f)) {
+      const float near = floorf(fmaxf(mx, st.top - 40.0f));
+      const float mn = near - (near - 11.0f) > 15.0f ? near : near - 11.0f;  // no 11 below where floats lie 16 apart
+      const bool move = mx - st.m > 15.0f || (mx > -INFINITY && st.m - mn > 8.0f);
       if (__any(move)) {
         st.refer_to(move ? mn : st.m);
         st.top = fmaxf(st.top, st.m + 11.0f);

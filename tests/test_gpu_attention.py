@@ -502,3 +502,33 @@ def test_a_key_that_no_row_can_weigh(dev, m, heads, groups, dim, dtype):
     k[:, :, 17, 3], k[:, :, 18, 3], k[:, :, 19, 5] = math.inf, math.nan, math.inf
     none = torch.full((1, m, heads), -math.inf, device=dev)
     assert (attention_weights(q.to(dev), k.to(dev), none, pos) == 0).all()
+
+
+@pytest.mark.parametrize("dtype,big", [(torch.float16, 9.0e2), (torch.float16, 1.5e4), (torch.float16, 3.6e4), (torch.bfloat16, 6.0e4), (torch.bfloat16, 1.0e7), (torch.bfloat16, 1.0e16)])
+@pytest.mark.parametrize("m,heads,groups,dim,ctx", [(1, 4, 2, 64, 300), (1, 4, 4, 64, 9000), (40, 4, 2, 64, 2000), (16, 8, 1, 128, 700)])
+def test_scores_that_fp32_hardly_resolves(dev, m, heads, groups, dim, ctx, dtype, big):
+    """Scores of 10^7 and far more, their differences exact multiples of a power of two: one key of a row leads all others
+    by more than the score's own error, and its value is the row's (the others' weights are below 2^-60)."""
+    from flint_amd.attention import tree_attention
+    g = torch.Generator(device=dev).manual_seed(ctx)
+    n = ctx + m
+    q = torch.zeros(1, m, heads, dim, device=dev)
+    q[..., :32] = big * (1 + torch.arange(m * heads, device=dev).view(1, m, heads, 1) % 5 / 8)
+    k = torch.zeros(1, groups, n, dim, device=dev)
+    level = torch.randint(1, 32, (1, groups, n), generator=g, device=dev) / 64
+    for sign in (1.0, -1.0):
+        k[..., :32] = (sign * big * (1 + level))[..., None]
+        lead = torch.randint(0, ctx, (groups,), generator=g, device=dev)
+        kk = k.clone()
+        kk[0, torch.arange(groups), lead, :32] = big * (1.75 if sign > 0 else -0.875)
+        v = torch.randn(1, groups, n, dim, generator=g, device=dev).to(dtype)
+        qd, kd = q.to(dtype), kk.to(dtype)
+        out, lse = tree_attention(qd, kd, v, ctx, None, 0.125, True)
+        rep = heads // groups
+        for j in range(groups):
+            s = torch.matmul(qd[0, :, j * rep:(j + 1) * rep].double(), kd[0, j].double().t().contiguous()) * 0.125
+            top = s.topk(2, -1).values
+            # sums of 32 products: an error of 32 2^-24 of the score; the lead is 1/8 of it and more than 60 by far
+            assert ((top[..., 0] - top[..., 1]) > 1e5).all()
+            assert torch.equal(out[0, :, j * rep:(j + 1) * rep], v[0, j, lead[j]].expand(m, rep, dim))
+            assert ((lse[0, :, j * rep:(j + 1) * rep].double() - top[..., 0]).abs() <= 2.0 ** -18 * top[..., 0].abs()).all()
